@@ -651,6 +651,78 @@ int vgdr_scalar_gates(int dtype, const void *x, const void *w_ab, const float *n
 int vgdr_swiglu(int dtype, const void *x, void *y, int64_t rows, int64_t hidden, hipStream_t stream);
 
 /*
+ * Speculative decoding (no reference counterpart: its Generator takes one token a
+ * step, infra/inference/generator.py).  A step feeds every stream its last token and
+ * up to 15 drafts; how many of them stand is known after the head, so the layers'
+ * states take a block's tokens at the next step (vgdr_draft_step), once
+ * vgdr_verify_drafts has counted them.
+ *
+ * vgdr_draft_block: what a block leaves behind.  Room for `capacity` (1..16) tokens per
+ * stream; 16-byte aligned.  k [B, capacity, H, dk], u [B, capacity, H, dv] and g ([B, capacity,
+ * H] or [B, capacity, H, dk]; NULL without a gate) in fp32: the block's keys as the recurrence
+ * takes them, its writes u_t = beta_t (v_t - S^T k_t) (v_t without the delta rule) and log-decays.
+ * x_q, x_k [B, capacity, H * dk], x_v [B, capacity, H * dv] in dtype: its raw conv inputs (NULL
+ * without a conv).
+ */
+typedef struct vgdr_draft_block {
+    float *k, *u, *g;
+    void *x_q, *x_k, *x_v;
+    int64_t capacity;
+} vgdr_draft_block;
+
+/*
+ * Commits, per stream b, the first accepted[b] (clamped to 0..capacity) tokens of the
+ * pending block to state [B, H, dk, dv] (fp32) and to the conv caches, in place; then forms
+ * the outputs o [B, L, H, dv] of L new tokens (0 <= L <= capacity; L = 0 commits only and
+ * leaves the pending block as it is), which become the pending block and move neither
+ * state nor caches.  Everything else as vgdr_decode_step_strided (q, k, v, gate rows of
+ * token b * L + t, ld_qk and ld_v elements apart; g, beta [B, L, H], g [B, L, H, dk] per
+ * channel, in fusion->gate_dtype where the kernel activates it), but that no intermediate is
+ * rounded to dtype and that the conv takes any kernel size 1..8.  Pending rows from L on
+ * are left as they were.  dk a multiple of 8 up to 128, dv a multiple of 8 up to 256.
+ */
+int vgdr_draft_step(int dtype, int gate_kind, int use_delta, const void *q, const void *k, const void *v,
+                    const void *g, const float *beta, void *o, float *state, const vgdr_draft_block *pending,
+                    const int32_t *accepted, int64_t B, int64_t L, int64_t H, int64_t dk, int64_t dv,
+                    int64_t ld_qk, int64_t ld_v, float scale, const vgdr_fusion *fusion,
+                    const vgdr_short_conv *conv, const vgdr_epilogue *epilogue, hipStream_t stream);
+
+/*
+ * Drafts against the target.  logits: row i of stream b (after the block's token i; V elements in
+ * dtype) at b * ld_stream + i * ld_row; drafts [B, K] (draft i is verified by row i), uniforms
+ * [B, K + 1] in [0, 1), temperature [B] (0, or anything that is not above it: greedy), n_drafts
+ * [B] (NULL: K each; clamped to 0..K).  With p_i = softmax(row i / T) and q_i the draft's
+ * probabilities (probs, in probs_dtype, rows as logits'; NULL: the draft is certain), draft i
+ * stands if all before it do and uniforms[i] q_i(d_i) < p_i(d_i).  The token behind the drafts
+ * that stand is the lowest v at which the running sum of r exceeds uniforms[K] times its whole: r = p where
+ * every draft stands, else max(p_i - q_i, 0) (p_i where that is zero everywhere).  Greedy: p is 1 at the
+ * row's lowest top.  tokens [B, K + 1]: the drafts that stand, that token, then -1; accepted [B].
+ * NaN logits have no mass; equal ones share it, +inf and a row of -inf alone included; a draft outside
+ * 0..V-1 never stands.  Sums and weights are 64-bit.  0 <= K <= 64, 1 <= V < 2^31 - 2^20.  workspace:
+ * vgdr_verify_drafts_workspace_size bytes, 16-byte aligned, calls that overlap have their own.
+ */
+int64_t vgdr_verify_drafts_workspace_size(int64_t B, int64_t K, int64_t V);
+int vgdr_verify_drafts(int dtype, const void *logits, int64_t ld_stream, int64_t ld_row, const int64_t *drafts,
+                       const float *uniforms, const float *temperature, const void *probs, int probs_dtype,
+                       int64_t ld_probs_stream, int64_t ld_probs_row, const int32_t *n_drafts, int64_t *tokens,
+                       int32_t *accepted, void *workspace, int64_t workspace_bytes, int64_t B, int64_t K, int64_t V,
+                       hipStream_t stream);
+
+/*
+ * Drafts from the streams' own text: history row b (ld elements apart, room for cap tokens of
+ * token_bytes 4 or 8 each) holds lengths[b] (clamped to 0..cap) tokens.  Of the places before
+ * its last token at which min_ngram or more of its last tokens end as well, the one where most do
+ * (max_ngram counted at most), the latest of those; drafts [B, K] are the tokens that followed it, read on
+ * from the first of them again where the text ends, and counts [B] = K; without such a place
+ * zeros and 0.  1 <= min_ngram <= max_ngram <= 16, 1 <= K <= 64.  workspace:
+ * vgdr_lookup_drafts_workspace_size bytes, 16-byte aligned (0: none), calls that overlap have their own.
+ */
+int64_t vgdr_lookup_drafts_workspace_size(int64_t B, int64_t cap);
+int vgdr_lookup_drafts(const void *history, int token_bytes, int64_t ld, int64_t cap, const int32_t *lengths,
+                       int64_t *drafts, int32_t *counts, void *workspace, int64_t workspace_bytes, int64_t B, int64_t K,
+                       int max_ngram, int min_ngram, hipStream_t stream);
+
+/*
  * Packed-batch schedule.  No reference counterpart (the reference has no
  * cu_seqlens, see infra/inference/generator.py:19-22); fla builds the same
  * integer tables for its varlen kernels.  Writes into `workspace`

@@ -51,6 +51,12 @@ class GateParams(ctypes.Structure):
                 ('param_dtype', ctypes.c_int)]
 
 
+class DraftBlock(ctypes.Structure):
+    """struct vgdr_draft_block: what a block of drafted tokens leaves behind."""
+    _fields_ = [('k', ctypes.c_void_p), ('u', ctypes.c_void_p), ('g', ctypes.c_void_p), ('x_q', ctypes.c_void_p),
+                ('x_k', ctypes.c_void_p), ('x_v', ctypes.c_void_p), ('capacity', ctypes.c_int64)]
+
+
 # every symbol the header declares, with its ctypes signature
 _P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
 _FZ = ctypes.POINTER(Fusion)
@@ -123,6 +129,12 @@ SIGNATURES = {
     'vgdr_causal_conv1d': (_I, [_I, _P, _P, _I, _P, _P, _P, _P, _L, _L, _L, _L, _I, _I, _P]),
     'vgdr_causal_conv1d_bwd_workspace_size': (_L, [_I, _L, _L, _L, _I]),
     'vgdr_causal_conv1d_bwd': (_I, [_I, _P, _P, _P, _P, _P, _P, _L, _L, _L, _L, _I, _I, _P]),
+    'vgdr_draft_step': (_I, [_I, _I, _I, _P, _P, _P, _P, _P, _P, _P, ctypes.POINTER(DraftBlock), _P,
+                             _L, _L, _L, _L, _L, _L, _L, _F, _FZ, _SC, _EP, _P]),
+    'vgdr_verify_drafts_workspace_size': (_L, [_L, _L, _L]),
+    'vgdr_verify_drafts': (_I, [_I, _P, _L, _L, _P, _P, _P, _P, _I, _L, _L, _P, _P, _P, _P, _L, _L, _L, _L, _P]),
+    'vgdr_lookup_drafts_workspace_size': (_L, [_L, _L]),
+    'vgdr_lookup_drafts': (_I, [_P, _I, _L, _L, _P, _P, _P, _P, _L, _L, _L, _I, _I, _P]),
     'vgdr_varlen_workspace_size': (_L, [_L]),
     'vgdr_varlen_prepare': (_I, [_P, _L, _L, _I, _P, _P]),
 }

@@ -1312,4 +1312,175 @@ int vgdr_varlen_prepare(const int32_t *cu_seqlens, int64_t n_seqs, int64_t n_tok
                       "vgdr_varlen_prepare launch");
 }
 
+int vgdr_draft_step(int dtype, int gate_kind, int use_delta, const void *q, const void *k, const void *v,
+                    const void *g, const float *beta, void *o, float *state, const vgdr_draft_block *pending,
+                    const int32_t *accepted, int64_t B, int64_t L, int64_t H, int64_t dk, int64_t dv,
+                    int64_t ld_qk, int64_t ld_v, float scale, const vgdr_fusion *fusion,
+                    const vgdr_short_conv *conv, const vgdr_epilogue *epilogue, hipStream_t stream) {
+    g_err[0] = 0;
+    const char *fn = "vgdr_draft_step";
+    if (dtype != VGDR_F32 && dtype != VGDR_BF16 && dtype != VGDR_F16)
+        return fail(VGDR_ERR_INVALID, "%s: unknown dtype %d", fn, dtype);
+    if (gate_kind < VGDR_GATE_NONE || gate_kind > VGDR_GATE_VECTOR)
+        return fail(VGDR_ERR_INVALID, "%s: unknown gate_kind %d", fn, gate_kind);
+    if (B < 0 || L < 0 || H <= 0)
+        return fail(VGDR_ERR_INVALID, "%s: bad sizes B=%lld L=%lld H=%lld", fn, (long long)B, (long long)L, (long long)H);
+    if (dk <= 0 || dk > 128 || dk % 8 || dv <= 0 || dv > 256 || dv % 8)
+        return fail(VGDR_ERR_UNSUPPORTED, "%s: dk=%lld dv=%lld (multiples of 8 up to 128 and 256)", fn, (long long)dk,
+                    (long long)dv);
+    if (!pending || pending->capacity < 1 || pending->capacity > vgdr::DRAFT_MAX)
+        return fail(pending ? VGDR_ERR_UNSUPPORTED : VGDR_ERR_INVALID, "%s: a pending block of 1 to %d tokens is required",
+                    fn, vgdr::DRAFT_MAX);
+    if (L > pending->capacity)
+        return fail(VGDR_ERR_INVALID, "%s: L=%lld tokens, room for %lld", fn, (long long)L, (long long)pending->capacity);
+    if (B > 0x7fffffffLL / H || H > 0x7fffffffLL / 256)
+        return fail(VGDR_ERR_INVALID, "%s: too many (stream, head) pairs", fn);
+    if (B == 0) return VGDR_OK;
+    vgdr::DraftParams p{};
+    int rc = check_fusion(fn, fusion, dtype, gate_kind, use_delta, false, p.fz);
+    if (rc) return rc;
+    rc = check_conv(fn, conv, dtype, p.cv);
+    if (rc) return rc;
+    rc = check_epilogue(fn, epilogue, dtype, p.ep);
+    if (rc) return rc;
+    if (p.fz.beta_sigmoid && !use_delta)
+        return fail(VGDR_ERR_INVALID, "%s: there is no beta to activate without the delta rule", fn);
+    if (!state || !accepted || !pending->k || !pending->u || (gate_kind != VGDR_GATE_NONE && !pending->g) ||
+        (conv && (!pending->x_q || !pending->x_k || !pending->x_v)))
+        return fail(VGDR_ERR_INVALID, "%s: state, accepted and every part of the pending block are required", fn);
+    for (const void *t : {(const void *)state, (const void *)pending->k, (const void *)pending->u,
+                          (const void *)pending->g, (const void *)pending->x_q, (const void *)pending->x_k,
+                          (const void *)pending->x_v, (const void *)p.cv.cq, (const void *)p.cv.ck,
+                          (const void *)p.cv.cv, q, k, v, (const void *)o})
+        if (!aligned16(t)) return fail(VGDR_ERR_INVALID, "%s: every tensor must be 16-byte aligned", fn);
+    if (L > 0) {
+        if (!q || !k || !v || !o) return fail(VGDR_ERR_INVALID, "%s: q, k, v and o are required", fn);
+        if (gate_kind != VGDR_GATE_NONE && !g) return fail(VGDR_ERR_INVALID, "%s: gate_kind %d needs g", fn, gate_kind);
+        if (gate_kind == VGDR_GATE_VECTOR && !aligned16(g))
+            return fail(VGDR_ERR_INVALID, "%s: a per-channel g must be 16-byte aligned", fn);
+        if (use_delta && !beta) return fail(VGDR_ERR_INVALID, "%s: the delta rule needs beta", fn);
+        if (ld_qk < H * dk || ld_v < H * dv || ld_qk % 8 || ld_v % 8)
+            return fail(VGDR_ERR_INVALID, "%s: row strides (%lld, %lld): multiples of 8, at least H*dk = %lld, H*dv = %lld",
+                        fn, (long long)ld_qk, (long long)ld_v, (long long)(H * dk), (long long)(H * dv));
+    }
+    p.q = q;
+    p.k = k;
+    p.v = v;
+    p.g = g;
+    p.beta = beta;
+    p.o = o;
+    p.S = state;
+    p.pk = pending->k;
+    p.pu = pending->u;
+    p.pg = pending->g;
+    p.xq = pending->x_q;
+    p.xk = pending->x_k;
+    p.xv = pending->x_v;
+    p.accepted = accepted;
+    p.ld_qk = ld_qk;
+    p.ld_v = ld_v;
+    p.N = B;
+    p.L = (int)L;
+    p.P = (int)pending->capacity;
+    p.H = (int)H;
+    p.dk = (int)dk;
+    p.dv = (int)dv;
+    p.dtype = dtype;
+    p.use_delta = use_delta ? 1 : 0;
+    p.scale = scale;
+    return hip_status(vgdr::draft_step(gate_kind, p, stream), "vgdr_draft_step launch");
+}
+
+static int check_verify(const char *fn, int64_t B, int64_t K, int64_t V) {
+    if (B < 0 || K < 0 || V < 1 || V >= 0x7ff00000LL)
+        return fail(VGDR_ERR_INVALID, "%s: bad sizes B=%lld K=%lld V=%lld", fn, (long long)B, (long long)K, (long long)V);
+    if (K > 64) return fail(VGDR_ERR_UNSUPPORTED, "%s: K=%lld drafts (at most 64)", fn, (long long)K);
+    if (B * (K + 1) > 0x1000000LL) return fail(VGDR_ERR_INVALID, "%s: too many rows", fn);
+    return VGDR_OK;
+}
+
+int64_t vgdr_verify_drafts_workspace_size(int64_t B, int64_t K, int64_t V) {
+    g_err[0] = 0;
+    if (check_verify("vgdr_verify_drafts_workspace_size", B, K, V)) return 0;
+    return vgdr::verify_workspace(B, K, V);
+}
+
+int vgdr_verify_drafts(int dtype, const void *logits, int64_t ld_stream, int64_t ld_row, const int64_t *drafts,
+                       const float *uniforms, const float *temperature, const void *probs, int probs_dtype,
+                       int64_t ld_probs_stream, int64_t ld_probs_row, const int32_t *n_drafts, int64_t *tokens,
+                       int32_t *accepted, void *workspace, int64_t workspace_bytes, int64_t B, int64_t K, int64_t V,
+                       hipStream_t stream) {
+    g_err[0] = 0;
+    const char *fn = "vgdr_verify_drafts";
+    for (int t : {dtype, probs ? probs_dtype : (int)VGDR_F32})
+        if (t != VGDR_F32 && t != VGDR_BF16 && t != VGDR_F16) return fail(VGDR_ERR_INVALID, "%s: unknown dtype %d", fn, t);
+    int rc = check_verify(fn, B, K, V);
+    if (rc) return rc;
+    if (B == 0) return VGDR_OK;
+    if (!logits || (K > 0 && !drafts) || !uniforms || !temperature || !tokens || !accepted)
+        return fail(VGDR_ERR_INVALID, "%s: logits, drafts, uniforms, temperature, tokens and accepted are required", fn);
+    if (ld_row < V || (B > 1 && ld_stream < 0) || (probs && ld_probs_row < V))
+        return fail(VGDR_ERR_INVALID, "%s: rows of %lld elements need strides of at least that", fn, (long long)V);
+    if (!workspace || !aligned16(workspace) || workspace_bytes < vgdr::verify_workspace(B, K, V))
+        return fail(VGDR_ERR_INVALID, "%s: a 16-byte aligned workspace of %lld bytes is required", fn,
+                    (long long)vgdr::verify_workspace(B, K, V));
+    vgdr::VerifyParams p{};
+    p.logits = logits;
+    p.drafts = drafts;
+    p.uniforms = uniforms;
+    p.temperature = temperature;
+    p.probs = K > 0 ? probs : nullptr;
+    p.n_drafts = n_drafts;
+    p.tokens = tokens;
+    p.accepted = accepted;
+    p.rows = reinterpret_cast<vgdr::RowMass *>(workspace);
+    p.ld_stream = ld_stream;
+    p.ld_row = ld_row;
+    p.ld_probs_stream = ld_probs_stream;
+    p.ld_probs_row = ld_probs_row;
+    p.N = B;
+    p.K = (int)K;
+    p.V = (int)V;
+    p.probs_dtype = probs_dtype;
+    return hip_status(vgdr::verify_drafts(dtype, p, stream), "vgdr_verify_drafts launch");
+}
+
+int64_t vgdr_lookup_drafts_workspace_size(int64_t B, int64_t cap) {
+    g_err[0] = 0;
+    (void)B;
+    (void)cap;
+    return 0;
+}
+
+int vgdr_lookup_drafts(const void *history, int token_bytes, int64_t ld, int64_t cap, const int32_t *lengths,
+                       int64_t *drafts, int32_t *counts, void *workspace, int64_t workspace_bytes, int64_t B, int64_t K,
+                       int max_ngram, int min_ngram, hipStream_t stream) {
+    g_err[0] = 0;
+    const char *fn = "vgdr_lookup_drafts";
+    if (token_bytes != 4 && token_bytes != 8)
+        return fail(VGDR_ERR_INVALID, "%s: tokens of %d bytes (4 or 8)", fn, token_bytes);
+    if (B < 0 || B > 0x1000000LL || cap < 0 || cap > 0x7fffffffLL || K < 1 || K > 64)
+        return fail(VGDR_ERR_INVALID, "%s: bad sizes B=%lld cap=%lld K=%lld", fn, (long long)B, (long long)cap, (long long)K);
+    if (min_ngram < 1 || max_ngram < min_ngram || max_ngram > 16)
+        return fail(VGDR_ERR_INVALID, "%s: 1 <= min_ngram <= max_ngram <= 16, got %d, %d", fn, min_ngram, max_ngram);
+    if (B == 0) return VGDR_OK;
+    if (!history || !lengths || !drafts || !counts)
+        return fail(VGDR_ERR_INVALID, "%s: history, lengths, drafts and counts are required", fn);
+    if (B > 1 && ld < cap) return fail(VGDR_ERR_INVALID, "%s: rows of %lld tokens, %lld apart", fn, (long long)cap, (long long)ld);
+    (void)workspace;
+    (void)workspace_bytes;
+    vgdr::LookupParams p{};
+    p.history = history;
+    p.lengths = lengths;
+    p.drafts = drafts;
+    p.counts = counts;
+    p.ld = ld;
+    p.cap = cap;
+    p.N = B;
+    p.K = (int)K;
+    p.longest = max_ngram;
+    p.shortest = min_ngram;
+    return hip_status(vgdr::lookup_drafts(token_bytes == 8, p, stream), "vgdr_lookup_drafts launch");
+}
+
 }  // extern "C"

@@ -350,6 +350,61 @@ hipError_t causal_conv_bwd(int dtype, const ConvBwdParams &p, hipStream_t stream
 hipError_t varlen_prepare(const int32_t *cu, int n_seqs, int64_t n_tokens, int chunk,
                           int32_t *ws, hipStream_t stream);
 
+// One speculative decoding step of a layer (gdr_draft.hip): N streams, L new tokens each behind a
+// pending block of room for P.  q, k, v and the epilogue's gate: rows of token (stream, t),
+// ld_qk (q, k) and ld_v (v, gate) elements apart.
+constexpr int DRAFT_MAX = 16;     // tokens of a block
+struct DraftParams {
+    const void *q, *k, *v;
+    const void *g;                // [N, L, H] fp32, [N, L, H, dk] fp32 or (fz.gate_16) the element type, or NULL
+    const float *beta;            // [N, L, H] (delta rule)
+    void *o;                      // [N, L, H, dv]
+    float *S;                     // [N, H, dk, dv], the committed state, moved in place
+    float *pk, *pu, *pg;          // the pending block: [N, P, H, dk], [N, P, H, dv], and g's shape with P
+    void *xq, *xk, *xv;           // its raw inputs [N, P, H d] (with a conv)
+    const int32_t *accepted;      // [N] pending tokens that stand (clamped to 0 .. P)
+    int64_t ld_qk, ld_v, N;
+    int L, P, H, dk, dv, dtype, use_delta;
+    float scale;
+    Fusion fz;
+    Epilogue ep;
+    ShortConv cv;
+};
+hipError_t draft_step(int gate, const DraftParams &p, hipStream_t stream);
+
+// Drafts against the target's logits (gdr_verify.hip), N streams of K drafts.
+struct RowMass {
+    double sum;                   // of e^{(x - top) / T} over the row
+    float top;
+    int at;                       // the lowest index of the top
+};
+struct VerifyParams {
+    const void *logits;           // row i of stream n at n ld_stream + i ld_row, V elements
+    const int64_t *drafts;        // [N, K]
+    const float *uniforms;        // [N, K + 1]
+    const float *temperature;     // [N]
+    const void *probs;            // rows as logits' with ld_probs_*, in probs_dtype; NULL: the drafts are certain
+    const int32_t *n_drafts;      // [N] or NULL (K)
+    int64_t *tokens;              // [N, K + 1]
+    int32_t *accepted;            // [N]
+    RowMass *rows;                // verify_workspace bytes
+    int64_t ld_stream, ld_row, ld_probs_stream, ld_probs_row, N;
+    int K, V, probs_dtype;
+};
+hipError_t verify_drafts(int dtype, const VerifyParams &p, hipStream_t stream);
+int64_t verify_workspace(int64_t N, int64_t K, int64_t V);
+
+// Drafts out of the streams' own text (gdr_verify.hip).
+struct LookupParams {
+    const void *history;          // [N] rows of cap tokens, ld apart, int32 or int64
+    const int32_t *lengths;       // [N]
+    int64_t *drafts;              // [N, K]
+    int32_t *counts;              // [N]
+    int64_t ld, cap, N;
+    int K, longest, shortest;
+};
+hipError_t lookup_drafts(bool wide, const LookupParams &p, hipStream_t stream);
+
 int device_cu_count();
 
 }  // namespace vgdr

@@ -1661,3 +1661,311 @@ def chunk_scan_vec(q, k, v, g, beta, S0, *, scale: float, delta: bool, chunk_siz
                                       _ptr(c.h0), _ptr(S), _ptr(c.cu), _ptr(ws), nbytes, c.B, c.T, c.H, c.dkp, c.dvp,
                                       c.N, scale, int(chunk_size), None, _stream(c.device)))
     return c.unpad_o(o), c.unpad_state(S)
+
+
+# --- speculative decoding -------------------------------------------------------
+
+MAX_DRAFT_BLOCK = 16         # tokens of a drafted block: a stream's last token and up to 15 drafts
+
+
+class DraftBlock:
+    """What a block of drafted tokens leaves behind in one layer until it is known how
+    many of them stand: per stream and token the keys k (N, P, H, dk) as the
+    recurrence takes them, the writes u (N, P, H, dv) and log-decays g ((N, P, H),
+    (N, P, H, dk) or None), fp32, and the raw conv inputs x = (xq, xk, xv), each (N,
+    P, H*d) in the compute type (None without a conv).  hip_draft_step reads and
+    rewrites it; P is the room, in tokens."""
+
+    __slots__ = ('k', 'u', 'g', 'x')
+
+    def __init__(self, k, u, g=None, x=None):
+        self.k, self.u, self.g, self.x = k, u, g, None if x is None else tuple(x)
+
+    @classmethod
+    def empty(cls, state, capacity: int, *, gate: str, conv_cache=None):
+        """An empty block of room for `capacity` tokens beside state (N, H, dk, dv) and the
+        conv caches (N, K, D); nothing of it stands yet (accepted 0)."""
+        if not 1 <= capacity <= MAX_DRAFT_BLOCK:
+            raise NotImplementedError(f'a drafted block holds 1 to {MAX_DRAFT_BLOCK} tokens; got {capacity}')
+        assert gate in ('none', 'scalar', 'vector'), gate
+        N, H, dk, dv = state.shape
+        new = lambda *s, dt=torch.float32: torch.zeros(N, capacity, *s, dtype=dt, device=state.device)  # noqa: E731
+        return cls(new(H, dk), new(H, dv), None if gate == 'none' else new(H) if gate == 'scalar' else new(H, dk),
+                   None if conv_cache is None else [new(c.shape[2], dt=c.dtype) for c in conv_cache])
+
+    @property
+    def capacity(self) -> int:
+        return self.k.shape[1]
+
+
+def _token_rows(t, width: int):
+    """The distance in elements from one token of t (N, L, width) or (N, L, H, d) to the
+    next, over all streams, where a kernel may read its rows in place; else None."""
+    e = t.element_size()
+    if t.dim() == 4 and t.shape[2] > 1 and t.stride(2) != t.shape[3]:
+        return None
+    if t.stride(-1) != 1 or t.data_ptr() % 16:
+        return None
+    N, L = t.shape[0], t.shape[1]
+    ld = t.stride(1) if L > 1 else t.stride(0) if N > 1 else width
+    if ld < width or ld % 8 or (N > 1 and t.stride(0) != L * ld):
+        return None
+    return ld
+
+
+def _in_place(name, t, shape, dtype, device):
+    assert t.shape == shape and t.dtype == dtype and t.device == device and t.is_contiguous() and t.data_ptr() % 16 == 0, \
+        f'{name} is read and written in place: {tuple(shape)}, {dtype}, contiguous, aligned, on {device}; got ' \
+        f'{tuple(t.shape)}, {t.dtype}, {t.device}'
+
+
+def _stream_counts(name, t, N, device):
+    """int32 (N,) counts of the streams for a kernel."""
+    assert t.shape == (N,) and t.device == device and not t.is_floating_point() and t.dtype != torch.bool, \
+        f'{name} must be ({N},) whole numbers on {device}; got {tuple(t.shape)}, {t.dtype}, {t.device}'
+    return t.to(torch.int32).contiguous()
+
+
+def hip_draft_step(qp, kp, vp, g, beta, state, pending, accepted, *, scale: float, delta: bool = True,
+                   conv_weights=None, conv_cache=None, l2norm: bool = True, beta_logits: bool = False,
+                   gate_in_kernel: bool = False, A_log=None, dt_bias=None, lower_bound: float | None = None,
+                   out_gate=None, out_norm_weight=None, out_norm_eps: float = 1e-6):
+    """One speculative decoding step of a layer, from the projections of a block of
+    drafted tokens to the input of W_o, in one kernel (vgdr_draft_step).
+
+    First the tokens of the last block that stand, accepted (N,) (whole numbers, on the
+    GPU; clamped to 0 .. the block's room), are committed from `pending` (DraftBlock) to
+    state (N, H, dk, dv) and conv_cache, in place.  Then the block's L tokens (1 <= L
+    <= the room of `pending`, at most 16) run behind them as hip_decode_step's tokens
+    do, one after the other, but on no state that is kept: the block becomes
+    `pending`, and the next call commits what stands of it.  A step that commits
+    nothing, such as the first, has accepted 0; commit_drafts commits without new tokens.
+
+    Arguments as hip_decode_step's: qp, kp (N, L, H*dk) or (N, L, H, dk), vp (N, L,
+    H*dv) or (N, L, H, dv), raw projections (with conv_weights and conv_cache; the
+    convolved and activated rows without), column blocks of one projection output among
+    them (read in place); g None, (N, L, H) fp32 log-decay or (N, L, H, dk) (with
+    gate_in_kernel its pre-activation); beta (N, L, H).  Returns o (N, L, H, dv) in
+    q's type.  Between the inputs and the outputs everything is fp32; hip_decode_step
+    rounds the conv's, the SiLU's, the norm's and the recurrence's results to q's type.
+    dk a multiple of 8 up to 128, dv a multiple of 8 up to 256.  No autograd."""
+    _check_device(qp, kp, vp, g, beta, state, accepted, out_gate, out_norm_weight, A_log, dt_bias)
+    _check_grad(qp, kp, vp, g, beta, state, out_gate, out_norm_weight, A_log, dt_bias, *(conv_weights or ()))
+    dev, dt = qp.device, qp.dtype
+    if dt not in _DTYPES or kp.dtype != dt or vp.dtype != dt:
+        raise NotImplementedError(f'q, k, v must share one of {list(_DTYPES)}; got {dt}, {kp.dtype}, {vp.dtype}')
+    assert state.dim() == 4, f'state must be (N, H, dk, dv); got {tuple(state.shape)}'
+    N, H, dk, dv = state.shape
+    L, P = qp.shape[1], pending.capacity
+    for name, t, d in (('q', qp, dk), ('k', kp, dk), ('v', vp, dv)):
+        assert t.shape in ((N, L, H * d), (N, L, H, d)) and t.device == dev, \
+            f'{name} must be {(N, L, H * d)} or {(N, L, H, d)} on {dev}; got {tuple(t.shape)}, {t.device}'
+    assert 1 <= L <= P, f'a block of 1 to {P} tokens (the pending block\'s room); got {L}'
+    gate = _gate_of(g)
+    assert g is None or g.shape == (N, L, H) + (() if gate == 'scalar' else (dk,)), \
+        f'g must be {(N, L, H)} or {(N, L, H, dk)}; got {tuple(g.shape)}'
+    if delta:
+        assert beta is not None and beta.shape == (N, L, H), f'the delta rule needs beta {(N, L, H)}'
+    assert not gate_in_kernel or gate == 'vector', 'the fused gate activation is a KDA (vector-gate) kernel'
+    assert delta or not beta_logits, 'there is no beta to activate without the delta rule'
+    fz = _Fusion(l2norm=l2norm, beta=beta_logits, gate=gate_in_kernel, A_log=A_log, dt_bias=dt_bias,
+                 lower_bound=lower_bound if gate_in_kernel else None)
+    ep = None
+    if out_gate is not None or out_norm_weight is not None:
+        assert out_gate is not None and out_gate.shape in ((N, L, H * dv), (N, L, H, dv)), \
+            f'the output gate must be {(N, L, H * dv)} or {(N, L, H, dv)}'
+        ep = _Epilogue(out_gate.reshape(N, L, H, dv), out_norm_weight, out_norm_eps)
+        if out_gate.dtype != dt:
+            raise NotImplementedError(f'the epilogue gate must have o\'s dtype {dt}; got {out_gate.dtype}')
+    # rows in place: q and k one stride apart, v and the gate one
+    lds = [_token_rows(t, w) for t, w in ((qp, H * dk), (kp, H * dk), (vp, H * dv))]
+    ld_gate = lds[2] if ep is None else _token_rows(out_gate, H * dv)
+    ogate = out_gate
+    if None in lds or ld_gate is None or lds[0] != lds[1] or lds[2] != ld_gate:
+        qp, kp, vp = _aligned(qp), _aligned(kp), _aligned(vp)
+        ogate = None if ep is None else _aligned(out_gate)
+        lds = [H * dk, H * dk, H * dv]
+    if g is not None:
+        g = _aligned(g) if gate_in_kernel and g.dtype == dt else _aligned(g.float())
+    beta = beta.float().contiguous() if delta else None
+    o = torch.empty(N, L, H, dv, dtype=dt, device=dev)
+    _draft_call(dt, gate, delta, (qp, kp, vp, g, beta, o), state, pending, accepted, L, lds[0], lds[2], float(scale), fz,
+                conv_weights, conv_cache, ep, ogate)
+    return o
+
+
+def commit_drafts(state, pending, accepted, *, conv_weights=None, conv_cache=None) -> None:
+    """hip_draft_step's first half alone: the accepted (N,) tokens of `pending` that stand
+    move into state and conv_cache, in place (the end of speculative decoding, or an
+    export).  Nothing of `pending` stands behind it: the next call's accepted is 0."""
+    _check_device(state, accepted)
+    _check_grad(state)
+    gate = 'none' if pending.g is None else 'scalar' if pending.g.dim() == 3 else 'vector'
+    dt = conv_cache[0].dtype if conv_cache is not None else torch.float32
+    if dt not in _DTYPES:
+        raise NotImplementedError(f'the conv caches must be one of {list(_DTYPES)}; got {dt}')
+    _draft_call(dt, gate, False, (None,) * 6, state, pending, accepted, 0, 0, 0, 1.0, _NO_FUSION, conv_weights, conv_cache,
+                None, None)
+
+
+def _draft_call(dt, gate, delta, operands, state, pending, accepted, L, ld_qk, ld_v, scale, fz, conv_weights, conv_cache,
+                ep, ogate):
+    dev = state.device
+    N, H, dk, dv = state.shape
+    P = pending.capacity
+    if dk % 8 or dk > 128 or dv % 8 or dv > 256:
+        raise NotImplementedError(f'dk={dk}, dv={dv}: drafted blocks take multiples of 8 up to 128 and 256')
+    if not 1 <= P <= MAX_DRAFT_BLOCK:
+        raise NotImplementedError(f'a drafted block holds 1 to {MAX_DRAFT_BLOCK} tokens; got room for {P}')
+    f32 = torch.float32
+    _in_place('state', state, (N, H, dk, dv), f32, dev)
+    _in_place('pending.k', pending.k, (N, P, H, dk), f32, dev)
+    _in_place('pending.u', pending.u, (N, P, H, dv), f32, dev)
+    assert (pending.g is None) == (gate == 'none'), f'the pending block was made for another gate than {gate!r}'
+    if pending.g is not None:
+        _in_place('pending.g', pending.g, (N, P, H) if gate == 'scalar' else (N, P, H, dk), f32, dev)
+    assert (conv_weights is None) == (conv_cache is None) == (pending.x is None), \
+        'a conv needs its weights, its caches and a pending block with its inputs'
+    sc, keep = None, []
+    if conv_cache is not None:
+        conv = _ShortConv(conv_weights, conv_cache)
+        widths = (H * dk, H * dk, H * dv)
+        for n, w, c, x, d in zip('qkv', conv.weights, conv_cache, pending.x, widths):
+            assert w.shape == (d, conv.K) and w.device == dev, \
+                f'conv weight must be ({d}, {conv.K}) or ({d}, 1, {conv.K}) on {dev}; got {tuple(w.shape)}'
+            _in_place(f'conv cache {n}', c, (N, conv.K, d), dt, dev)
+            _in_place(f'pending.x {n}', x, (N, P, d), dt, dev)
+        wdt = f32 if all(w.dtype == f32 for w in conv.weights) else dt
+        keep += [w.to(wdt).contiguous() for w in conv.weights]
+        sc = _lib.ShortConv(weight_q=_ptr(keep[0]), weight_k=_ptr(keep[1]), weight_v=_ptr(keep[2]),
+                            cache_q=_ptr(conv_cache[0]), cache_k=_ptr(conv_cache[1]), cache_v=_ptr(conv_cache[2]),
+                            kernel_size=conv.K, weight_dtype=_DTYPES[wdt])
+    q, k, v, g, beta, o = operands
+    for t in (g, beta, ogate, *(fz.A_log, fz.dt_bias), *((ep.gamma,) if ep is not None else ())):
+        assert t is None or t.device == dev, f'every tensor must be on {dev}; got {t.device}'
+    fzs = None
+    if fz.any:
+        fzs = _lib.Fusion(int(fz.l2norm), int(fz.beta), int(fz.gate), _lib.VGDR_F32, None, None, 0, 0.0)
+        if fz.gate:
+            assert fz.A_log.numel() == H and fz.dt_bias.numel() == H * dk, f'A_log has {H} and dt_bias {H * dk} elements'
+            params = [t.detach().float().contiguous() for t in (fz.A_log, fz.dt_bias)]
+            keep += params
+            fzs.A_log, fzs.dt_bias, fzs.gate_dtype = _ptr(params[0]), _ptr(params[1]), _DTYPES[g.dtype]
+            if fz.lower_bound is not None:
+                fzs.lower_bound_set, fzs.lower_bound = 1, float(fz.lower_bound)
+    eps = None
+    if ep is not None:
+        gamma = ep.gamma if ep.gamma.dtype in (f32, dt) else ep.gamma.float()
+        gamma = gamma.contiguous()
+        keep.append(gamma)
+        eps = _lib.Epilogue(gate=_ptr(ogate), gamma=_ptr(gamma), gamma_dtype=_DTYPES[gamma.dtype], eps=ep.eps)
+    acc = _stream_counts('accepted', accepted, N, dev)
+    xs = pending.x or (None,) * 3
+    blk = _lib.DraftBlock(_ptr(pending.k), _ptr(pending.u), _ptr(pending.g), _ptr(xs[0]), _ptr(xs[1]), _ptr(xs[2]), P)
+    kind = {'none': _lib.VGDR_GATE_NONE, 'scalar': _lib.VGDR_GATE_SCALAR, 'vector': _lib.VGDR_GATE_VECTOR}[gate]
+    ref = lambda s: None if s is None else ctypes.byref(s)  # noqa: E731
+    with torch.cuda.device(dev):
+        _lib.check(_lib.load().vgdr_draft_step(
+            _DTYPES[dt], kind, int(delta), _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _ptr(o), _ptr(state), ref(blk),
+            _ptr(acc), N, L, H, dk, dv, ld_qk, ld_v, scale, ref(fzs), ref(sc), ref(eps), _stream(dev)))
+
+
+def verify_drafts(logits, drafts, uniforms, *, temperature=1.0, draft_probs=None, n_drafts=None):
+    """Which drafted tokens stand before the target's probabilities, and the token that
+    follows them, from given random numbers (vgdr_verify_drafts).
+
+    logits (N, K + 1, V), fp32, bf16 or fp16: the target's, row i after the block's token
+    i, so that row i judges draft i and the last row follows the last draft; any strides over
+    whole rows.  drafts (N, K) whole numbers (K = 0: a token is sampled, nothing verified).  uniforms
+    (N, K + 1) fp32 in [0, 1): one per draft, the last for the token behind them.  temperature: a
+    number or (N,); 0 is greedy.  draft_probs (N, K, V): the probabilities that the drafts were drawn
+    from; None: the drafts were certain (looked up, or greedy).  n_drafts (N,): how many of its
+    K a stream has.
+
+    With p = softmax(logits / temperature) and q the draft's: draft i stands if all before it do
+    and uniforms[i] q_i(d_i) < p_i(d_i); the token behind the last that stands is drawn from
+    max(p - q, 0) of the first refused draft's row, or from p where none was refused, as the
+    lowest id at which the running sum exceeds uniforms[K] times the whole.  So the tokens are
+    distributed as the target's own, one by one.  Weights and sums are 64-bit.
+
+    NaN logits have no mass, equal ones (+inf among them, and a row of -inf alone) share it, a draft
+    outside the vocabulary never stands, and where q covers all of p the token is drawn from p.
+    Returns (tokens (N, K + 1) int64: the drafts that stand, the token, then -1; accepted (N,) int32).
+    No autograd: logits that require grad are refused."""
+    _check_device(logits, drafts, uniforms, draft_probs, n_drafts)
+    _check_grad(logits, draft_probs)
+    assert logits.dim() == 3 and logits.shape[1] >= 1 and logits.shape[2] >= 1, \
+        f'logits must be (N, K + 1, V); got {tuple(logits.shape)}'
+    N, L, V = logits.shape
+    K, dev = L - 1, logits.device
+    if logits.dtype not in _DTYPES:
+        raise NotImplementedError(f'logits must be one of {list(_DTYPES)}; got {logits.dtype}')
+    if K > 64:
+        raise NotImplementedError(f'{K} drafts (at most 64)')
+    assert drafts.shape == (N, K) and not drafts.is_floating_point() and drafts.dtype != torch.bool, \
+        f'drafts must be {(N, K)} whole numbers; got {tuple(drafts.shape)}, {drafts.dtype}'
+    assert uniforms.shape == (N, L) and uniforms.dtype == torch.float32, \
+        f'uniforms must be {(N, L)} in fp32; got {tuple(uniforms.shape)}, {uniforms.dtype}'
+    x = logits if logits.stride(2) == 1 and logits.stride(1) >= V and logits.stride(0) >= 0 else logits.contiguous()
+    if isinstance(temperature, torch.Tensor):
+        assert temperature.shape == (N,) and temperature.is_floating_point(), \
+            f'temperature must be a number or ({N},); got {tuple(temperature.shape)}, {temperature.dtype}'
+        _check_device(temperature)
+        T = temperature.float().contiguous()
+    else:
+        assert temperature >= 0, f'temperature must not be negative; got {temperature}'
+        T = torch.full((N,), float(temperature), device=dev)
+    q = None
+    if draft_probs is not None:
+        assert draft_probs.shape == (N, K, V), f'draft_probs must be {(N, K, V)}; got {tuple(draft_probs.shape)}'
+        if draft_probs.dtype not in _DTYPES:
+            raise NotImplementedError(f'draft_probs must be one of {list(_DTYPES)}; got {draft_probs.dtype}')
+        q = draft_probs
+        if K and not (q.stride(2) == 1 and q.stride(1) >= V and q.stride(0) >= 0):
+            q = q.contiguous()
+    nd = None if n_drafts is None else _stream_counts('n_drafts', n_drafts, N, dev)
+    d, u = drafts.to(torch.int64).contiguous(), uniforms.contiguous()
+    for t in (d, u, T, q):
+        assert t is None or t.device == dev, f'every tensor must be on {dev}; got {t.device}'
+    tokens = torch.empty(N, L, dtype=torch.int64, device=dev)
+    accepted = torch.empty(N, dtype=torch.int32, device=dev)
+    lib = _lib.load()
+    nbytes = lib.vgdr_verify_drafts_workspace_size(N, K, V)
+    ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        _lib.check(lib.vgdr_verify_drafts(
+            _DTYPES[x.dtype], _ptr(x), x.stride(0), max(x.stride(1), V) if L == 1 else x.stride(1), _ptr(d), _ptr(u), _ptr(T),
+            _ptr(q), 0 if q is None else _DTYPES[q.dtype], 0 if q is None else q.stride(0),
+            0 if q is None else max(q.stride(1), V), _ptr(nd), _ptr(tokens), _ptr(accepted), _ptr(ws), nbytes, N, K, V,
+            _stream(dev)))
+    return tokens, accepted
+
+
+def lookup_drafts(history, lengths, n, *, max_ngram: int = 3, min_ngram: int = 1):
+    """n drafted tokens for each stream out of its own text (vgdr_lookup_drafts).
+
+    history (N, cap) int32 or int64, row b holding lengths[b] (whole numbers, clamped to 0 ..
+    cap) tokens, any row stride.  Of the places before a row's last token at which its last
+    min_ngram or more tokens have stood before, the one where most of them agree (max_ngram
+    counted at most), and of those the latest; the drafts are the tokens that followed, read on
+    from the first of them again where the text ends.  Returns (drafts (N, n) int64, counts (N,)
+    int32: n, or 0 and zeros without such a place)."""
+    _check_device(history, lengths)
+    assert history.dim() == 2, f'history must be (N, cap); got {tuple(history.shape)}'
+    if history.dtype not in (torch.int32, torch.int64):
+        raise NotImplementedError(f'history must be int32 or int64; got {history.dtype}')
+    assert 1 <= n <= 64, f'1 to 64 drafts; got {n}'
+    assert 1 <= min_ngram <= max_ngram <= 16, f'1 <= min_ngram <= max_ngram <= 16; got {min_ngram}, {max_ngram}'
+    N, cap = history.shape
+    dev = history.device
+    h = history if (history.stride(1) == 1 or cap <= 1) and (history.stride(0) >= cap or N <= 1) else history.contiguous()
+    lens = _stream_counts('lengths', lengths, N, dev)
+    drafts = torch.empty(N, n, dtype=torch.int64, device=dev)
+    counts = torch.empty(N, dtype=torch.int32, device=dev)
+    lib = _lib.load()
+    nbytes = lib.vgdr_lookup_drafts_workspace_size(N, cap)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with torch.cuda.device(dev):
+        _lib.check(lib.vgdr_lookup_drafts(_ptr(h), h.element_size(), max(h.stride(0), cap), cap, _ptr(lens), _ptr(drafts),
+                                          _ptr(counts), _ptr(ws), nbytes, N, n, max_ngram, min_ngram, _stream(dev)))
+    return drafts, counts
