@@ -1387,6 +1387,7 @@ int vgdr_draft_step(int dtype, int gate_kind, int use_delta, const void *q, cons
     p.dv = (int)dv;
     p.dtype = dtype;
     p.use_delta = use_delta ? 1 : 0;
+    p.conv4 = conv && p.cv.K == 4 && aligned16(p.cv.wq) && aligned16(p.cv.wk) && aligned16(p.cv.wv);
     p.scale = scale;
     return hip_status(vgdr::draft_step(gate_kind, p, stream), "vgdr_draft_step launch");
 }

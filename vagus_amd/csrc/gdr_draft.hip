@@ -40,61 +40,91 @@ __device__ __forceinline__ f32x2 buffer_load_nt2(__amdgpu_buffer_rsrc_t r, uint3
 __device__ __forceinline__ void buffer_store_nt2(f32x2 x, __amdgpu_buffer_rsrc_t r, uint32_t voff) {
     __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, x), r, (int)voff, 0, CPOL_NT);
 }
+__device__ __forceinline__ float buffer_load1(__amdgpu_buffer_rsrc_t r, uint32_t voff) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, (int)voff, 0, 0));
+}
+__device__ __forceinline__ f32x2 buffer_load2(__amdgpu_buffer_rsrc_t r, uint32_t voff) {
+    return __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(r, (int)voff, 0, 0));
+}
+constexpr uint32_t NOWHERE = 0x40000000u;                          // an offset behind every block: reads zeros
 
-// Two neighbouring channels of this (stream, head)'s q, k or v through the short conv: the cache moves
-// to the a-th pending input, the block's inputs become pending, and put(t, x0, x1) takes the
-// activated values.  TAPS: 4, all loads in flight at once; 0: any number up to 8, one token
-// after the other (right-aligned in 8 places).
-template <typename E, int LT, int TAPS, typename F>
-__device__ __forceinline__ void draft_conv(const DraftParams &p, const E *src, int64_t ld, int64_t n, int a, int which, int col,
-                                           F put) {
-    constexpr int T = TAPS ? TAPS : 8;
-    const int K = TAPS ? TAPS : p.cv.K, skip = T - K;
-    const int64_t D = (int64_t)p.H * (which < 2 ? p.dk : p.dv);
-    E *cache = reinterpret_cast<E *>(which == 0 ? p.cv.cq : which == 1 ? p.cv.ck : p.cv.cv) + n * K * D + col;
-    E *pend = reinterpret_cast<E *>(which == 0 ? p.xq : which == 1 ? p.xk : p.xv) + n * p.P * D + col;
-    const void *wp = which == 0 ? p.cv.wq : which == 1 ? p.cv.wk : p.cv.wv;
-    const int wt = p.cv.w_f32 ? 0 : p.dtype;
-    constexpr int NEW = TAPS ? LT : 1;
-    Pair<E> x[T + NEW];                                            // the K last inputs, then the block's
-    f32x2 w[T];
-    unroll<T>([&](auto r) {
+// by value: a choice among a parameter block's members would put the block into scratch memory
+__device__ __forceinline__ uint64_t pick(int which, const void *q, const void *k, const void *v) {
+    const uint64_t a = (uint64_t)q, b = (uint64_t)k, c = (uint64_t)v;
+    return which == 0 ? a : which == 1 ? b : c;
+}
+
+// Two neighbouring channels of this (stream, head)'s q, k or v: where they are.
+template <typename E> struct ChannelPair {
+    const E *src;                 // the block's inputs, ld apart
+    E *cache, *pend;              // the conv's last K inputs and the pending block's, D apart
+    const void *w;                // the conv's weights of the two
+    int64_t ld, D;
+    int which, c;                 // 0 q, 1 k, 2 v; channel in the head
+
+    __device__ __forceinline__ ChannelPair(const DraftParams &p, int64_t n, int h, int cp) {
+        const int c2 = 2 * cp, K = p.cv.K;
+        which = c2 < p.dk ? 0 : c2 < 2 * p.dk ? 1 : 2;
+        c = which == 0 ? c2 : which == 1 ? c2 - p.dk : c2 - 2 * p.dk;
+        const int d = which < 2 ? p.dk : p.dv, col = h * d + c;
+        ld = which < 2 ? p.ld_qk : p.ld_v;
+        D = (int64_t)p.H * d;
+        src = reinterpret_cast<const E *>(pick(which, p.q, p.k, p.v)) + n * p.L * ld + col;
+        cache = reinterpret_cast<E *>(pick(which, p.cv.cq, p.cv.ck, p.cv.cv)) + n * K * D + col;
+        pend = reinterpret_cast<E *>(pick(which, p.xq, p.xk, p.xv)) + n * p.P * D + col;
+        w = reinterpret_cast<const char *>(pick(which, p.cv.wq, p.cv.wk, p.cv.wv)) + (int64_t)col * K * (p.cv.w_f32 ? 4 : (int)sizeof(E));
+    }
+};
+
+// The short conv of any number of taps up to 8, one token after the other: the cache moves to the
+// a-th pending input, the block's inputs become pending, put(t, x0, x1) takes the activated values.
+template <typename E, typename F>
+__device__ __forceinline__ void draft_conv_any(const DraftParams &p, const ChannelPair<E> &at, int a, F put) {
+    const int K = p.cv.K, skip = 8 - K, wt = p.cv.w_f32 ? 0 : p.dtype;
+    Pair<E> x[9];                                                  // right-aligned: the K last inputs, then a token's
+    f32x2 w[8];
+    unroll<8>([&](auto r) {
         x[r] = Pair<E>{(E)0.f, (E)0.f};
         w[r] = f32x2{0.f, 0.f};
-        if (TAPS || r >= skip) {
-            const int at = a + r - skip;                           // of the K cached and P pending inputs
-            x[r] = *reinterpret_cast<const Pair<E> *>(at < K ? cache + at * D : pend + (at - K) * D);
-            w[r] = f32x2{param_f(wp, wt, (int64_t)col * K + r - skip), param_f(wp, wt, (int64_t)(col + 1) * K + r - skip)};
+        if (r >= skip) {
+            const int i = a + r - skip;                            // of the K cached and P pending inputs
+            x[r] = *reinterpret_cast<const Pair<E> *>(i < K ? at.cache + i * at.D : at.pend + (i - K) * at.D);
+            w[r] = f32x2{param_f(at.w, wt, r - skip), param_f(at.w, wt, K + r - skip)};
         }
     });
-    if (TAPS && p.L > 0)
-        unroll<NEW>([&](auto t) { x[T + t] = *reinterpret_cast<const Pair<E> *>(src + (t < p.L ? (int)t : p.L - 1) * ld); });
-    unroll<T>([&](auto r) {
-        if (TAPS || r >= skip) *reinterpret_cast<Pair<E> *>(cache + (r - skip) * D) = x[r];
+    unroll<8>([&](auto r) {
+        if (r >= skip) *reinterpret_cast<Pair<E> *>(at.cache + (r - skip) * at.D) = x[r];
     });
-    auto token = [&](int t, auto at) {                             // at: the token's place behind the window in x
-        *reinterpret_cast<Pair<E> *>(pend + t * D) = x[T + at];
+#pragma nounroll
+    for (int t = 0; t < p.L; ++t) {
+        x[8] = *reinterpret_cast<const Pair<E> *>(at.src + t * at.ld);
+        *reinterpret_cast<Pair<E> *>(at.pend + t * at.D) = x[8];
         f32x2 y = {0.f, 0.f};
-        unroll<T>([&](auto r) {
-            if (TAPS || r >= skip) {
-                y[0] += w[r][0] * (float)x[at + 1 + r][0];
-                y[1] += w[r][1] * (float)x[at + 1 + r][1];
+        unroll<8>([&](auto r) {
+            if (r >= skip) {
+                y[0] += w[r][0] * (float)x[1 + r][0];
+                y[1] += w[r][1] * (float)x[1 + r][1];
             }
         });
-        put(t, y[0] / (1.f + expf(-y[0])), y[1] / (1.f + expf(-y[1])));
-    };
-    if (TAPS) {
-        unroll<NEW>([&](auto t) {
-            if (t < p.L) token(t, t);
-        });
-    } else {
-#pragma nounroll
-        for (int t = 0; t < p.L; ++t) {
-            x[T] = *reinterpret_cast<const Pair<E> *>(src + t * ld);
-            token(t, std::integral_constant<int, 0>{});
-            unroll<T>([&](auto r) { x[r] = x[r + 1]; });
-        }
+        put(t, y[0] * sigmoidf_(y[0]), y[1] * sigmoidf_(y[1]));
+        unroll<8>([&](auto r) { x[r] = x[r + 1]; });
     }
+}
+
+// inclusive sums over the lanes behind, within a row of 16
+__device__ __forceinline__ float row_suffix16(float x) {
+    x += dpp_f<0x101>(x);                                          // row_shl:1
+    x += dpp_f<0x102>(x);
+    x += dpp_f<0x104>(x);
+    x += dpp_f<0x108>(x);
+    return x;
+}
+__device__ __forceinline__ float row_prefix16(float x) {
+    x += dpp_f<0x111>(x);                                          // row_shr:1
+    x += dpp_f<0x112>(x);
+    x += dpp_f<0x114>(x);
+    x += dpp_f<0x118>(x);
+    return x;
 }
 
 }  // namespace
@@ -102,174 +132,227 @@ __device__ __forceinline__ void draft_conv(const DraftParams &p, const E *src, i
 // One workgroup per (stream, head), a wave per 32 columns of the state, which it holds in the
 // C layout of 16 x 16 tiles: lane 16 g + r has rows 16 i + 4 g + j (j < 4) of columns 2 r, 2 r + 1, so a
 // row's 32 columns are one 128-byte line. As it lies it is the B operand of the product with [K; Q].
-// RT: row tiles (dk <= 16 RT). LT: room of the pending block and tokens (8 or 16).
+// What does not need the state (conv, gates, A and B) is loaded ahead of it and done while it
+// arrives.  q and k are kept unnormalised: the norms are A's and q's own diagonals and scale the
+// results.  RT: row tiles (dk <= 16 RT). LT: room of the pending block and tokens (8 or 16).
 template <typename E, int GATE, int RT, int LT, int NT>
-__global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(LT == 16 && NT == 256 ? 3 : 4))) draft_block_kernel(const DraftParams p) {
-    constexpr int DKP = 16 * RT, LDK = DKP + 4, WLD = DKP + 16, DVM = NT / 2, LP = DKP / 16;
-    constexpr int SHARED = LT * WLD > 2 * LT * DVM ? LT * WLD : 2 * LT * DVM;
-    __shared__ __attribute__((aligned(16))) float kk[LT][LDK], qq[LT][LDK], vv[LT][DVM];
-    __shared__ __attribute__((aligned(16))) float both[SHARED];   // ws, then the products with the state
-    __shared__ __attribute__((aligned(16))) float es[GATE == 2 ? LT : 1][GATE == 2 ? DKP : LT], ds[DKP];
-    __shared__ __attribute__((aligned(16))) float aa[LT][LT], bb[LT][LT], betas[LT], decay[LT];
+__global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(LT == 16 && NT == 256 ? 3 : 4)))
+draft_block_kernel(const DraftParams p) {
+    constexpr int DKP = 16 * RT, LDK = DKP + 4, WLD = DKP + 16, DVM = NT / 2, NC = DKP / 64;
+    __shared__ __attribute__((aligned(16))) float kk[LT][LDK], qq[LT][LDK], vv[LT][DVM], ws[LT][WLD], prod[2 * LT][DVM];
+    __shared__ __attribute__((aligned(16))) float es[GATE == 2 ? LT : 1][GATE == 2 ? DKP : 16];  // e^{g_t}
+    __shared__ __attribute__((aligned(16))) float eg[GATE == 2 ? LT : 1][GATE == 2 ? LDK : 16];  // e^{G_t}
+    __shared__ __attribute__((aligned(16))) float ds[GATE == 2 ? DKP : 16], aa[LT][LT], bb[LT][LT];
+    __shared__ float betas[LT], rk[LT], rq[LT];
     const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 63, waves = nt >> 6;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), g4 = lane >> 4, r16 = lane & 15;
     const int64_t n = blockIdx.x / p.H;
     const int h = blockIdx.x - (int)n * p.H;
-    const int dk = p.dk, dv = p.dv, L = p.L, P = p.P, pairs = dk + dv / 2;
+    const int dk = p.dk, dv = p.dv, L = p.L, P = p.P, H = p.H, pairs = dk + dv / 2;
     int a = p.accepted[n];
     a = a < 0 ? 0 : a > P ? P : a;
+    const bool fast = p.conv4;
 
-    // the state; rows and columns beyond it read zeros and are not stored
+    // --- loads ahead of the state ---
+    const ChannelPair<E> at(p, n, h, tid < pairs ? tid : pairs - 1);
+    Pair<E> x[4 + LT];                                             // four taps: the last inputs, then the block's
+    u32x4 wraw[2];
+    if (fast) {
+        unroll<4>([&](auto r) {
+            const int i = a + r;
+            x[r] = *reinterpret_cast<const Pair<E> *>(i < 4 ? at.cache + i * at.D : at.pend + (i - 4) * at.D);
+        });
+        wraw[0] = *reinterpret_cast<const u32x4 *>(at.w);
+        if (p.cv.w_f32 || sizeof(E) == 4) wraw[1] = reinterpret_cast<const u32x4 *>(at.w)[1];
+        if (L > 0)
+            unroll<LT>([&](auto t) { x[4 + t] = *reinterpret_cast<const Pair<E> *>(at.src + (t < L ? (int)t : L - 1) * at.ld); });
+    }
+    // scalar gate: lane r of every row of 16 has token r's
+    const bool has_g = GATE == 2 || p.pg != nullptr;
+    float gp = 0.f, gn = 0.f, be = 0.f;
+    if (GATE == 1 && has_g) {
+        if (r16 < a) gp = p.pg[(n * P + r16) * H + h];
+        if (r16 < L) gn = reinterpret_cast<const float *>(p.g)[(n * L + r16) * H + h];
+    }
+    if (p.use_delta && r16 < L) be = p.beta[(n * L + r16) * H + h];
+    // the pending keys (and per-channel decays), a channel to a thread
+    float pk[LT], pg[GATE == 2 ? LT : 1];
+    {
+        const uint32_t row = (uint32_t)(H * dk) * 4u, o0 = (uint32_t)(h * dk + tid) * 4u;
+        const __amdgpu_buffer_rsrc_t rk_ = buffer_rsrc(p.pk + n * P * H * dk, (uint32_t)P * row);
+        unroll<LT>([&](auto t) { pk[t] = buffer_load1(rk_, t < a && tid < dk ? o0 + t * row : NOWHERE); });
+        if (GATE == 2) {
+            const __amdgpu_buffer_rsrc_t rg_ = buffer_rsrc(p.pg + n * P * H * dk, (uint32_t)P * row);
+            unroll<LT>([&](auto t) { pg[GATE == 2 ? t : 0] = buffer_load1(rg_, t < a && tid < dk ? o0 + t * row : NOWHERE); });
+        }
+    }
+    // the pending writes as the commit's B operand: token 4 s + g, this lane's columns
     const int col = 32 * wave + 2 * r16;
+    f32x2 pu[LT / 4];
+    {
+        const uint32_t row = (uint32_t)(H * dv) * 4u, o0 = (uint32_t)(h * dv + col) * 4u;
+        const __amdgpu_buffer_rsrc_t ru = buffer_rsrc(p.pu + n * P * H * dv, (uint32_t)P * row);
+        unroll<LT / 4>([&](auto s) {
+            const int t = 4 * s + g4;
+            pu[s] = buffer_load2(ru, t < a && col < dv ? o0 + t * row : NOWHERE);
+        });
+    }
+    // --- the state; rows and columns beyond it read zeros and are not stored ---
     const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(p.S + (int64_t)blockIdx.x * dk * dv, (uint32_t)(dk * dv) * 4u);
-    const uint32_t v0 = col < dv ? (uint32_t)(4 * g4 * dv + col) * 4u : 0x40000000u, row = (uint32_t)dv * 4u;
+    const uint32_t v0 = col < dv ? (uint32_t)(4 * g4 * dv + col) * 4u : NOWHERE, row = (uint32_t)dv * 4u;
     f32x4 S[RT][2];
     unroll<RT>([&](auto i) {
         unroll<4>([&](auto j) {
-            const f32x2 x = buffer_load_nt2(rs, v0 + (16 * i + j) * row);
-            S[i][0][j.value] = x[0];
-            S[i][1][j.value] = x[1];
+            const f32x2 y = buffer_load_nt2(rs, v0 + (16 * i + j) * row);
+            S[i][0][j.value] = y[0];
+            S[i][1][j.value] = y[1];
         });
     });
-    // the pending writes as the commit's B operand: token 4 s + g, this lane's columns
-    f32x2 pu[LT / 4];
-    unroll<LT / 4>([&](auto s) {
-        const int t = 4 * s + g4;
-        pu[s] = f32x2{0.f, 0.f};
-        if (t < a && col < dv) pu[s] = *reinterpret_cast<const f32x2 *>(p.pu + ((n * P + t) * p.H + h) * dv + col);
-    });
-    // the accepted writes' weights at their block's end, a channel to a thread
-    float *ws = both;
-    const bool has_g = GATE == 2 || p.pg != nullptr;
-    if (tid < DKP) {
-        float pk[LT], pg[LT], run = 1.f;
-        unroll<LT>([&](auto t) {
-            const int64_t at = (n * P + t) * p.H + h;
-            pk[t] = pg[t] = 0.f;
-            if (t < a && tid < dk) {
-                pk[t] = p.pk[at * dk + tid];
-                if (has_g) pg[t] = p.pg[GATE == 2 ? at * dk + tid : at];
+
+    // --- without the state ---
+    {
+        float *to = at.which == 0 ? &qq[0][at.c] : at.which == 1 ? &kk[0][at.c] : &vv[0][at.c];
+        const int ld = at.which < 2 ? LDK : DVM;
+        auto put = [&](int t, float y0, float y1) { *reinterpret_cast<f32x2 *>(to + t * ld) = f32x2{y0, y1}; };
+        if (fast) {
+            float w[8];
+            if (p.cv.w_f32 || sizeof(E) == 4) {
+                unroll<8>([&](auto i) { w[i] = __builtin_bit_cast(float, (unsigned)wraw[i / 4][i % 4]); });
+            } else {
+                typedef E E8 __attribute__((ext_vector_type(8)));
+                struct W16 { E8 e; };
+                if constexpr (sizeof(E) == 2) {
+                    const E8 e = __builtin_bit_cast(E8, wraw[0]);
+                    unroll<8>([&](auto i) { w[i] = (float)e[i.value]; });
+                }
             }
-        });
-        unroll<LT>([&](auto s) {
-            constexpr int t = LT - 1 - s;
-            ws[t * WLD + tid] = t < a ? run * pk[t] : 0.f;
-            if (t < a) run *= expf(pg[t]);
-        });
-        ds[tid] = run;
-    }
-    for (int cp = tid; cp < pairs; cp += nt) {
-        const int c2 = 2 * cp, which = c2 < dk ? 0 : c2 < 2 * dk ? 1 : 2;
-        const int c = which == 0 ? c2 : which == 1 ? c2 - dk : c2 - 2 * dk, cc = h * (which < 2 ? dk : dv) + c;
-        const int64_t ld_in = which < 2 ? p.ld_qk : p.ld_v;
-        const E *src = reinterpret_cast<const E *>(which == 0 ? p.q : which == 1 ? p.k : p.v) + n * L * ld_in + cc;
-        float *to = which == 0 ? &qq[0][c] : which == 1 ? &kk[0][c] : &vv[0][c];
-        const int ld = which < 2 ? LDK : DVM;
-        auto put = [&](int t, float x, float y) { *reinterpret_cast<f32x2 *>(to + t * ld) = f32x2{x, y}; };
-        if (p.cv.K == 4) draft_conv<E, LT, 4>(p, src, ld_in, n, a, which, cc, put);
-        else if (p.cv.K) draft_conv<E, LT, 0>(p, src, ld_in, n, a, which, cc, put);
-        else
-            for (int t = 0; t < L; ++t) {
-                const Pair<E> x = *reinterpret_cast<const Pair<E> *>(src + t * ld_in);
-                put(t, (float)x[0], (float)x[1]);
+            if (tid < pairs) {
+                unroll<4>([&](auto r) { *reinterpret_cast<Pair<E> *>(at.cache + r * at.D) = x[r]; });
+                unroll<LT>([&](auto t) {
+                    if (t < L) {
+                        *reinterpret_cast<Pair<E> *>(at.pend + t * at.D) = x[4 + t];
+                        f32x2 y = {0.f, 0.f};
+                        unroll<4>([&](auto r) {
+                            y[0] += w[r] * (float)x[t + 1 + r][0];
+                            y[1] += w[4 + r] * (float)x[t + 1 + r][1];
+                        });
+                        put(t, y[0] * sigmoidf_(y[0]), y[1] * sigmoidf_(y[1]));
+                    }
+                });
             }
+        } else if (tid < pairs) {
+            if (p.cv.K) draft_conv_any<E>(p, at, a, put);
+            else
+                for (int t = 0; t < L; ++t) {
+                    const Pair<E> y = *reinterpret_cast<const Pair<E> *>(at.src + t * at.ld);
+                    put(t, (float)y[0], (float)y[1]);
+                }
+        }
     }
+    // what the accepted writes weigh at their block's end
+    if (GATE == 2) {
+        if (tid < DKP) {
+            float run = 1.f;
+            unroll<LT>([&](auto s) {
+                constexpr int t = LT - 1 - s;
+                ws[t][tid] = run * pk[t];
+                run *= __expf(pg[GATE == 2 ? t : 0]);              // 1 behind the accepted
+            });
+            ds[tid] = run;
+        }
+    } else {
+        if (tid < DKP) unroll<LT>([&](auto t) { ws[t][tid] = pk[t]; });
+        const float back = row_suffix16(gp), after = dpp_f<0x101>(back);
+        const float weight = __expf(after);
+        unroll<LT / 4>([&](auto s) { pu[s] *= __shfl(weight, 4 * s + g4); });
+        if (tid < 16) {
+            ds[tid] = __expf(__shfl(back, 0));
+            es[0][tid] = __expf(gn);
+            eg[0][tid] = __expf(row_prefix16(gn));
+        }
+    }
+    if (tid < L) betas[tid] = p.fz.beta_sigmoid ? sigmoidf_(be) : be;
     if (dk < DKP)
         for (int c = dk + tid; c < DKP; c += nt)
             for (int t = 0; t < LT; ++t) {
                 kk[t][c] = qq[t][c] = 0.f;
-                if (GATE == 2) es[t][c] = 1.f;
+                if (GATE == 2) es[t][c] = eg[t][c] = 1.f;
             }
     lds_barrier();
-    // q, k to unit length, the decays and beta; from here on the pending block is the new one's
-    if (L > 0) {
-        if (p.fz.qk_l2norm) {
-            for (int r = wave; r < 2 * L; r += waves) {
-                float *x = r < L ? qq[r] : kk[r - L];
-                float s = 0.f;
-                for (int c = lane; c < dk; c += 64) s += x[c] * x[c];
-                s = rsqrtf(wave_sum64(s) + 1e-6f);
-                for (int c = lane; c < dk; c += 64) x[c] *= s;
+    // from here on the pending block is the new one's
+    if (GATE == 1 && has_g && tid < L) p.pg[(n * P + tid) * H + h] = gn;
+    if (GATE == 2) {
+        for (int i = tid; i < L * (dk / 2); i += nt) {
+            const int t = i / (dk / 2), c = 2 * (i - t * (dk / 2));
+            const int64_t o = ((n * L + t) * H + h) * dk + c;
+            f32x2 g;
+            if (p.fz.gate_16) {
+                const Pair<E> e = *reinterpret_cast<const Pair<E> *>(reinterpret_cast<const E *>(p.g) + o);
+                g = f32x2{(float)e[0], (float)e[1]};
+            } else {
+                g = *reinterpret_cast<const f32x2 *>(reinterpret_cast<const float *>(p.g) + o);
             }
-        }
-        if (GATE == 1 && tid < L) {
-            float g = 0.f;
-            if (has_g) {
-                g = reinterpret_cast<const float *>(p.g)[(n * L + tid) * p.H + h];
-                p.pg[(n * P + tid) * p.H + h] = g;
+            if (p.fz.gate_act) {
+                const float al = p.fz.A_log[h];
+                g[0] = gate_activation(g[0], al, p.fz.dt_bias[h * dk + c], p.fz.lb_set, p.fz.lb);
+                g[1] = gate_activation(g[1], al, p.fz.dt_bias[h * dk + c + 1], p.fz.lb_set, p.fz.lb);
             }
-            es[0][tid] = expf(g);
-        }
-        if (GATE == 2) {
-            for (int i = tid; i < L * dk; i += nt) {
-                const int t = i / dk, c = i - t * dk;
-                const int64_t at = ((n * L + t) * p.H + h) * dk + c;
-                float g = p.fz.gate_16 ? (float)reinterpret_cast<const E *>(p.g)[at] : reinterpret_cast<const float *>(p.g)[at];
-                if (p.fz.gate_act) {
-                    const float z = g + p.fz.dt_bias[h * dk + c], al = expf(p.fz.A_log[h]);
-                    g = p.fz.lb_set ? p.fz.lb / (1.f + expf(-al * z)) : -al * (z > 20.f ? z : log1pf(expf(z)));
-                }
-                p.pg[((n * P + t) * p.H + h) * dk + c] = g;
-                es[t][c] = expf(g);
-            }
-        }
-        if (tid < L) {
-            const float b = p.use_delta ? p.beta[(n * L + tid) * p.H + h] : 0.f;
-            betas[tid] = p.fz.beta_sigmoid ? 1.f / (1.f + expf(-b)) : b;
-        }
-        lds_barrier();
-        for (int i = tid; i < L * dk; i += nt) {
-            const int t = i / dk, c = i - t * dk;
-            p.pk[((n * P + t) * p.H + h) * dk + c] = kk[t][c];
-        }
-        // A and B: 16 lanes share the channels of key j, decayed from token to token
-        for (int j = tid >> 4; j < L; j += nt >> 4) {
-            float x[LP];
-#pragma unroll
-            for (int c = 0; c < LP; ++c) x[c] = kk[j][r16 * LP + c];
-            for (int t = j; t < L; ++t) {
-                float sa = 0.f, sb = 0.f;
-#pragma unroll
-                for (int c = 0; c < LP; ++c) {
-                    if (t > j) x[c] *= es[GATE == 2 ? t : 0][GATE == 2 ? r16 * LP + c : t];
-                    sa += kk[t][r16 * LP + c] * x[c];
-                    sb += qq[t][r16 * LP + c] * x[c];
-                }
-                sa = row_sum16(sa);
-                sb = row_sum16(sb);
-                if (r16 == 0) {
-                    aa[t][j] = sa;
-                    bb[t][j] = sb;
-                }
-            }
-        }
-        if (GATE == 2) {
-            lds_barrier();
-            for (int c = tid; c < dk; c += nt) {
-                float run = 1.f;
-                for (int t = 0; t < L; ++t) {
-                    run *= es[t][c];
-                    kk[t][c] *= run;
-                    qq[t][c] *= run;
-                }
-            }
-        } else if (tid == 0) {
-            float run = 1.f;
-            for (int t = 0; t < L; ++t) {
-                run *= es[0][t];
-                decay[t] = run;
-            }
+            *reinterpret_cast<f32x2 *>(p.pg + ((n * P + t) * H + h) * dk + c) = g;
+            *reinterpret_cast<f32x2 *>(&es[t][c]) = f32x2{__expf(g[0]), __expf(g[1])};
         }
         lds_barrier();
     }
+    // A and B: 16 lanes share the channels of key j, which decays from token to token
+    for (int j = wave + waves * g4; j < L; j += 4 * waves) {
+        f32x4 y[NC];
+        unroll<NC>([&](auto c) { y[c] = ld4(&kk[j][64 * c + 4 * r16]); });
+        for (int t = j; t < L; ++t) {
+            float sa = 0.f, sb = 0.f, sq = 0.f;
+            const float e1 = GATE == 2 ? 1.f : es[0][t];
+            unroll<NC>([&](auto c) {
+                const f32x4 k4 = ld4(&kk[t][64 * c + 4 * r16]), q4 = ld4(&qq[t][64 * c + 4 * r16]);
+                if (t > j) y[c] *= GATE == 2 ? ld4(&es[GATE == 2 ? t : 0][64 * c + 4 * r16]) : f32x4{e1, e1, e1, e1};
+                unroll<4>([&](auto i) {
+                    sa += k4[i.value] * y[c][i.value];
+                    sb += q4[i.value] * y[c][i.value];
+                    sq += q4[i.value] * q4[i.value];
+                });
+            });
+            sa = row_sum16(sa);
+            sb = row_sum16(sb);
+            if (t == j) sq = row_sum16(sq);
+            if (r16 == 0) {
+                aa[t][j] = sa;
+                bb[t][j] = sb;
+                if (t == j) {
+                    rk[t] = p.fz.qk_l2norm ? rsqrtf(sa + 1e-6f) : 1.f;
+                    rq[t] = p.scale * (p.fz.qk_l2norm ? rsqrtf(sq + 1e-6f) : 1.f);
+                }
+            }
+        }
+    }
+    if (GATE == 2)
+        for (int c = tid; c < dk; c += nt) {
+            float run = 1.f;
+            for (int t = 0; t < L; ++t) {
+                run *= es[t][c];
+                eg[t][c] = run;
+            }
+        }
+    lds_barrier();
+    for (int i = tid; i < L * (dk / 2); i += nt) {
+        const int t = i / (dk / 2), c = 2 * (i - t * (dk / 2));
+        const f32x2 y = *reinterpret_cast<const f32x2 *>(&kk[t][c]);
+        *reinterpret_cast<f32x2 *>(p.pk + ((n * P + t) * H + h) * dk + c) = f32x2{y[0] * rk[t], y[1] * rk[t]};
+    }
 
-    // commit
+    // --- commit ---
     unroll<RT>([&](auto i) {
-        const f32x4 d = ld4(&ds[16 * i + 4 * g4]);
+        const f32x4 d = GATE == 2 ? ld4(&ds[GATE == 2 ? 16 * i + 4 * g4 : 0]) : f32x4{ds[0], ds[0], ds[0], ds[0]};
         S[i][0] *= d;
         S[i][1] *= d;
         unroll<LT / 4>([&](auto s) {
-            const float w = ws[(4 * s + g4) * WLD + 16 * i + r16];
+            const float w = ws[4 * s + g4][16 * i + r16];
             S[i][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(w, pu[s][0], S[i][0], 0, 0, 0);
             S[i][1] = __builtin_amdgcn_mfma_f32_16x16x4f32(w, pu[s][1], S[i][1], 0, 0, 0);
         });
@@ -281,48 +364,49 @@ __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(LT == 1
     });
     if (L == 0) return;
 
-    // [K; Q] S: rows 0 .. LT - 1 are K's, LT .. 2 LT - 1 Q's
+    // --- [K; Q] S: rows 0 .. LT - 1 are K's, LT .. 2 LT - 1 Q's ---
     f32x4 z[LT / 8][2];
     unroll<LT / 8>([&](auto m) { z[m][0] = z[m][1] = f32x4{0.f, 0.f, 0.f, 0.f}; });
     unroll<RT>([&](auto i) {
         unroll<LT / 8>([&](auto m) {
-            const float *x = LT == 16 ? (m ? qq[r16] : kk[r16]) : (r16 < 8 ? kk[r16 & 7] : qq[r16 & 7]);
-            const f32x4 f = ld4(x + 16 * i + 4 * g4);
+            const int c = 16 * i + 4 * g4;
+            f32x4 f = ld4(LT == 16 ? (m ? &qq[r16 % LT][c] : &kk[r16 % LT][c]) : (r16 < 8 ? &kk[r16 & 7][c] : &qq[r16 & 7][c]));
+            if (GATE == 2) f *= ld4(&eg[GATE == 2 ? r16 % LT : 0][c]);
             z[m][0] = mfma_kb1(f, S[i][0], z[m][0]);
             z[m][1] = mfma_kb1(f, S[i][1], z[m][1]);
         });
     });
-    lds_barrier();                                                 // ws is read no more
-    float *prod = both;
-    unroll<LT / 8>([&](auto m) {
+    unroll<LT / 8>([&](auto m) {                                   // read below by this wave alone
         unroll<4>([&](auto j) {
-            *reinterpret_cast<f32x2 *>(&prod[(16 * m + 4 * g4 + j) * DVM + col]) = f32x2{z[m][0][j.value], z[m][1][j.value]};
+            *reinterpret_cast<f32x2 *>(&prod[16 * m + 4 * g4 + j][col]) = f32x2{z[m][0][j.value], z[m][1][j.value]};
         });
     });
-    lds_barrier();
     // the block's writes and outputs, a column to a lane (both halves of the wave the same)
     {
         const int c = 32 * wave + (lane & 31);
-        float u[LT];
+        float u[LT];                                               // rk_t u_t
         unroll<LT>([&](auto t) {
             u[t] = 0.f;
             if (t < L) {
-                float s = prod[t * DVM + c];
-                if (GATE == 1) s *= decay[t];
+                float s = prod[t][c], o = prod[LT + t][c], v = vv[t][c];
+                const float k1 = rk[t];
+                if (GATE == 1) {
+                    s *= eg[0][t];
+                    o *= eg[0][t];
+                }
                 unroll<t>([&](auto j) { s += aa[t][j] * u[j]; });
-                u[t] = p.use_delta ? betas[t] * (vv[t][c] - s) : vv[t][c];
-                if (lane < 32 && c < dv) p.pu[((n * P + t) * p.H + h) * dv + c] = u[t];
-                float o = prod[(LT + t) * DVM + c];
-                if (GATE == 1) o *= decay[t];
+                if (p.use_delta) v = betas[t] * (v - k1 * s);
+                if (lane < 32 && c < dv) p.pu[((n * P + t) * H + h) * dv + c] = v;
+                u[t] = k1 * v;
                 unroll<t + 1>([&](auto j) { o += bb[t][j] * u[j]; });
-                if (lane < 32) vv[t][c] = p.scale * o;
+                if (lane < 32) vv[t][c] = rq[t] * o;
             }
         });
     }
     lds_barrier();
-    // the outputs, a wave per token
+    // --- the outputs, a wave per token ---
     for (int t = wave; t < L; t += waves) {
-        E *out = reinterpret_cast<E *>(p.o) + ((n * L + t) * p.H + h) * dv;
+        E *out = reinterpret_cast<E *>(p.o) + ((n * L + t) * H + h) * dv;
         const E *gate = reinterpret_cast<const E *>(p.ep.gate) + (n * L + t) * p.ld_v + h * dv;
         float r = 1.f;
         if (p.ep.gate) {
@@ -331,23 +415,25 @@ __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(LT == 1
             r = rsqrtf(wave_sum64(s) / (float)dv + p.ep.eps);
         }
         for (int c = 2 * lane; c < dv; c += 128) {
-            f32x2 x = *reinterpret_cast<const f32x2 *>(&vv[t][c]);
+            f32x2 y = *reinterpret_cast<const f32x2 *>(&vv[t][c]);
             if (p.ep.gate) {
-                const Pair<E> z = *reinterpret_cast<const Pair<E> *>(gate + c);
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
-                    x[b] = x[b] * r * param_f(p.ep.gamma, p.ep.gamma_f32 ? 0 : p.dtype, c + b) *
-                           ((float)z[b] / (1.f + expf(-(float)z[b])));
+                const Pair<E> b = *reinterpret_cast<const Pair<E> *>(gate + c);
+                f32x2 gm;
+                if (p.ep.gamma_f32) gm = reinterpret_cast<const f32x2 *>(p.ep.gamma)[c / 2];
+                else gm = f32x2{(float)reinterpret_cast<const E *>(p.ep.gamma)[c], (float)reinterpret_cast<const E *>(p.ep.gamma)[c + 1]};
+                y[0] *= r * gm[0] * ((float)b[0] * sigmoidf_((float)b[0]));
+                y[1] *= r * gm[1] * ((float)b[1] * sigmoidf_((float)b[1]));
             }
-            *reinterpret_cast<Pair<E> *>(out + c) = Pair<E>{(E)x[0], (E)x[1]};
+            *reinterpret_cast<Pair<E> *>(out + c) = Pair<E>{(E)y[0], (E)y[1]};
         }
     }
 }
 
 template <typename E, int GATE, int RT, int LT>
 static hipError_t draft_launch(const DraftParams &p, hipStream_t stream) {
-    // a wave per 32 columns, and a thread per key channel
-    const int by_cols = (p.dv + 31) / 32, waves = by_cols > RT / 4 ? by_cols : RT / 4;
+    // a wave per 32 columns, a thread per key channel and per pair of q, k, v channels
+    const int cols = (p.dv + 31) / 32, pairs = (p.dk + p.dv / 2 + 63) / 64, key = RT / 4;
+    const int waves = cols > pairs ? (cols > key ? cols : key) : (pairs > key ? pairs : key);
     const dim3 grid((unsigned)(p.N * p.H)), block(64 * waves);
     if (p.dv <= 128) draft_block_kernel<E, GATE, RT, LT, 256><<<grid, block, 0, stream>>>(p);
     else draft_block_kernel<E, GATE, RT, LT, 512><<<grid, block, 0, stream>>>(p);

@@ -365,6 +365,7 @@ struct DraftParams {
     const int32_t *accepted;      // [N] pending tokens that stand (clamped to 0 .. P)
     int64_t ld_qk, ld_v, N;
     int L, P, H, dk, dv, dtype, use_delta;
+    int conv4;                    // four taps whose weights are 16-byte aligned
     float scale;
     Fusion fz;
     Epilogue ep;
