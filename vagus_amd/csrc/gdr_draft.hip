@@ -34,17 +34,11 @@ namespace {
 template <typename E> using Pair = E __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-__device__ __forceinline__ f32x2 buffer_load_nt2(__amdgpu_buffer_rsrc_t r, uint32_t voff) {
-    return __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(r, (int)voff, 0, CPOL_NT));
-}
-__device__ __forceinline__ void buffer_store_nt2(f32x2 x, __amdgpu_buffer_rsrc_t r, uint32_t voff) {
-    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, x), r, (int)voff, 0, CPOL_NT);
-}
 __device__ __forceinline__ float buffer_load1(__amdgpu_buffer_rsrc_t r, uint32_t voff) {
     return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, (int)voff, 0, 0));
 }
-__device__ __forceinline__ f32x2 buffer_load2(__amdgpu_buffer_rsrc_t r, uint32_t voff) {
-    return __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(r, (int)voff, 0, 0));
+__device__ __forceinline__ f32x4 buffer_load4(__amdgpu_buffer_rsrc_t r, uint32_t voff) {
+    return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)voff, 0, 0));
 }
 constexpr uint32_t NOWHERE = 0x40000000u;                          // an offset behind every block: reads zeros
 
@@ -129,103 +123,66 @@ __device__ __forceinline__ float row_prefix16(float x) {
 
 }  // namespace
 
-// One workgroup per (stream, head), a wave per 32 columns of the state, which it holds in the
-// C layout of 16 x 16 tiles: lane 16 g + r has rows 16 i + 4 g + j (j < 4) of columns 2 r, 2 r + 1, so a
-// row's 32 columns are one 128-byte line. As it lies it is the B operand of the product with [K; Q].
-// What does not need the state (conv, gates, A and B) is loaded ahead of it and done while it
-// arrives.  q and k are kept unnormalised: the norms are A's and q's own diagonals and scale the
-// results.  RT: row tiles (dk <= 16 RT). LT: room of the pending block and tokens (8 or 16).
+// One workgroup per (stream, head). A wave holds 64 rows x 64 columns of the state in the C layout of
+// 16 x 16 tiles: lane 16 g + r has rows 16 i + 4 g + j (i, j < 4) of columns 4 r .. 4 r + 3, so that an
+// access touches four rows of 256 bytes. As it lies it is the B operand of the product with [K; Q], whose
+// two halves of rows (dk > 64) meet in LDS.  q and k are kept unnormalised: the norms are A's and
+// q's own diagonals and scale the results.  RT: row tiles (dk <= 16 RT). LT: room of the pending
+// block and tokens (8 or 16).  At least 128 (RT 4) or 256 threads, and a thread per pair of q, k, v channels.
 template <typename E, int GATE, int RT, int LT, int NT>
-__global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(LT == 16 && NT == 256 ? 3 : 4)))
+__global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(LT == 8 ? 4 : NT == 256 ? 3 : 2)))
 draft_block_kernel(const DraftParams p) {
-    constexpr int DKP = 16 * RT, LDK = DKP + 4, WLD = DKP + 16, DVM = NT / 2, NC = DKP / 64;
+    constexpr int DKP = 16 * RT, LDK = DKP + 4, WLD = DKP + 16, DVM = NT / 2, NC = DKP / 64, HALVES = RT / 4, LG = LT / 4;
     __shared__ __attribute__((aligned(16))) float kk[LT][LDK], qq[LT][LDK], vv[LT][DVM], ws[LT][WLD], prod[2 * LT][DVM];
     __shared__ __attribute__((aligned(16))) float es[GATE == 2 ? LT : 1][GATE == 2 ? DKP : 16];  // e^{g_t}
     __shared__ __attribute__((aligned(16))) float eg[GATE == 2 ? LT : 1][GATE == 2 ? LDK : 16];  // e^{G_t}
     __shared__ __attribute__((aligned(16))) float ds[GATE == 2 ? DKP : 16], aa[LT][LT], bb[LT][LT];
-    __shared__ float betas[LT], rk[LT], rq[LT];
+    __shared__ float betas[16], rk[LT], rq[LT];
     const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 63, waves = nt >> 6;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), g4 = lane >> 4, r16 = lane & 15;
     const int64_t n = blockIdx.x / p.H;
     const int h = blockIdx.x - (int)n * p.H;
     const int dk = p.dk, dv = p.dv, L = p.L, P = p.P, H = p.H, pairs = dk + dv / 2;
     int a = p.accepted[n];
-    a = a < 0 ? 0 : a > P ? P : a;
-    const bool fast = p.conv4;
-
-    // --- loads ahead of the state ---
-    const ChannelPair<E> at(p, n, h, tid < pairs ? tid : pairs - 1);
-    Pair<E> x[4 + LT];                                             // four taps: the last inputs, then the block's
-    u32x4 wraw[2];
-    if (fast) {
-        unroll<4>([&](auto r) {
-            const int i = a + r;
-            x[r] = *reinterpret_cast<const Pair<E> *>(i < 4 ? at.cache + i * at.D : at.pend + (i - 4) * at.D);
-        });
-        wraw[0] = *reinterpret_cast<const u32x4 *>(at.w);
-        if (p.cv.w_f32 || sizeof(E) == 4) wraw[1] = reinterpret_cast<const u32x4 *>(at.w)[1];
-        if (L > 0)
-            unroll<LT>([&](auto t) { x[4 + t] = *reinterpret_cast<const Pair<E> *>(at.src + (t < L ? (int)t : L - 1) * at.ld); });
-    }
-    // scalar gate: lane r of every row of 16 has token r's
-    const bool has_g = GATE == 2 || p.pg != nullptr;
-    float gp = 0.f, gn = 0.f, be = 0.f;
-    if (GATE == 1 && has_g) {
-        if (r16 < a) gp = p.pg[(n * P + r16) * H + h];
-        if (r16 < L) gn = reinterpret_cast<const float *>(p.g)[(n * L + r16) * H + h];
-    }
-    if (p.use_delta && r16 < L) be = p.beta[(n * L + r16) * H + h];
-    // the pending keys (and per-channel decays), a channel to a thread
-    float pk[LT], pg[GATE == 2 ? LT : 1];
-    {
-        const uint32_t row = (uint32_t)(H * dk) * 4u, o0 = (uint32_t)(h * dk + tid) * 4u;
-        const __amdgpu_buffer_rsrc_t rk_ = buffer_rsrc(p.pk + n * P * H * dk, (uint32_t)P * row);
-        unroll<LT>([&](auto t) { pk[t] = buffer_load1(rk_, t < a && tid < dk ? o0 + t * row : NOWHERE); });
-        if (GATE == 2) {
-            const __amdgpu_buffer_rsrc_t rg_ = buffer_rsrc(p.pg + n * P * H * dk, (uint32_t)P * row);
-            unroll<LT>([&](auto t) { pg[GATE == 2 ? t : 0] = buffer_load1(rg_, t < a && tid < dk ? o0 + t * row : NOWHERE); });
-        }
-    }
-    // the pending writes as the commit's B operand: token 4 s + g, this lane's columns
-    const int col = 32 * wave + 2 * r16;
-    f32x2 pu[LT / 4];
-    {
-        const uint32_t row = (uint32_t)(H * dv) * 4u, o0 = (uint32_t)(h * dv + col) * 4u;
-        const __amdgpu_buffer_rsrc_t ru = buffer_rsrc(p.pu + n * P * H * dv, (uint32_t)P * row);
-        unroll<LT / 4>([&](auto s) {
-            const int t = 4 * s + g4;
-            pu[s] = buffer_load2(ru, t < a && col < dv ? o0 + t * row : NOWHERE);
-        });
-    }
     // --- the state; rows and columns beyond it read zeros and are not stored ---
+    const int half = wave % HALVES, col = 64 * (wave / HALVES) + 4 * r16;
     const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(p.S + (int64_t)blockIdx.x * dk * dv, (uint32_t)(dk * dv) * 4u);
-    const uint32_t v0 = col < dv ? (uint32_t)(4 * g4 * dv + col) * 4u : NOWHERE, row = (uint32_t)dv * 4u;
-    f32x4 S[RT][2];
-    unroll<RT>([&](auto i) {
+    const uint32_t row = (uint32_t)dv * 4u, v0 = col < dv ? (uint32_t)((64 * half + 4 * g4) * dv + col) * 4u : NOWHERE;
+    f32x4 S[4][4];                                                 // [row tile][column of the lane's four]
+    unroll<4>([&](auto i) {
         unroll<4>([&](auto j) {
-            const f32x2 y = buffer_load_nt2(rs, v0 + (16 * i + j) * row);
-            S[i][0][j.value] = y[0];
-            S[i][1][j.value] = y[1];
+            const f32x4 y = buffer_load_nt4(rs, v0 + (16 * i + j) * row, 0);
+            unroll<4>([&](auto c) { S[i][c][j.value] = y[c.value]; });
         });
     });
 
-    // --- without the state ---
+    // --- without the state: the short conv, a thread to two channels ---
+    a = a < 0 ? 0 : a > P ? P : a;
     {
+        const ChannelPair<E> at(p, n, h, tid < pairs ? tid : pairs - 1);
         float *to = at.which == 0 ? &qq[0][at.c] : at.which == 1 ? &kk[0][at.c] : &vv[0][at.c];
         const int ld = at.which < 2 ? LDK : DVM;
         auto put = [&](int t, float y0, float y1) { *reinterpret_cast<f32x2 *>(to + t * ld) = f32x2{y0, y1}; };
-        if (fast) {
-            float w[8];
-            if (p.cv.w_f32 || sizeof(E) == 4) {
-                unroll<8>([&](auto i) { w[i] = __builtin_bit_cast(float, (unsigned)wraw[i / 4][i % 4]); });
-            } else {
-                typedef E E8 __attribute__((ext_vector_type(8)));
-                struct W16 { E8 e; };
-                if constexpr (sizeof(E) == 2) {
-                    const E8 e = __builtin_bit_cast(E8, wraw[0]);
-                    unroll<8>([&](auto i) { w[i] = (float)e[i.value]; });
-                }
-            }
+        if (p.conv4) {
+            Pair<E> x[4 + LT];                                     // the last inputs, then the block's
+            u32x4 wraw[2];
+            const bool w32 = sizeof(E) == 4 || p.cv.w_f32;
+            unroll<4>([&](auto r) {
+                const int i = a + r;
+                x[r] = *reinterpret_cast<const Pair<E> *>(i < 4 ? at.cache + i * at.D : at.pend + (i - 4) * at.D);
+            });
+            wraw[0] = *reinterpret_cast<const u32x4 *>(at.w);
+            wraw[1] = reinterpret_cast<const u32x4 *>(at.w)[w32 ? 1 : 0];
+            if (L > 0)
+                unroll<LT>([&](auto t) { x[4 + t] = *reinterpret_cast<const Pair<E> *>(at.src + (t < L ? (int)t : L - 1) * at.ld); });
+            f32x2 w[4];
+            unroll<8>([&](auto i) {
+                const unsigned word = w32 ? wraw[i / 4][i % 4] : wraw[0][i / 2];
+                float f = __builtin_bit_cast(float, word);
+                if constexpr (sizeof(E) == 2)
+                    if (!w32) f = (float)__builtin_bit_cast(E, (unsigned short)(i % 2 ? word >> 16 : word));
+                w[i % 4][i / 4] = f;
+            });
             if (tid < pairs) {
                 unroll<4>([&](auto r) { *reinterpret_cast<Pair<E> *>(at.cache + r * at.D) = x[r]; });
                 unroll<LT>([&](auto t) {
@@ -233,8 +190,8 @@ draft_block_kernel(const DraftParams p) {
                         *reinterpret_cast<Pair<E> *>(at.pend + t * at.D) = x[4 + t];
                         f32x2 y = {0.f, 0.f};
                         unroll<4>([&](auto r) {
-                            y[0] += w[r] * (float)x[t + 1 + r][0];
-                            y[1] += w[4 + r] * (float)x[t + 1 + r][1];
+                            y[0] += w[r][0] * (float)x[t + 1 + r][0];
+                            y[1] += w[r][1] * (float)x[t + 1 + r][1];
                         });
                         put(t, y[0] * sigmoidf_(y[0]), y[1] * sigmoidf_(y[1]));
                     }
@@ -249,59 +206,71 @@ draft_block_kernel(const DraftParams p) {
                 }
         }
     }
-    // what the accepted writes weigh at their block's end
-    if (GATE == 2) {
-        if (tid < DKP) {
-            float run = 1.f;
-            unroll<LT>([&](auto s) {
-                constexpr int t = LT - 1 - s;
-                ws[t][tid] = run * pk[t];
-                run *= __expf(pg[GATE == 2 ? t : 0]);              // 1 behind the accepted
-            });
-            ds[tid] = run;
-        }
-    } else {
-        if (tid < DKP) unroll<LT>([&](auto t) { ws[t][tid] = pk[t]; });
-        const float back = row_suffix16(gp), after = dpp_f<0x101>(back);
-        const float weight = __expf(after);
-        unroll<LT / 4>([&](auto s) { pu[s] *= __shfl(weight, 4 * s + g4); });
-        if (tid < 16) {
-            ds[tid] = __expf(__shfl(back, 0));
-            es[0][tid] = __expf(gn);
-            eg[0][tid] = __expf(row_prefix16(gn));
-        }
+    // scalar gate and beta: lane r of every row of 16 has token r's
+    const bool has_g = GATE == 2 || p.pg != nullptr;
+    float gp = 0.f, gn = 0.f, be = 0.f;
+    f32x2 gv[GATE == 2 ? LG : 1];                                  // per channel: two channels of some tokens
+    if (GATE == 1 && has_g) {
+        if (r16 < a) gp = p.pg[(n * P + r16) * H + h];
+        if (r16 < L) gn = reinterpret_cast<const float *>(p.g)[(n * L + r16) * H + h];
     }
-    if (tid < L) betas[tid] = p.fz.beta_sigmoid ? sigmoidf_(be) : be;
+    if (p.use_delta && r16 < L) be = p.beta[(n * L + r16) * H + h];
+    if (GATE == 2) {
+        unroll<LG>([&](auto m) {
+            const int i = tid + m * nt, t = i / (DKP / 2), c = 2 * (i % (DKP / 2));
+            f32x2 &g = gv[GATE == 2 ? m : 0];
+            g = f32x2{0.f, 0.f};
+            if (t < L && c < dk) {
+                const int64_t o = ((n * L + t) * H + h) * dk + c;
+                if (p.fz.gate_16) {
+                    const Pair<E> e = *reinterpret_cast<const Pair<E> *>(reinterpret_cast<const E *>(p.g) + o);
+                    g = f32x2{(float)e[0], (float)e[1]};
+                } else {
+                    g = *reinterpret_cast<const f32x2 *>(reinterpret_cast<const float *>(p.g) + o);
+                }
+            }
+        });
+    }
+    // the pending keys (and per-channel decays), a channel to a thread, and writes, as the commit's B
+    // operand: token 4 s + g, this lane's columns
+    float pk[LT], pg[GATE == 2 ? LT : 1];
+    f32x4 pu[LG];
+    {
+        const uint32_t kr = (uint32_t)(H * dk) * 4u, k0 = (uint32_t)(h * dk + tid) * 4u;
+        const uint32_t ur = (uint32_t)(H * dv) * 4u, u0 = (uint32_t)(h * dv + col) * 4u;
+        const __amdgpu_buffer_rsrc_t bk = buffer_rsrc(p.pk + n * P * H * dk, (uint32_t)P * kr);
+        const __amdgpu_buffer_rsrc_t bu = buffer_rsrc(p.pu + n * P * H * dv, (uint32_t)P * ur);
+        unroll<LT>([&](auto t) { pk[t] = buffer_load1(bk, t < a && tid < dk ? k0 + t * kr : NOWHERE); });
+        if (GATE == 2) {
+            const __amdgpu_buffer_rsrc_t bg = buffer_rsrc(p.pg + n * P * H * dk, (uint32_t)P * kr);
+            unroll<LT>([&](auto t) { pg[GATE == 2 ? t : 0] = buffer_load1(bg, t < a && tid < dk ? k0 + t * kr : NOWHERE); });
+        }
+        unroll<LG>([&](auto s) {
+            const int t = 4 * s + g4;
+            pu[s] = buffer_load4(bu, t < a && col < dv ? u0 + t * ur : NOWHERE);
+        });
+    }
+    if (GATE == 2) {
+        unroll<LG>([&](auto m) {
+            const int i = tid + m * nt, t = i / (DKP / 2), c = 2 * (i % (DKP / 2));
+            f32x2 &g = gv[GATE == 2 ? m : 0];
+            if (p.fz.gate_act) {
+                const int cc = c < dk ? h * dk + c : 0;
+                const float al = p.fz.A_log[h];
+                g[0] = gate_activation(g[0], al, p.fz.dt_bias[cc], p.fz.lb_set, p.fz.lb);
+                g[1] = gate_activation(g[1], al, p.fz.dt_bias[cc + 1], p.fz.lb_set, p.fz.lb);
+            }
+            if (t < LT) *reinterpret_cast<f32x2 *>(&es[GATE == 2 ? t : 0][c]) = f32x2{__expf(g[0]), __expf(g[1])};
+        });
+    } else if (tid < 16) {
+        es[0][tid] = __expf(gn);
+        eg[0][tid] = __expf(row_prefix16(gn));
+    }
+    if (tid < 16) betas[tid] = p.fz.beta_sigmoid ? sigmoidf_(be) : be;
     if (dk < DKP)
         for (int c = dk + tid; c < DKP; c += nt)
-            for (int t = 0; t < LT; ++t) {
-                kk[t][c] = qq[t][c] = 0.f;
-                if (GATE == 2) es[t][c] = eg[t][c] = 1.f;
-            }
+            for (int t = 0; t < LT; ++t) kk[t][c] = qq[t][c] = 0.f;
     lds_barrier();
-    // from here on the pending block is the new one's
-    if (GATE == 1 && has_g && tid < L) p.pg[(n * P + tid) * H + h] = gn;
-    if (GATE == 2) {
-        for (int i = tid; i < L * (dk / 2); i += nt) {
-            const int t = i / (dk / 2), c = 2 * (i - t * (dk / 2));
-            const int64_t o = ((n * L + t) * H + h) * dk + c;
-            f32x2 g;
-            if (p.fz.gate_16) {
-                const Pair<E> e = *reinterpret_cast<const Pair<E> *>(reinterpret_cast<const E *>(p.g) + o);
-                g = f32x2{(float)e[0], (float)e[1]};
-            } else {
-                g = *reinterpret_cast<const f32x2 *>(reinterpret_cast<const float *>(p.g) + o);
-            }
-            if (p.fz.gate_act) {
-                const float al = p.fz.A_log[h];
-                g[0] = gate_activation(g[0], al, p.fz.dt_bias[h * dk + c], p.fz.lb_set, p.fz.lb);
-                g[1] = gate_activation(g[1], al, p.fz.dt_bias[h * dk + c + 1], p.fz.lb_set, p.fz.lb);
-            }
-            *reinterpret_cast<f32x2 *>(p.pg + ((n * P + t) * H + h) * dk + c) = g;
-            *reinterpret_cast<f32x2 *>(&es[t][c]) = f32x2{__expf(g[0]), __expf(g[1])};
-        }
-        lds_barrier();
-    }
     // A and B: 16 lanes share the channels of key j, which decays from token to token
     for (int j = wave + waves * g4; j < L; j += 4 * waves) {
         f32x4 y[NC];
@@ -331,59 +300,98 @@ draft_block_kernel(const DraftParams p) {
             }
         }
     }
-    if (GATE == 2)
+    // what the accepted writes weigh at their block's end
+    if (GATE == 2) {
         for (int c = tid; c < dk; c += nt) {
             float run = 1.f;
             for (int t = 0; t < L; ++t) {
-                run *= es[t][c];
-                eg[t][c] = run;
+                run *= es[GATE == 2 ? t : 0][c];
+                eg[GATE == 2 ? t : 0][c] = run;
             }
         }
+        if (dk < DKP)
+            for (int c = dk + tid; c < DKP; c += nt)
+                for (int t = 0; t < LT; ++t) eg[GATE == 2 ? t : 0][c] = 1.f;
+        if (tid < DKP) {
+            float run = 1.f;
+            unroll<LT>([&](auto s) {
+                constexpr int t = LT - 1 - s;
+                ws[t][tid] = run * pk[t];
+                run *= __expf(pg[GATE == 2 ? t : 0]);              // 1 behind the accepted
+            });
+            ds[GATE == 2 ? tid : 0] = run;
+        }
+    } else {
+        if (tid < DKP) unroll<LT>([&](auto t) { ws[t][tid] = pk[t]; });
+        const float back = row_suffix16(gp), weight = __expf(dpp_f<0x101>(back));
+        unroll<LG>([&](auto s) { pu[s] *= __shfl(weight, 4 * s + g4); });
+        if (tid < 16) ds[0] = __expf(__shfl(back, 0));
+    }
     lds_barrier();
-    for (int i = tid; i < L * (dk / 2); i += nt) {
-        const int t = i / (dk / 2), c = 2 * (i - t * (dk / 2));
+    // the pending block has been read: from here on it is the new one's
+    if (GATE == 1 && has_g && tid < L) p.pg[(n * P + tid) * H + h] = gn;
+    if (GATE == 2)
+        unroll<LG>([&](auto m) {
+            const int i = tid + m * nt, t = i / (DKP / 2), c = 2 * (i % (DKP / 2));
+            if (t < L && c < dk) *reinterpret_cast<f32x2 *>(p.pg + ((n * P + t) * H + h) * dk + c) = gv[GATE == 2 ? m : 0];
+        });
+    for (int i = tid; i < L * (DKP / 2); i += nt) {
+        const int t = i / (DKP / 2), c = 2 * (i % (DKP / 2));
         const f32x2 y = *reinterpret_cast<const f32x2 *>(&kk[t][c]);
-        *reinterpret_cast<f32x2 *>(p.pk + ((n * P + t) * H + h) * dk + c) = f32x2{y[0] * rk[t], y[1] * rk[t]};
+        if (c < dk) *reinterpret_cast<f32x2 *>(p.pk + ((n * P + t) * H + h) * dk + c) = f32x2{y[0] * rk[t], y[1] * rk[t]};
     }
 
     // --- commit ---
-    unroll<RT>([&](auto i) {
-        const f32x4 d = GATE == 2 ? ld4(&ds[GATE == 2 ? 16 * i + 4 * g4 : 0]) : f32x4{ds[0], ds[0], ds[0], ds[0]};
-        S[i][0] *= d;
-        S[i][1] *= d;
-        unroll<LT / 4>([&](auto s) {
-            const float w = ws[4 * s + g4][16 * i + r16];
-            S[i][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(w, pu[s][0], S[i][0], 0, 0, 0);
-            S[i][1] = __builtin_amdgcn_mfma_f32_16x16x4f32(w, pu[s][1], S[i][1], 0, 0, 0);
+    unroll<4>([&](auto i) {
+        const int k0 = 64 * half + 16 * i;
+        const f32x4 d = GATE == 2 ? ld4(&ds[GATE == 2 ? k0 + 4 * g4 : 0]) : f32x4{ds[0], ds[0], ds[0], ds[0]};
+        unroll<4>([&](auto c) { S[i][c] *= d; });
+        unroll<LG>([&](auto s) {
+            const float w = ws[4 * s + g4][k0 + r16];
+            unroll<4>([&](auto c) { S[i][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(w, pu[s][c.value], S[i][c], 0, 0, 0); });
         });
     });
     uint32_t v1 = v0;
-    asm volatile("" : "+v"(v1));                                   // the loads' 32 addresses are not kept for the stores
-    unroll<RT>([&](auto i) {
-        unroll<4>([&](auto j) { buffer_store_nt2(f32x2{S[i][0][j.value], S[i][1][j.value]}, rs, v1 + (16 * i + j) * row); });
+    asm volatile("" : "+v"(v1));                                   // the loads' addresses are not kept for the stores
+    unroll<4>([&](auto i) {
+        unroll<4>([&](auto j) {
+            buffer_store_nt4(f32x4{S[i][0][j.value], S[i][1][j.value], S[i][2][j.value], S[i][3][j.value]}, rs,
+                             v1 + (16 * i + j) * row, 0);
+        });
     });
     if (L == 0) return;
 
     // --- [K; Q] S: rows 0 .. LT - 1 are K's, LT .. 2 LT - 1 Q's ---
-    f32x4 z[LT / 8][2];
-    unroll<LT / 8>([&](auto m) { z[m][0] = z[m][1] = f32x4{0.f, 0.f, 0.f, 0.f}; });
-    unroll<RT>([&](auto i) {
+    f32x4 z[LT / 8][4];
+    unroll<LT / 8>([&](auto m) { unroll<4>([&](auto c) { z[m][c] = f32x4{0.f, 0.f, 0.f, 0.f}; }); });
+    unroll<4>([&](auto i) {
         unroll<LT / 8>([&](auto m) {
-            const int c = 16 * i + 4 * g4;
-            f32x4 f = ld4(LT == 16 ? (m ? &qq[r16 % LT][c] : &kk[r16 % LT][c]) : (r16 < 8 ? &kk[r16 & 7][c] : &qq[r16 & 7][c]));
-            if (GATE == 2) f *= ld4(&eg[GATE == 2 ? r16 % LT : 0][c]);
-            z[m][0] = mfma_kb1(f, S[i][0], z[m][0]);
-            z[m][1] = mfma_kb1(f, S[i][1], z[m][1]);
+            const int k0 = 64 * half + 16 * i + 4 * g4;
+            f32x4 f = ld4(LT == 16 ? (m ? &qq[r16 % LT][k0] : &kk[r16 % LT][k0]) : (r16 < 8 ? &kk[r16 & 7][k0] : &qq[r16 & 7][k0]));
+            if (GATE == 2) f *= ld4(&eg[GATE == 2 ? r16 % LT : 0][k0]);
+            unroll<4>([&](auto c) { z[m][c] = mfma_kb1(f, S[i][c], z[m][c]); });
         });
     });
-    unroll<LT / 8>([&](auto m) {                                   // read below by this wave alone
-        unroll<4>([&](auto j) {
-            *reinterpret_cast<f32x2 *>(&prod[16 * m + 4 * g4 + j][col]) = f32x2{z[m][0][j.value], z[m][1][j.value]};
+    const bool mine = col - 4 * r16 < dv;                          // a wave with columns
+    auto exchange = [&](auto f) {
+        unroll<LT / 8>([&](auto m) {
+            unroll<4>([&](auto j) {
+                f(*reinterpret_cast<f32x4 *>(&prod[16 * m + 4 * g4 + j][col]), m, j);
+            });
         });
-    });
-    // the block's writes and outputs, a column to a lane (both halves of the wave the same)
-    {
-        const int c = 32 * wave + (lane & 31);
+    };
+    if (HALVES == 2) {
+        if (mine && half == 1)
+            exchange([&](f32x4 &x, auto m, auto j) { x = f32x4{z[m][0][j.value], z[m][1][j.value], z[m][2][j.value], z[m][3][j.value]}; });
+        lds_barrier();
+    }
+    // the block's writes and outputs, a column to a lane
+    if (mine && half == 0) {
+        exchange([&](f32x4 &x, auto m, auto j) {
+            const f32x4 y = {z[m][0][j.value], z[m][1][j.value], z[m][2][j.value], z[m][3][j.value]};
+            x = HALVES == 2 ? x + y : y;
+        });
+        const int c = 64 * (wave / HALVES) + lane;
         float u[LT];                                               // rk_t u_t
         unroll<LT>([&](auto t) {
             u[t] = 0.f;
@@ -396,10 +404,10 @@ draft_block_kernel(const DraftParams p) {
                 }
                 unroll<t>([&](auto j) { s += aa[t][j] * u[j]; });
                 if (p.use_delta) v = betas[t] * (v - k1 * s);
-                if (lane < 32 && c < dv) p.pu[((n * P + t) * H + h) * dv + c] = v;
+                if (c < dv) p.pu[((n * P + t) * H + h) * dv + c] = v;
                 u[t] = k1 * v;
                 unroll<t + 1>([&](auto j) { o += bb[t][j] * u[j]; });
-                if (lane < 32) vv[t][c] = rq[t] * o;
+                vv[t][c] = rq[t] * o;
             }
         });
     }
@@ -431,9 +439,8 @@ draft_block_kernel(const DraftParams p) {
 
 template <typename E, int GATE, int RT, int LT>
 static hipError_t draft_launch(const DraftParams &p, hipStream_t stream) {
-    // a wave per 32 columns, a thread per key channel and per pair of q, k, v channels
-    const int cols = (p.dv + 31) / 32, pairs = (p.dk + p.dv / 2 + 63) / 64, key = RT / 4;
-    const int waves = cols > pairs ? (cols > key ? cols : key) : (pairs > key ? pairs : key);
+    const int tiles = RT / 4 * ((p.dv + 63) / 64), pairs = (p.dk + p.dv / 2 + 63) / 64, least = RT / 2;
+    const int waves = tiles > pairs ? (tiles > least ? tiles : least) : (pairs > least ? pairs : least);
     const dim3 grid((unsigned)(p.N * p.H)), block(64 * waves);
     if (p.dv <= 128) draft_block_kernel<E, GATE, RT, LT, 256><<<grid, block, 0, stream>>>(p);
     else draft_block_kernel<E, GATE, RT, LT, 512><<<grid, block, 0, stream>>>(p);
