@@ -37,6 +37,9 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ float buffer_load1(__amdgpu_buffer_rsrc_t r, uint32_t voff) {
     return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, (int)voff, 0, 0));
 }
+__device__ __forceinline__ f32x2 buffer_load2(__amdgpu_buffer_rsrc_t r, uint32_t voff) {
+    return __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(r, (int)voff, 0, 0));
+}
 __device__ __forceinline__ f32x4 buffer_load4(__amdgpu_buffer_rsrc_t r, uint32_t voff) {
     return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)voff, 0, 0));
 }
@@ -130,14 +133,14 @@ __device__ __forceinline__ float row_prefix16(float x) {
 // q's own diagonals and scale the results.  RT: row tiles (dk <= 16 RT). LT: room of the pending
 // block and tokens (8 or 16).  At least 128 (RT 4) or 256 threads, and a thread per pair of q, k, v channels.
 template <typename E, int GATE, int RT, int LT, int NT>
-__global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(LT == 8 ? 4 : NT == 256 ? 3 : 2)))
+__global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(GATE == 2 && RT == 8 ? (NT == 256 ? 3 : 2) : LT == 8 ? 4 : NT == 256 ? 3 : 2)))
 draft_block_kernel(const DraftParams p) {
     constexpr int DKP = 16 * RT, LDK = DKP + 4, WLD = DKP + 16, DVM = NT / 2, NC = DKP / 64, HALVES = RT / 4, LG = LT / 4;
     __shared__ __attribute__((aligned(16))) float kk[LT][LDK], qq[LT][LDK], vv[LT][DVM], ws[LT][WLD], prod[2 * LT][DVM];
     __shared__ __attribute__((aligned(16))) float es[GATE == 2 ? LT : 1][GATE == 2 ? DKP : 16];  // e^{g_t}
     __shared__ __attribute__((aligned(16))) float eg[GATE == 2 ? LT : 1][GATE == 2 ? LDK : 16];  // e^{G_t}
     __shared__ __attribute__((aligned(16))) float ds[GATE == 2 ? DKP : 16], aa[LT][LT], bb[LT][LT];
-    __shared__ float betas[16], rk[LT], rq[LT];
+    __shared__ float betas[16], rk[LT], rq[LT], squares[NT / 128][LT];
     const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 63, waves = nt >> 6;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), g4 = lane >> 4, r16 = lane & 15;
     const int64_t n = blockIdx.x / p.H;
@@ -156,8 +159,32 @@ draft_block_kernel(const DraftParams p) {
         });
     });
 
-    // --- without the state: the short conv, a thread to two channels ---
+    // --- without the state ---
     a = a < 0 ? 0 : a > P ? P : a;
+    // scalar gate and beta: lane r of every row of 16 has token r's
+    const bool has_g = GATE == 2 || p.pg != nullptr;
+    const uint32_t lane_h = (uint32_t)(r16 * H + h) * 4u;
+    const float be = buffer_load1(buffer_rsrc(p.use_delta ? p.beta + n * L * H : nullptr, p.use_delta ? (uint32_t)(L * H) * 4u : 0u), lane_h);
+    float gp = 0.f, gn = 0.f;
+    f32x2 gv[GATE == 2 ? LG : 1], dt_bias[GATE == 2 ? LG : 1];     // per channel: two channels of some tokens
+    if (GATE == 1) {
+        gp = buffer_load1(buffer_rsrc(p.pg + (has_g ? n * P * H : 0), has_g ? (uint32_t)(P * H) * 4u : 0u), r16 < a ? lane_h : NOWHERE);
+        gn = buffer_load1(buffer_rsrc(reinterpret_cast<const float *>(p.g) + (has_g ? n * L * H : 0), has_g ? (uint32_t)(L * H) * 4u : 0u), lane_h);
+    }
+    if (GATE == 2) {
+        const uint32_t e = p.fz.gate_16 ? 2 : 4;
+        const __amdgpu_buffer_rsrc_t bg = buffer_rsrc(reinterpret_cast<const char *>(p.g) + n * L * H * dk * e, (uint32_t)(L * H * dk) * e);
+        const __amdgpu_buffer_rsrc_t bb_ = buffer_rsrc(p.fz.dt_bias, p.fz.gate_act ? (uint32_t)(H * dk) * 4u : 0u);
+        unroll<LG>([&](auto m) {
+            const int i = tid + m * nt, t = i / (DKP / 2), c = 2 * (i % (DKP / 2));
+            const uint32_t o = t < L && c < dk ? (uint32_t)((t * H + h) * dk + c) * e : NOWHERE;
+            f32x2 &g = gv[GATE == 2 ? m : 0];
+            if (p.fz.gate_16) g[0] = buffer_load1(bg, o);          // both halves
+            else g = buffer_load2(bg, o);
+            dt_bias[GATE == 2 ? m : 0] = buffer_load2(bb_, c < dk ? (uint32_t)(h * dk + c) * 4u : NOWHERE);
+        });
+    }
+    // the short conv, a thread to two channels
     {
         const ChannelPair<E> at(p, n, h, tid < pairs ? tid : pairs - 1);
         float *to = at.which == 0 ? &qq[0][at.c] : at.which == 1 ? &kk[0][at.c] : &vv[0][at.c];
@@ -206,31 +233,6 @@ draft_block_kernel(const DraftParams p) {
                 }
         }
     }
-    // scalar gate and beta: lane r of every row of 16 has token r's
-    const bool has_g = GATE == 2 || p.pg != nullptr;
-    float gp = 0.f, gn = 0.f, be = 0.f;
-    f32x2 gv[GATE == 2 ? LG : 1];                                  // per channel: two channels of some tokens
-    if (GATE == 1 && has_g) {
-        if (r16 < a) gp = p.pg[(n * P + r16) * H + h];
-        if (r16 < L) gn = reinterpret_cast<const float *>(p.g)[(n * L + r16) * H + h];
-    }
-    if (p.use_delta && r16 < L) be = p.beta[(n * L + r16) * H + h];
-    if (GATE == 2) {
-        unroll<LG>([&](auto m) {
-            const int i = tid + m * nt, t = i / (DKP / 2), c = 2 * (i % (DKP / 2));
-            f32x2 &g = gv[GATE == 2 ? m : 0];
-            g = f32x2{0.f, 0.f};
-            if (t < L && c < dk) {
-                const int64_t o = ((n * L + t) * H + h) * dk + c;
-                if (p.fz.gate_16) {
-                    const Pair<E> e = *reinterpret_cast<const Pair<E> *>(reinterpret_cast<const E *>(p.g) + o);
-                    g = f32x2{(float)e[0], (float)e[1]};
-                } else {
-                    g = *reinterpret_cast<const f32x2 *>(reinterpret_cast<const float *>(p.g) + o);
-                }
-            }
-        });
-    }
     // the pending keys (and per-channel decays), a channel to a thread, and writes, as the commit's B
     // operand: token 4 s + g, this lane's columns
     float pk[LT], pg[GATE == 2 ? LT : 1];
@@ -251,14 +253,18 @@ draft_block_kernel(const DraftParams p) {
         });
     }
     if (GATE == 2) {
+        const float al = p.fz.gate_act ? p.fz.A_log[h] : 0.f;
         unroll<LG>([&](auto m) {
             const int i = tid + m * nt, t = i / (DKP / 2), c = 2 * (i % (DKP / 2));
-            f32x2 &g = gv[GATE == 2 ? m : 0];
+            f32x2 &g = gv[GATE == 2 ? m : 0], &b = dt_bias[GATE == 2 ? m : 0];
+            if constexpr (sizeof(E) == 2)
+                if (p.fz.gate_16) {
+                    const Pair<E> x = __builtin_bit_cast(Pair<E>, g[0]);
+                    g = f32x2{(float)x[0], (float)x[1]};
+                }
             if (p.fz.gate_act) {
-                const int cc = c < dk ? h * dk + c : 0;
-                const float al = p.fz.A_log[h];
-                g[0] = gate_activation(g[0], al, p.fz.dt_bias[cc], p.fz.lb_set, p.fz.lb);
-                g[1] = gate_activation(g[1], al, p.fz.dt_bias[cc + 1], p.fz.lb_set, p.fz.lb);
+                g[0] = gate_activation(g[0], al, b[0], p.fz.lb_set, p.fz.lb);
+                g[1] = gate_activation(g[1], al, b[1], p.fz.lb_set, p.fz.lb);
             }
             if (t < LT) *reinterpret_cast<f32x2 *>(&es[GATE == 2 ? t : 0][c]) = f32x2{__expf(g[0]), __expf(g[1])};
         });
@@ -351,6 +357,7 @@ draft_block_kernel(const DraftParams p) {
             unroll<4>([&](auto c) { S[i][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(w, pu[s][c.value], S[i][c], 0, 0, 0); });
         });
     });
+    if (L == 0) {
     uint32_t v1 = v0;
     asm volatile("" : "+v"(v1));                                   // the loads' addresses are not kept for the stores
     unroll<4>([&](auto i) {
@@ -359,7 +366,27 @@ draft_block_kernel(const DraftParams p) {
                              v1 + (16 * i + j) * row, 0);
         });
     });
-    if (L == 0) return;
+        return;
+    }
+
+    // the output gate's rows and gamma, for the end
+    const int half_dv = dv / 2;
+    Pair<E> ogate[LG];
+    f32x2 gamma[LG];
+    unroll<LG>([&](auto m) {
+        const int i = tid + m * nt, t = i / half_dv, c = 2 * (i - t * half_dv);
+        ogate[m] = Pair<E>{(E)0.f, (E)0.f};
+        gamma[m] = f32x2{0.f, 0.f};
+        if (p.ep.gate && t < L) {
+            ogate[m] = *reinterpret_cast<const Pair<E> *>(reinterpret_cast<const E *>(p.ep.gate) + (n * L + t) * p.ld_v + h * dv + c);
+            if (p.ep.gamma_f32) {
+                gamma[m] = reinterpret_cast<const f32x2 *>(p.ep.gamma)[c / 2];
+            } else {
+                const Pair<E> y = reinterpret_cast<const Pair<E> *>(p.ep.gamma)[c / 2];
+                gamma[m] = f32x2{(float)y[0], (float)y[1]};
+            }
+        }
+    });
 
     // --- [K; Q] S: rows 0 .. LT - 1 are K's, LT .. 2 LT - 1 Q's ---
     f32x4 z[LT / 8][4];
@@ -370,6 +397,14 @@ draft_block_kernel(const DraftParams p) {
             f32x4 f = ld4(LT == 16 ? (m ? &qq[r16 % LT][k0] : &kk[r16 % LT][k0]) : (r16 < 8 ? &kk[r16 & 7][k0] : &qq[r16 & 7][k0]));
             if (GATE == 2) f *= ld4(&eg[GATE == 2 ? r16 % LT : 0][k0]);
             unroll<4>([&](auto c) { z[m][c] = mfma_kb1(f, S[i][c], z[m][c]); });
+        });
+    });
+    uint32_t v1 = v0;
+    asm volatile("" : "+v"(v1));                                   // the loads' addresses are not kept for the stores
+    unroll<4>([&](auto i) {
+        unroll<4>([&](auto j) {
+            buffer_store_nt4(f32x4{S[i][0][j.value], S[i][1][j.value], S[i][2][j.value], S[i][3][j.value]}, rs,
+                             v1 + (16 * i + j) * row, 0);
         });
     });
     const bool mine = col - 4 * r16 < dv;                          // a wave with columns
@@ -407,40 +442,41 @@ draft_block_kernel(const DraftParams p) {
                 if (c < dv) p.pu[((n * P + t) * H + h) * dv + c] = v;
                 u[t] = k1 * v;
                 unroll<t + 1>([&](auto j) { o += bb[t][j] * u[j]; });
-                vv[t][c] = rq[t] * o;
+                o *= rq[t];
+                vv[t][c] = o;
+                if (p.ep.gate) {
+                    const float q = wave_sum64(c < dv ? o * o : 0.f);
+                    if (lane == 0) squares[wave / HALVES][t] = q;
+                }
             }
         });
     }
     lds_barrier();
-    // --- the outputs, a wave per token ---
-    for (int t = wave; t < L; t += waves) {
-        E *out = reinterpret_cast<E *>(p.o) + ((n * L + t) * H + h) * dv;
-        const E *gate = reinterpret_cast<const E *>(p.ep.gate) + (n * L + t) * p.ld_v + h * dv;
-        float r = 1.f;
-        if (p.ep.gate) {
-            float s = 0.f;
-            for (int c = lane; c < dv; c += 64) s += vv[t][c] * vv[t][c];
-            r = rsqrtf(wave_sum64(s) / (float)dv + p.ep.eps);
-        }
-        for (int c = 2 * lane; c < dv; c += 128) {
+    // --- the outputs, a thread to two columns of up to LG tokens ---
+    unroll<LG>([&](auto m) {
+        const int i = tid + m * nt, t = i / half_dv, c = 2 * (i - t * half_dv);
+        if (t < L) {
             f32x2 y = *reinterpret_cast<const f32x2 *>(&vv[t][c]);
             if (p.ep.gate) {
-                const Pair<E> b = *reinterpret_cast<const Pair<E> *>(gate + c);
-                f32x2 gm;
-                if (p.ep.gamma_f32) gm = reinterpret_cast<const f32x2 *>(p.ep.gamma)[c / 2];
-                else gm = f32x2{(float)reinterpret_cast<const E *>(p.ep.gamma)[c], (float)reinterpret_cast<const E *>(p.ep.gamma)[c + 1]};
-                y[0] *= r * gm[0] * ((float)b[0] * sigmoidf_((float)b[0]));
-                y[1] *= r * gm[1] * ((float)b[1] * sigmoidf_((float)b[1]));
+                float s = squares[0][t];
+                for (int b = 1; 64 * b < dv; ++b) s += squares[b][t];
+                const float r = rsqrtf(s / (float)dv + p.ep.eps);
+                y[0] *= r * gamma[m][0] * ((float)ogate[m][0] * sigmoidf_((float)ogate[m][0]));
+                y[1] *= r * gamma[m][1] * ((float)ogate[m][1] * sigmoidf_((float)ogate[m][1]));
             }
-            *reinterpret_cast<Pair<E> *>(out + c) = Pair<E>{(E)y[0], (E)y[1]};
+            *reinterpret_cast<Pair<E> *>(reinterpret_cast<E *>(p.o) + ((n * L + t) * H + h) * dv + c) = Pair<E>{(E)y[0], (E)y[1]};
         }
-    }
+    });
 }
 
 template <typename E, int GATE, int RT, int LT>
 static hipError_t draft_launch(const DraftParams &p, hipStream_t stream) {
-    const int tiles = RT / 4 * ((p.dv + 63) / 64), pairs = (p.dk + p.dv / 2 + 63) / 64, least = RT / 2;
-    const int waves = tiles > pairs ? (tiles > least ? tiles : least) : (pairs > least ? pairs : least);
+    // a wave per 64 x 64 of the state, a thread per pair of q, k, v channels and per two key or value channels of
+    // LT / 4 tokens
+    const int tiles = RT / 4 * ((p.dv + 63) / 64), pairs = (p.dk + p.dv / 2 + 63) / 64, least = (p.dv + 31) / 32;
+    int waves = tiles > pairs ? tiles : pairs;
+    waves = waves > least ? waves : least;
+    waves = waves > RT / 2 ? waves : RT / 2;
     const dim3 grid((unsigned)(p.N * p.H)), block(64 * waves);
     if (p.dv <= 128) draft_block_kernel<E, GATE, RT, LT, 256><<<grid, block, 0, stream>>>(p);
     else draft_block_kernel<E, GATE, RT, LT, 512><<<grid, block, 0, stream>>>(p);

@@ -1701,29 +1701,46 @@ class DraftBlock:
 def _token_rows(t, width: int):
     """The distance in elements from one token of t (N, L, width) or (N, L, H, d) to the
     next, over all streams, where a kernel may read its rows in place; else None."""
-    e = t.element_size()
-    if t.dim() == 4 and t.shape[2] > 1 and t.stride(2) != t.shape[3]:
+    st, sh = t.stride(), t.shape
+    if st[-1] != 1 or t.data_ptr() % 16 or (len(sh) == 4 and sh[2] > 1 and st[2] != sh[3]):
         return None
-    if t.stride(-1) != 1 or t.data_ptr() % 16:
-        return None
-    N, L = t.shape[0], t.shape[1]
-    ld = t.stride(1) if L > 1 else t.stride(0) if N > 1 else width
-    if ld < width or ld % 8 or (N > 1 and t.stride(0) != L * ld):
+    N, L = sh[0], sh[1]
+    ld = st[1] if L > 1 else st[0] if N > 1 else width
+    if ld < width or ld % 8 or (N > 1 and st[0] != L * ld):
         return None
     return ld
 
 
-def _in_place(name, t, shape, dtype, device):
-    assert t.shape == shape and t.dtype == dtype and t.device == device and t.is_contiguous() and t.data_ptr() % 16 == 0, \
-        f'{name} is read and written in place: {tuple(shape)}, {dtype}, contiguous, aligned, on {device}; got ' \
-        f'{tuple(t.shape)}, {t.dtype}, {t.device}'
+def _in_place(name, t, shape, dtype, index):
+    """t as a kernel reads and writes it where it lies: its address."""
+    p = t.data_ptr()
+    if not (t.shape == shape and t.dtype is dtype and t.get_device() == index and t.is_contiguous() and p % 16 == 0):
+        raise AssertionError(f'{name} is read and written in place: {tuple(shape)}, {dtype}, contiguous, aligned, on GPU '
+                             f'{index}; got {tuple(t.shape)}, {t.dtype}, {t.device}')
+    return p
 
 
-def _stream_counts(name, t, N, device):
+def _stream_counts(name, t, N, index):
     """int32 (N,) counts of the streams for a kernel."""
-    assert t.shape == (N,) and t.device == device and not t.is_floating_point() and t.dtype != torch.bool, \
-        f'{name} must be ({N},) whole numbers on {device}; got {tuple(t.shape)}, {t.dtype}, {t.device}'
-    return t.to(torch.int32).contiguous()
+    assert t.shape == (N,) and t.get_device() == index and not t.is_floating_point() and t.dtype is not torch.bool, \
+        f'{name} must be ({N},) whole numbers on GPU {index}; got {tuple(t.shape)}, {t.dtype}, {t.device}'
+    return t if t.dtype is torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+
+
+def _launch(index, fn, *args):
+    """fn(*args, stream) on GPU `index`'s current stream, with that GPU current."""
+    if index == torch.cuda.current_device():
+        _lib.check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
+    else:
+        with torch.cuda.device(index):
+            _lib.check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
+
+
+def _all_on(index, *ts):
+    for t in ts:
+        if t is not None and t.get_device() != index:
+            _check_device(t)
+            raise AssertionError(f'every tensor must be on GPU {index}; got {t.device}')
 
 
 def hip_draft_step(qp, kp, vp, g, beta, state, pending, accepted, *, scale: float, delta: bool = True,
@@ -1749,48 +1766,57 @@ def hip_draft_step(qp, kp, vp, g, beta, state, pending, accepted, *, scale: floa
     q's type.  Between the inputs and the outputs everything is fp32; hip_decode_step
     rounds the conv's, the SiLU's, the norm's and the recurrence's results to q's type.
     dk a multiple of 8 up to 128, dv a multiple of 8 up to 256.  No autograd."""
-    _check_device(qp, kp, vp, g, beta, state, accepted, out_gate, out_norm_weight, A_log, dt_bias)
-    _check_grad(qp, kp, vp, g, beta, state, out_gate, out_norm_weight, A_log, dt_bias, *(conv_weights or ()))
-    dev, dt = qp.device, qp.dtype
-    if dt not in _DTYPES or kp.dtype != dt or vp.dtype != dt:
+    index, dt = qp.get_device(), qp.dtype
+    if index < 0:
+        _check_device(qp)
+    _all_on(index, kp, vp, g, beta, state, accepted, out_gate, out_norm_weight, A_log, dt_bias, *(conv_weights or ()))
+    if torch.is_grad_enabled():
+        _check_grad(qp, kp, vp, g, beta, state, out_gate, out_norm_weight, A_log, dt_bias, *(conv_weights or ()))
+    if dt not in _DTYPES or kp.dtype is not dt or vp.dtype is not dt:
         raise NotImplementedError(f'q, k, v must share one of {list(_DTYPES)}; got {dt}, {kp.dtype}, {vp.dtype}')
     assert state.dim() == 4, f'state must be (N, H, dk, dv); got {tuple(state.shape)}'
     N, H, dk, dv = state.shape
     L, P = qp.shape[1], pending.capacity
     for name, t, d in (('q', qp, dk), ('k', kp, dk), ('v', vp, dv)):
-        assert t.shape in ((N, L, H * d), (N, L, H, d)) and t.device == dev, \
-            f'{name} must be {(N, L, H * d)} or {(N, L, H, d)} on {dev}; got {tuple(t.shape)}, {t.device}'
+        assert t.shape == (N, L, H * d) or t.shape == (N, L, H, d), \
+            f'{name} must be {(N, L, H * d)} or {(N, L, H, d)}; got {tuple(t.shape)}'
     assert 1 <= L <= P, f'a block of 1 to {P} tokens (the pending block\'s room); got {L}'
     gate = _gate_of(g)
-    assert g is None or g.shape == (N, L, H) + (() if gate == 'scalar' else (dk,)), \
+    assert g is None or g.shape == ((N, L, H) if gate == 'scalar' else (N, L, H, dk)), \
         f'g must be {(N, L, H)} or {(N, L, H, dk)}; got {tuple(g.shape)}'
     if delta:
         assert beta is not None and beta.shape == (N, L, H), f'the delta rule needs beta {(N, L, H)}'
     assert not gate_in_kernel or gate == 'vector', 'the fused gate activation is a KDA (vector-gate) kernel'
     assert delta or not beta_logits, 'there is no beta to activate without the delta rule'
-    fz = _Fusion(l2norm=l2norm, beta=beta_logits, gate=gate_in_kernel, A_log=A_log, dt_bias=dt_bias,
-                 lower_bound=lower_bound if gate_in_kernel else None)
-    ep = None
-    if out_gate is not None or out_norm_weight is not None:
-        assert out_gate is not None and out_gate.shape in ((N, L, H * dv), (N, L, H, dv)), \
-            f'the output gate must be {(N, L, H * dv)} or {(N, L, H, dv)}'
-        ep = _Epilogue(out_gate.reshape(N, L, H, dv), out_norm_weight, out_norm_eps)
-        if out_gate.dtype != dt:
+    fusion = None
+    if l2norm or beta_logits or gate_in_kernel:
+        fusion = _Fusion(l2norm=l2norm, beta=beta_logits, gate=gate_in_kernel, A_log=A_log, dt_bias=dt_bias,
+                         lower_bound=lower_bound if gate_in_kernel else None)
+    epilogue = out_gate is not None or out_norm_weight is not None
+    if epilogue:
+        assert out_gate is not None and out_norm_weight is not None, 'the output epilogue needs the gate and the norm weight'
+        assert out_gate.shape == (N, L, H * dv) or out_gate.shape == (N, L, H, dv), \
+            f'the output gate must be {(N, L, H * dv)} or {(N, L, H, dv)}; got {tuple(out_gate.shape)}'
+        assert out_norm_weight.shape == (dv,), f'the norm weight must be ({dv},); got {tuple(out_norm_weight.shape)}'
+        assert out_norm_eps > 0, 'the RMSNorm eps must be positive'
+        if out_gate.dtype is not dt:
             raise NotImplementedError(f'the epilogue gate must have o\'s dtype {dt}; got {out_gate.dtype}')
     # rows in place: q and k one stride apart, v and the gate one
-    lds = [_token_rows(t, w) for t, w in ((qp, H * dk), (kp, H * dk), (vp, H * dv))]
-    ld_gate = lds[2] if ep is None else _token_rows(out_gate, H * dv)
-    ogate = out_gate
-    if None in lds or ld_gate is None or lds[0] != lds[1] or lds[2] != ld_gate:
+    ld_qk, ld_v = _token_rows(qp, H * dk), _token_rows(vp, H * dv)
+    if (ld_qk is None or ld_v is None or _token_rows(kp, H * dk) != ld_qk
+            or (epilogue and _token_rows(out_gate, H * dv) != ld_v)):
         qp, kp, vp = _aligned(qp), _aligned(kp), _aligned(vp)
-        ogate = None if ep is None else _aligned(out_gate)
-        lds = [H * dk, H * dk, H * dv]
-    if g is not None:
-        g = _aligned(g) if gate_in_kernel and g.dtype == dt else _aligned(g.float())
-    beta = beta.float().contiguous() if delta else None
-    o = torch.empty(N, L, H, dv, dtype=dt, device=dev)
-    _draft_call(dt, gate, delta, (qp, kp, vp, g, beta, o), state, pending, accepted, L, lds[0], lds[2], float(scale), fz,
-                conv_weights, conv_cache, ep, ogate)
+        out_gate = _aligned(out_gate)
+        ld_qk, ld_v = H * dk, H * dv
+    if g is not None and (g.dtype is not torch.float32 or not g.is_contiguous() or g.data_ptr() % 16):
+        g = _aligned(g if gate_in_kernel and g.dtype is dt else g.float())
+    if not delta:
+        beta = None
+    elif beta.dtype is not torch.float32 or not beta.is_contiguous():
+        beta = beta.float().contiguous()
+    o = torch.empty((N, L, H, dv), dtype=dt, device=qp.device)
+    _draft_call(index, dt, gate, delta, (qp, kp, vp, g, beta, o), state, pending, accepted, L, ld_qk, ld_v, float(scale), fusion,
+                conv_weights, conv_cache, out_gate if epilogue else None, out_norm_weight, out_norm_eps)
     return o
 
 
@@ -1798,19 +1824,24 @@ def commit_drafts(state, pending, accepted, *, conv_weights=None, conv_cache=Non
     """hip_draft_step's first half alone: the accepted (N,) tokens of `pending` that stand
     move into state and conv_cache, in place (the end of speculative decoding, or an
     export).  Nothing of `pending` stands behind it: the next call's accepted is 0."""
-    _check_device(state, accepted)
+    index = state.get_device()
+    if index < 0:
+        _check_device(state)
+    _all_on(index, accepted)
     _check_grad(state)
     gate = 'none' if pending.g is None else 'scalar' if pending.g.dim() == 3 else 'vector'
     dt = conv_cache[0].dtype if conv_cache is not None else torch.float32
     if dt not in _DTYPES:
         raise NotImplementedError(f'the conv caches must be one of {list(_DTYPES)}; got {dt}')
-    _draft_call(dt, gate, False, (None,) * 6, state, pending, accepted, 0, 0, 0, 1.0, _NO_FUSION, conv_weights, conv_cache,
-                None, None)
+    _draft_call(index, dt, gate, False, (None,) * 6, state, pending, accepted, 0, 0, 0, 1.0, None, conv_weights, conv_cache,
+                None, None, 1.0)
 
 
-def _draft_call(dt, gate, delta, operands, state, pending, accepted, L, ld_qk, ld_v, scale, fz, conv_weights, conv_cache,
-                ep, ogate):
-    dev = state.device
+_GATE_KINDS = {'none': _lib.VGDR_GATE_NONE, 'scalar': _lib.VGDR_GATE_SCALAR, 'vector': _lib.VGDR_GATE_VECTOR}
+
+
+def _draft_call(index, dt, gate, delta, operands, state, pending, accepted, L, ld_qk, ld_v, scale, fusion, conv_weights,
+                conv_cache, out_gate, gamma, eps):
     N, H, dk, dv = state.shape
     P = pending.capacity
     if dk % 8 or dk > 128 or dv % 8 or dv > 256:
@@ -1818,56 +1849,51 @@ def _draft_call(dt, gate, delta, operands, state, pending, accepted, L, ld_qk, l
     if not 1 <= P <= MAX_DRAFT_BLOCK:
         raise NotImplementedError(f'a drafted block holds 1 to {MAX_DRAFT_BLOCK} tokens; got room for {P}')
     f32 = torch.float32
-    _in_place('state', state, (N, H, dk, dv), f32, dev)
-    _in_place('pending.k', pending.k, (N, P, H, dk), f32, dev)
-    _in_place('pending.u', pending.u, (N, P, H, dv), f32, dev)
+    S = _in_place('state', state, (N, H, dk, dv), f32, index)
+    blk = _lib.DraftBlock(k=_in_place('pending.k', pending.k, (N, P, H, dk), f32, index),
+                          u=_in_place('pending.u', pending.u, (N, P, H, dv), f32, index), capacity=P)
     assert (pending.g is None) == (gate == 'none'), f'the pending block was made for another gate than {gate!r}'
     if pending.g is not None:
-        _in_place('pending.g', pending.g, (N, P, H) if gate == 'scalar' else (N, P, H, dk), f32, dev)
+        blk.g = _in_place('pending.g', pending.g, (N, P, H) if gate == 'scalar' else (N, P, H, dk), f32, index)
     assert (conv_weights is None) == (conv_cache is None) == (pending.x is None), \
         'a conv needs its weights, its caches and a pending block with its inputs'
-    sc, keep = None, []
+    conv = keep = None
     if conv_cache is not None:
-        conv = _ShortConv(conv_weights, conv_cache)
-        widths = (H * dk, H * dk, H * dv)
-        for n, w, c, x, d in zip('qkv', conv.weights, conv_cache, pending.x, widths):
-            assert w.shape == (d, conv.K) and w.device == dev, \
-                f'conv weight must be ({d}, {conv.K}) or ({d}, 1, {conv.K}) on {dev}; got {tuple(w.shape)}'
-            _in_place(f'conv cache {n}', c, (N, conv.K, d), dt, dev)
-            _in_place(f'pending.x {n}', x, (N, P, d), dt, dev)
-        wdt = f32 if all(w.dtype == f32 for w in conv.weights) else dt
-        keep += [w.to(wdt).contiguous() for w in conv.weights]
-        sc = _lib.ShortConv(weight_q=_ptr(keep[0]), weight_k=_ptr(keep[1]), weight_v=_ptr(keep[2]),
-                            cache_q=_ptr(conv_cache[0]), cache_k=_ptr(conv_cache[1]), cache_v=_ptr(conv_cache[2]),
-                            kernel_size=conv.K, weight_dtype=_DTYPES[wdt])
+        assert len(conv_weights) == len(conv_cache) == len(pending.x) == 3, 'the short conv is that of q, k and v'
+        K = conv_weights[0].shape[-1]
+        wdt = f32 if all(w.dtype is f32 for w in conv_weights) else dt
+        conv = _lib.ShortConv(kernel_size=K, weight_dtype=_DTYPES[wdt])
+        keep, at, xs = [], [], []
+        for name, w, c, x, d in zip('qkv', conv_weights, conv_cache, pending.x, (H * dk, H * dk, H * dv)):
+            assert w.shape == (d, 1, K) or w.shape == (d, K), f'conv weight must be ({d}, {K}) or ({d}, 1, {K}); got {tuple(w.shape)}'
+            at.append(_in_place(f'conv cache {name}', c, (N, K, d), dt, index))
+            xs.append(_in_place(f'pending.x {name}', x, (N, P, d), dt, index))
+            keep.append(w if w.dtype is wdt and w.is_contiguous() else w.to(wdt).contiguous())
+        _all_on(index, *keep)
+        conv.weight_q, conv.weight_k, conv.weight_v = (w.data_ptr() for w in keep)
+        conv.cache_q, conv.cache_k, conv.cache_v = at
+        blk.x_q, blk.x_k, blk.x_v = xs
     q, k, v, g, beta, o = operands
-    for t in (g, beta, ogate, *(fz.A_log, fz.dt_bias), *((ep.gamma,) if ep is not None else ())):
-        assert t is None or t.device == dev, f'every tensor must be on {dev}; got {t.device}'
-    fzs = None
-    if fz.any:
-        fzs = _lib.Fusion(int(fz.l2norm), int(fz.beta), int(fz.gate), _lib.VGDR_F32, None, None, 0, 0.0)
-        if fz.gate:
-            assert fz.A_log.numel() == H and fz.dt_bias.numel() == H * dk, f'A_log has {H} and dt_bias {H * dk} elements'
-            params = [t.detach().float().contiguous() for t in (fz.A_log, fz.dt_bias)]
-            keep += params
-            fzs.A_log, fzs.dt_bias, fzs.gate_dtype = _ptr(params[0]), _ptr(params[1]), _DTYPES[g.dtype]
-            if fz.lower_bound is not None:
-                fzs.lower_bound_set, fzs.lower_bound = 1, float(fz.lower_bound)
-    eps = None
-    if ep is not None:
-        gamma = ep.gamma if ep.gamma.dtype in (f32, dt) else ep.gamma.float()
-        gamma = gamma.contiguous()
-        keep.append(gamma)
-        eps = _lib.Epilogue(gate=_ptr(ogate), gamma=_ptr(gamma), gamma_dtype=_DTYPES[gamma.dtype], eps=ep.eps)
-    acc = _stream_counts('accepted', accepted, N, dev)
-    xs = pending.x or (None,) * 3
-    blk = _lib.DraftBlock(_ptr(pending.k), _ptr(pending.u), _ptr(pending.g), _ptr(xs[0]), _ptr(xs[1]), _ptr(xs[2]), P)
-    kind = {'none': _lib.VGDR_GATE_NONE, 'scalar': _lib.VGDR_GATE_SCALAR, 'vector': _lib.VGDR_GATE_VECTOR}[gate]
-    ref = lambda s: None if s is None else ctypes.byref(s)  # noqa: E731
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().vgdr_draft_step(
-            _DTYPES[dt], kind, int(delta), _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _ptr(o), _ptr(state), ref(blk),
-            _ptr(acc), N, L, H, dk, dv, ld_qk, ld_v, scale, ref(fzs), ref(sc), ref(eps), _stream(dev)))
+    fz = None
+    if fusion is not None:
+        fz = _lib.Fusion(int(fusion.l2norm), int(fusion.beta), int(fusion.gate), _lib.VGDR_F32, None, None, 0, 0.0)
+        if fusion.gate:
+            assert fusion.A_log.numel() == H and fusion.dt_bias.numel() == H * dk, f'A_log has {H} and dt_bias {H * dk} elements'
+            params = [t if t.dtype is f32 and t.is_contiguous() else t.detach().float().contiguous()
+                      for t in (fusion.A_log, fusion.dt_bias)]
+            fz.A_log, fz.dt_bias, fz.gate_dtype = params[0].data_ptr(), params[1].data_ptr(), _DTYPES[g.dtype]
+            if fusion.lower_bound is not None:
+                fz.lower_bound_set, fz.lower_bound = 1, float(fusion.lower_bound)
+    ep = None
+    if out_gate is not None:
+        if gamma.dtype not in (f32, dt) or not gamma.is_contiguous() or gamma.data_ptr() % 16:
+            gamma = _aligned(gamma if gamma.dtype in (f32, dt) else gamma.float())
+        ep = _lib.Epilogue(gate=out_gate.data_ptr(), gamma=gamma.data_ptr(), gamma_dtype=_DTYPES[gamma.dtype], eps=float(eps))
+    acc = _stream_counts('accepted', accepted, N, index)
+    ref = ctypes.byref
+    _launch(index, _lib.load().vgdr_draft_step, _DTYPES[dt], _GATE_KINDS[gate], int(delta), _ptr(q), _ptr(k), _ptr(v), _ptr(g),
+            _ptr(beta), _ptr(o), S, ref(blk), acc.data_ptr(), N, L, H, dk, dv, ld_qk, ld_v, scale, None if fz is None else ref(fz),
+            None if conv is None else ref(conv), None if ep is None else ref(ep))
 
 
 def verify_drafts(logits, drafts, uniforms, *, temperature=1.0, draft_probs=None, n_drafts=None):
@@ -1892,52 +1918,50 @@ def verify_drafts(logits, drafts, uniforms, *, temperature=1.0, draft_probs=None
     outside the vocabulary never stands, and where q covers all of p the token is drawn from p.
     Returns (tokens (N, K + 1) int64: the drafts that stand, the token, then -1; accepted (N,) int32).
     No autograd: logits that require grad are refused."""
-    _check_device(logits, drafts, uniforms, draft_probs, n_drafts)
+    index = logits.get_device()
+    if index < 0:
+        _check_device(logits)
+    tensor_T = isinstance(temperature, torch.Tensor)
+    _all_on(index, drafts, uniforms, draft_probs, n_drafts, temperature if tensor_T else None)
     _check_grad(logits, draft_probs)
     assert logits.dim() == 3 and logits.shape[1] >= 1 and logits.shape[2] >= 1, \
         f'logits must be (N, K + 1, V); got {tuple(logits.shape)}'
     N, L, V = logits.shape
-    K, dev = L - 1, logits.device
+    K = L - 1
     if logits.dtype not in _DTYPES:
         raise NotImplementedError(f'logits must be one of {list(_DTYPES)}; got {logits.dtype}')
     if K > 64:
         raise NotImplementedError(f'{K} drafts (at most 64)')
-    assert drafts.shape == (N, K) and not drafts.is_floating_point() and drafts.dtype != torch.bool, \
+    assert drafts.shape == (N, K) and not drafts.is_floating_point() and drafts.dtype is not torch.bool, \
         f'drafts must be {(N, K)} whole numbers; got {tuple(drafts.shape)}, {drafts.dtype}'
-    assert uniforms.shape == (N, L) and uniforms.dtype == torch.float32, \
+    assert uniforms.shape == (N, L) and uniforms.dtype is torch.float32, \
         f'uniforms must be {(N, L)} in fp32; got {tuple(uniforms.shape)}, {uniforms.dtype}'
-    x = logits if logits.stride(2) == 1 and logits.stride(1) >= V and logits.stride(0) >= 0 else logits.contiguous()
-    if isinstance(temperature, torch.Tensor):
+    rows = lambda t: t if t.stride(2) == 1 and t.stride(1) >= V and t.stride(0) >= 0 else t.contiguous()  # noqa: E731
+    x = rows(logits)
+    if tensor_T:
         assert temperature.shape == (N,) and temperature.is_floating_point(), \
             f'temperature must be a number or ({N},); got {tuple(temperature.shape)}, {temperature.dtype}'
-        _check_device(temperature)
         T = temperature.float().contiguous()
     else:
         assert temperature >= 0, f'temperature must not be negative; got {temperature}'
-        T = torch.full((N,), float(temperature), device=dev)
+        T = torch.full((N,), float(temperature), device=logits.device)
     q = None
     if draft_probs is not None:
         assert draft_probs.shape == (N, K, V), f'draft_probs must be {(N, K, V)}; got {tuple(draft_probs.shape)}'
         if draft_probs.dtype not in _DTYPES:
             raise NotImplementedError(f'draft_probs must be one of {list(_DTYPES)}; got {draft_probs.dtype}')
-        q = draft_probs
-        if K and not (q.stride(2) == 1 and q.stride(1) >= V and q.stride(0) >= 0):
-            q = q.contiguous()
-    nd = None if n_drafts is None else _stream_counts('n_drafts', n_drafts, N, dev)
-    d, u = drafts.to(torch.int64).contiguous(), uniforms.contiguous()
-    for t in (d, u, T, q):
-        assert t is None or t.device == dev, f'every tensor must be on {dev}; got {t.device}'
-    tokens = torch.empty(N, L, dtype=torch.int64, device=dev)
-    accepted = torch.empty(N, dtype=torch.int32, device=dev)
+        q = rows(draft_probs) if K else None
+    nd = None if n_drafts is None else _stream_counts('n_drafts', n_drafts, N, index)
+    d = drafts if drafts.dtype is torch.int64 and drafts.is_contiguous() else drafts.to(torch.int64).contiguous()
+    u = uniforms.contiguous()
+    tokens = torch.empty((N, L), dtype=torch.int64, device=logits.device)
+    accepted = torch.empty((N,), dtype=torch.int32, device=logits.device)
     lib = _lib.load()
     nbytes = lib.vgdr_verify_drafts_workspace_size(N, K, V)
-    ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        _lib.check(lib.vgdr_verify_drafts(
-            _DTYPES[x.dtype], _ptr(x), x.stride(0), max(x.stride(1), V) if L == 1 else x.stride(1), _ptr(d), _ptr(u), _ptr(T),
-            _ptr(q), 0 if q is None else _DTYPES[q.dtype], 0 if q is None else q.stride(0),
-            0 if q is None else max(q.stride(1), V), _ptr(nd), _ptr(tokens), _ptr(accepted), _ptr(ws), nbytes, N, K, V,
-            _stream(dev)))
+    ws = torch.empty((max(nbytes, 1),), dtype=torch.uint8, device=logits.device)
+    _launch(index, lib.vgdr_verify_drafts, _DTYPES[x.dtype], x.data_ptr(), x.stride(0), max(x.stride(1), V) if L == 1 else x.stride(1),
+            d.data_ptr(), u.data_ptr(), T.data_ptr(), _ptr(q), 0 if q is None else _DTYPES[q.dtype], 0 if q is None else q.stride(0),
+            0 if q is None else max(q.stride(1), V), _ptr(nd), tokens.data_ptr(), accepted.data_ptr(), ws.data_ptr(), nbytes, N, K, V)
     return tokens, accepted
 
 
@@ -1950,22 +1974,23 @@ def lookup_drafts(history, lengths, n, *, max_ngram: int = 3, min_ngram: int = 1
     counted at most), and of those the latest; the drafts are the tokens that followed, read on
     from the first of them again where the text ends.  Returns (drafts (N, n) int64, counts (N,)
     int32: n, or 0 and zeros without such a place)."""
-    _check_device(history, lengths)
+    index = history.get_device()
+    if index < 0:
+        _check_device(history)
+    _all_on(index, lengths)
     assert history.dim() == 2, f'history must be (N, cap); got {tuple(history.shape)}'
     if history.dtype not in (torch.int32, torch.int64):
         raise NotImplementedError(f'history must be int32 or int64; got {history.dtype}')
     assert 1 <= n <= 64, f'1 to 64 drafts; got {n}'
     assert 1 <= min_ngram <= max_ngram <= 16, f'1 <= min_ngram <= max_ngram <= 16; got {min_ngram}, {max_ngram}'
     N, cap = history.shape
-    dev = history.device
     h = history if (history.stride(1) == 1 or cap <= 1) and (history.stride(0) >= cap or N <= 1) else history.contiguous()
-    lens = _stream_counts('lengths', lengths, N, dev)
-    drafts = torch.empty(N, n, dtype=torch.int64, device=dev)
-    counts = torch.empty(N, dtype=torch.int32, device=dev)
+    lens = _stream_counts('lengths', lengths, N, index)
+    drafts = torch.empty((N, n), dtype=torch.int64, device=history.device)
+    counts = torch.empty((N,), dtype=torch.int32, device=history.device)
     lib = _lib.load()
     nbytes = lib.vgdr_lookup_drafts_workspace_size(N, cap)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    with torch.cuda.device(dev):
-        _lib.check(lib.vgdr_lookup_drafts(_ptr(h), h.element_size(), max(h.stride(0), cap), cap, _ptr(lens), _ptr(drafts),
-                                          _ptr(counts), _ptr(ws), nbytes, N, n, max_ngram, min_ngram, _stream(dev)))
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=history.device) if nbytes else None
+    _launch(index, lib.vgdr_lookup_drafts, h.data_ptr(), h.element_size(), max(h.stride(0), cap), cap, lens.data_ptr(),
+            drafts.data_ptr(), counts.data_ptr(), _ptr(ws), nbytes, N, n, max_ngram, min_ngram)
     return drafts, counts
