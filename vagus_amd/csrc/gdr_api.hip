@@ -1434,7 +1434,6 @@ int vgdr_verify_drafts(int dtype, const void *logits, int64_t ld_stream, int64_t
     p.n_drafts = n_drafts;
     p.tokens = tokens;
     p.accepted = accepted;
-    p.rows = reinterpret_cast<vgdr::RowMass *>(workspace);
     p.ld_stream = ld_stream;
     p.ld_row = ld_row;
     p.ld_probs_stream = ld_probs_stream;
@@ -1443,7 +1442,7 @@ int vgdr_verify_drafts(int dtype, const void *logits, int64_t ld_stream, int64_t
     p.K = (int)K;
     p.V = (int)V;
     p.probs_dtype = probs_dtype;
-    return hip_status(vgdr::verify_drafts(dtype, p, stream), "vgdr_verify_drafts launch");
+    return hip_status(vgdr::verify_drafts(dtype, p, workspace, stream), "vgdr_verify_drafts launch");
 }
 
 int64_t vgdr_lookup_drafts_workspace_size(int64_t B, int64_t cap) {

@@ -374,10 +374,14 @@ struct DraftParams {
 hipError_t draft_step(int gate, const DraftParams &p, hipStream_t stream);
 
 // Drafts against the target's logits (gdr_verify.hip), N streams of K drafts.
-struct RowMass {
-    double sum;                   // of e^{(x - top) / T} over the row
+struct RowMass {                  // a chunk of a row
+    float sum;                    // of e^{(x - top) / T}
     float top;
-    int at;                       // the lowest index of the top
+    int at;                       // (greedy) the lowest id that has the top; -1 where the chunk has none of the row
+};
+struct Stood {                    // a stream's drafts that stand, and the top of the row behind them
+    int count;
+    float top;
 };
 struct VerifyParams {
     const void *logits;           // row i of stream n at n ld_stream + i ld_row, V elements
@@ -388,11 +392,15 @@ struct VerifyParams {
     const int32_t *n_drafts;      // [N] or NULL (K)
     int64_t *tokens;              // [N, K + 1]
     int32_t *accepted;            // [N]
-    RowMass *rows;                // verify_workspace bytes
     int64_t ld_stream, ld_row, ld_probs_stream, ld_probs_row, N;
     int K, V, probs_dtype;
+    // set by verify_drafts, in the workspace: [N, K + 1, chunks], [N, 2, blocks] and [N]
+    RowMass *rows;
+    double *sums;
+    Stood *stood;
+    int64_t chunks, blocks;
 };
-hipError_t verify_drafts(int dtype, const VerifyParams &p, hipStream_t stream);
+hipError_t verify_drafts(int dtype, VerifyParams p, void *workspace, hipStream_t stream);
 int64_t verify_workspace(int64_t N, int64_t K, int64_t V);
 
 // Drafts out of the streams' own text (gdr_verify.hip).
