@@ -1447,9 +1447,7 @@ int vgdr_verify_drafts(int dtype, const void *logits, int64_t ld_stream, int64_t
 
 int64_t vgdr_lookup_drafts_workspace_size(int64_t B, int64_t cap) {
     g_err[0] = 0;
-    (void)B;
-    (void)cap;
-    return 0;
+    return B < 0 || B > 0x1000000LL || cap < 0 || cap > 0x7fffffffLL ? 0 : vgdr::lookup_workspace(B, cap);
 }
 
 int vgdr_lookup_drafts(const void *history, int token_bytes, int64_t ld, int64_t cap, const int32_t *lengths,
@@ -1467,8 +1465,9 @@ int vgdr_lookup_drafts(const void *history, int token_bytes, int64_t ld, int64_t
     if (!history || !lengths || !drafts || !counts)
         return fail(VGDR_ERR_INVALID, "%s: history, lengths, drafts and counts are required", fn);
     if (B > 1 && ld < cap) return fail(VGDR_ERR_INVALID, "%s: rows of %lld tokens, %lld apart", fn, (long long)cap, (long long)ld);
-    (void)workspace;
-    (void)workspace_bytes;
+    const int64_t need = vgdr::lookup_workspace(B, cap);
+    if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need))
+        return fail(VGDR_ERR_INVALID, "%s: a 16-byte aligned workspace of %lld bytes is required", fn, (long long)need);
     vgdr::LookupParams p{};
     p.history = history;
     p.lengths = lengths;
@@ -1480,7 +1479,7 @@ int vgdr_lookup_drafts(const void *history, int token_bytes, int64_t ld, int64_t
     p.K = (int)K;
     p.longest = max_ngram;
     p.shortest = min_ngram;
-    return hip_status(vgdr::lookup_drafts(token_bytes == 8, p, stream), "vgdr_lookup_drafts launch");
+    return hip_status(vgdr::lookup_drafts(token_bytes == 8, p, workspace, stream), "vgdr_lookup_drafts launch");
 }
 
 }  // extern "C"

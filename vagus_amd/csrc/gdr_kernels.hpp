@@ -411,8 +411,12 @@ struct LookupParams {
     int32_t *counts;              // [N]
     int64_t ld, cap, N;
     int K, longest, shortest;
+    // set by lookup_drafts: runs of `run` places a text is read in, and (runs > 1) each one's best
+    int64_t runs, run;
+    long long *best;
 };
-hipError_t lookup_drafts(bool wide, const LookupParams &p, hipStream_t stream);
+hipError_t lookup_drafts(bool wide, LookupParams p, void *workspace, hipStream_t stream);
+int64_t lookup_workspace(int64_t N, int64_t cap);
 
 int device_cu_count();
 

@@ -473,38 +473,112 @@ hipError_t verify_drafts(int dtype, VerifyParams p, void *workspace, hipStream_t
     return hipGetLastError();
 }
 
-constexpr int ROW_THREADS = 256;
+namespace {
 
-// Per stream: of all places e < n - 1 of its n tokens at which at least `shortest` of the last
-// tokens end as well, the one where most of them do (up to `longest`), of those the last; the
-// drafts are what follows it, again from there where the text ends.
-template <typename I>
-__global__ void __launch_bounds__(ROW_THREADS) lookup_kernel(const LookupParams p) {
-    __shared__ long long keys[ROW_THREADS];
-    const int tid = threadIdx.x;
-    const int64_t b = blockIdx.x;
-    const I *text = reinterpret_cast<const I *>(p.history) + b * p.ld;
-    int64_t n = p.lengths[b];
-    n = n < 0 ? 0 : n > p.cap ? p.cap : n;
-    long long best = -1;
-    for (int64_t e = tid; e < n - 1; e += ROW_THREADS) {
-        int m = 0;
-        while (m < p.longest && m <= e && text[e - m] == text[n - 1 - m]) ++m;
-        const long long key = ((long long)m << 40) | e;
-        if (m >= p.shortest && key > best) best = key;
+constexpr int LOOK_THREADS = 256, LOOK_EACH = 8;                   // places a thread has in flight
+constexpr int64_t LOOK_RUN = 8192;                                 // places of a workgroup, at the least
+
+__device__ __forceinline__ long long wave_best(long long x) {
+    for (int m = 32; m; m >>= 1) {
+        const long long y = __shfl_xor(x, m);
+        x = y > x ? y : x;
     }
-    keys[tid] = best;
-    __syncthreads();
-    for (int j = 0; j < ROW_THREADS; ++j) best = keys[j] > best ? keys[j] : best;
-    const int64_t start = (best & ((1LL << 40) - 1)) + 1;
-    for (int64_t i = tid; i < p.K; i += ROW_THREADS)
-        p.drafts[b * p.K + i] = best < 0 ? 0 : (int64_t)text[start + i % (n - start)];
-    if (tid == 0) p.counts[b] = best < 0 ? 0 : p.K;
+    return x;
 }
 
-hipError_t lookup_drafts(bool wide, const LookupParams &p, hipStream_t stream) {
-    if (wide) lookup_kernel<int64_t><<<dim3((unsigned)p.N), dim3(ROW_THREADS), 0, stream>>>(p);
-    else lookup_kernel<int32_t><<<dim3((unsigned)p.N), dim3(ROW_THREADS), 0, stream>>>(p);
+// the drafts behind place best % 2^40 (best < 0: none), over the threads of a wave
+template <typename I>
+__device__ __forceinline__ void lookup_finish(const LookupParams &p, int64_t b, const I *text, int64_t n, long long best, int lane) {
+    const int64_t start = (best & ((1LL << 40) - 1)) + 1;
+    if (lane < p.K) p.drafts[b * p.K + lane] = best < 0 ? 0 : (int64_t)text[start + lane % (n - start)];
+    if (lane == 0) p.counts[b] = best < 0 ? 0 : p.K;
+}
+__device__ __forceinline__ int64_t lookup_length(const LookupParams &p, int64_t b) {
+    const int64_t n = p.lengths[b];
+    return n < 0 ? 0 : n > p.cap ? p.cap : n;
+}
+
+}  // namespace
+
+// Per stream: of all places e < n - 1 of its n tokens at which at least `shortest` of the last
+// tokens end as well, the one where most of them do (up to `longest`), of those the last, as the
+// largest 2^40 matches + e; the drafts are what follows it, again from there where the text ends.
+// gridDim.x workgroups read a run of it each; a lone one finishes, else their bests are left
+// for lookup_finish_kernel.  Bound by the text's read; a thread has eight places in flight (one after the
+// other, 64 texts of 131,072: 215 us).
+template <typename I>
+__global__ void __launch_bounds__(LOOK_THREADS) lookup_kernel(const LookupParams p) {
+    __shared__ long long keys[LOOK_THREADS / 64];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int64_t b = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
+    if (b >= p.N) return;
+    const I *text = reinterpret_cast<const I *>(p.history) + b * p.ld;
+    const int64_t n = lookup_length(p, b);
+    const int64_t first = blockIdx.x * p.run, end = first + p.run < n - 1 ? first + p.run : n - 1;
+    long long best = -1;
+    const I last = n > 0 ? text[n - 1] : (I)0;
+    for (int64_t e0 = first; e0 < end; e0 += LOOK_THREADS * LOOK_EACH) {
+        I here[LOOK_EACH];
+        unroll<LOOK_EACH>([&](auto j) {
+            const int64_t e = e0 + j * LOOK_THREADS + tid;
+            here[j] = text[e < end ? e : end - 1];
+        });
+        unroll<LOOK_EACH>([&](auto j) {
+            const int64_t e = e0 + j * LOOK_THREADS + tid;
+            if (here[j] == last && e < end) {
+                int m = 1;
+                while (m < p.longest && m <= e && text[e - m] == text[n - 1 - m]) ++m;
+                const long long key = ((long long)m << 40) | e;
+                if (m >= p.shortest && key > best) best = key;
+            }
+        });
+    }
+    best = wave_best(best);
+    if (lane == 0) keys[tid >> 6] = best;
+    __syncthreads();
+    if (tid >= 64) return;
+    for (int k = 0; k < LOOK_THREADS / 64; ++k) best = keys[k] > best ? keys[k] : best;
+    if (gridDim.x == 1) lookup_finish<I>(p, b, text, n, best, lane);
+    else if (lane == 0) p.best[b * gridDim.x + blockIdx.x] = best;
+}
+
+template <typename I>
+__global__ void __launch_bounds__(64) lookup_finish_kernel(const LookupParams p) {
+    const int lane = threadIdx.x;
+    const int64_t b = blockIdx.x;
+    long long best = -1;
+    for (int64_t k = lane; k < p.runs; k += 64) {
+        const long long key = p.best[b * p.runs + k];
+        best = key > best ? key : best;
+    }
+    best = wave_best(best);
+    lookup_finish<I>(p, b, reinterpret_cast<const I *>(p.history) + b * p.ld, lookup_length(p, b), best, lane);
+}
+
+// Runs a text is read in: one of up to LOOK_RUN places (a second launch costs what they do), and above as many of that
+// size as make 1,024 workgroups.
+static int64_t lookup_runs(int64_t N, int64_t cap) {
+    const int64_t most = (cap + LOOK_RUN - 1) / LOOK_RUN, share = 1024 / (N > 0 ? N : 1);
+    const int64_t runs = most < share ? most : share;
+    return runs > 1 ? runs : 1;
+}
+int64_t lookup_workspace(int64_t N, int64_t cap) {
+    const int64_t runs = lookup_runs(N, cap);
+    return runs > 1 ? N * runs * (int64_t)sizeof(long long) : 0;
+}
+
+template <typename I> static void lookup_typed(const LookupParams &p, hipStream_t stream) {
+    const int64_t ny = p.N < 32768 ? p.N : 32768;
+    lookup_kernel<I><<<dim3((unsigned)p.runs, (unsigned)ny, (unsigned)((p.N + ny - 1) / ny)), dim3(LOOK_THREADS), 0, stream>>>(p);
+    if (p.runs > 1) lookup_finish_kernel<I><<<dim3((unsigned)p.N), dim3(64), 0, stream>>>(p);
+}
+
+hipError_t lookup_drafts(bool wide, LookupParams p, void *workspace, hipStream_t stream) {
+    p.runs = lookup_runs(p.N, p.cap);
+    p.run = (p.cap + p.runs - 1) / p.runs;
+    p.best = reinterpret_cast<long long *>(workspace);
+    if (wide) lookup_typed<int64_t>(p, stream);
+    else lookup_typed<int32_t>(p, stream);
     return hipGetLastError();
 }
 
