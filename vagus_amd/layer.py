@@ -29,6 +29,8 @@ Streaming: a one-token ``decode_step`` is one kernel from the projections to
 the input of W_o (short conv with its cache, L2 norm, beta sigmoid, gate,
 recurrence updating the state in place, epilogue); a longer block runs the
 conv continuing from the cache and the chunked scan from the state.
+``draft_step`` runs a block of drafted tokens for speculative decoding: the state takes
+of it what the next call says stands.
 ``prefill_packed`` pushes ragged sequences, packed with cu_seqlens, into cache
 rows: the continuous batching the reference's Generator cannot do
 (generator.py:19-22).
@@ -556,6 +558,63 @@ class GatedDeltaNet(nn.Module):
             self.state.copy_(S)
         self.cache_len += L
         return self._output(o, x)
+
+    def begin_drafts(self, capacity: int) -> None:
+        """Room for blocks of up to `capacity` drafted tokens a stream (draft_step), none pending.
+        Buffers of the right shape are kept, so a recorded draft_step stays valid."""
+        assert self.state.shape[0] > 0, 'No state allocated. Call reset_cache or load_cache first.'
+        if type(self)._write is not GatedDeltaNet._write:
+            raise NotImplementedError('drafted blocks write beta_t k_t: a layer with a write of its own decodes token by token')
+        caches = self._caches() if self.short_conv_size is not None else None
+        d = getattr(self, '_drafted', None)
+        if (d is None or d.capacity != capacity or d.u.shape[:1] != self.state.shape[:1] or d.u.device != self.state.device
+                or (caches is not None and d.x[0].dtype != caches[0].dtype)):
+            self._drafted = ops.DraftBlock.empty(self.state, capacity, gate=self.gate, conv_cache=caches)
+
+    @torch.no_grad()
+    def draft_step(self, x, accepted):
+        """One step of speculative decoding (after begin_drafts): the first accepted (N,) tokens of
+        the last block stand and move into the state and the conv caches; the block x (N,
+        L, dim) runs behind them, each token as decode_step's, and waits for the next call (or
+        commit_drafts) to hear how many of it stand.  Returns the layer's output (N, L, dim).
+        The reference decodes one token a step (linear_attention.py:918-952).  cache_len is not
+        advanced: the streams advance by different counts."""
+        N, L = x.shape[0], x.shape[1]
+        assert getattr(self, '_drafted', None) is not None, 'No drafted block allocated. Call begin_drafts first.'
+        assert N == self.state.shape[0], 'Batch size does not match the state. Reset or load cache first.'
+        self._pick_impl(x)
+        H, dk, dv = self.head_count, self.key_head_dim, self.value_head_dim
+        vec = self.gate == 'vector'
+        qp, kp, vp, og, g, beta, gp = self._decode_inputs(x.reshape(N * L, 1, self.dim))
+        if gp is not None:
+            # the scalar gate and the beta logits by the gate kernel, the weights as the module holds them now
+            _, wa, wb, A_log, dt_bias = gp
+            g, beta = ops.scalar_gates(x.reshape(N * L, self.dim), torch.cat([wa, wb]) if self.delta else wa,
+                                       -A_log.float().exp(), dt_bias, with_beta=self.delta)
+        rows = lambda t, *s: None if t is None else t.reshape(N, L, *s)  # noqa: E731
+        conv = {}
+        if self.short_conv_size is not None:
+            conv = dict(conv_weights=self._conv_weights(), conv_cache=self._caches())
+        else:
+            qp, kp, vp = F.silu(qp), F.silu(kp), F.silu(vp)
+        o = ops.hip_draft_step(rows(qp, H * dk), rows(kp, H * dk), rows(vp, H * dv), rows(g, *((H, dk) if vec else (H,))),
+                               rows(beta, H), self.state, self._drafted, accepted, scale=self.scale, delta=self.delta,
+                               beta_logits=self.delta, gate_in_kernel=vec, A_log=self.A_log if vec else None,
+                               dt_bias=self.dt_bias if vec else None, lower_bound=self.gate_lower_bound,
+                               out_gate=rows(og, H * dv), out_norm_weight=self.o_norm.gamma, out_norm_eps=self.o_norm.eps,
+                               **conv)
+        o = o.reshape(N, L, H * dv)
+        return self.wo(o) if self.out_proj else o
+
+    @torch.no_grad()
+    def commit_drafts(self, accepted) -> None:
+        """The last block's accepted (N,) tokens move into the state and the conv caches, without a
+        new block: what follows (decode_step, export_cache, a draft_step with accepted 0) starts from there."""
+        assert getattr(self, '_drafted', None) is not None, 'No drafted block allocated. Call begin_drafts first.'
+        conv = {}
+        if self.short_conv_size is not None:
+            conv = dict(conv_weights=self._conv_weights(), conv_cache=self._caches())
+        ops.commit_drafts(self.state, self._drafted, accepted, **conv)
 
     @torch.no_grad()
     def prefill_packed(self, x, cu_seqlens, *, rows=None):

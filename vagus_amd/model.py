@@ -20,7 +20,10 @@ replayed.  Its stream convention is the reference Generator's
 (generator.py:8-17): prefill consumes all but the last token of each prompt,
 which becomes the pending token; a decode step feeds the pending tokens,
 takes the logits' argmax (sampling.py:30-35 at temperature 0) and makes it
-pending.
+pending.  ``RaggedGenerator.generate_drafted`` feeds a block a step, the pending
+token and tokens drafted from the stream's own text, keeps those that the
+model's probabilities let stand, and samples the token behind them: as many tokens for
+one read of the weights and the states, greedy or at a temperature.
 """
 from __future__ import annotations
 
@@ -244,6 +247,26 @@ class GDNLM(nn.Module):
             return None
         return self.head(_add_norm(self.rms_head, x, delta, inplace=True)[1])
 
+    def begin_drafts(self, capacity: int) -> None:
+        """Room for drafted blocks of up to `capacity` tokens a stream in every layer."""
+        for blk in self.blocks:
+            blk.att.begin_drafts(capacity)
+
+    @torch.no_grad()
+    def draft_step(self, tokens, accepted):
+        """One step of speculative decoding (GatedDeltaNet.draft_step through every layer): the last
+        block's accepted (N,) tokens are committed, the block tokens (N, L) runs behind them;
+        logits (N, L, vocab), row i after token i."""
+        x = self.embedding(tokens)
+        delta = None
+        for blk in self.blocks:
+            x, delta = blk._stream(x, delta, lambda h, blk=blk: blk.att.draft_step(h, accepted))
+        return self.head(_add_norm(self.rms_head, x, delta, inplace=True)[1])
+
+    def commit_drafts(self, accepted) -> None:
+        for blk in self.blocks:
+            blk.att.commit_drafts(accepted)
+
     @torch.no_grad()
     def prefill_packed(self, tokens, cu_seqlens, *, rows=None, last_logits: bool = True):
         """Consume ragged token blocks, packed as tokens (T,) or (1, T) with
@@ -272,6 +295,8 @@ class RaggedGenerator:
         self.fed_len: list[int] = []
         self._graph = None
         self._graph_key = None
+        self._text: list = []                         # the streams' tokens since the prefill: (ids, cu), then (N, n) blocks
+        self._drafted: dict | None = None             # generate_drafted's buffers and recorded step
 
     def reset(self, batch_size: int) -> None:
         """batch_size empty streams.  The caches are zeroed in place when the
@@ -284,6 +309,7 @@ class RaggedGenerator:
             self.pending.zero_()
         self.batch_size = batch_size
         self.fed_len = [0] * batch_size
+        self._text = []
 
     @torch.no_grad()
     def prefill(self, prompts) -> None:
@@ -306,6 +332,7 @@ class RaggedGenerator:
         self.reset(N)
         last = (cu[1:] - 1).long()
         self.pending.copy_(ids.index_select(0, last))
+        self._text = [(ids, lens)]
         keep = torch.ones(ids.numel(), dtype=torch.bool, device=self.device)
         keep[last] = False
         body = ids[keep]
@@ -361,4 +388,107 @@ class RaggedGenerator:
                         blk.att.cache_len = n
                     self._graph_key = self._fingerprint()
             self.fed_len = [n + 1 for n in self.fed_len]
+        self._text.append(out.clone())                # out is the caller's
         return out
+
+    def _texts(self, room: int):
+        """(the streams' tokens so far, the pending one last (N, cap) int64, their counts (N,) int32),
+        with room for `room` more each."""
+        assert self._text and isinstance(self._text[0], tuple), 'prefill first'
+        ids, lens = self._text[0]
+        more = torch.cat(self._text[1:], 1) if len(self._text) > 1 else ids.new_empty(self.batch_size, 0)
+        width = more.shape[1]
+        cap = -(-(max(lens) + width + room) // 256) * 256
+        text = torch.zeros(self.batch_size, cap, dtype=torch.int64, device=self.device)
+        at = 0
+        for b, n in enumerate(lens):
+            text[b, :n] = ids[at:at + n]
+            text[b, n:n + width] = more[b]
+            at += n
+        return text, torch.tensor([n + width for n in lens], dtype=torch.int32, device=self.device)
+
+    def _drafted_step(self, s: dict) -> None:
+        """One step of generate_drafted over its buffers s, all on the GPU: drafts out of the text,
+        the block through the model (which commits what stood of the last), what of it stands,
+        and the text, the pending tokens and the counts moved on."""
+        K, text, length = s['K'], s['text'], s['length']
+        drafts, found = ops.lookup_drafts(text, length, K, max_ngram=s['max_ngram'], min_ngram=s['min_ngram'])
+        # no stream makes more tokens than it is asked for: the token behind the drafts is one
+        n_drafts = torch.minimum(found, (s['left'] - 1).clamp_(min=0))
+        logits = self.model.draft_step(torch.cat([self.pending[:, None], drafts], 1), s['commit'])
+        tokens, accepted = ops.verify_drafts(logits, drafts, s['uniforms'], temperature=s['temperature'], n_drafts=n_drafts)
+        alive = s['left'] > 0
+        made = torch.where(alive, accepted + 1, 0)
+        last = tokens.gather(1, accepted[:, None].long())[:, 0]
+        self.pending.copy_(torch.where(alive, last, self.pending))
+        at = length[:, None].long() + s['places']
+        text.scatter_(1, at, torch.where(s['places'] < made[:, None], tokens, text.gather(1, at)))
+        length.add_(made)
+        s['left'].sub_(made)
+        s['commit'].copy_(made)
+
+    @torch.no_grad()
+    def generate_drafted(self, steps: int, *, drafts: int = 4, max_ngram: int = 3, min_ngram: int = 1,
+                         temperature: float = 0.0, generator: torch.Generator | None = None,
+                         graph: bool = True) -> torch.Tensor:
+        """`steps` tokens for every stream, (N, steps) int64, by speculative decoding: each step feeds
+        the pending token and up to `drafts` (1 to 15) tokens drafted from the stream's own text
+        (ops.lookup_drafts), and keeps those that stand before the model's probabilities and the token
+        behind them (ops.verify_drafts).  At temperature 0 these are generate's tokens, up to the
+        rounding of the logits; above, samples of the softmax at that temperature from `generator`'s
+        uniform numbers.  The streams advance by different counts a step, and the call ends when
+        the slowest has its tokens.  With graph=True the first step runs eagerly, and the recorded step is
+        replayed; as in generate the layers' cache_len counters are not advanced."""
+        assert self.pending is not None and self.batch_size > 0, 'prefill first'
+        assert 1 <= drafts < ops.MAX_DRAFT_BLOCK, f'1 to {ops.MAX_DRAFT_BLOCK - 1} drafts a step; got {drafts}'
+        assert temperature >= 0, f'temperature must not be negative; got {temperature}'
+        N, dev = self.batch_size, self.device
+        if steps <= 0:
+            return torch.empty(N, 0, dtype=torch.int64, device=dev)
+        text, length = self._texts(steps + drafts + 1)
+        self.model.begin_drafts(drafts + 1)
+        kind = (N, drafts, text.shape[1], max_ngram, min_ngram)
+        s = self._drafted
+        if s is None or s['kind'] != kind:
+            new = lambda *shape, dt=torch.int32: torch.zeros(*shape, dtype=dt, device=dev)  # noqa: E731
+            s = self._drafted = dict(kind=kind, K=drafts, max_ngram=max_ngram, min_ngram=min_ngram, text=text, length=length,
+                                     left=new(N), commit=new(N), uniforms=new(N, drafts + 1, dt=torch.float32),
+                                     temperature=new(N, dt=torch.float32), places=torch.arange(drafts + 1, device=dev)[None],
+                                     graph=None, key=None)
+        else:
+            s['text'].copy_(text)
+            s['length'].copy_(length)
+        start = length.long()
+        s['left'].fill_(steps)
+        s['commit'].zero_()
+        s['temperature'].fill_(temperature)
+        taken = 0
+        # every step makes a token, so the fewest steps are known; past them the counts are asked for
+        while taken * (drafts + 1) < steps or int(s['left'].max()) > 0:
+            if temperature > 0:
+                s['uniforms'].uniform_(generator=generator)
+            if graph and s['graph'] is not None and s['key'] != self._fingerprint() + self._drafted_fingerprint():
+                s['graph'] = None                     # a captured tensor moved or changed: record again
+            if graph and s['graph'] is not None:
+                s['graph'].replay()
+            else:
+                self._drafted_step(s)
+                if graph:
+                    s['graph'] = torch.cuda.CUDAGraph()
+                    with torch.cuda.graph(s['graph']):
+                        self._drafted_step(s)
+                    s['key'] = self._fingerprint() + self._drafted_fingerprint()
+            taken += 1
+        self.model.commit_drafts(s['commit'])
+        s['commit'].zero_()
+        out = s['text'].gather(1, start[:, None] + torch.arange(steps, device=dev)[None])
+        self.fed_len = [n + steps for n in self.fed_len]
+        self._text.append(out.clone())                # out is the caller's
+        self.drafted_steps = taken
+        return out
+
+    def _drafted_fingerprint(self) -> tuple:
+        """What a recorded drafted step holds by address beside _fingerprint: the pending tokens and
+        every layer's drafted block."""
+        ds = [blk.att._drafted for blk in self.model.blocks]
+        return (self.pending.data_ptr(),) + tuple(t.data_ptr() for d in ds for t in (d.k, d.u, *(d.x or ())))
