@@ -4,7 +4,7 @@
 //    the token that follows them.  row_mass_kernel reads every row once, each wave a chunk of 2048
 //    logits held in registers: its top, and where it is (greedy streams) or sum e^{(x - top) / T}
 //    in fp32, which decides u q Z < w but where the two are within 1e-5.  stand_kernel decides, and
-//    of the one row that a stream samples sums the weights in 64 bits, in blocks of 256 over several
+//    of the one row that a stream samples sums the weights in 64 bits, in blocks of 512 over several
 //    workgroups: the running sums meet the uniform number at up to V borders, so an fp32
 //    sum's error (5e-7) would choose another token once in some ten streams of 100,000 ids, a
 //    64-bit one's (1e-14) never in practice.  rest_kernel does the same with what the draft's probabilities
@@ -19,8 +19,9 @@ namespace vgdr {
 
 namespace {
 
-constexpr int CHUNK = 2048, BLOCK = 256;                           // logits of a wave: in row_mass, in choose
+constexpr int CHUNK = 2048, BLOCK = 512, EACH = BLOCK / 64;        // logits of a wave in row_mass, in the others; a lane's
 constexpr int ROW_WAVES = 4, WAVES = 8;                            // of a workgroup: in row_mass, in the others
+constexpr int64_t SHARE = 512;
 constexpr double LOG2E = 1.4426950408889634;
 
 // A row in pieces on 16-byte boundaries: it starts at place `first` of the first.
@@ -103,26 +104,36 @@ __device__ __forceinline__ int passing_lane(double own, double upto, double goal
     return past ? __ffsll((unsigned long long)past) - 1 : any ? 63 - __clzll((long long)any) : -1;
 }
 
-// e^{(x - top) / T} in 64 bits, c = log2(e) / T: 2^n 2^f, n whole, |f| <= 1/2, by the exponential
-// series of f ln 2 up to its 11th power (6e-15 off). Nothing below 2^-1022 and for NaN; the top is 1
-// whatever its value (a NaN beside a top of -inf counts as it).
-__device__ __forceinline__ double mass(float x, float top, double c) {
+// e^{(x - top) / T} in 64 bits for a finite top, c = log2(e) / T: 2^n 2^f, n whole, |f| <= 1/2, by the exponential
+// series of f ln 2 up to its 10th power (2e-13 off). n is rounded off and added to the exponent as an
+// integer: the 64-bit rounding, conversion and scaling instructions run at a fraction of an addition's rate.
+// Nothing below 2^-1000 and for NaN.
+__device__ __forceinline__ double mass_finite(float x, float top, double c) {
+    constexpr double L1 = 0.6931471805599453, L2 = L1 * L1 / 2, L3 = L2 * L1 / 3, L4 = L3 * L1 / 4, L5 = L4 * L1 / 5,
+                     L6 = L5 * L1 / 6, L7 = L6 * L1 / 7, L8 = L7 * L1 / 8, L9 = L8 * L1 / 9, L10 = L9 * L1 / 10;
+    constexpr double ROUND = 6755399441055744.0;                   // 1.5 2^52: the sum's last bit is worth 1
     const double y = ((double)x - (double)top) * c;
-    const double n = rint(y), f = (y - n) * 0.6931471805599453;
-    double s = 1.0 / 39916800;
-    s = fma(s, f, 1.0 / 3628800);
-    s = fma(s, f, 1.0 / 362880);
-    s = fma(s, f, 1.0 / 40320);
-    s = fma(s, f, 1.0 / 5040);
-    s = fma(s, f, 1.0 / 720);
-    s = fma(s, f, 1.0 / 120);
-    s = fma(s, f, 1.0 / 24);
-    s = fma(s, f, 1.0 / 6);
-    s = fma(s, f, 0.5);
+    const double r = y + ROUND, f = y - (r - ROUND);
+    double s = fma(L10, f, L9);
+    s = fma(s, f, L8);
+    s = fma(s, f, L7);
+    s = fma(s, f, L6);
+    s = fma(s, f, L5);
+    s = fma(s, f, L4);
+    s = fma(s, f, L3);
+    s = fma(s, f, L2);
+    s = fma(s, f, L1);
     s = fma(s, f, 1.0);
-    s = fma(s, f, 1.0);
-    s = y >= -1022.0 ? ldexp(s, (int)n) : 0.0;
-    return fmaxf(x, -__builtin_inff()) == top ? 1.0 : s;
+    const uint64_t u = __builtin_bit_cast(uint64_t, s);
+    const uint32_t hi = (uint32_t)(u >> 32) + ((uint32_t)__builtin_bit_cast(uint64_t, r) << 20);
+    s = __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)u);
+    return y >= -1000.0 ? s : 0.0;
+}
+// the same for any top: of an infinite one what equals it counts 1 (NaN as -inf), all else nothing
+__device__ __forceinline__ bool infinite(float top) { return fabsf(top) == __builtin_inff(); }
+__device__ __forceinline__ double mass(float x, float top, double c) {
+    if (infinite(top)) return fmaxf(x, -__builtin_inff()) == top ? 1.0 : 0.0;
+    return mass_finite(x, top, c);
 }
 
 }  // namespace
@@ -188,30 +199,68 @@ template <typename E> struct Sampled {
     int q_dtype;
     double z;
 
-    // the weights of block b's logits 4 lane .. 4 lane + 3
-    __device__ __forceinline__ void four(int64_t b, int lane, double (&w)[4]) const {
-        typedef E E4 __attribute__((ext_vector_type(4)));
-        const int64_t at = b * BLOCK + 4 * lane;
-        unroll<4>([&](auto e) { w[e] = 0.0; });
-        if (at >= row.end) return;                                 // else within the row's last 16 bytes
-        const E4 x = *reinterpret_cast<const E4 *>(row.base + at);
+    // block b's logits EACH lane .. EACH lane + EACH - 1 as they lie, in whole units of 16 bytes of the row
+    struct Raw { u32x4 u[EACH * sizeof(E) / 16]; };
+    __device__ __forceinline__ Raw raw(int64_t b, int lane) const {
+        Raw r;
+        unroll<EACH * (int)sizeof(E) / 16>([&](auto k) {
+            const int64_t at = b * BLOCK + EACH * lane + Row<E>::UNIT * k;
+            r.u[k] = at < row.end ? *reinterpret_cast<const u32x4 *>(row.base + at) : u32x4{0, 0, 0, 0};
+        });
+        return r;
+    }
+    // their weights
+    __device__ __forceinline__ void weigh(const Raw &r, int64_t b, int lane, double (&w)[EACH]) const {
+        const int64_t at = b * BLOCK + EACH * lane;
+        float x[EACH], qv[EACH];
+        unroll<EACH>([&](auto e) {
+            if constexpr (sizeof(E) == 2)
+                x[e] = (float)__builtin_bit_cast(E, (unsigned short)(r.u[0][e / 2] >> (e % 2 * 16)));
+            else x[e] = __builtin_bit_cast(float, (unsigned)r.u[e / 4][e % 4]);
+        });
         const int v0 = (int)(at - row.first);
-        float qv[4] = {0.f, 0.f, 0.f, 0.f};
-        if (q)
-            unroll<4>([&](auto e) {
-                const int v = v0 + e;
-                qv[e] = param_f(q, q_dtype, v < 0 ? 0 : v < V ? v : V - 1);
+        unroll<EACH>([&](auto e) { qv[e] = 0.f; });
+        if (q) {
+            auto fetch = [&](auto *q0) __attribute__((always_inline)) {  // ids outside the row: its nearest end's
+                unroll<EACH>([&](auto e) {
+                    const int v = v0 + e;
+                    qv[e] = (float)q0[v < 0 ? 0 : v < V ? v : V - 1];
+                });
+            };
+            if (q_dtype == 0) fetch(reinterpret_cast<const float *>(q));
+            else if (q_dtype == 1) fetch(reinterpret_cast<const __bf16 *>(q));
+            else fetch(reinterpret_cast<const _Float16 *>(q));
+        }
+        if (infinite(top)) {
+            unroll<EACH>([&](auto e) { w[e] = fmaxf(x[e], -__builtin_inff()) == top ? 1.0 : 0.0; });
+        } else {
+            unroll<EACH>([&](auto e) {
+                w[e] = mass_finite(x[e], top, c);
+                if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
             });
-        unroll<4>([&](auto e) {
+        }
+        if (q) unroll<EACH>([&](auto e) { w[e] = fmax(w[e] - z * (double)qv[e], 0.0); });
+        unroll<EACH>([&](auto e) {
             const int v = v0 + e;
-            const double m = fmax(mass((float)x[e.value], top, c) - z * (double)qv[e], 0.0);
-            w[e] = v >= 0 && v < V && v != without ? m : 0.0;
+            if (v < 0 || v >= V || v == without) w[e] = 0.0;
         });
     }
-    __device__ __forceinline__ double block_sum(int64_t b, int lane) const {
-        double w[4];
-        four(b, lane, w);
-        return wave_sum((w[0] + w[1]) + (w[2] + w[3]));
+    __device__ __forceinline__ static double sum(const double (&w)[EACH]) {
+        double s = 0.0;
+        unroll<EACH>([&](auto e) { s += w[e]; });
+        return s;
+    }
+    // f(b, sum of its weights) for the blocks b = first, first + step, ..; a block's logits are loaded two ahead
+    template <typename F> __device__ __forceinline__ void sums(int64_t first, int64_t step, int64_t blocks, int lane, F f) const {
+        Raw r0 = raw(first, lane), r1 = raw(first + step, lane);
+        for (int64_t b = first; b < blocks; b += step) {
+            const Raw r2 = raw(b + 2 * step, lane);
+            double w[EACH];
+            weigh(r0, b, lane, w);
+            f(b, wave_sum(sum(w)));
+            r0 = r1;
+            r1 = r2;
+        }
     }
 };
 
@@ -328,11 +377,10 @@ __global__ void __launch_bounds__(64 * WAVES) stand_kernel(const VerifyParams p)
         // the whole row in every workgroup where a draft is near, else this one's blocks: one copy of the code
         const int64_t first = near ? wave : (int64_t)blockIdx.x * WAVES + wave, step = near ? WAVES : (int64_t)gridDim.x * WAVES;
         double z = 0.0;
-        for (int64_t b = first; b < blocks; b += step) {
-            const double s = row.block_sum(b, lane);
+        row.sums(first, step, blocks, lane, [&](int64_t b, double s) __attribute__((always_inline)) {
             z += s;
             if (!near && lane == 0) sums[b] = s;
-        }
+        });
         if (!near) break;
         if (lane == 0) part[wave] = z;
         __syncthreads();
@@ -365,10 +413,10 @@ __global__ void __launch_bounds__(64 * WAVES) rest_kernel(const VerifyParams p) 
     Sampled<E> row = sampled_row<E>(p, n, st.count, n_drafts, st.top, LOG2E / (double)t);
     row.q = probs_row(p, n, st.count);
     row.z = group_sum(sums, blocks, wave, lane, part);
-    for (int64_t b = (int64_t)blockIdx.x * WAVES + wave; b < blocks; b += (int64_t)gridDim.x * WAVES) {
-        const double s = row.block_sum(b, lane);
-        if (lane == 0) sums[blocks + b] = s;
-    }
+    row.sums((int64_t)blockIdx.x * WAVES + wave, (int64_t)gridDim.x * WAVES, blocks, lane,
+             [&](int64_t b, double s) __attribute__((always_inline)) {
+                 if (lane == 0) sums[blocks + b] = s;
+             });
 }
 
 // The token of a sampled stream: the first id at which the running sum passes u times the whole.
@@ -422,17 +470,17 @@ __global__ void __launch_bounds__(64 * WAVES) choose_kernel(const VerifyParams p
         base = lane_d(upto, 63);
     }
     if (block < 0) return;
-    double w[4];
-    row.four(block, lane, w);
-    const double own = (w[0] + w[1]) + (w[2] + w[3]), upto = start + wave_prefix(own);
+    double w[EACH];
+    row.weigh(row.raw(block, lane), block, lane, w);
+    const double own = row.sum(w), upto = start + wave_prefix(own);
     const int l = passing_lane(own, upto, goal, passed);
     double run = upto - own;
     int last = -1;
     bool over = false;
-    unroll<4>([&](auto e) {
+    unroll<EACH>([&](auto e) {
         run += w[e];
         if (w[e] > 0.0 && !over) {
-            last = (int)(block * BLOCK + 4 * lane + e - row.row.first);
+            last = (int)(block * BLOCK + EACH * lane + e - row.row.first);
             over = run > goal;
         }
     });
@@ -453,8 +501,8 @@ template <typename E> static void verify_typed(const VerifyParams &p, hipStream_
     const int64_t rows = p.N * (p.K + 1), ry = rows < 32768 ? rows : 32768, ny = p.N < 32768 ? p.N : 32768;
     row_mass_kernel<E><<<dim3((unsigned)((p.chunks + ROW_WAVES - 1) / ROW_WAVES), (unsigned)ry, (unsigned)((rows + ry - 1) / ry)),
                          dim3(64 * ROW_WAVES), 0, stream>>>(p);
-    // a block to a wave, up to 1,024 workgroups (64 streams of 32,000: 16 each; 128 of 131,072: 8 each)
-    const int64_t most = (p.blocks + WAVES - 1) / WAVES, share = 1024 / p.N > 1 ? 1024 / p.N : 1;
+    // a block to a wave, up to SHARE workgroups of a decision's latency each (64 streams of 32,000: 8 each; 128 of 131,072: 4)
+    const int64_t most = (p.blocks + WAVES - 1) / WAVES, share = SHARE / p.N > 1 ? SHARE / p.N : 1;
     const dim3 grid((unsigned)(most < share ? most : share), (unsigned)ny, (unsigned)((p.N + ny - 1) / ny));
     stand_kernel<E><<<grid, dim3(64 * WAVES), 0, stream>>>(p);
     if (p.probs) rest_kernel<E><<<grid, dim3(64 * WAVES), 0, stream>>>(p);
