@@ -677,9 +677,11 @@ typedef struct vgdr_draft_block {
  * leaves the pending block as it is), which become the pending block and move neither
  * state nor caches.  Everything else as vgdr_decode_step_strided (q, k, v, gate rows of
  * token b * L + t, ld_qk and ld_v elements apart; g, beta [B, L, H], g [B, L, H, dk] per
- * channel, in fusion->gate_dtype where the kernel activates it), but that no intermediate is
+ * channel, in fusion->gate_dtype where the kernel activates it: the scalar gate's too, -exp(A_log)
+ * softplus(f + dt_bias) with A_log and dt_bias [H]), but that no intermediate is
  * rounded to dtype and that the conv takes any kernel size 1..8.  Pending rows from L on
- * are left as they were.  dk a multiple of 8 up to 128, dv a multiple of 8 up to 256.
+ * are left as they were.  dk a multiple of 8 up to 128, dv a multiple of 8 up to 256, H * dk and
+ * H * dv up to 2^24.
  */
 int vgdr_draft_step(int dtype, int gate_kind, int use_delta, const void *q, const void *k, const void *v,
                     const void *g, const float *beta, void *o, float *state, const vgdr_draft_block *pending,

@@ -41,6 +41,8 @@ def make(N, L, H, dk, dv, *, P=None, dtype=torch.float32, gate='scalar', delta=T
     if gate == 'vector':
         c['g_in'] = randn(N, L, H, dk).to(dtype) if c['act'] else F.logsigmoid(randn(N, L, H, dk) + 3)
     c['A_log'], c['dt_bias'] = torch.rand(H, generator=r), randn(H * dk) - 2
+    if gate == 'scalar' and act == 'scalar':
+        c['act'], c['g_in'], c['dt_bias'] = True, randn(N, L, H).to(dtype), c['dt_bias'][:H]
     c['lower'] = None
     c['gamma'] = 1 + 0.2 * randn(dv) if epilogue else None
     D = (H * dk, H * dk, H * dv)
@@ -84,8 +86,8 @@ def reference(c, accepted):
         for t in range(L):
             g = None if c['g_in'] is None else c['g_in'][n, t].double()
             if c['act']:
-                z = g + c['dt_bias'].double().view(H, dk)
-                A = c['A_log'].double().exp()[:, None]
+                z = g + c['dt_bias'].double().view(g.shape)
+                A = c['A_log'].double().exp().view((H,) + (1,) * (g.dim() - 1))
                 g = -A * F.softplus(z) if c['lower'] is None else c['lower'] * torch.sigmoid(A * z)
             M = decay(M, g)
             u = v[t]
@@ -174,6 +176,10 @@ CASES = [
     dict(N=4, L=2, P=7, H=2, dk=64, dv=64),
     dict(N=4, L=1, P=16, H=2, dk=128, dv=128, dtype=torch.bfloat16, gate='vector'),
     dict(N=1, L=5, P=6, H=2, dk=128, dv=64, wide=True),
+    # the scalar gate's activation in the kernel
+    dict(N=3, L=5, H=3, dk=64, dv=64, act='scalar'),
+    dict(N=2, L=11, H=2, dk=128, dv=128, act='scalar', dtype=torch.bfloat16),
+    dict(N=2, L=4, H=5, dk=64, dv=128, act='scalar', dtype=torch.float16, delta=False),
 ]
 
 
@@ -365,8 +371,12 @@ def test_refusals():
         call(beta=None)
     with pytest.raises(AssertionError, match='no beta to activate'):
         call(delta=False)
-    with pytest.raises(AssertionError, match='vector-gate'):
+    with pytest.raises(AssertionError, match='needs A_log'):
         call(gate_in_kernel=True)
+    with pytest.raises(AssertionError, match='A_log has 2 and dt_bias 2'):
+        call(gate_in_kernel=True, A_log=torch.zeros(2, device='cuda'), dt_bias=torch.zeros(128, device='cuda'))
+    with pytest.raises(AssertionError, match='bounded'):
+        call(gate_in_kernel=True, A_log=torch.zeros(2, device='cuda'), dt_bias=torch.zeros(2, device='cuda'), lower_bound=-2.0)
     with pytest.raises(NotImplementedError, match='share one'):
         call(k=k.half())
     with pytest.raises(NotImplementedError, match='backward'):
@@ -409,6 +419,9 @@ def test_entry_point_refuses_before_it_launches():
     assert _call(conv=conv, pending=_lib.DraftBlock(16, 32, 48, None, None, None, 4)) == bad
     assert _call(conv=_lib.ShortConv(16, 32, 48, 64, 80, 96, 9, 1)) == no
     assert _call(fz=_lib.Fusion(1, 1, 0, 0, None, None, 0, 0.0), delta=0) == bad
-    assert _call(fz=_lib.Fusion(1, 0, 1, 0, 16, 32, 0, 0.0)) == bad
+    assert _call(gate=0, fz=_lib.Fusion(1, 0, 1, 0, 16, 32, 0, 0.0)) == bad           # no gate to activate
+    assert _call(fz=_lib.Fusion(1, 0, 1, 0, 16, 32, 1, -2.0)) == bad                  # the scalar gate has no bounded form
+    assert _call(fz=_lib.Fusion(1, 0, 1, 0, None, 32, 0, 0.0)) == bad
     assert _call(ep=_lib.Epilogue(None, 16, 0, 1e-6)) == bad
+    assert _call(H=1 << 19, ld_qk=1 << 25, ld_v=1 << 25) == no and _call(B=1 << 31) == no
     assert _call(B=0) == _lib.VGDR_OK

@@ -1333,12 +1333,17 @@ int vgdr_draft_step(int dtype, int gate_kind, int use_delta, const void *q, cons
                     fn, vgdr::DRAFT_MAX);
     if (L > pending->capacity)
         return fail(VGDR_ERR_INVALID, "%s: L=%lld tokens, room for %lld", fn, (long long)L, (long long)pending->capacity);
-    if (B > 0x7fffffffLL / H || H > 0x7fffffffLL / 256)
-        return fail(VGDR_ERR_INVALID, "%s: too many (stream, head) pairs", fn);
+    // a stream's pending block lies within 2^30 bytes: the kernels' 32-bit offsets
+    if (B > 0x7fffffffLL / H || H > 0x1000000LL / (dk > dv ? dk : dv))
+        return fail(VGDR_ERR_UNSUPPORTED, "%s: too many (stream, head) pairs", fn);
     if (B == 0) return VGDR_OK;
     vgdr::DraftParams p{};
-    int rc = check_fusion(fn, fusion, dtype, gate_kind, use_delta, false, p.fz);
+    // (the scalar gate's activation as well, which the other entry points take from their own projections)
+    int rc = check_fusion(fn, fusion, dtype, gate_kind == VGDR_GATE_SCALAR ? (int)VGDR_GATE_VECTOR : gate_kind, use_delta, false,
+                          p.fz);
     if (rc) return rc;
+    if (p.fz.lb_set && gate_kind == VGDR_GATE_SCALAR)
+        return fail(VGDR_ERR_INVALID, "%s: the bounded decay is a per-channel gate's", fn);
     rc = check_conv(fn, conv, dtype, p.cv);
     if (rc) return rc;
     rc = check_epilogue(fn, epilogue, dtype, p.ep);

@@ -169,7 +169,15 @@ draft_block_kernel(const DraftParams p) {
     f32x2 gv[GATE == 2 ? LG : 1], dt_bias[GATE == 2 ? LG : 1];     // per channel: two channels of some tokens
     if (GATE == 1) {
         gp = buffer_load1(buffer_rsrc(p.pg + (has_g ? n * P * H : 0), has_g ? (uint32_t)(P * H) * 4u : 0u), r16 < a ? lane_h : NOWHERE);
-        gn = buffer_load1(buffer_rsrc(reinterpret_cast<const float *>(p.g) + (has_g ? n * L * H : 0), has_g ? (uint32_t)(L * H) * 4u : 0u), lane_h);
+        const uint32_t e = p.fz.gate_16 ? 2 : 4;
+        const __amdgpu_buffer_rsrc_t bg = buffer_rsrc(reinterpret_cast<const char *>(p.g) + (has_g ? n * L * H * e : 0),
+                                                      has_g ? (uint32_t)(L * H) * e : 0u);
+        if constexpr (sizeof(E) == 2) {
+            if (p.fz.gate_16) gn = (float)__builtin_bit_cast(E, __builtin_amdgcn_raw_buffer_load_b16(bg, (int)(lane_h / 2), 0, 0));
+            else gn = buffer_load1(bg, lane_h);
+        } else {
+            gn = buffer_load1(bg, lane_h);
+        }
     }
     if (GATE == 2) {
         const uint32_t e = p.fz.gate_16 ? 2 : 4;
@@ -269,6 +277,7 @@ draft_block_kernel(const DraftParams p) {
             if (t < LT) *reinterpret_cast<f32x2 *>(&es[GATE == 2 ? t : 0][c]) = f32x2{__expf(g[0]), __expf(g[1])};
         });
     } else if (tid < 16) {
+        if (p.fz.gate_act) gn = -__expf(p.fz.A_log[h]) * softplusf_(gn + p.fz.dt_bias[h]);
         es[0][tid] = __expf(gn);
         eg[0][tid] = __expf(row_prefix16(gn));
     }

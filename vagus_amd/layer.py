@@ -465,7 +465,7 @@ class GatedDeltaNet(nn.Module):
         return (self.short_conv_size is not None and self.key_head_dim in (64, 128)
                 and (self.value_head_dim in (64, 128) or (self.value_head_dim == 256 and self.short_conv_size == 4)))
 
-    def _decode_inputs(self, x):
+    def _decode_inputs(self, x, *, raw_gate: bool = False):
         """(qp, kp, vp, out_gate, g, beta, gate_proj) for the one-token decode kernel,
         from x (B, 1, dim): the projections, the KDA gate's pre-activation and the beta
         logits.  One launch forms them (ops.project_rows; W_a2 follows as its own)
@@ -476,12 +476,16 @@ class GatedDeltaNet(nn.Module):
         beta are None and gate_proj = (x, W_a, W_b, A_log, dt_bias): the decode kernel
         forms them itself.  The values are those of the separate projections and of
         _gates(raw_gate=vector, raw_beta=delta) up to the sums' order.
+        raw_gate (draft_step): W_a is one of the projections, g the scalar gate's pre-activation and
+        gate_proj (A_log, dt_bias); where the modules are called one by one g is the
+        log-decay and gate_proj None.
         Projections that are not plain bias-free nn.Linear modules of x's type, an
         overridden _gates, and batches that the launch does not take are called one
         by one."""
         B = x.shape[0]
         H, dk, dv = self.head_count, self.key_head_dim, self.value_head_dim
-        vec, scalar = self.gate == 'vector', self.gate == 'scalar'
+        vec, scalar = self.gate == 'vector', self.gate == 'scalar' and not raw_gate
+        raw_gate = raw_gate and self.gate == 'scalar'
         names = self._input_projections()
         mods = [self._modules.get(n) for n in names]
         x2 = x.reshape(B, -1)
@@ -492,7 +496,7 @@ class GatedDeltaNet(nn.Module):
             plain = all(t is not None and t.dtype == x.dtype for t in w.values()) and not torch.is_autocast_enabled('cuda')
             y = None
             if plain and ops.project_rows_fits(x2, list(w.values())):
-                y, at, beta = ops.project_rows(x2, [w[n] for n in names if n not in ('wa', 'wb')],
+                y, at, beta = ops.project_rows(x2, [w[n] for n in names if n != 'wb' and (raw_gate or n != 'wa')],
                                                None if scalar else w.get('wb'))
             elif plain and B > ops._PROJECT_ROWS:
                 # one GEMM over the weights stacked for this call, to rows of whole 16-byte units
@@ -509,8 +513,11 @@ class GatedDeltaNet(nn.Module):
                 if vec:
                     f = y.as_strided((B, w['wa1'].shape[0]), (ld, 1), off + at[4])
                     g = self.wa2(f).view(B, 1, H, dk)
+                elif raw_gate:
+                    g = y.as_strided((B, 1, H), (ld, H, 1), off + at[4])
                 return (qp, kp, vp, og, g, None if beta is None else beta.view(B, 1, H),
-                        (x, w['wa'], w.get('wb'), self.A_log, self.dt_bias) if scalar else None)
+                        (x, w['wa'], w.get('wb'), self.A_log, self.dt_bias) if scalar
+                        else (self.A_log, self.dt_bias) if raw_gate else None)
         g, beta = self._gates(x, raw_gate=vec, raw_beta=self.delta)
         return self.wq(x), self.wk(x), self.wv(x), self.wg(x), g, beta if self.delta else None, None
 
@@ -585,12 +592,8 @@ class GatedDeltaNet(nn.Module):
         self._pick_impl(x)
         H, dk, dv = self.head_count, self.key_head_dim, self.value_head_dim
         vec = self.gate == 'vector'
-        qp, kp, vp, og, g, beta, gp = self._decode_inputs(x.reshape(N * L, 1, self.dim))
-        if gp is not None:
-            # the scalar gate and the beta logits by the gate kernel, the weights as the module holds them now
-            _, wa, wb, A_log, dt_bias = gp
-            g, beta = ops.scalar_gates(x.reshape(N * L, self.dim), torch.cat([wa, wb]) if self.delta else wa,
-                                       -A_log.float().exp(), dt_bias, with_beta=self.delta)
+        qp, kp, vp, og, g, beta, gate = self._decode_inputs(x.reshape(N * L, 1, self.dim), raw_gate=True)
+        raw = vec or gate is not None                          # g is the gate's pre-activation
         rows = lambda t, *s: None if t is None else t.reshape(N, L, *s)  # noqa: E731
         conv = {}
         if self.short_conv_size is not None:
@@ -599,8 +602,8 @@ class GatedDeltaNet(nn.Module):
             qp, kp, vp = F.silu(qp), F.silu(kp), F.silu(vp)
         o = ops.hip_draft_step(rows(qp, H * dk), rows(kp, H * dk), rows(vp, H * dv), rows(g, *((H, dk) if vec else (H,))),
                                rows(beta, H), self.state, self._drafted, accepted, scale=self.scale, delta=self.delta,
-                               beta_logits=self.delta, gate_in_kernel=vec, A_log=self.A_log if vec else None,
-                               dt_bias=self.dt_bias if vec else None, lower_bound=self.gate_lower_bound,
+                               beta_logits=self.delta, gate_in_kernel=raw, A_log=self.A_log if raw else None,
+                               dt_bias=self.dt_bias if raw else None, lower_bound=self.gate_lower_bound,
                                out_gate=rows(og, H * dv), out_norm_weight=self.o_norm.gamma, out_norm_eps=self.o_norm.eps,
                                **conv)
         o = o.reshape(N, L, H * dv)

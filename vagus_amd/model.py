@@ -332,7 +332,7 @@ class RaggedGenerator:
         self.reset(N)
         last = (cu[1:] - 1).long()
         self.pending.copy_(ids.index_select(0, last))
-        self._text = [(ids, lens)]
+        self._text = [(ids.clone(), lens)]            # ids may be the caller's
         keep = torch.ones(ids.numel(), dtype=torch.bool, device=self.device)
         keep[last] = False
         body = ids[keep]

@@ -1751,8 +1751,9 @@ def hip_draft_step(qp, kp, vp, g, beta, state, pending, accepted, *, scale: floa
     drafted tokens to the input of W_o, in one kernel (vgdr_draft_step).
 
     First the tokens of the last block that stand, accepted (N,) (whole numbers, on the
-    GPU; clamped to 0 .. the block's room), are committed from `pending` (DraftBlock) to
-    state (N, H, dk, dv) and conv_cache, in place.  Then the block's L tokens (1 <= L
+    GPU; clamped to 0 .. the block's room; that the last block had as many is the caller's
+    word), are committed from `pending` (DraftBlock) to state (N, H, dk, dv) and
+    conv_cache, in place.  Then the block's L tokens (1 <= L
     <= the room of `pending`, at most 16) run behind them as hip_decode_step's tokens
     do, one after the other, but on no state that is kept: the block becomes
     `pending`, and the next call commits what stands of it.  A step that commits
@@ -1761,8 +1762,9 @@ def hip_draft_step(qp, kp, vp, g, beta, state, pending, accepted, *, scale: floa
     Arguments as hip_decode_step's: qp, kp (N, L, H*dk) or (N, L, H, dk), vp (N, L,
     H*dv) or (N, L, H, dv), raw projections (with conv_weights and conv_cache; the
     convolved and activated rows without), column blocks of one projection output among
-    them (read in place); g None, (N, L, H) fp32 log-decay or (N, L, H, dk) (with
-    gate_in_kernel its pre-activation); beta (N, L, H).  Returns o (N, L, H, dv) in
+    them (read in place); g None, (N, L, H) or (N, L, H, dk) log-decay, with
+    gate_in_kernel its pre-activation (the scalar gate's as well: -exp(A_log) softplus(g + dt_bias), A_log
+    and dt_bias (H,)); beta (N, L, H).  Returns o (N, L, H, dv) in
     q's type.  Between the inputs and the outputs everything is fp32; hip_decode_step
     rounds the conv's, the SiLU's, the norm's and the recurrence's results to q's type.
     dk a multiple of 8 up to 128, dv a multiple of 8 up to 256.  No autograd."""
@@ -1777,16 +1779,18 @@ def hip_draft_step(qp, kp, vp, g, beta, state, pending, accepted, *, scale: floa
     assert state.dim() == 4, f'state must be (N, H, dk, dv); got {tuple(state.shape)}'
     N, H, dk, dv = state.shape
     L, P = qp.shape[1], pending.capacity
-    for name, t, d in (('q', qp, dk), ('k', kp, dk), ('v', vp, dv)):
-        assert t.shape == (N, L, H * d) or t.shape == (N, L, H, d), \
-            f'{name} must be {(N, L, H * d)} or {(N, L, H, d)}; got {tuple(t.shape)}'
+    for t, d in ((qp, dk), (kp, dk), (vp, dv)):
+        ts = t.shape
+        assert ts == (N, L, H * d) or ts == (N, L, H, d), \
+            f'q, k, v must be (N, L, H*d) or (N, L, H, d), here {(N, L, H * d)}; got {tuple(ts)}'
     assert 1 <= L <= P, f'a block of 1 to {P} tokens (the pending block\'s room); got {L}'
     gate = _gate_of(g)
     assert g is None or g.shape == ((N, L, H) if gate == 'scalar' else (N, L, H, dk)), \
         f'g must be {(N, L, H)} or {(N, L, H, dk)}; got {tuple(g.shape)}'
     if delta:
         assert beta is not None and beta.shape == (N, L, H), f'the delta rule needs beta {(N, L, H)}'
-    assert not gate_in_kernel or gate == 'vector', 'the fused gate activation is a KDA (vector-gate) kernel'
+    assert not gate_in_kernel or gate != 'none', 'the fused gate activation needs g'
+    assert lower_bound is None or not gate_in_kernel or gate == 'vector', 'the bounded decay is a vector gate\'s'
     assert delta or not beta_logits, 'there is no beta to activate without the delta rule'
     fusion = None
     if l2norm or beta_logits or gate_in_kernel:
@@ -1827,7 +1831,7 @@ def commit_drafts(state, pending, accepted, *, conv_weights=None, conv_cache=Non
     index = state.get_device()
     if index < 0:
         _check_device(state)
-    _all_on(index, accepted)
+    _all_on(index, accepted, *(conv_weights or ()))
     _check_grad(state)
     gate = 'none' if pending.g is None else 'scalar' if pending.g.dim() == 3 else 'vector'
     dt = conv_cache[0].dtype if conv_cache is not None else torch.float32
@@ -1850,8 +1854,8 @@ def _draft_call(index, dt, gate, delta, operands, state, pending, accepted, L, l
         raise NotImplementedError(f'a drafted block holds 1 to {MAX_DRAFT_BLOCK} tokens; got room for {P}')
     f32 = torch.float32
     S = _in_place('state', state, (N, H, dk, dv), f32, index)
-    blk = _lib.DraftBlock(k=_in_place('pending.k', pending.k, (N, P, H, dk), f32, index),
-                          u=_in_place('pending.u', pending.u, (N, P, H, dv), f32, index), capacity=P)
+    blk = _lib.DraftBlock(_in_place('pending.k', pending.k, (N, P, H, dk), f32, index),
+                          _in_place('pending.u', pending.u, (N, P, H, dv), f32, index), None, None, None, None, P)
     assert (pending.g is None) == (gate == 'none'), f'the pending block was made for another gate than {gate!r}'
     if pending.g is not None:
         blk.g = _in_place('pending.g', pending.g, (N, P, H) if gate == 'scalar' else (N, P, H, dk), f32, index)
@@ -1859,26 +1863,27 @@ def _draft_call(index, dt, gate, delta, operands, state, pending, accepted, L, l
         'a conv needs its weights, its caches and a pending block with its inputs'
     conv = keep = None
     if conv_cache is not None:
-        assert len(conv_weights) == len(conv_cache) == len(pending.x) == 3, 'the short conv is that of q, k and v'
-        K = conv_weights[0].shape[-1]
-        wdt = f32 if all(w.dtype is f32 for w in conv_weights) else dt
-        conv = _lib.ShortConv(kernel_size=K, weight_dtype=_DTYPES[wdt])
-        keep, at, xs = [], [], []
-        for name, w, c, x, d in zip('qkv', conv_weights, conv_cache, pending.x, (H * dk, H * dk, H * dv)):
-            assert w.shape == (d, 1, K) or w.shape == (d, K), f'conv weight must be ({d}, {K}) or ({d}, 1, {K}); got {tuple(w.shape)}'
-            at.append(_in_place(f'conv cache {name}', c, (N, K, d), dt, index))
-            xs.append(_in_place(f'pending.x {name}', x, (N, P, d), dt, index))
-            keep.append(w if w.dtype is wdt and w.is_contiguous() else w.to(wdt).contiguous())
-        _all_on(index, *keep)
-        conv.weight_q, conv.weight_k, conv.weight_v = (w.data_ptr() for w in keep)
-        conv.cache_q, conv.cache_k, conv.cache_v = at
-        blk.x_q, blk.x_k, blk.x_v = xs
+        (wq, wk, wv), (cq, ck, cv), (xq, xk, xv) = conv_weights, conv_cache, pending.x
+        K, Dk, Dv = wq.shape[-1], H * dk, H * dv
+        for w, d in ((wq, Dk), (wk, Dk), (wv, Dv)):
+            ws = w.shape
+            assert ws[0] == d and ws[-1] == K and w.numel() == d * K, \
+                f'conv weight must be ({d}, {K}) or ({d}, 1, {K}); got {tuple(ws)}'
+        wdt = f32 if wq.dtype is wk.dtype is wv.dtype is f32 else dt
+        keep = [w if w.dtype is wdt and w.is_contiguous() else w.to(wdt).contiguous() for w in (wq, wk, wv)]
+        cs, xs = (N, K, Dk), (N, P, Dk)
+        conv = _lib.ShortConv(keep[0].data_ptr(), keep[1].data_ptr(), keep[2].data_ptr(), _in_place('conv cache q', cq, cs, dt, index),
+                              _in_place('conv cache k', ck, cs, dt, index), _in_place('conv cache v', cv, (N, K, Dv), dt, index),
+                              K, _DTYPES[wdt])
+        blk.x_q, blk.x_k = _in_place('pending.x q', xq, xs, dt, index), _in_place('pending.x k', xk, xs, dt, index)
+        blk.x_v = _in_place('pending.x v', xv, (N, P, Dv), dt, index)
     q, k, v, g, beta, o = operands
     fz = None
     if fusion is not None:
         fz = _lib.Fusion(int(fusion.l2norm), int(fusion.beta), int(fusion.gate), _lib.VGDR_F32, None, None, 0, 0.0)
         if fusion.gate:
-            assert fusion.A_log.numel() == H and fusion.dt_bias.numel() == H * dk, f'A_log has {H} and dt_bias {H * dk} elements'
+            n_dt = H if gate == 'scalar' else H * dk
+            assert fusion.A_log.numel() == H and fusion.dt_bias.numel() == n_dt, f'A_log has {H} and dt_bias {n_dt} elements'
             params = [t if t.dtype is f32 and t.is_contiguous() else t.detach().float().contiguous()
                       for t in (fusion.A_log, fusion.dt_bias)]
             fz.A_log, fz.dt_bias, fz.gate_dtype = params[0].data_ptr(), params[1].data_ptr(), _DTYPES[g.dtype]
@@ -1888,7 +1893,7 @@ def _draft_call(index, dt, gate, delta, operands, state, pending, accepted, L, l
     if out_gate is not None:
         if gamma.dtype not in (f32, dt) or not gamma.is_contiguous() or gamma.data_ptr() % 16:
             gamma = _aligned(gamma if gamma.dtype in (f32, dt) else gamma.float())
-        ep = _lib.Epilogue(gate=out_gate.data_ptr(), gamma=gamma.data_ptr(), gamma_dtype=_DTYPES[gamma.dtype], eps=float(eps))
+        ep = _lib.Epilogue(out_gate.data_ptr(), gamma.data_ptr(), _DTYPES[gamma.dtype], float(eps))
     acc = _stream_counts('accepted', accepted, N, index)
     ref = ctypes.byref
     _launch(index, _lib.load().vgdr_draft_step, _DTYPES[dt], _GATE_KINDS[gate], int(delta), _ptr(q), _ptr(k), _ptr(v), _ptr(g),
@@ -1904,7 +1909,7 @@ def verify_drafts(logits, drafts, uniforms, *, temperature=1.0, draft_probs=None
     i, so that row i judges draft i and the last row follows the last draft; any strides over
     whole rows.  drafts (N, K) whole numbers (K = 0: a token is sampled, nothing verified).  uniforms
     (N, K + 1) fp32 in [0, 1): one per draft, the last for the token behind them.  temperature: a
-    number or (N,); 0 is greedy.  draft_probs (N, K, V): the probabilities that the drafts were drawn
+    number or (N,); 0 (in a tensor anything not above it) is greedy.  draft_probs (N, K, V): the probabilities that the drafts were drawn
     from; None: the drafts were certain (looked up, or greedy).  n_drafts (N,): how many of its
     K a stream has.
 
