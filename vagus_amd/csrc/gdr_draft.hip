@@ -286,33 +286,77 @@ draft_block_kernel(const DraftParams p) {
         for (int c = dk + tid; c < DKP; c += nt)
             for (int t = 0; t < LT; ++t) kk[t][c] = qq[t][c] = 0.f;
     lds_barrier();
-    // A and B: 16 lanes share the channels of key j, which decays from token to token
-    for (int j = wave + waves * g4; j < L; j += 4 * waves) {
-        f32x4 y[NC];
-        unroll<NC>([&](auto c) { y[c] = ld4(&kk[j][64 * c + 4 * r16]); });
-        for (int t = j; t < L; ++t) {
-            float sa = 0.f, sb = 0.f, sq = 0.f;
-            const float e1 = GATE == 2 ? 1.f : es[0][t];
-            unroll<NC>([&](auto c) {
-                const f32x4 k4 = ld4(&kk[t][64 * c + 4 * r16]), q4 = ld4(&qq[t][64 * c + 4 * r16]);
-                if (t > j) y[c] *= GATE == 2 ? ld4(&es[GATE == 2 ? t : 0][64 * c + 4 * r16]) : f32x4{e1, e1, e1, e1};
-                unroll<4>([&](auto i) {
-                    sa += k4[i.value] * y[c][i.value];
-                    sb += q4[i.value] * y[c][i.value];
-                    sq += q4[i.value] * q4[i.value];
+    // A and B
+    if (GATE == 2) {
+        // per channel: 16 lanes share the channels of key j, which decays from token to token
+        for (int j = wave + waves * g4; j < L; j += 4 * waves) {
+            f32x4 y[NC];
+            unroll<NC>([&](auto c) { y[c] = ld4(&kk[j][64 * c + 4 * r16]); });
+            for (int t = j; t < L; ++t) {
+                float sa = 0.f, sb = 0.f, sq = 0.f;
+                unroll<NC>([&](auto c) {
+                    const f32x4 k4 = ld4(&kk[t][64 * c + 4 * r16]), q4 = ld4(&qq[t][64 * c + 4 * r16]);
+                    if (t > j) y[c] *= ld4(&es[GATE == 2 ? t : 0][64 * c + 4 * r16]);
+                    unroll<4>([&](auto i) {
+                        sa += k4[i.value] * y[c][i.value];
+                        sb += q4[i.value] * y[c][i.value];
+                        sq += q4[i.value] * q4[i.value];
+                    });
                 });
-            });
-            sa = row_sum16(sa);
-            sb = row_sum16(sb);
-            if (t == j) sq = row_sum16(sq);
-            if (r16 == 0) {
-                aa[t][j] = sa;
-                bb[t][j] = sb;
-                if (t == j) {
-                    rk[t] = p.fz.qk_l2norm ? rsqrtf(sa + 1e-6f) : 1.f;
-                    rq[t] = p.scale * (p.fz.qk_l2norm ? rsqrtf(sq + 1e-6f) : 1.f);
+                sa = row_sum16(sa);
+                sb = row_sum16(sb);
+                if (t == j) sq = row_sum16(sq);
+                if (r16 == 0) {
+                    aa[t][j] = sa;
+                    bb[t][j] = sb;
+                    if (t == j) {
+                        rk[t] = p.fz.qk_l2norm ? rsqrtf(sa + 1e-6f) : 1.f;
+                        rq[t] = p.scale * (p.fz.qk_l2norm ? rsqrtf(sq + 1e-6f) : 1.f);
+                    }
                 }
             }
+        }
+    } else {
+        // [K; Q] K^T by MFMA, two tiles of channels to a wave, joined in LDS in a fixed order, and the tokens'
+        // decays between (blocks of 16, 128 streams of 16 heads: 97 us with the loop above)
+        constexpr int SHARES = RT / 2, TILES = LT / 8;
+        float *shares = &prod[0][0];                               // [SHARES][TILES][16][16]
+        if (wave < SHARES) {
+            f32x4 y[TILES];
+            unroll<TILES>([&](auto m) { y[m] = f32x4{0.f, 0.f, 0.f, 0.f}; });
+            unroll<2>([&](auto s) {
+                const int c = 16 * (2 * wave + s) + 4 * g4;
+                const f32x4 k4 = ld4(&kk[r16 % LT][c]), q4 = ld4(&qq[r16 % LT][c]);
+                if (LT == 8) {
+                    y[0] = mfma_kb1(r16 < 8 ? k4 : q4, k4, y[0]);
+                } else {
+                    y[0] = mfma_kb1(k4, k4, y[0]);
+                    y[TILES - 1] = mfma_kb1(q4, k4, y[TILES - 1]);
+                }
+            });
+            unroll<TILES>([&](auto m) {
+                unroll<4>([&](auto j) { shares[((wave * TILES + m) * 16 + 4 * g4 + j) * 16 + r16] = y[m][j.value]; });
+            });
+        }
+        for (int t = wave; t < L; t += waves) {
+            float s = 0.f;
+            for (int c = lane; c < dk; c += 64) s += qq[t][c] * qq[t][c];
+            s = wave_sum64(s);
+            if (lane == 0) rq[t] = p.scale * (p.fz.qk_l2norm ? rsqrtf(s + 1e-6f) : 1.f);
+        }
+        lds_barrier();
+        for (int i = tid; i < L * LT; i += nt) {
+            const int t = i / LT, j = i % LT;
+            if (j > t) continue;
+            float sa = 0.f, sb = 0.f, run = 1.f;
+            unroll<SHARES>([&](auto w) {
+                sa += shares[(w * TILES * 16 + t) * 16 + j];
+                sb += shares[(w * TILES * 16 + LT + t) * 16 + j];
+            });
+            for (int e = j + 1; e <= t; ++e) run *= es[0][e];
+            aa[t][j] = run * sa;
+            bb[t][j] = run * sb;
+            if (j == t) rk[t] = p.fz.qk_l2norm ? rsqrtf(sa + 1e-6f) : 1.f;
         }
     }
     // what the accepted writes weigh at their block's end
