@@ -128,10 +128,22 @@ __device__ __forceinline__ float row_prefix16(float x) {
 
 // One workgroup per (stream, head). A wave holds 64 rows x 64 columns of the state in the C layout of
 // 16 x 16 tiles: lane 16 g + r has rows 16 i + 4 g + j (i, j < 4) of columns 4 r .. 4 r + 3, so that an
-// access touches four rows of 256 bytes. As it lies it is the B operand of the product with [K; Q], whose
+// access touches four rows of 256 bytes (32 columns a wave, 128 bytes a row: a bare copy of the state
+// took 42 us where this takes 26). As it lies it is the B operand of the product with [K; Q], whose
 // two halves of rows (dk > 64) meet in LDS.  q and k are kept unnormalised: the norms are A's and
 // q's own diagonals and scale the results.  RT: row tiles (dk <= 16 RT). LT: room of the pending
-// block and tokens (8 or 16).  At least 128 (RT 4) or 256 threads, and a thread per pair of q, k, v channels.
+// block and tokens: 16, or 8, whose [K; Q] is one tile of 16 rows and which leaves registers and LDS
+// for four workgroups a CU (three at 16).  At least 128 (RT 4) or 256 threads, two per value
+// channel, and one per pair of q, k, v channels.
+//
+// Bound by the state's way in and out: 64 streams of 16 128 x 128 heads, bf16, blocks of 5: 28 us for 161 MB
+// (5.7 TB/s; the traffic counters read 156 MB), of which the products and the solve, which the
+// stores cover in part, are 5; 128 streams, blocks of 16: 93-97 us for 411 MB, where the product with the state costs
+// 9, the solve 13 and the outputs 6. One workgroup a CU (64 streams of 4 128 x 256 heads, per-channel
+// gates, blocks of 8) is a chain of latencies: 25 us for 83 MB. One stream: 10 us.
+// Measured and left out: the operands' loads ahead of the state's (b64 31.1 -> 33.1 us), stores before
+// the products (32.6) or behind the solve (32.9), ws and the products in one LDS area for a fourth
+// workgroup at 16 tokens (97 -> 135 us with the registers that takes).
 template <typename E, int GATE, int RT, int LT, int NT>
 __global__ void __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(GATE == 2 && RT == 8 ? (NT == 256 ? 3 : 2) : LT == 8 ? 4 : NT == 256 ? 3 : 2)))
 draft_block_kernel(const DraftParams p) {
