@@ -103,6 +103,27 @@ def test_borders_of_the_uniform_numbers():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('V,dtype,probs', [(32000, torch.bfloat16, False), (1003, torch.float32, True), (131071, torch.float16, True)])
+def test_uniforms_at_the_acceptance_border(V, dtype, probs):
+    """Uniform numbers that are the fp32 neighbours of p(d) / q(d), half a step (2^-24) from it or less:
+    what an fp32 sum cannot tell, and 64 bits can."""
+    N = 24
+    x, d, u, q = make(N, 2, V, dtype, probs, seed=12)
+    if probs:
+        q = q.to(torch.float16)
+    p = torch.softmax(x.double(), -1)
+    pd = p[:, :2].gather(2, d[..., None])[..., 0]
+    if probs:
+        pd = pd / q.double().gather(2, d[..., None])[..., 0]
+    at = pd.float().clamp(max=1 - 2.0 ** -24)
+    for way in (0.0, 2.0, None):
+        u[:, :2] = at if way is None else torch.nextafter(at, torch.full_like(at, way)).clamp(0, 1 - 2.0 ** -24)
+        _, counts = check(x, d, u, 1.0, q)
+        if way is not None and not probs:
+            assert int((counts > 0).sum()) == (N if way == 0.0 else 0)
+
+
+@pytest.mark.gpu
 def test_masks_infinities_and_nan():
     V = 600
     x, d, u, q = make(6, 2, V, torch.float32, True, seed=5)
@@ -212,6 +233,45 @@ def test_streams_and_graphs():
         want = ops.verify_drafts(x, d, u, draft_probs=q)
         assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
         assert looked[1].tolist() == [3, 3]
+
+
+@pytest.mark.gpu
+def test_two_graphs_replayed_in_turn():
+    """Each recorded call has its own workspace; other work runs between the replays."""
+    sides = []
+    for seed in (1, 2):
+        x, d, u, q = (t.cuda() for t in make(6, 3, 9001, torch.bfloat16, True, seed))
+        h = torch.randint(0, 3, (3, 30000), device='cuda', generator=torch.Generator('cuda').manual_seed(seed))
+        n = torch.tensor([30000, 7, 12345], device='cuda', dtype=torch.int32)
+        ops.verify_drafts(x, d, u, draft_probs=q), ops.lookup_drafts(h, n, 5, max_ngram=16)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.verify_drafts(x, d, u, draft_probs=q) + ops.lookup_drafts(h, n, 5, max_ngram=16)
+        sides.append((graph, out, (x, d, u, q, h, n)))
+    for step in range(3):
+        for graph, out, (x, d, u, q, h, n) in sides:
+            u.copy_(torch.rand(6, 4, generator=torch.Generator().manual_seed(step)))
+            h[1, :7] = torch.tensor([1, 2, step, 9, 1, 2, step], device='cuda')
+        for graph, out, _ in sides + sides[::-1]:
+            graph.replay()
+        torch.cuda.synchronize()
+        for graph, out, (x, d, u, q, h, n) in sides:
+            want = ops.verify_drafts(x, d, u, draft_probs=q) + ops.lookup_drafts(h, n, 5, max_ngram=16)
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.gpu
+def test_more_streams_than_a_grid_dimension():
+    n = 40000
+    h = torch.arange(12, device='cuda').remainder(5).expand(n, 12).contiguous()
+    h[:, -1] = torch.arange(n, device='cuda') % 5
+    drafts, counts = ops.lookup_drafts(h, torch.full((n,), 12, device='cuda'), 2, max_ngram=2)
+    want = [looked_up(h[b].tolist(), 12, 2, 2, 1) for b in range(5)]
+    for b in range(5):
+        assert bool((drafts[b::5] == torch.tensor(want[b][0], device='cuda')).all())
+    assert bool((counts == 2).all())
+    empty = ops.lookup_drafts(h[:3, :0], torch.tensor([0, 5, -1], device='cuda'), 2)
+    assert empty[0].tolist() == [[0, 0]] * 3 and empty[1].tolist() == [0, 0, 0]
 
 
 @pytest.mark.gpu

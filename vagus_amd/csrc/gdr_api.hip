@@ -1467,7 +1467,7 @@ int vgdr_lookup_drafts(const void *history, int token_bytes, int64_t ld, int64_t
     if (min_ngram < 1 || max_ngram < min_ngram || max_ngram > 16)
         return fail(VGDR_ERR_INVALID, "%s: 1 <= min_ngram <= max_ngram <= 16, got %d, %d", fn, min_ngram, max_ngram);
     if (B == 0) return VGDR_OK;
-    if (!history || !lengths || !drafts || !counts)
+    if ((cap > 0 && !history) || !lengths || !drafts || !counts)
         return fail(VGDR_ERR_INVALID, "%s: history, lengths, drafts and counts are required", fn);
     if (B > 1 && ld < cap) return fail(VGDR_ERR_INVALID, "%s: rows of %lld tokens, %lld apart", fn, (long long)cap, (long long)ld);
     const int64_t need = vgdr::lookup_workspace(B, cap);
