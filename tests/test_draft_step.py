@@ -329,6 +329,28 @@ def test_streams_and_graphs():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('L', [1, 4])
+def test_layouts_of_the_inputs(L):
+    """(N, L, H, d) operands, rows of one buffer at any place, transposed streams: the same bits."""
+    c = make(3, L, 2, 64, 128, gate='vector', dtype=torch.bfloat16, seed=97)
+    accepted = [0, L, 1]
+    want, want_state = run(c, accepted)[:2]
+    acc = torch.tensor(accepted, device='cuda')
+
+    def again(f):
+        (q, k, v), g, beta, state, pending, cache, kw = device(c)
+        kw['out_gate'] = f(kw['out_gate'])
+        g, beta = (t.transpose(0, 1).contiguous().transpose(0, 1) for t in (g, beta))
+        return ops.hip_draft_step(f(q), f(k), f(v), g, beta, state, pending, acc, **kw), state
+
+    shift = lambda t: torch.cat([t[..., :3], t], -1)[..., 3:]  # noqa: E731 -- rows 6 bytes off their alignment
+    for f in (lambda t: t.view(3, L, 2, -1), shift, lambda t: t.transpose(0, 1).contiguous().transpose(0, 1),
+              lambda t: torch.cat([t, t], 1)[:, :L], lambda t: t.view(3, L, 2, -1).transpose(1, 2).contiguous().transpose(1, 2)):
+        o, s = again(f)
+        assert torch.equal(o, want) and torch.equal(s, want_state)
+
+
+@pytest.mark.gpu
 def test_no_streams():
     c = make(1, 3, 2, 64, 64, seed=95)
     (q, k, v), g, beta, state, pending, cache, kw = device(c)

@@ -56,7 +56,7 @@ def rel(x, ref):
 @pytest.mark.parametrize('gate,dtype,kw', [
     ('scalar', torch.float32, {}), ('vector', torch.float32, {}), ('none', torch.float32, {}),
     ('scalar', torch.float32, dict(delta=False)), ('vector', torch.float32, dict(gate_lower_bound=-3.0)),
-    ('scalar', torch.float32, dict(short_conv_size=3)), ('scalar', torch.float32, dict(key_head_dim=32, value_head_dim=128)),
+    ('scalar', torch.float32, dict(short_conv_size=3)), ('vector', torch.float32, dict(short_conv_size=None)), ('scalar', torch.float32, dict(key_head_dim=32, value_head_dim=128)),
     ('scalar', torch.float32, dict(out_proj=False, value_head_dim=128)),
     ('scalar', torch.bfloat16, {}), ('vector', torch.bfloat16, dict(value_head_dim=256))])
 def test_layer_blocks_are_its_one_token_steps(gate, dtype, kw):
@@ -90,6 +90,26 @@ def test_layer_blocks_are_its_one_token_steps(gate, dtype, kw):
             for n in ('qp_cache', 'kp_cache', 'vp_cache'):
                 # the projections' order of sums differs between one row and twelve
                 assert rel(got[n][b], end[n][0]) <= (1e-5 if dtype == torch.float32 else 2 ** -8)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('gate', ['scalar', 'vector', 'none'])
+def test_many_rows(gate):
+    """70 streams of 4 tokens: more rows than one projection launch takes (256), as the blocks of 10
+    streams each, which it does."""
+    m = layer(gate, torch.float32)
+    x = torch.randn(70, 4, 128, generator=torch.Generator().manual_seed(8)).cuda()
+    zero, two = (torch.full((70,), n, dtype=torch.int32, device='cuda') for n in (0, 2))
+    m.reset_cache(70)
+    m.begin_drafts(4)
+    m.draft_step(x, zero)
+    got, state = m.draft_step(x.flip(1), two), m.state.clone()
+    for b in range(0, 70, 10):
+        m.reset_cache(10)
+        m.begin_drafts(4)
+        m.draft_step(x[b:b + 10], zero[:10])
+        want = m.draft_step(x[b:b + 10].flip(1), two[:10])
+        assert rel(got[b:b + 10], want) <= 1e-5 and rel(state[b:b + 10], m.state) <= 1e-5
 
 
 @pytest.mark.gpu
