@@ -194,6 +194,23 @@ def test_drafted_and_one_token_calls_in_turn():
 
 
 @pytest.mark.gpu
+def test_a_recorded_step_knows_every_tensor_of_its_blocks():
+    """A block's log-decays that lie elsewhere: the step is recorded again."""
+    m = varied(torch.float32)
+    ps = repeating([12, 33, 8], seed=4)
+    gen = RaggedGenerator(m)
+    gen.prefill(ps)
+    want = gen.generate_drafted(30)
+    att = m.blocks[1].att
+    for name in ('k', 'u', 'g'):
+        key, old = gen._drafted_fingerprint(), getattr(att._drafted, name)
+        setattr(att._drafted, name, torch.zeros_like(old))
+        assert gen._drafted_fingerprint() != key
+    gen.prefill(ps)
+    assert torch.equal(gen.generate_drafted(30), want)
+
+
+@pytest.mark.gpu
 def test_sampled_decoding():
     """The same uniform numbers give the same tokens, eagerly and replayed; at a temperature near 0
     they are the greedy ones; every token is in the vocabulary."""

@@ -491,4 +491,5 @@ class RaggedGenerator:
         """What a recorded drafted step holds by address beside _fingerprint: the pending tokens and
         every layer's drafted block."""
         ds = [blk.att._drafted for blk in self.model.blocks]
-        return (self.pending.data_ptr(),) + tuple(t.data_ptr() for d in ds for t in (d.k, d.u, *(d.x or ())))
+        return (self.pending.data_ptr(),) + tuple(t.data_ptr() for d in ds for t in (d.k, d.u, d.g, *(d.x or ()))
+                                              if t is not None)
