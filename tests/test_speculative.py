@@ -56,7 +56,8 @@ def rel(x, ref):
 @pytest.mark.parametrize('gate,dtype,kw', [
     ('scalar', torch.float32, {}), ('vector', torch.float32, {}), ('none', torch.float32, {}),
     ('scalar', torch.float32, dict(delta=False)), ('vector', torch.float32, dict(gate_lower_bound=-3.0)),
-    ('scalar', torch.float32, dict(short_conv_size=3)), ('vector', torch.float32, dict(short_conv_size=None)), ('scalar', torch.float32, dict(key_head_dim=32, value_head_dim=128)),
+    ('scalar', torch.float32, dict(short_conv_size=3)), ('vector', torch.float32, dict(short_conv_size=None)),
+    ('scalar', torch.float32, dict(key_head_dim=32, value_head_dim=128)),
     ('scalar', torch.float32, dict(out_proj=False, value_head_dim=128)),
     ('scalar', torch.bfloat16, {}), ('vector', torch.bfloat16, dict(value_head_dim=256))])
 def test_layer_blocks_are_its_one_token_steps(gate, dtype, kw):
