@@ -659,7 +659,7 @@ int vgdr_swiglu(int dtype, const void *x, void *y, int64_t rows, int64_t hidden,
  *
  * vgdr_draft_block: what a block leaves behind.  Room for `capacity` (1..16) tokens per
  * stream; 16-byte aligned.  k [B, capacity, H, dk], u [B, capacity, H, dv] and g ([B, capacity,
- * H] or [B, capacity, H, dk]; NULL without a gate) in fp32: the block's keys as the recurrence
+ * H] or [B, capacity, H, dk]; ignored without a gate, may be NULL) in fp32: the block's keys as the recurrence
  * takes them, its writes u_t = beta_t (v_t - S^T k_t) (v_t without the delta rule) and log-decays.
  * x_q, x_k [B, capacity, H * dk], x_v [B, capacity, H * dv] in dtype: its raw conv inputs (NULL
  * without a conv).

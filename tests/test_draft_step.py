@@ -10,6 +10,8 @@ epilogue), so its error is under (dk + 2 L + K + 30) 2^-24 of the terms' size, a
 norm. o is then rounded once to its type: half a step more, 2^-8 (bf16) or 2^-11 (fp16) of
 each value. Caches and raw inputs are copies: equal bits.
 """
+import ctypes
+
 import pytest
 import torch
 import torch.nn.functional as F
@@ -412,6 +414,34 @@ def test_refusals():
     with pytest.raises(NotImplementedError, match='multiples of 8'):
         ops.hip_draft_step(z[..., :60], z[..., :60], z, None, torch.zeros(1, 1, 1, device='cuda'), s,
                            ops.DraftBlock.empty(s, 1, gate='none'), acc[:1], scale=1.0)
+
+
+@pytest.mark.gpu
+def test_without_a_gate_log_decays_are_not_looked_at():
+    """The C entry without a gate: log-decays, or room for them in the block, change no bit and stay as they are."""
+    c = make(3, 4, 2, 64, 64, gate='none', K=0, epilogue=False, l2norm=False, logits=False, seed=98)
+    accepted = torch.tensor([0, 4, 2], dtype=torch.int32, device='cuda')
+    lib = _lib.load()
+
+    def call(g, room):
+        (q, k, v), _, beta, state, pending, _, _ = device(c)
+        pg = torch.full((3, 4, 2), -1.5, device='cuda') if room else None
+        gs = torch.full((3, 4, 2), -0.5, device='cuda') if g else None
+        blk = _lib.DraftBlock(pending.k.data_ptr(), pending.u.data_ptr(), pg.data_ptr() if room else None, None, None, None, 4)
+        outs = []
+        for L in (4, 0):                                   # a block behind the last one's, and its commit alone
+            o = torch.zeros(3, 4, 2, 64, device='cuda')
+            _lib.check(lib.vgdr_draft_step(
+                _lib.VGDR_F32, _lib.VGDR_GATE_NONE, 1, q.data_ptr(), k.data_ptr(), v.data_ptr(), gs.data_ptr() if g else None,
+                beta.data_ptr(), o.data_ptr(), state.data_ptr(), ctypes.byref(blk), accepted.data_ptr(), 3, L, 2, 64, 64, 128, 128,
+                0.125, None, None, None, torch.cuda.current_stream().cuda_stream))
+            outs += [o, state.clone()]
+        assert not room or bool((pg == -1.5).all())
+        return [*outs, pending.k, pending.u]
+
+    want = call(False, False)
+    for g, room in ((True, True), (False, True), (True, False)):
+        assert all(torch.equal(x, y) for x, y in zip(call(g, room), want)), (g, room)
 
 
 def _call(**over):

@@ -1371,13 +1371,14 @@ int vgdr_draft_step(int dtype, int gate_kind, int use_delta, const void *q, cons
     p.q = q;
     p.k = k;
     p.v = v;
-    p.g = g;
+    // without a gate neither log-decays nor room for them are looked at: the kernel has a gate where pg is set
+    p.g = gate_kind == VGDR_GATE_NONE ? nullptr : g;
     p.beta = beta;
     p.o = o;
     p.S = state;
     p.pk = pending->k;
     p.pu = pending->u;
-    p.pg = pending->g;
+    p.pg = gate_kind == VGDR_GATE_NONE ? nullptr : pending->g;
     p.xq = pending->x_q;
     p.xk = pending->x_k;
     p.xv = pending->x_v;
