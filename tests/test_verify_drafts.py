@@ -275,6 +275,37 @@ def test_more_streams_than_a_grid_dimension():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('K', [0, 1])
+def test_eight_million_streams(K):
+    """2^23 streams, sampled and greedy: the choosing workgroups' threads pass 2^32."""
+    n, V = 1 << 23, 3
+    r = torch.Generator('cuda').manual_seed(12)
+    x = torch.randn(n, K + 1, V, generator=r, device='cuda')
+    T = (torch.arange(n, device='cuda') % 4 > 0).float()
+    drafts = torch.randint(0, V, (n, K), generator=r, device='cuda')
+    u = torch.rand(n, K + 1, generator=r, device='cuda')
+    tokens, accepted = ops.verify_drafts(x, drafts, u, temperature=T)
+    p = torch.where(T[:, None, None] > 0, x.double().softmax(-1),
+                    torch.nn.functional.one_hot(x.argmax(-1), V).double())
+    stood = u[:, 0].double() < p[:, 0].gather(1, drafts)[:, 0] if K else torch.zeros(n, dtype=torch.bool, device='cuda')
+    # the row behind what stands, without a refused draft
+    rest = p[torch.arange(n, device='cuda'), stood.long()]
+    if K:
+        refused = (~stood[:, None] & (T[:, None] > 0)) & (torch.arange(V, device='cuda')[None] == drafts)
+        rest = torch.where(refused, 0.0, rest)
+    one, two = rest[:, 0], rest[:, 0] + rest[:, 1]
+    goal = u[:, K].double() * (two + rest[:, 2])
+    last = torch.where(one > goal, 0, torch.where(two > goal, 1, 2))
+    want = torch.full((n, K + 1), -1, device='cuda')
+    if K:
+        want[:, 0] = torch.where(stood, drafts[:, 0], last)
+        want[:, 1] = torch.where(stood, last, -1)
+    else:
+        want[:, 0] = last
+    assert torch.equal(accepted, stood.int()) and torch.equal(tokens, want)
+
+
+@pytest.mark.gpu
 def test_refusals():
     x, d, u, q = (t.cuda() for t in make(2, 3, 50, torch.float32, True, seed=11))
     with pytest.raises(AssertionError, match='drafts'):

@@ -425,7 +425,8 @@ template <typename E>
 __global__ void __launch_bounds__(64 * WAVES) choose_kernel(const VerifyParams p) {
     __shared__ double part[WAVES], part2[WAVES];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), K = p.K;
-    const int64_t n = blockIdx.x, blocks = p.blocks;
+    const int64_t n = blockIdx.y + (int64_t)blockIdx.z * gridDim.y, blocks = p.blocks;
+    if (n >= p.N) return;
     const float t = p.temperature[n];
     const Stood st = p.stood[n];
     const int n_drafts = drafts_of(p, n);
@@ -498,7 +499,7 @@ int64_t verify_workspace(int64_t N, int64_t K, int64_t V) {
 }
 
 template <typename E> static void verify_typed(const VerifyParams &p, hipStream_t stream) {
-    // rows and streams over two grid dimensions of at most 65,535
+    // rows and streams over two grid dimensions of at most 65,535: one dimension holds under 2^32 threads, 2^23 streams
     const int64_t rows = p.N * (p.K + 1), ry = rows < 32768 ? rows : 32768, ny = p.N < 32768 ? p.N : 32768;
     row_mass_kernel<E><<<dim3((unsigned)((p.chunks + ROW_WAVES - 1) / ROW_WAVES), (unsigned)ry, (unsigned)((rows + ry - 1) / ry)),
                          dim3(64 * ROW_WAVES), 0, stream>>>(p);
@@ -507,7 +508,7 @@ template <typename E> static void verify_typed(const VerifyParams &p, hipStream_
     const dim3 grid((unsigned)(most < share ? most : share), (unsigned)ny, (unsigned)((p.N + ny - 1) / ny));
     stand_kernel<E><<<grid, dim3(64 * WAVES), 0, stream>>>(p);
     if (p.probs) rest_kernel<E><<<grid, dim3(64 * WAVES), 0, stream>>>(p);
-    choose_kernel<E><<<dim3((unsigned)p.N), dim3(64 * WAVES), 0, stream>>>(p);
+    choose_kernel<E><<<dim3(1, grid.y, grid.z), dim3(64 * WAVES), 0, stream>>>(p);
 }
 
 hipError_t verify_drafts(int dtype, VerifyParams p, void *workspace, hipStream_t stream) {
