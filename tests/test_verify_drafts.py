@@ -417,3 +417,12 @@ def test_entry_points_refuse_before_they_launch():
     assert lookup(tb=2) == bad and lookup(ld=99) == bad and lookup(K=0) == bad and lookup(K=65) == bad
     assert lookup(hi=17) == bad and lookup(lo=0) == bad and lookup(hi=1, lo=2) == bad and lookup(h=None) == bad
     assert lookup(cap=-1) == bad and lookup(B=0) == _lib.VGDR_OK
+
+
+def test_row_counts_past_64_bits_are_refused():
+    """B (K + 1) rows are counted without an overflow."""
+    L = _lib.load()
+    for B, K in ((1 << 62, 3), ((1 << 63) - 1, 1), (1 << 24, 1)):
+        assert L.vgdr_verify_drafts_workspace_size(B, K, 100) == 0 and b'too many rows' in L.vgdr_last_error()
+        rc = L.vgdr_verify_drafts(0, 16, 400, 100, 32, 48, 64, None, 0, 0, 0, None, 80, 96, 112, 1 << 62, B, K, 100, None)
+        assert rc == _lib.VGDR_ERR_INVALID and b'too many rows' in L.vgdr_last_error()

@@ -1402,7 +1402,7 @@ static int check_verify(const char *fn, int64_t B, int64_t K, int64_t V) {
     if (B < 0 || K < 0 || V < 1 || V >= 0x7ff00000LL)
         return fail(VGDR_ERR_INVALID, "%s: bad sizes B=%lld K=%lld V=%lld", fn, (long long)B, (long long)K, (long long)V);
     if (K > 64) return fail(VGDR_ERR_UNSUPPORTED, "%s: K=%lld drafts (at most 64)", fn, (long long)K);
-    if (B * (K + 1) > 0x1000000LL) return fail(VGDR_ERR_INVALID, "%s: too many rows", fn);
+    if (B > 0x1000000LL / (K + 1)) return fail(VGDR_ERR_INVALID, "%s: too many rows", fn);
     return VGDR_OK;
 }
 
