@@ -681,7 +681,7 @@ typedef struct vgdr_draft_block {
  * softplus(f + dt_bias) with A_log and dt_bias [H]), but that no intermediate is
  * rounded to dtype and that the conv takes any kernel size 1..8.  Pending rows from L on
  * are left as they were.  dk a multiple of 8 up to 128, dv a multiple of 8 up to 256, H * dk and
- * H * dv up to 2^24.
+ * H * dv up to 2^24, B * H under 2^32 threads, of which a workgroup of one has 128 to 512.
  */
 int vgdr_draft_step(int dtype, int gate_kind, int use_delta, const void *q, const void *k, const void *v,
                     const void *g, const float *beta, void *o, float *state, const vgdr_draft_block *pending,

@@ -477,3 +477,12 @@ def test_entry_point_refuses_before_it_launches():
     assert _call(ep=_lib.Epilogue(None, 16, 0, 1e-6)) == bad
     assert _call(H=1 << 19, ld_qk=1 << 25, ld_v=1 << 25) == no and _call(B=1 << 31) == no
     assert _call(B=0) == _lib.VGDR_OK
+
+
+def test_more_heads_than_a_launch_holds_are_refused():
+    """A workgroup of 128 (dk, dv up to 64), 256 (up to 128) or 512 threads a (stream, head): under 2^32 threads a launch."""
+    no = _lib.VGDR_ERR_UNSUPPORTED
+    for d, threads in (((64, 64), 128), ((128, 128), 256), ((128, 256), 512)):
+        ld = [max(2 * n, 128) for n in d]
+        assert _call(B=(1 << 31) // threads, H=2, dk=d[0], dv=d[1], ld_qk=ld[0], ld_v=ld[1]) == no
+        assert b'too many' in _lib.load().vgdr_last_error()

@@ -1333,8 +1333,8 @@ int vgdr_draft_step(int dtype, int gate_kind, int use_delta, const void *q, cons
                     fn, vgdr::DRAFT_MAX);
     if (L > pending->capacity)
         return fail(VGDR_ERR_INVALID, "%s: L=%lld tokens, room for %lld", fn, (long long)L, (long long)pending->capacity);
-    // a stream's pending block lies within 2^30 bytes: the kernels' 32-bit offsets
-    if (B > 0x7fffffffLL / H || H > 0x1000000LL / (dk > dv ? dk : dv))
+    // a stream's pending block lies within 2^30 bytes: the kernels' 32-bit offsets; a launch holds under 2^32 threads
+    if (H > 0x1000000LL / (dk > dv ? dk : dv) || B > 0xffffffffLL / vgdr::draft_threads(dk, dv) / H)
         return fail(VGDR_ERR_UNSUPPORTED, "%s: too many (stream, head) pairs", fn);
     if (B == 0) return VGDR_OK;
     vgdr::DraftParams p{};

@@ -534,15 +534,18 @@ draft_block_kernel(const DraftParams p) {
     });
 }
 
+// a wave per 64 x 64 of the state, a thread per pair of q, k, v channels and per two key or value channels of
+// LT / 4 tokens
+int64_t draft_threads(int64_t dk, int64_t dv) {
+    const int64_t rt = dk <= 64 ? 4 : 8, tiles = rt / 4 * ((dv + 63) / 64), pairs = (dk + dv / 2 + 63) / 64, least = (dv + 31) / 32;
+    int64_t waves = tiles > pairs ? tiles : pairs;
+    waves = waves > least ? waves : least;
+    return 64 * (waves > rt / 2 ? waves : rt / 2);
+}
+
 template <typename E, int GATE, int RT, int LT>
 static hipError_t draft_launch(const DraftParams &p, hipStream_t stream) {
-    // a wave per 64 x 64 of the state, a thread per pair of q, k, v channels and per two key or value channels of
-    // LT / 4 tokens
-    const int tiles = RT / 4 * ((p.dv + 63) / 64), pairs = (p.dk + p.dv / 2 + 63) / 64, least = (p.dv + 31) / 32;
-    int waves = tiles > pairs ? tiles : pairs;
-    waves = waves > least ? waves : least;
-    waves = waves > RT / 2 ? waves : RT / 2;
-    const dim3 grid((unsigned)(p.N * p.H)), block(64 * waves);
+    const dim3 grid((unsigned)(p.N * p.H)), block((unsigned)draft_threads(p.dk, p.dv));
     if (p.dv <= 128) draft_block_kernel<E, GATE, RT, LT, 256><<<grid, block, 0, stream>>>(p);
     else draft_block_kernel<E, GATE, RT, LT, 512><<<grid, block, 0, stream>>>(p);
     return hipGetLastError();

@@ -372,6 +372,7 @@ struct DraftParams {
     ShortConv cv;
 };
 hipError_t draft_step(int gate, const DraftParams &p, hipStream_t stream);
+int64_t draft_threads(int64_t dk, int64_t dv);    // of the workgroup of a (stream, head)
 
 // Drafts against the target's logits (gdr_verify.hip), N streams of K drafts.
 struct RowMass {                  // a chunk of a row
