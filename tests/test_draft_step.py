@@ -444,6 +444,27 @@ def test_without_a_gate_log_decays_are_not_looked_at():
         assert all(torch.equal(x, y) for x, y in zip(call(g, room), want)), (g, room)
 
 
+@pytest.mark.parametrize('dtype', [torch.int64, torch.uint32, torch.int32, torch.int16, torch.uint8])
+def test_counts_of_wider_types_do_not_wrap(dtype):
+    """Counts are clamped by the kernels: one that int32 does not hold must not come in as another."""
+    counts = [n for n in (0, 5, 127, 2 ** 31 - 1, 2 ** 31, 2 ** 32 - 1, 2 ** 32 + 3, 2 ** 62, -1, -2 ** 32 + 3)
+              if torch.iinfo(dtype).min <= n <= torch.iinfo(dtype).max]
+    t = torch.tensor(counts, dtype=torch.int64).to(dtype)
+    got = ops._stream_counts('counts', t, len(counts), -1)
+    assert got.dtype == torch.int32
+    room = 2 ** 31 - 1                                         # as the kernels clamp, for the largest room there is
+    assert [min(max(n, 0), room) for n in got.tolist()] == [min(max(n, 0), room) for n in counts]
+
+
+@pytest.mark.gpu
+def test_counts_that_int32_does_not_hold():
+    """2^32 + 1 accepted tokens are as many as there is room for, -2^32 + 1 are none."""
+    c = make(2, 4, 2, 64, 64, seed=51)
+    args, g, beta, state, pending, cache, kw = device(c)
+    o = ops.hip_draft_step(*args, g, beta, state, pending, torch.tensor([2 ** 32 + 1, -2 ** 32 + 1], device='cuda'), **kw)
+    check(c, o, state, pending, cache, reference(c, [4, 0]))
+
+
 def _call(**over):
     blk = _lib.DraftBlock(16, 32, 48, 64, 80, 96, over.pop('P', 4))
     a = dict(dtype=1, gate=1, delta=1, q=16, k=32, v=48, g=64, beta=80, o=96, state=112, pending=blk, acc=128, B=2, L=3,

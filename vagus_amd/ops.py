@@ -1721,9 +1721,11 @@ def _in_place(name, t, shape, dtype, index):
 
 
 def _stream_counts(name, t, N, index):
-    """int32 (N,) counts of the streams for a kernel."""
+    """int32 (N,) counts of the streams for a kernel; what int32 does not hold stays beyond every bound."""
     assert t.shape == (N,) and t.get_device() == index and not t.is_floating_point() and t.dtype is not torch.bool, \
         f'{name} must be ({N},) whole numbers on GPU {index}; got {tuple(t.shape)}, {t.dtype}, {t.device}'
+    if t.dtype is not torch.int32 and torch.iinfo(t.dtype).max > 0x7fffffff:
+        t = t.to(torch.int64).clamp(-1, 0x7fffffff)
     return t if t.dtype is torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
 
 
