@@ -9,6 +9,8 @@ recurrence's results (2^-8 each, five in a row) where the block does not, the st
 2e-2, the other tests' bar against the oracle. Tokens: fp32 logits of 211 random ids
 are not within 1e-5 of each other at their top, so greedy tokens are equal.
 """
+import gc
+
 import pytest
 import torch
 
@@ -269,3 +271,57 @@ def test_model_logits_of_a_block():
     m.begin_drafts(6)
     got = m.draft_step(block, torch.zeros(2, dtype=torch.int32, device='cuda'))
     assert rel(got, want) <= 1e-4
+
+
+class Chain(torch.nn.Module):
+    """Stands for a model on the CPU: the token behind t is 5 t + 3 modulo 97."""
+    blocks = ()
+
+    def __init__(self):
+        super().__init__()
+        self.scale = torch.nn.Parameter(torch.ones(1))
+
+    def reset_cache(self, batch_size):
+        pass
+
+    def prefill_packed(self, tokens, cu_seqlens, *, rows=None, last_logits=True):
+        pass
+
+    def decode_step(self, tokens, *, return_logits=True):
+        return torch.nn.functional.one_hot((5 * tokens + 3) % 97, 97).float()
+
+
+def test_texts_of_the_streams():
+    """The streams' texts: their prompts and what every call made since, of any length; a prefill starts anew."""
+    gen = RaggedGenerator(Chain())
+    for lens, calls in (([5, 1, 9], (3, 0, 1, 600, 2, 1300)), ([5, 1, 9], ()), ([2], (1, 255, 1)), ([4, 300], (7,))):
+        ps = prompts(lens, 6, 97)
+        gen.prefill((torch.cat(ps), torch.tensor([0] + lens).cumsum(0)))
+        outs = []
+        for n in calls:
+            out = gen.generate(n, graph=False)
+            outs.append(out.clone())
+            out.fill_(-7)                              # the caller's to write
+        text, length = gen._texts(11)
+        assert text.shape[1] >= int(length.max()) + 11 and length.dtype == torch.int32
+        for b, p in enumerate(ps):
+            want = torch.cat([p] + [o[b] for o in outs])
+            assert length[b] == want.numel() and torch.equal(text[b, :want.numel()], want)
+            assert not text[b, want.numel():].any()
+
+
+def test_one_token_calls_hold_no_tensors_of_their_own():
+    """A server of one-token calls that never drafts: as many tensors behind 300 of them as behind two."""
+    gen = RaggedGenerator(Chain())
+    gen.prefill(prompts([5, 9], 6, 97))
+
+    def held():
+        gc.collect()
+        return sum(type(t) is torch.Tensor for t in gc.get_objects())
+
+    for _ in range(2):
+        gen.generate(1, graph=False)
+    before = held()
+    for _ in range(300):
+        gen.generate(1, graph=False)
+    assert held() <= before

@@ -295,7 +295,9 @@ class RaggedGenerator:
         self.fed_len: list[int] = []
         self._graph = None
         self._graph_key = None
-        self._text: list = []                         # the streams' tokens since the prefill: (ids, cu), then (N, n) blocks
+        self._prompts: tuple | None = None            # the last prefill's (ids (T,), their counts)
+        self._made: torch.Tensor | None = None        # (N, room): what was generated since, in the first _made_len columns
+        self._made_len = 0
         self._drafted: dict | None = None             # generate_drafted's buffers and recorded step
 
     def reset(self, batch_size: int) -> None:
@@ -305,11 +307,12 @@ class RaggedGenerator:
         if self.pending is None or batch_size != self.batch_size:
             self.pending = torch.zeros(batch_size, dtype=torch.int64, device=self.device)
             self._graph = None
+            self._made = None
         else:
             self.pending.zero_()
         self.batch_size = batch_size
         self.fed_len = [0] * batch_size
-        self._text = []
+        self._prompts, self._made_len = None, 0
 
     @torch.no_grad()
     def prefill(self, prompts) -> None:
@@ -332,7 +335,7 @@ class RaggedGenerator:
         self.reset(N)
         last = (cu[1:] - 1).long()
         self.pending.copy_(ids.index_select(0, last))
-        self._text = [(ids.clone(), lens)]            # ids may be the caller's
+        self._prompts = (ids.clone(), lens)           # ids may be the caller's
         keep = torch.ones(ids.numel(), dtype=torch.bool, device=self.device)
         keep[last] = False
         body = ids[keep]
@@ -388,24 +391,38 @@ class RaggedGenerator:
                         blk.att.cache_len = n
                     self._graph_key = self._fingerprint()
             self.fed_len = [n + 1 for n in self.fed_len]
-        self._text.append(out.clone())                # out is the caller's
+        self._keep(out)
         return out
+
+    def _keep(self, out) -> None:
+        """Generated tokens out (N, n) join the streams' texts, as a copy (out is the caller's) in a buffer
+        whose room doubles: a call adds no tensor of its own."""
+        n = out.shape[1]
+        if self._prompts is None or n == 0:
+            return
+        end = self._made_len + n
+        if self._made is None or end > self._made.shape[1]:
+            made = torch.empty(self.batch_size, max(256, 2 * end), dtype=torch.int64, device=self.device)
+            if self._made_len:
+                made[:, :self._made_len].copy_(self._made[:, :self._made_len])
+            self._made = made
+        self._made[:, self._made_len:end].copy_(out)
+        self._made_len = end
 
     def _texts(self, room: int):
         """(the streams' tokens so far, the pending one last (N, cap) int64, their counts (N,) int32),
         with room for `room` more each."""
-        assert self._text and isinstance(self._text[0], tuple), 'prefill first'
-        ids, lens = self._text[0]
-        more = torch.cat(self._text[1:], 1) if len(self._text) > 1 else ids.new_empty(self.batch_size, 0)
-        width = more.shape[1]
+        assert self._prompts is not None, 'prefill first'
+        ids, lens = self._prompts
+        width, dev = self._made_len, self.device
         cap = -(-(max(lens) + width + room) // 256) * 256
-        text = torch.zeros(self.batch_size, cap, dtype=torch.int64, device=self.device)
-        at = 0
-        for b, n in enumerate(lens):
-            text[b, :n] = ids[at:at + n]
-            text[b, n:n + width] = more[b]
-            at += n
-        return text, torch.tensor([n + width for n in lens], dtype=torch.int32, device=self.device)
+        text = torch.zeros(self.batch_size, cap, dtype=torch.int64, device=dev)
+        n = torch.tensor(lens, dtype=torch.int64, device=dev)
+        row = torch.repeat_interleave(torch.arange(self.batch_size, device=dev), n, output_size=sum(lens))
+        text[row, torch.arange(row.numel(), device=dev) - (n.cumsum(0) - n)[row]] = ids[:row.numel()]
+        if width:
+            text.scatter_(1, n[:, None] + torch.arange(width, device=dev), self._made[:, :width])
+        return text, (n + width).to(torch.int32)
 
     def _drafted_step(self, s: dict) -> None:
         """One step of generate_drafted over its buffers s, all on the GPU: drafts out of the text,
@@ -483,7 +500,7 @@ class RaggedGenerator:
         s['commit'].zero_()
         out = s['text'].gather(1, start[:, None] + torch.arange(steps, device=dev)[None])
         self.fed_len = [n + steps for n in self.fed_len]
-        self._text.append(out.clone())                # out is the caller's
+        self._keep(out)
         self.drafted_steps = taken
         return out
 
