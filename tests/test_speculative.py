@@ -173,6 +173,15 @@ def test_drafted_tokens_are_the_greedy_ones(gate):
     assert len(set(want[1].tolist())) > 5              # a text, not one token
 
 
+def test_drafted_steps_are_the_last_calls():
+    """drafted_steps is there before the first call, and 0 behind a call that takes none."""
+    gen = RaggedGenerator(Chain())
+    assert gen.drafted_steps == 0
+    gen.prefill(prompts([5], 6, 97))
+    gen.drafted_steps = 9                              # as an earlier call leaves it
+    assert gen.generate_drafted(0).shape == (1, 0) and gen.drafted_steps == 0
+
+
 @pytest.mark.gpu
 def test_drafted_and_one_token_calls_in_turn():
     """generate, generate_drafted and generate again go on where the last call ended; a

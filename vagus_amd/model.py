@@ -299,6 +299,7 @@ class RaggedGenerator:
         self._made: torch.Tensor | None = None        # (N, room): what was generated since, in the first _made_len columns
         self._made_len = 0
         self._drafted: dict | None = None             # generate_drafted's buffers and recorded step
+        self.drafted_steps = 0                        # steps that the last generate_drafted took
 
     def reset(self, batch_size: int) -> None:
         """batch_size empty streams.  The caches are zeroed in place when the
@@ -460,6 +461,7 @@ class RaggedGenerator:
         assert 1 <= drafts < ops.MAX_DRAFT_BLOCK, f'1 to {ops.MAX_DRAFT_BLOCK - 1} drafts a step; got {drafts}'
         assert temperature >= 0, f'temperature must not be negative; got {temperature}'
         N, dev = self.batch_size, self.device
+        self.drafted_steps = 0
         if steps <= 0:
             return torch.empty(N, 0, dtype=torch.int64, device=dev)
         text, length = self._texts(steps + drafts + 1)
