@@ -9,6 +9,7 @@ recurrence's results (2^-8 each, five in a row) where the block does not, the st
 2e-2, the other tests' bar against the oracle. Tokens: fp32 logits of 211 random ids
 are not within 1e-5 of each other at their top, so greedy tokens are equal.
 """
+import contextlib
 import gc
 
 import pytest
@@ -334,3 +335,27 @@ def test_one_token_calls_hold_no_tensors_of_their_own():
     for _ in range(300):
         gen.generate(1, graph=False)
     assert held() <= before
+
+
+def test_steps_are_recorded_on_the_models_gpu(monkeypatch):
+    """The capture stream is one of the generator's device, whichever is current: seen with torch's calls replaced."""
+    gen = RaggedGenerator(Chain())
+    gen.prefill(prompts([5, 9], 6, 97))
+    seen = []
+
+    class Graph:
+        def replay(self):
+            gen._step()
+
+    @contextlib.contextmanager
+    def entered(*args, **kw):
+        seen.append((args, kw))
+        yield
+
+    monkeypatch.setattr(torch.cuda, 'CUDAGraph', Graph)
+    monkeypatch.setattr(torch.cuda, 'graph', entered)
+    monkeypatch.setattr(torch.cuda, 'device', entered)
+    monkeypatch.setattr(torch.cuda, 'Stream', lambda device=None, **kw: ('stream', device))
+    gen.generate(3)
+    assert seen[0] == ((gen.device,), {})
+    assert seen[1][1] == dict(stream=('stream', gen.device))

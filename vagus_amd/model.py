@@ -345,6 +345,14 @@ class RaggedGenerator:
             self.model.prefill_packed(body, cu_body, last_logits=False)
         self.fed_len = [n - 1 for n in lens]
 
+    def _record(self, step) -> torch.cuda.CUDAGraph:
+        """step() as a HIP graph, on a stream of the model's GPU: torch's own capture stream is one of whichever
+        GPU was current first, and on another the step would run instead of being recorded."""
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.device(self.device), torch.cuda.graph(graph, stream=torch.cuda.Stream(self.device)):
+            step()
+        return graph
+
     def _step(self):
         logits = self.model.decode_step(self.pending[:, None], return_logits=True)
         nxt = logits[:, -1].float().argmax(dim=-1)
@@ -385,9 +393,7 @@ class RaggedGenerator:
                 if graph and self._graph is None:
                     # recording runs no kernel: the layers' cache_len must not count it
                     lens = [blk.att.cache_len for blk in self.model.blocks]
-                    self._graph = torch.cuda.CUDAGraph()
-                    with torch.cuda.graph(self._graph):
-                        self._step()
+                    self._graph = self._record(self._step)
                     for blk, n in zip(self.model.blocks, lens):
                         blk.att.cache_len = n
                     self._graph_key = self._fingerprint()
@@ -493,9 +499,7 @@ class RaggedGenerator:
             else:
                 self._drafted_step(s)
                 if graph:
-                    s['graph'] = torch.cuda.CUDAGraph()
-                    with torch.cuda.graph(s['graph']):
-                        self._drafted_step(s)
+                    s['graph'] = self._record(lambda: self._drafted_step(s))
                     s['key'] = self._fingerprint() + self._drafted_fingerprint()
             taken += 1
         self.model.commit_drafts(s['commit'])
