@@ -15,7 +15,7 @@ import gc
 import pytest
 import torch
 
-from test_model import prompts
+from test_model import prompts, tiny
 from vagus_amd.layer import GatedDeltaNet
 from vagus_amd.model import GDNLM, RaggedGenerator
 
@@ -254,6 +254,56 @@ def test_bf16_model_runs():
         assert out.shape == (64, 12) and int(out.min()) >= 0 and int(out.max()) < 211
         for blk in m.blocks:
             assert torch.isfinite(blk.att.state).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('drafts,graph', [(4, True), (1, True), (15, False)])
+def test_drafts_stand(drafts, graph):
+    """A model that repeats each stream's last token for ever: behind one step, whose drafts may fall, the
+    text ends in that token twice and every draft is it, so that each step makes drafts + 1 tokens."""
+    m = tiny(torch.float32)
+    lens, steps = [5, 70, 19, 1, 2], 41
+    ps = [p.clone() for p in prompts(lens)]
+    gen = RaggedGenerator(m)
+    gen.prefill(ps)
+    want = gen.generate(steps)
+    assert torch.equal(want.cpu(), torch.stack([p[-1].expand(steps) for p in ps]))        # the premise
+    states = [blk.att.export_cache()['state'] for blk in m.blocks]
+    gen.prefill(ps)
+    assert torch.equal(gen.generate_drafted(steps, drafts=drafts, graph=graph), want)
+    assert -(-steps // (drafts + 1)) <= gen.drafted_steps <= 1 + -(-(steps - 1) // (drafts + 1))
+    for blk, s in zip(m.blocks, states):
+        assert rel(blk.att.state, s) <= 41e-5          # a step's bar, 41 steps
+
+
+@pytest.mark.gpu
+def test_sampled_drafts_stand():
+    """At a temperature too: one that leaves the repeated token nearly all of the mass."""
+    m = tiny(torch.float32)
+    ps = prompts([5, 70, 19])
+    gen = RaggedGenerator(m)
+    gen.prefill(ps)
+    got = gen.generate_drafted(41, drafts=4, temperature=1e-3, generator=torch.Generator('cuda').manual_seed(3))
+    assert torch.equal(got.cpu(), torch.stack([p[-1].expand(41) for p in ps]))
+    assert 9 <= gen.drafted_steps <= 1 + 8
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('gate', ['scalar', 'vector'])
+def test_bf16_logits_of_a_block(gate):
+    """Blocks of 5 through 64 bf16 streams (320 rows: the stacked projections), all of the first one's tokens
+    standing: each token's logits against the one-token steps'. Either is within 2e-2 of the oracle's by the
+    model's own bar, so they are within twice that of each other."""
+    m = tiny(torch.bfloat16, gate)
+    toks = torch.stack(prompts([10] * 64, seed=10)).cuda()
+    m.reset_cache(64)
+    want = torch.cat([m.decode_step(toks[:, t:t + 1]) for t in range(10)], 1)
+    m.reset_cache(64)
+    m.begin_drafts(5)
+    counts = torch.zeros(64, dtype=torch.int32, device='cuda')
+    got = torch.cat([m.draft_step(toks[:, :5], counts), m.draft_step(toks[:, 5:], counts + 5)], 1)
+    for t in range(10):
+        assert rel(got[:, t], want[:, t]) <= 4e-2, t
 
 
 @pytest.mark.gpu
