@@ -700,7 +700,8 @@ int vgdr_draft_step(int dtype, int gate_kind, int use_delta, const void *q, cons
  * every draft stands, else max(p_i - q_i, 0) (p_i where that is zero everywhere).  Greedy: p is 1 at the
  * row's lowest top.  tokens [B, K + 1]: the drafts that stand, that token, then -1; accepted [B].
  * NaN logits have no mass; equal ones share it, +inf and a row of -inf alone included; a draft outside
- * 0..V-1 never stands.  Sums and weights are 64-bit.  0 <= K <= 64, 1 <= V < 2^31 - 2^20.  workspace:
+ * 0..V-1 never stands.  The sampled row's weights and sums are 64-bit; a draft is judged by fp32 sums, and
+ * by 64-bit ones where the two sides are within 1e-5 of each other.  0 <= K <= 64, 1 <= V < 2^31 - 2^20.  workspace:
  * vgdr_verify_drafts_workspace_size bytes, 16-byte aligned, calls that overlap have their own.
  */
 int64_t vgdr_verify_drafts_workspace_size(int64_t B, int64_t K, int64_t V);

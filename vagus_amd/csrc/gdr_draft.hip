@@ -132,15 +132,21 @@ __device__ __forceinline__ float row_prefix16(float x) {
 // took 42 us where this takes 26). As it lies it is the B operand of the product with [K; Q], whose
 // two halves of rows (dk > 64) meet in LDS.  q and k are kept unnormalised: the norms are A's and
 // q's own diagonals and scale the results.  RT: row tiles (dk <= 16 RT). LT: room of the pending
-// block and tokens: 16, or 8, whose [K; Q] is one tile of 16 rows and which leaves registers and LDS
-// for four workgroups a CU (three at 16).  At least 128 (RT 4) or 256 threads, two per value
-// channel, and one per pair of q, k, v channels.
+// block and tokens: 16, or 8, whose [K; Q] is one tile of 16 rows and which, without per-channel gates, leaves
+// registers and LDS for four workgroups a CU (three at 16).  Per-channel gates of dk > 64 take 147 registers a
+// thread at 8 tokens (three waves a SIMD) and at 16 and dv <= 128 283 with 70 KB of LDS: one wave a SIMD, since pk, pg
+// and the operands in flight live beside the state across A and B. At 8 tokens the per-channel kernels of dk <= 64 and
+// the fp32 ones of other gates keep 5 to 17 registers in scratch memory (7 in fp32 at 16 and dv <= 128).  At least 128 (RT 4) or 256 threads,
+// two per value channel, and one per pair of q, k, v channels.
 //
 // Bound by the state's way in and out: 64 streams of 16 128 x 128 heads, bf16, blocks of 5: 28 us for 161 MB
-// (5.7 TB/s; the traffic counters read 156 MB), of which the products and the solve, which the
-// stores cover in part, are 5; 128 streams, blocks of 16: 93-97 us for 411 MB, where the product with the state costs
+// (5.7 TB/s) on one state again and again, which the last-level cache holds in part, 29-30 (5.4) on eight in turn;
+// 160 MB pass behind the L2. The products and the solve, which the stores cover in part, are 5 of it;
+// 128 streams, blocks of 16: 93-97 us for 411 MB (99 on several in turn), where the product with the state costs
 // 9, the solve 13 and the outputs 6. One workgroup a CU (64 streams of 4 128 x 256 heads, per-channel
-// gates, blocks of 8) is a chain of latencies: 25 us for 83 MB. One stream: 10 us.
+// gates, blocks of 8) is a chain of latencies: 25 us for 83 MB. One stream: 10 us.  Per-channel gates on
+// the first case's heads: 41 us for 166 MB, 106 for 222 MB at 16 tokens (54 without), where A and B, walked a key at a
+// time, and the one wave a SIMD show. The commit alone (L = 0): 23.5 us, per-channel 26.4.
 // Measured and left out: the operands' loads ahead of the state's (b64 31.1 -> 33.1 us), stores before
 // the products (32.6) or behind the solve (32.9), ws and the products in one LDS area for a fourth
 // workgroup at 16 tokens (97 -> 135 us with the registers that takes).

@@ -6,8 +6,8 @@
 //    in fp32, which decides u q Z < w but where the two are within 1e-5.  stand_kernel decides, and
 //    of the one row that a stream samples sums the weights in 64 bits, in blocks of 512 over several
 //    workgroups: the running sums meet the uniform number at up to V borders, so an fp32
-//    sum's error (5e-7) would choose another token once in some ten streams of 100,000 ids, a
-//    64-bit one's (1e-14) never in practice.  rest_kernel does the same with what the draft's probabilities
+//    sum's error (5e-7) would choose another token once in some ten streams of 100,000 ids, the
+//    64-bit weights' (2e-13, their exponential's) never in practice.  rest_kernel does the same with what the draft's probabilities
 //    leave of the row, and choose_kernel finds the token.  The last workgroup of a stream to finish
 //    does not do it: the fence that takes writes the L2 back (58 us a call at 64 streams of 32,000
 //    ids); nor does one workgroup do all: 26 us with the weights on 64 of 256 CUs.

@@ -458,9 +458,11 @@ class RaggedGenerator:
         """`steps` tokens for every stream, (N, steps) int64, by speculative decoding: each step feeds
         the pending token and up to `drafts` (1 to 15) tokens drafted from the stream's own text
         (ops.lookup_drafts), and keeps those that stand before the model's probabilities and the token
-        behind them (ops.verify_drafts).  At temperature 0 these are generate's tokens, up to the
-        rounding of the logits; above, samples of the softmax at that temperature from `generator`'s
-        uniform numbers.  The streams advance by different counts a step, and the call ends when
+        behind them (ops.verify_drafts).  At temperature 0 these are generate's tokens where roundings do
+        not decide: in bf16 and fp16 the one-token step rounds the conv's, the norm's and the recurrence's
+        results and a block does not, so that the logits differ by these, and close ones may change places;
+        above, samples of the softmax at that temperature from `generator`'s uniform numbers.  A
+        stream without an earlier occurrence still takes its part in the whole block, whose drafts then fall.  The streams advance by different counts a step, and the call ends when
         the slowest has its tokens.  With graph=True the first step runs eagerly, and the recorded step is
         replayed; as in generate the layers' cache_len counters are not advanced."""
         assert self.pending is not None and self.batch_size > 0, 'prefill first'

@@ -1919,7 +1919,8 @@ def verify_drafts(logits, drafts, uniforms, *, temperature=1.0, draft_probs=None
     and uniforms[i] q_i(d_i) < p_i(d_i); the token behind the last that stands is drawn from
     max(p - q, 0) of the first refused draft's row, or from p where none was refused, as the
     lowest id at which the running sum exceeds uniforms[K] times the whole.  So the tokens are
-    distributed as the target's own, one by one.  Weights and sums are 64-bit.
+    distributed as the target's own, one by one.  The sampled row's weights and sums are 64-bit; a
+    draft is judged by fp32 sums, and by 64-bit ones where the two sides are within 1e-5 of each other.
 
     NaN logits have no mass, equal ones (+inf among them, and a row of -inf alone) share it, a draft
     outside the vocabulary never stands, and where q covers all of p the token is drawn from p.
