@@ -409,3 +409,31 @@ def test_steps_are_recorded_on_the_models_gpu(monkeypatch):
     gen.generate(3)
     assert seen[0] == ((gen.device,), {})
     assert seen[1][1] == dict(stream=('stream', gen.device))
+
+
+def test_calls_within_and_outside_inference_mode():
+    """The text that one call leaves in inference mode is the next one's to write on outside of it."""
+    gen = RaggedGenerator(Chain())
+    gen.prefill(prompts([5, 9], 6, 97))
+    with torch.inference_mode():
+        a = gen.generate(3, graph=False)
+    b = gen.generate(2, graph=False)
+    text, length = gen._texts(1)
+    assert torch.equal(text[0, 5:10], torch.cat([a, b], 1)[0]) and length.tolist() == [10, 14]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('graph', [True, False])
+def test_drafted_calls_within_and_outside_inference_mode(graph):
+    m = varied(torch.float32)
+    ps = repeating([12, 33, 8], seed=4)
+    gen = RaggedGenerator(m)
+    gen.prefill(ps)
+    want = gen.generate(30)
+    gen.prefill(ps)
+    with torch.inference_mode():
+        a = gen.generate_drafted(10, graph=graph)
+    b = gen.generate_drafted(10, graph=graph)
+    with torch.inference_mode():
+        c = gen.generate_drafted(10, graph=graph)
+    assert torch.equal(torch.cat([a, b, c], 1), want)

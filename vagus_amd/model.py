@@ -409,7 +409,8 @@ class RaggedGenerator:
             return
         end = self._made_len + n
         if self._made is None or end > self._made.shape[1]:
-            made = torch.empty(self.batch_size, max(256, 2 * end), dtype=torch.int64, device=self.device)
+            with torch.inference_mode(False):         # the next call may come from outside of it
+                made = torch.empty(self.batch_size, max(256, 2 * end), dtype=torch.int64, device=self.device)
             if self._made_len:
                 made[:, :self._made_len].copy_(self._made[:, :self._made_len])
             self._made = made
@@ -478,13 +479,13 @@ class RaggedGenerator:
         s = self._drafted
         if s is None or s['kind'] != kind:
             new = lambda *shape, dt=torch.int32: torch.zeros(*shape, dtype=dt, device=dev)  # noqa: E731
-            s = self._drafted = dict(kind=kind, K=drafts, max_ngram=max_ngram, min_ngram=min_ngram, text=text, length=length,
-                                     left=new(N), commit=new(N), uniforms=new(N, drafts + 1, dt=torch.float32),
-                                     temperature=new(N, dt=torch.float32), places=torch.arange(drafts + 1, device=dev)[None],
-                                     graph=None, key=None)
-        else:
-            s['text'].copy_(text)
-            s['length'].copy_(length)
+            with torch.inference_mode(False):         # kept for calls from outside of it too
+                s = self._drafted = dict(kind=kind, K=drafts, max_ngram=max_ngram, min_ngram=min_ngram,
+                                         text=new(*text.shape, dt=torch.int64), length=new(N), left=new(N), commit=new(N),
+                                         uniforms=new(N, drafts + 1, dt=torch.float32), temperature=new(N, dt=torch.float32),
+                                         places=torch.arange(drafts + 1, device=dev)[None], graph=None, key=None)
+        s['text'].copy_(text)
+        s['length'].copy_(length)
         start = length.long()
         s['left'].fill_(steps)
         s['commit'].zero_()
