@@ -726,6 +726,50 @@ int vgdr_lookup_drafts(const void *history, int token_bytes, int64_t ld, int64_t
                        int max_ngram, int min_ngram, hipStream_t stream);
 
 /*
+ * Block-scaled numbers: 32 consecutive elements of a row share a scale 2^(b - 127), held as the byte b in 1..254; b = 255:
+ * the block had a NaN or an infinity, its values are NaN.  8-bit values are e4m3, 4-bit ones e2m1; the scale
+ * is the smallest power of two (at least 2^-126) with amax <= 464 scale (8 bits) or 7 scale (4 bits), elements
+ * are rounded to nearest, ties to even, and saturate at 448 and 6.
+ *
+ * VGDR_MX8, beside the element types: rows in 8 bits, values [rows, 128 ceil(K / 128)] with bytes
+ * [rows, 4 ceil(K / 128)]; padded columns are zeros with b = 1.
+ *
+ * 4-bit weights [n, K]: with C = ceil(K / 128) and T = ceil(n / 16), values [T][C][4][16][16] bytes: byte i of
+ * [t][c][g][r] holds columns 128 c + 32 g + 2 i (low half) and + 1 of row 16 t + r; scale bytes
+ * [T][ceil(C / 4)][4][16][4]: [t][c / 4][g][r][c % 4].  A gated pair (n / 2 rows each): T = 2 ceil(n / 2 / 16), tile 2 i has
+ * rows 16 i.. of the first half, tile 2 i + 1 those of the second.  Padded rows and columns are zeros with b = 1.
+ *
+ * Every pointer is 16-byte aligned but x and w of vgdr_mx_quantize and vgdr_mx_weight; ld: elements from a row to the
+ * next.  No entry point has a backward.
+ */
+#define VGDR_MX8 3
+
+/* Rows x [rows, cols] in dtype to 8 bits. */
+int vgdr_mx_quantize(int dtype, const void *x, int64_t ldx, void *values, void *scales, int64_t rows, int64_t cols,
+                     hipStream_t stream);
+/* Weights w [rows, cols] in dtype to 4 bits in the tiles' order; gated: rows is even. */
+int vgdr_mx_weight(int dtype, const void *w, int64_t ldw, void *values, void *scales, int64_t rows, int64_t cols, int gated,
+                   hipStream_t stream);
+/* h = x + residual (rounded to dtype; residual NULL: h = x), written to x_out (may be NULL or x), and the norm
+ * h rsqrt(mean h^2 + eps) gamma (infra/components/norm_layer.py:15-23) formed in 64 bits and rounded once, to
+ * 8-bit rows; y (may be NULL): the norm in dtype with vgdr_rms_norm's roundings.  x, residual [rows, dim] dense; dim a
+ * multiple of 8, at most 16384. */
+int vgdr_mx_rms_norm(int dtype, const void *x, const void *residual, void *x_out, const void *gamma, void *y, void *values,
+                     void *scales, int64_t rows, int64_t dim, float eps, hipStream_t stream);
+/*
+ * y [rows, n] = x W^T for x [rows, k] (x_dtype: an element type with ldx a multiple of 8, or VGDR_MX8 with
+ * x_scales) and 4-bit weights of n rows, in out_dtype (an element type).  gated: y [rows, n / 2] =
+ * silu(x W1^T) (x W2^T) (the FFN's input half, infra/components/ffn.py:48-50) with sums, activation and product in fp32
+ * and one rounding, in an element type or VGDR_MX8 (y_scales).  Products and sums are fp32: bf16, fp16 and fp32 rows
+ * meet the weights exactly (as one, two and three bf16 numbers an element).  workspace:
+ * vgdr_mx_linear_workspace_size bytes (0: none), calls that overlap have their own.  At most 2^24 rows of weights and columns.
+ */
+int64_t vgdr_mx_linear_workspace_size(int x_dtype, int64_t rows, int64_t k);
+int vgdr_mx_linear(int x_dtype, const void *x, int64_t ldx, const void *x_scales, const void *w_values, const void *w_scales,
+                   int gated, int out_dtype, void *y, void *y_scales, void *workspace, int64_t workspace_bytes, int64_t rows,
+                   int64_t n, int64_t k, hipStream_t stream);
+
+/*
  * Packed-batch schedule.  No reference counterpart (the reference has no
  * cu_seqlens, see infra/inference/generator.py:19-22); fla builds the same
  * integer tables for its varlen kernels.  Writes into `workspace`

@@ -13,7 +13,7 @@ import threading
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), 'libvagus_gdr.so')
 
 VGDR_OK, VGDR_ERR_INVALID, VGDR_ERR_UNSUPPORTED, VGDR_ERR_HIP = 0, 1, 2, 3
-VGDR_F32, VGDR_BF16, VGDR_F16 = 0, 1, 2
+VGDR_F32, VGDR_BF16, VGDR_F16, VGDR_MX8 = 0, 1, 2, 3
 VGDR_GATE_NONE, VGDR_GATE_SCALAR, VGDR_GATE_VECTOR = 0, 1, 2
 
 
@@ -116,6 +116,11 @@ SIGNATURES = {
     'vgdr_project_rows': (_I, [_I, _I, ctypes.POINTER(_P), ctypes.POINTER(_L), _P, _L, _P, _L, _I, _P, _L, _L,
                                _P]),
     'vgdr_rms_norm': (_I, [_I, _P, _P, _P, _P, _P, _L, _L, _F, _P]),
+    'vgdr_mx_quantize': (_I, [_I, _P, _L, _P, _P, _L, _L, _P]),
+    'vgdr_mx_weight': (_I, [_I, _P, _L, _P, _P, _L, _L, _I, _P]),
+    'vgdr_mx_rms_norm': (_I, [_I, _P, _P, _P, _P, _P, _P, _P, _L, _L, _F, _P]),
+    'vgdr_mx_linear_workspace_size': (_L, [_I, _L, _L]),
+    'vgdr_mx_linear': (_I, [_I, _P, _L, _P, _P, _P, _I, _I, _P, _P, _P, _L, _L, _L, _L, _P]),
     'vgdr_scalar_gates': (_I, [_I, _P, _P, _P, _P, _P, _P, _L, _L, _L, _P]),
     'vgdr_swiglu': (_I, [_I, _P, _P, _L, _L, _P]),
     'vgdr_recurrent_fwd_w': (_I, [_I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P,

@@ -30,6 +30,18 @@ int hip_status(hipError_t e, const char *what) {
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+constexpr int64_t MX_MOST = 1 << 24;              // rows of weights, columns
+
+// checks of what is rounded to block-scaled numbers
+int check_mx_source(const char *fn, int dtype, int64_t ld, int64_t rows, int64_t cols) {
+    if (dtype != VGDR_F32 && dtype != VGDR_BF16 && dtype != VGDR_F16)
+        return fail(VGDR_ERR_INVALID, "%s: unknown dtype %d", fn, dtype);
+    if (rows < 0 || cols < 1 || cols > MX_MOST)
+        return fail(VGDR_ERR_INVALID, "%s: rows=%lld cols=%lld", fn, (long long)rows, (long long)cols);
+    if (ld < cols) return fail(VGDR_ERR_INVALID, "%s: rows %lld apart for %lld columns", fn, (long long)ld, (long long)cols);
+    return VGDR_OK;
+}
+
 // checks shared by both scan entry points; returns VGDR_OK or an error code
 int check_common(const char *fn, int dtype, int gate_kind, int use_delta, const void *q, const void *k,
                  const void *v, const float *g, const float *beta, const void *o,
@@ -1153,6 +1165,118 @@ int vgdr_rms_norm(int dtype, const void *x, const void *residual, void *x_out, c
         return fail(VGDR_ERR_INVALID, "vgdr_rms_norm: y must not alias x, residual or x_out");
     return hip_status(vgdr::rms_norm(dtype, x, residual, x_out, gamma, y, rows, (int)dim, eps, stream),
                       "vgdr_rms_norm launch");
+}
+
+int vgdr_mx_quantize(int dtype, const void *x, int64_t ldx, void *values, void *scales, int64_t rows, int64_t cols,
+                     hipStream_t stream) {
+    g_err[0] = 0;
+    const char *fn = "vgdr_mx_quantize";
+    if (int rc = check_mx_source(fn, dtype, ldx, rows, cols)) return rc;
+    if (rows == 0) return VGDR_OK;
+    if (rows > (int64_t)0x7fffffff * 256 / ((cols + 127) / 128 * 16))
+        return fail(VGDR_ERR_INVALID, "%s: too many rows", fn);
+    if (!x || !values || !scales) return fail(VGDR_ERR_INVALID, "%s: x, values and scales are required", fn);
+    if (!aligned16(values) || !aligned16(scales)) return fail(VGDR_ERR_INVALID, "%s: values and scales must be 16-byte aligned", fn);
+    if (x == values) return fail(VGDR_ERR_INVALID, "%s: values must not alias x", fn);
+    vgdr::MxQuantize p{vgdr::MX_ROWS, x, ldx, rows, cols, (uint8_t *)values, (uint8_t *)scales, false};
+    return hip_status(vgdr::mx_quantize(dtype, p, stream), "vgdr_mx_quantize launch");
+}
+
+int vgdr_mx_weight(int dtype, const void *w, int64_t ldw, void *values, void *scales, int64_t rows, int64_t cols, int gated,
+                   hipStream_t stream) {
+    g_err[0] = 0;
+    const char *fn = "vgdr_mx_weight";
+    if (int rc = check_mx_source(fn, dtype, ldw, rows, cols)) return rc;
+    if (rows < 1 || rows > MX_MOST) return fail(VGDR_ERR_INVALID, "%s: rows=%lld (1 to 2^24)", fn, (long long)rows);
+    if (gated != 0 && gated != 1) return fail(VGDR_ERR_INVALID, "%s: gated=%d", fn, gated);
+    if (gated && rows % 2) return fail(VGDR_ERR_INVALID, "%s: a gated pair has an even number of rows, got %lld", fn, (long long)rows);
+    if ((rows + 31) / 16 * ((cols + 511) / 512) > 0x7fffffffLL) return fail(VGDR_ERR_INVALID, "%s: too many tiles", fn);
+    if (!w || !values || !scales) return fail(VGDR_ERR_INVALID, "%s: w, values and scales are required", fn);
+    if (!aligned16(values) || !aligned16(scales)) return fail(VGDR_ERR_INVALID, "%s: values and scales must be 16-byte aligned", fn);
+    vgdr::MxQuantize p{vgdr::MX_WEIGHT, w, ldw, rows, cols, (uint8_t *)values, (uint8_t *)scales, gated != 0};
+    return hip_status(vgdr::mx_quantize(dtype, p, stream), "vgdr_mx_weight launch");
+}
+
+int vgdr_mx_rms_norm(int dtype, const void *x, const void *residual, void *x_out, const void *gamma, void *y, void *values,
+                     void *scales, int64_t rows, int64_t dim, float eps, hipStream_t stream) {
+    g_err[0] = 0;
+    const char *fn = "vgdr_mx_rms_norm";
+    if (dtype != VGDR_F32 && dtype != VGDR_BF16 && dtype != VGDR_F16)
+        return fail(VGDR_ERR_INVALID, "%s: unknown dtype %d", fn, dtype);
+    if (rows < 0) return fail(VGDR_ERR_INVALID, "%s: rows=%lld", fn, (long long)rows);
+    if (dim <= 0 || dim % 8 || dim > 16384)
+        return fail(VGDR_ERR_UNSUPPORTED, "%s: dim=%lld (supported: a multiple of 8, at most 16384)", fn, (long long)dim);
+    if (!(eps >= 0.f)) return fail(VGDR_ERR_INVALID, "%s: eps must be >= 0", fn);
+    if (rows == 0) return VGDR_OK;
+    if (rows > 0x7fffffffLL) return fail(VGDR_ERR_INVALID, "%s: too many rows", fn);
+    if (!x || !gamma || !values || !scales) return fail(VGDR_ERR_INVALID, "%s: x, gamma, values and scales are required", fn);
+    if (!aligned16(x) || !aligned16(gamma) || !aligned16(values) || !aligned16(scales) || !aligned16(residual) ||
+        !aligned16(x_out) || !aligned16(y))
+        return fail(VGDR_ERR_INVALID, "%s: every tensor must be 16-byte aligned", fn);
+    if (values == x || (residual && values == residual) || (x_out && values == x_out) ||
+        (y && (y == x || y == residual || y == x_out || y == values)))
+        return fail(VGDR_ERR_INVALID, "%s: values and y must not alias x, residual or x_out", fn);
+    vgdr::MxNorm p{x, residual, x_out, y, gamma, (uint8_t *)values, (uint8_t *)scales, rows, (int)dim, eps};
+    return hip_status(vgdr::mx_rms_norm(dtype, p, stream), "vgdr_mx_rms_norm launch");
+}
+
+int64_t vgdr_mx_linear_workspace_size(int x_dtype, int64_t rows, int64_t k) {
+    if (rows <= 0 || k <= 0 || k > MX_MOST || rows > 0x7fffffffLL) return 0;
+    if (x_dtype == VGDR_F32 || x_dtype == VGDR_F16 || (x_dtype == VGDR_BF16 && k % 128))
+        return (x_dtype == VGDR_F32 ? 3 : x_dtype == VGDR_F16 ? 2 : 1) * rows * ((k + 127) / 128 * 256);
+    return 0;
+}
+
+int vgdr_mx_linear(int x_dtype, const void *x, int64_t ldx, const void *x_scales, const void *w_values, const void *w_scales,
+                   int gated, int out_dtype, void *y, void *y_scales, void *workspace, int64_t workspace_bytes, int64_t rows,
+                   int64_t n, int64_t k, hipStream_t stream) {
+    g_err[0] = 0;
+    const char *fn = "vgdr_mx_linear";
+    const bool x8 = x_dtype == VGDR_MX8, y8 = out_dtype == VGDR_MX8;
+    if (x_dtype < VGDR_F32 || x_dtype > VGDR_MX8) return fail(VGDR_ERR_INVALID, "%s: unknown x_dtype %d", fn, x_dtype);
+    if (out_dtype < VGDR_F32 || out_dtype > VGDR_MX8) return fail(VGDR_ERR_INVALID, "%s: unknown out_dtype %d", fn, out_dtype);
+    if (gated != 0 && gated != 1) return fail(VGDR_ERR_INVALID, "%s: gated=%d", fn, gated);
+    if (y8 && !gated) return fail(VGDR_ERR_UNSUPPORTED, "%s: 8-bit results are the gated product's", fn);
+    if (rows < 0 || rows > 0x7fffffffLL) return fail(VGDR_ERR_INVALID, "%s: rows=%lld", fn, (long long)rows);
+    if (n < 1 || k < 1 || n > MX_MOST || k > MX_MOST)
+        return fail(VGDR_ERR_INVALID, "%s: n=%lld k=%lld (1 to 2^24)", fn, (long long)n, (long long)k);
+    if (gated && n % 2) return fail(VGDR_ERR_INVALID, "%s: a gated pair has an even number of rows, got %lld", fn, (long long)n);
+    if (rows == 0) return VGDR_OK;
+    if ((rows + 63) / 64 * ((n + 255) / 128) > 0x7fffffffLL) return fail(VGDR_ERR_INVALID, "%s: too many rows", fn);
+    if (!x || !w_values || !w_scales || !y || (x8 && !x_scales) || (y8 && !y_scales))
+        return fail(VGDR_ERR_INVALID, "%s: x, the weights, y and the scales of 8-bit rows are required", fn);
+    if (!aligned16(x) || !aligned16(x_scales) || !aligned16(w_values) || !aligned16(w_scales) || !aligned16(y) || !aligned16(y_scales))
+        return fail(VGDR_ERR_INVALID, "%s: every tensor must be 16-byte aligned", fn);
+    if (!x8 && (ldx % 8 || ldx < k)) return fail(VGDR_ERR_INVALID, "%s: ldx=%lld (a multiple of 8, at least k)", fn, (long long)ldx);
+    if (y == x || y == w_values) return fail(VGDR_ERR_INVALID, "%s: y must not alias an input", fn);
+    const int64_t need = vgdr_mx_linear_workspace_size(x_dtype, rows, k);
+    if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+        return fail(VGDR_ERR_INVALID, "%s: the workspace has %lld bytes, 16-byte aligned; got %lld", fn, (long long)need,
+                    (long long)(workspace ? workspace_bytes : 0));
+    vgdr::MxLinear p{};
+    p.C = (int)((k + 127) / 128);
+    p.T = (int)(gated ? 2 * ((n / 2 + 15) / 16) : (n + 15) / 16);
+    p.N = (int)(gated ? n / 2 : n);
+    p.x = x;
+    p.ldx = x8 ? 128 * (int64_t)p.C : ldx;
+    p.planes = 1;
+    if (need) {
+        vgdr::MxQuantize q{vgdr::MX_PLANES, x, ldx, rows, k, (uint8_t *)workspace, nullptr, false};
+        if (int rc = hip_status(vgdr::mx_quantize(x_dtype, q, stream), "vgdr_mx_linear launch")) return rc;
+        p.x = workspace;
+        p.ldx = 128 * (int64_t)p.C;
+        p.planes = x_dtype == VGDR_F32 ? 3 : x_dtype == VGDR_F16 ? 2 : 1;
+    }
+    p.x_scales = (const uint8_t *)x_scales;
+    p.w = (const uint8_t *)w_values;
+    p.w_scales = (const uint8_t *)w_scales;
+    p.y = y;
+    p.y_scales = (uint8_t *)y_scales;
+    p.rows = rows;
+    p.out = out_dtype;
+    p.x8 = x8;
+    p.gated = gated != 0;
+    return hip_status(vgdr::mx_linear(p, stream), "vgdr_mx_linear launch");
 }
 
 int vgdr_scalar_gates(int dtype, const void *x, const void *w_ab, const float *neg_exp_a, const float *dt_bias,

@@ -44,32 +44,6 @@ namespace vgdr {
 // units are XOR-swizzled within each row (unit c of row r sits at unit
 // position c ^ (r % UPR)), so that the fragment reads of 16 consecutive rows
 // at one column spread over all LDS banks.
-// global -> LDS copies of 16 / 4 bytes per lane: lane L writes LDS base + L * size
-// (global_load_lds_dword{,x4}; the LDS base goes in M0).  Written as inline asm
-// on purpose: the compiler then does not know that the instruction writes LDS,
-// so it never makes later LDS reads of the *other* double-buffer slot wait for
-// the copy.  Completion is managed explicitly: dma_wait() (s_waitcnt vmcnt(0))
-// by every issuing wave, then a barrier, before any lane reads the slot; the
-// memory clobber keeps the compiler from moving LDS accesses across the copy.
-// M0 is set inside the asm and is otherwise unused by these kernels (no
-// movrel / LDS-parameter instructions), so clobbering it is safe here.  An
-// LDS DMA that reads M0 needs one wait state after the SALU write of M0
-// (a GFX9-family hazard), hence the s_nop between the two.
-__device__ __forceinline__ uint32_t lds_addr(const void *p) {
-    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char *)p;
-}
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-__device__ __forceinline__ void lds_dma16(const void *src, void *lds_base) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
-                 :: "v"(src), "s"(__builtin_amdgcn_readfirstlane(lds_addr(lds_base))) : "memory", "m0");
-}
-__device__ __forceinline__ void lds_dma4(const void *src, void *lds_base) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off"
-                 :: "v"(src), "s"(__builtin_amdgcn_readfirstlane(lds_addr(lds_base))) : "memory", "m0");
-}
-#pragma clang diagnostic pop
-
 template <typename E, int NCOL>
 struct Swz {
     static constexpr int VE = 16 / sizeof(E);

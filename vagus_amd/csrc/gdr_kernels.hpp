@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace vgdr {
 
 // Sequence geometry shared by the chunk kernels: a dense batch (cu == NULL,
@@ -418,6 +420,43 @@ struct LookupParams {
 };
 hipError_t lookup_drafts(bool wide, LookupParams p, void *workspace, hipStream_t stream);
 int64_t lookup_workspace(int64_t N, int64_t cap);
+
+// Block-scaled numbers (gdr_mx.hip; the formats: gdr_mx.hpp).
+enum MxKind { MX_ROWS, MX_WEIGHT, MX_PLANES };
+struct MxQuantize {
+    MxKind kind;
+    const void *x;                // [rows, K], ldx elements apart
+    int64_t ldx, rows, K;
+    uint8_t *values, *scales;     // MX_PLANES: bf16 [P][rows][Kp], none
+    bool gated;                   // MX_WEIGHT: two halves whose tiles take turns
+};
+hipError_t mx_quantize(int dtype, const MxQuantize &p, hipStream_t stream);
+template <typename E> constexpr int mx_planes() { return sizeof(E) == 4 ? 3 : std::is_same<E, _Float16>::value ? 2 : 1; }
+
+struct MxNorm {
+    const void *x, *residual;     // [rows, dim]; the residual or NULL
+    void *x_out, *y;              // their sum, the norm in the element type; each may be NULL
+    const void *gamma;
+    uint8_t *values, *scales;
+    int64_t rows;
+    int dim;
+    float eps;
+};
+hipError_t mx_rms_norm(int dtype, const MxNorm &p, hipStream_t stream);
+
+// Products with 4-bit weights (gdr_mx_linear.hip).
+constexpr int MX8 = 3;            // beside the element types: rows in 8 bits with scales
+struct MxLinear {
+    const void *x;                // bf16 [planes][rows][ldx], or 8-bit [rows][128 C]
+    const uint8_t *x_scales;      // [rows][4 C]
+    const uint8_t *w, *w_scales;  // T tiles of 16 rows, C tiles of 128 columns
+    void *y;                      // [rows, N] in `out`; MX8: [rows, 128 ceil(N / 128)]
+    uint8_t *y_scales;
+    int64_t rows, ldx;
+    int planes, T, C, N, out;     // N: the output's columns
+    bool x8, gated;
+};
+hipError_t mx_linear(const MxLinear &p, hipStream_t stream);
 
 int device_cu_count();
 

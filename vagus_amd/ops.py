@@ -2002,3 +2002,220 @@ def lookup_drafts(history, lengths, n, *, max_ngram: int = 3, min_ngram: int = 1
     _launch(index, lib.vgdr_lookup_drafts, h.data_ptr(), h.element_size(), max(h.stride(0), cap), cap, lens.data_ptr(),
             drafts.data_ptr(), counts.data_ptr(), _ptr(ws), nbytes, N, n, max_ngram, min_ngram)
     return drafts, counts
+
+
+# --- block-scaled numbers ------------------------------------------------------
+
+
+def _blocks_of(n: int) -> int:
+    """Tiles of 128 columns that n columns take."""
+    return -(-n // 128)
+
+
+def _powers(scales):
+    """The scale bytes' numbers, fp32: 2^(b - 127), NaN for 255."""
+    b = scales.to(torch.int32)
+    return torch.where(b == 255, float('nan'), (b << 23).view(torch.float32))
+
+
+class MXRows:
+    """Rows in 8 bits, a scale for each 32 elements (vagus_gdr.h, VGDR_MX8): values (..., 128 ceil(size / 128)) in
+    float8_e4m3fn, scales (..., 4 ceil(size / 128)) uint8, the exponents of two plus 127 (255: NaN); columns from `size` on
+    are zeros.  What mx_quantize, mx_rms_norm and mx_swiglu return and mx_linear and mx_swiglu take."""
+
+    __slots__ = ('values', 'scales', 'size')
+
+    def __init__(self, values, scales, size: int):
+        C = _blocks_of(size)
+        assert size >= 1 and values.dtype is torch.float8_e4m3fn and values.shape[-1] == 128 * C, \
+            f'values must be (..., {128 * C}) in float8_e4m3fn for {size} columns; got {tuple(values.shape)}, {values.dtype}'
+        assert scales.dtype is torch.uint8 and scales.shape == (*values.shape[:-1], 4 * C), \
+            f'scales must be {(*values.shape[:-1], 4 * C)} in uint8; got {tuple(scales.shape)}, {scales.dtype}'
+        self.values, self.scales, self.size = values, scales, size
+
+    @property
+    def shape(self) -> torch.Size:
+        return torch.Size((*self.values.shape[:-1], self.size))
+
+    @property
+    def device(self):
+        return self.values.device
+
+    def dequantize(self, dtype=torch.float32):
+        v = self.values.float().unflatten(-1, (-1, 32)) * _powers(self.scales)[..., None]
+        return v.flatten(-2)[..., :self.size].to(dtype)
+
+
+class MXWeight:
+    """A linear map's weights in 4 bits, a scale for each 32 elements of a row, in the order in which the kernels'
+    matrix instructions take them (vagus_gdr.h): values (T, C, 4, 16, 16) and scales (T, ceil(C / 4), 4, 16, 4),
+    uint8, for T tiles of 16 rows and C of 128 columns; shape (n, k).  gated: two maps of n / 2
+    rows whose tiles take turns (mx_swiglu).  mx_weight makes them."""
+
+    __slots__ = ('values', 'scales', 'shape', 'gated')
+
+    def __init__(self, values, scales, shape, gated: bool = False):
+        n, k = shape
+        assert n >= 1 and k >= 1 and not (gated and n % 2), f'a weight of shape {tuple(shape)}' + (', gated' if gated else '')
+        T, C = (2 * -(-n // 32) if gated else -(-n // 16)), _blocks_of(k)
+        want = ((T, C, 4, 16, 16), (T, -(-C // 4), 4, 16, 4))
+        for name, t, w in zip(('values', 'scales'), (values, scales), want):
+            assert t.dtype is torch.uint8 and t.shape == w and t.is_contiguous() and t.data_ptr() % 16 == 0, \
+                f'{name} must be {w} in uint8, contiguous, aligned; got {tuple(t.shape)}, {t.dtype}'
+        self.values, self.scales, self.shape, self.gated = values, scales, torch.Size(shape), gated
+
+    @property
+    def device(self):
+        return self.values.device
+
+    def dequantize(self, dtype=torch.float32):
+        """The numbers that the bytes stand for, (n, k)."""
+        n, k = self.shape
+        T, C = self.values.shape[:2]
+        number = torch.tensor([0, .5, 1, 1.5, 2, 3, 4, 6], device=self.device)
+        number = torch.cat([number, -number])
+        code = torch.stack([self.values & 15, self.values >> 4], -1).flatten(-2)          # (T, C, 4, 16, 32)
+        s = _powers(self.scales).permute(0, 1, 4, 2, 3).flatten(1, 2)[:, :C]               # (T, C, 4, 16)
+        w = (number[code.long()] * s[..., None]).permute(0, 3, 1, 2, 4).reshape(T, 16, 128 * C)[..., :k]
+        if self.gated:
+            w = w.unflatten(0, (-1, 2)).transpose(0, 1).reshape(2, -1, k)[:, :n // 2]
+        return w.reshape(-1, k)[:n].to(dtype)
+
+
+def _mx_source(name, t, dims=None):
+    """(t as rows (R, K), their distance in elements) for a kernel that rounds them."""
+    if t.get_device() < 0:
+        _check_device(t)
+    _check_grad(t)
+    if t.dtype not in _DTYPES:
+        raise NotImplementedError(f'{name} must be one of {list(_DTYPES)}; got {t.dtype}')
+    assert t.dim() >= 1 and t.shape[-1] >= 1 and (dims is None or t.dim() == dims), f'{name}: shape {tuple(t.shape)}'
+    K = t.shape[-1]
+    if t.dim() != 2:
+        t = t.reshape(-1, K)
+    if (t.stride(1) != 1 and K > 1) or (t.stride(0) < K and t.shape[0] > 1):
+        t = t.contiguous()
+    return t, t.stride(0) if t.shape[0] > 1 else K
+
+
+def _mx_rows(lead, K: int, device) -> MXRows:
+    C = _blocks_of(K)
+    return MXRows(torch.empty((*lead, 128 * C), dtype=torch.float8_e4m3fn, device=device),
+                  torch.empty((*lead, 4 * C), dtype=torch.uint8, device=device), K)
+
+
+def mx_quantize(x) -> MXRows:
+    """x (..., K), fp32, bf16 or fp16, as rows in 8 bits (vgdr_mx_quantize): a scale for each 32 elements of a row, the smallest
+    power of two with amax <= 464 scale, elements rounded to nearest, ties to even.  A block with a NaN or an infinity is
+    NaN.  No autograd."""
+    rows, ld = _mx_source('x', x)
+    out = _mx_rows(x.shape[:-1], x.shape[-1], x.device)
+    _launch(x.get_device(), _lib.load().vgdr_mx_quantize, _DTYPES[x.dtype], rows.data_ptr(), ld, out.values.data_ptr(),
+            out.scales.data_ptr(), rows.shape[0], x.shape[-1])
+    return out
+
+
+def mx_weight(w, gated: bool = False) -> MXWeight:
+    """w (n, k), fp32, bf16 or fp16, as 4-bit weights (vgdr_mx_weight): a scale for each 32 elements of a row, the smallest
+    power of two with amax <= 7 scale, elements rounded to nearest, ties to even.  gated: w is the FFN's input
+    projection, its two halves' rows for mx_swiglu.  Done once, where the model is made ready to serve."""
+    rows, ld = _mx_source('w', w.detach(), dims=2)
+    n, k = w.shape
+    assert n >= 1 and not (gated and n % 2), f'w of shape {tuple(w.shape)}' + (', gated' if gated else '')
+    T, C = (2 * -(-n // 32) if gated else -(-n // 16)), _blocks_of(k)
+    out = MXWeight(torch.empty((T, C, 4, 16, 16), dtype=torch.uint8, device=w.device),
+                   torch.empty((T, -(-C // 4), 4, 16, 4), dtype=torch.uint8, device=w.device), (n, k), gated)
+    _launch(w.get_device(), _lib.load().vgdr_mx_weight, _DTYPES[w.dtype], rows.data_ptr(), ld, out.values.data_ptr(),
+            out.scales.data_ptr(), n, k, int(gated))
+    return out
+
+
+def mx_rms_norm(x, weight, eps: float = 1e-6, residual=None, out_residual=None, norm_out: bool = False):
+    """rms_norm with its result as rows in 8 bits (vgdr_mx_rms_norm): h = x + residual, rounded to x's dtype (into
+    out_residual, a new tensor by default), and h rsqrt(mean h^2 + eps) weight, formed in 64 bits and rounded once, to
+    the bytes that mx_quantize would give of it.  Returns the MXRows; with norm_out also the norm
+    in x's dtype, rounded as rms_norm's; with residual also h: rows, (rows, h), (rows, y) or (rows, y, h).
+    x, residual, weight in one dtype, the last dim a multiple of 8; no autograd."""
+    index = x.get_device()
+    if index < 0:
+        _check_device(x)
+    _all_on(index, weight, residual, out_residual)
+    _check_grad(x, weight, residual)
+    if x.dtype not in _DTYPES:
+        raise NotImplementedError(f'x must be one of {list(_DTYPES)}; got {x.dtype}')
+    D = x.shape[-1]
+    assert weight.shape == (D,) and weight.dtype == x.dtype, \
+        f'weight must be ({D},) in {x.dtype}; got {tuple(weight.shape)} {weight.dtype}'
+    xs, w = _aligned(x), _aligned(weight)
+    r = h = None
+    if residual is not None:
+        assert residual.shape == x.shape and residual.dtype == x.dtype, 'residual must match x'
+        r = _aligned(residual)
+        if out_residual is None:
+            h = torch.empty_like(xs)
+        else:
+            assert out_residual.shape == x.shape and out_residual.dtype == x.dtype and out_residual.is_contiguous() \
+                and out_residual.data_ptr() % 16 == 0, 'out_residual: contiguous, aligned, shaped and typed as x'
+            h = out_residual
+    out = _mx_rows(x.shape[:-1], D, x.device)
+    y = torch.empty_like(xs) if norm_out else None
+    _launch(index, _lib.load().vgdr_mx_rms_norm, _DTYPES[x.dtype], xs.data_ptr(), _ptr(r), _ptr(h), w.data_ptr(), _ptr(y),
+            out.values.data_ptr(), out.scales.data_ptr(), xs.numel() // max(D, 1), D, float(eps))
+    got = (out,) + ((y,) if norm_out else ()) + ((h,) if residual is not None else ())
+    return got if len(got) > 1 else out
+
+
+def _mx_product(x, w: MXWeight, gated: bool, quantize: bool, out_dtype):
+    assert isinstance(w, MXWeight) and w.gated == gated, \
+        f'{"mx_swiglu takes a gated" if gated else "mx_linear takes an ungated"} MXWeight (mx_weight); got {type(w).__name__}'
+    n, k = w.shape
+    rows8 = isinstance(x, MXRows)
+    assert (x.size if rows8 else x.shape[-1] if x.dim() else 0) == k, f'x must be (..., {k}); got {tuple(x.shape)}'
+    index = x.values.get_device() if rows8 else x.get_device()
+    if index < 0:
+        _check_device(x.values if rows8 else x)
+    _all_on(index, w.values, w.scales, x.scales if rows8 else None)
+    xs = ws = None
+    if rows8:
+        dt = torch.bfloat16 if out_dtype is None else out_dtype
+        v, xs = _aligned(x.values), _aligned(x.scales)
+        code, ld = _lib.VGDR_MX8, 0
+    else:
+        dt = x.dtype if out_dtype is None else out_dtype
+        v, ld = _mx_source('x', x)
+        if v.data_ptr() % 16 or ld % 8:
+            pad = -k % 8                                              # rows of whole 16-byte units
+            v = F.pad(v, (0, pad)) if pad else v.clone(memory_format=torch.contiguous_format)
+            ld = k + pad
+        code = _DTYPES[x.dtype]
+    if dt not in _DTYPES:
+        raise NotImplementedError(f'out_dtype must be one of {list(_DTYPES)}; got {dt}')
+    lead, cols = x.shape[:-1], n // 2 if gated else n
+    R = v.numel() // v.shape[-1]
+    lib = _lib.load()
+    nbytes = lib.vgdr_mx_linear_workspace_size(code, R, k)
+    if nbytes:
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=v.device)
+    if quantize:
+        y = _mx_rows(lead, cols, v.device)
+        yp, ys, out = y.values.data_ptr(), y.scales.data_ptr(), _lib.VGDR_MX8
+    else:
+        y = torch.empty((*lead, cols), dtype=dt, device=v.device)
+        yp, ys, out = y.data_ptr(), None, _DTYPES[dt]
+    _launch(index, lib.vgdr_mx_linear, code, v.data_ptr(), ld, _ptr(xs), w.values.data_ptr(), w.scales.data_ptr(), int(gated),
+            out, yp, ys, _ptr(ws), nbytes, R, n, k)
+    return y
+
+
+def mx_linear(x, w: MXWeight, out_dtype=None):
+    """F.linear(x, w) with 4-bit weights (vgdr_mx_linear), for one row as for a batch of prompts: x (..., k) in fp32, bf16 or
+    fp16, which meets the weights exactly, or MXRows; fp32 sums, rounded once to out_dtype (x's; bf16
+    for MXRows).  A block of weights or of an MXRows that is NaN makes NaN what it takes part in.  No autograd."""
+    return _mx_product(x, w, False, False, out_dtype)
+
+
+def mx_swiglu(x, w: MXWeight, quantize: bool = False, out_dtype=None):
+    """swiglu(F.linear(x, w)) with gated 4-bit weights (mx_weight(w, gated=True)) in one kernel: both products, the
+    activation and their product in fp32, rounded once (the module rounds four times, infra/components/ffn.py:48-50),
+    to out_dtype as mx_linear, or with `quantize` to MXRows, which the FFN's second product reads.  No autograd."""
+    return _mx_product(x, w, True, quantize, out_dtype)
