@@ -42,85 +42,90 @@ __device__ __forceinline__ float gated_product(float a, float b, bool accurate) 
     return a * sigmoidf_(a) * b;
 }
 
-// y[row][col .. col + 3] in type `out`; columns from N on are dropped
-__device__ __forceinline__ void store4(const MxLinear &p, int64_t row, int col, f32x4 v) {
-    if (row >= p.rows || col >= p.N) return;
-    const int64_t at = row * p.N + col;
-    const bool whole = (p.N & 3) == 0;                                // and col + 3 < N, the address aligned
-    if (p.out == 0) {
-        float *y = reinterpret_cast<float *>(p.y) + at;
-        if (whole) {
-            *reinterpret_cast<f32x4 *>(y) = v;
-            return;
-        }
+// y[row][col .. col + 4 V - 1] in type `out`; columns from N on are dropped
+template <typename E, int V>
+__device__ __forceinline__ void store_as(const MxLinear &p, int64_t row, int col, const f32x4 *v) {
+    typedef E EV __attribute__((ext_vector_type(4 * V)));
+    typedef E E4 __attribute__((ext_vector_type(4)));
+    E *y = reinterpret_cast<E *>(p.y) + row * p.N + col;
+    EV o;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (col + j < p.N) y[j] = v[j];
-    } else if (p.out == 1) {
-        __bf16 *y = reinterpret_cast<__bf16 *>(p.y) + at;
-        const bf16x4 o = Elem<__bf16>::cvt(v);
-        if (whole) {
-            *reinterpret_cast<bf16x4 *>(y) = o;
-            return;
-        }
+    for (int j = 0; j < 4 * V; ++j) o[j] = (E)v[j / 4][j % 4];
+    if (p.N % (4 * V) == 0) {                                         // and col + 4 V <= N, the address aligned
+        if constexpr (sizeof(EV) <= 16) {
+            *reinterpret_cast<EV *>(y) = o;
+        } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (col + j < p.N) y[j] = o[j];
-    } else {
-        _Float16 *y = reinterpret_cast<_Float16 *>(p.y) + at;
-        const f16x4 o = Elem<_Float16>::cvt(v);
-        if (whole) {
-            *reinterpret_cast<f16x4 *>(y) = o;
-            return;
+            for (int h = 0; h < V; ++h) *reinterpret_cast<E4 *>(y + 4 * h) = E4{o[4 * h], o[4 * h + 1], o[4 * h + 2], o[4 * h + 3]};
         }
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (col + j < p.N) y[j] = o[j];
+        return;
     }
+#pragma unroll
+    for (int j = 0; j < 4 * V; ++j)
+        if (col + j < p.N) y[j] = o[j];
+}
+template <int V>
+__device__ __forceinline__ void store(const MxLinear &p, int64_t row, int col, const f32x4 *v) {
+    if (row >= p.rows || col >= p.N) return;
+    if (p.out == 0) store_as<float, V>(p, row, col, v);
+    else if (p.out == 1) store_as<__bf16, V>(p, row, col, v);
+    else store_as<_Float16, V>(p, row, col, v);
 }
 
-// The results of one tile of 16 rows and MT consecutive weight tiles from tile t0 on, acc[MT].
+// Which weight row MFMA row r of weight tile a meets, of the MT tiles from t0 on.  Results come out four
+// to a lane, of the rows 4 g .. + 3 of a tile; two tiles of the same kind (of the same weight, where they are gated) are
+// taken as 32 rows of which MFMA row 4 g + j of the h-th is row 8 g + 4 h + j, so that a lane ends up with eight
+// neighbouring columns, a row of y with 64 bytes in one store, and an 8-bit block with eight bytes a lane.
+struct WeightRow {
+    int tile, row;
+};
+template <bool GATED, int MT>
+__device__ __forceinline__ WeightRow weight_row(int a, int t0, int r) {
+    if constexpr (MT == 1) return {t0, r};
+    const int h = GATED ? a / 2 % 2 : a % 2;
+    const int first = GATED ? t0 + a / 4 * 4 + a % 2 : t0 + a / 2 * 2;
+    return {first + (r >> 3) * (GATED ? 2 : 1), 8 * (r >> 2 & 1) + 4 * h + (r & 3)};
+}
+
+// The results of row `row` (MFMA column r) from the MT weight tiles from t0 on, acc[MT].
 template <bool GATED, int MT>
 __device__ __forceinline__ void epilogue(const MxLinear &p, int64_t row, int t0, int g, const f32x4 *acc) {
     if constexpr (!GATED) {
+        if constexpr (MT == 1) {
+            store<1>(p, row, 16 * t0 + 4 * g, acc);
+        } else {
 #pragma unroll
-        for (int a = 0; a < MT; ++a)
-            if (t0 + a < p.T) store4(p, row, 16 * (t0 + a) + 4 * g, acc[a]);
-    } else {
-        f32x4 v[MT / 2];
-#pragma unroll
-        for (int a = 0; a < MT / 2; ++a)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[a][j] = gated_product(acc[2 * a][j], acc[2 * a + 1][j], p.out == 0);
-        if (p.out != MX8) {
-#pragma unroll
-            for (int a = 0; a < MT / 2; ++a)
-                if (t0 + 2 * a < p.T) store4(p, row, 8 * t0 + 16 * a + 4 * g, v[a]);
-            return;
+            for (int q = 0; q < MT / 2; ++q) store<2>(p, row, 16 * (t0 + 2 * q) + 8 * g, acc + 2 * q);
         }
-        if constexpr (MT % 4 == 0) {
-            // two pairs of tiles are a block of 32 columns, whose values are in the four lanes of row r
+    } else {
+        static_assert(MT % 4 == 0, "two pairs of gated tiles are a block of 32 columns");
+#pragma unroll
+        for (int q = 0; q < MT / 4; ++q) {
+            f32x4 v[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    v[h][j] = gated_product(acc[4 * q + 2 * h][j], acc[4 * q + 2 * h + 1][j], p.out == 0);
+            const int col = 8 * (t0 + 4 * q) + 8 * g;
+            if (p.out != MX8) {
+                store<2>(p, row, col, v);
+                continue;
+            }
             const int64_t Np = (p.N + 127) / 128 * 128;
+            uint32_t amax = 0;
+            float f[8];
 #pragma unroll
-            for (int q = 0; q < MT / 4; ++q) {
-                uint32_t amax = 0;
-                float f[2][4];
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        f[h][j] = t0 + 4 * q + 2 * h < p.T ? v[2 * q + h][j] : 0.f;   // past the weights: padding
-                        amax = max(amax, abs_bits(f[h][j]));
-                    }
-                amax = max(amax, (uint32_t)__shfl_xor((int)amax, 16));
-                amax = max(amax, (uint32_t)__shfl_xor((int)amax, 32));
-                const int b = mx_scale<8>(amax), col = 8 * t0 + 32 * q;
-                if (row < p.rows && col < Np) {
-                    uint8_t *y = reinterpret_cast<uint8_t *>(p.y) + row * Np + col + 4 * g;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) *reinterpret_cast<uint32_t *>(y + 16 * h) = mx_pack8(f[h], b);
-                    if (g == 0) p.y_scales[(row * Np + col) / 32] = (uint8_t)b;
-                }
+            for (int j = 0; j < 8; ++j) {
+                f[j] = col + j < p.N ? v[j / 4][j % 4] : 0.f;                       // past the weights: padding
+                amax = max(amax, abs_bits(f[j]));
+            }
+            amax = max(amax, (uint32_t)__shfl_xor((int)amax, 16));
+            amax = max(amax, (uint32_t)__shfl_xor((int)amax, 32));
+            const int b = mx_scale<8>(amax);
+            if (row < p.rows && col < Np) {
+                *reinterpret_cast<u32x2 *>(reinterpret_cast<uint8_t *>(p.y) + row * Np + col) = u32x2{mx_pack8(f, b), mx_pack8(f + 4, b)};
+                if (g == 0) p.y_scales[(row * Np + col) / 32] = (uint8_t)b;
             }
         }
     }
@@ -128,12 +133,14 @@ __device__ __forceinline__ void epilogue(const MxLinear &p, int64_t row, int t0,
 
 }  // namespace
 
-// Few rows: a workgroup owns MT weight tiles and 16 NB rows; its NWV waves take every NWV-th K tile and
-// meet in LDS, in a fixed order.  A wave stages its rows' tiles through an LDS region of its own (a load
-// covers whole rows, and no barrier is needed for it).
+// Few rows: a workgroup owns MT weight tiles and 16 NB rows; its NWV waves take every NWV-th K tile, the next one's loads
+// ahead of this one's products, and meet in LDS, in a fixed order.  A wave passes its rows' tiles through an LDS
+// region of its own, which needs no barrier: a load covers whole rows of a tile there, where fragments
+// straight from global memory would have every lane in a line of its own, and the address unit bounds those
+// (64 rows, K 5632, N 2048: 9.6 us; 64 rows, K and N 8192: 25).
 template <bool X8, bool GATED, int MT, int NB, int NWV>
 __global__ void __launch_bounds__(64 * NWV) mx_few_rows_kernel(const MxLinear p) {
-    constexpr int ROW = X8 ? 128 : 256, PITCH = ROW + 16, LR = 1024 / ROW, NL = 16 * NB / LR;
+    constexpr int ROW = X8 ? 128 : 256, PITCH = ROW + 16, LR = 1024 / ROW, NX = 16 * NB / LR;
     constexpr int STAGE = 16 * NB * PITCH, RED = NWV / 2 * MT * NB * 64 * 16;
     constexpr int LDS = STAGE * NWV > RED ? STAGE * NWV : RED;
     __shared__ __attribute__((aligned(16))) char lds[LDS];
@@ -146,25 +153,24 @@ __global__ void __launch_bounds__(64 * NWV) mx_few_rows_kernel(const MxLinear p)
     const uint8_t *w[MT], *ws[MT];
 #pragma unroll
     for (int a = 0; a < MT; ++a) {
-        const int t = t0 + a < p.T ? t0 + a : p.T - 1;
-        w[a] = p.w + (int64_t)t * p.C * 1024 + lane * 16;
-        ws[a] = p.w_scales + (int64_t)t * C4 * 256 + lane * 4;
+        const WeightRow at = weight_row<GATED, MT>(a, t0, r);
+        const int64_t t = at.tile < p.T ? at.tile : p.T - 1;            // past the end: the last one again, not stored
+        w[a] = p.w + t * p.C * 1024 + (16 * g + at.row) * 16;
+        ws[a] = p.w_scales + t * C4 * 256 + (16 * g + at.row) * 4;
     }
     // a lane loads 16 bytes of row lane / (64 / LR) + LR i; rows past the end are the last one again
     const int lr = lane / (64 / LR), lk = lane % (64 / LR) * 16;
-    const char *src[NL];
+    const char *x[NX];
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
+    for (int i = 0; i < NX; ++i) {
         const int64_t row = b0 + LR * i + lr < p.rows ? b0 + LR * i + lr : p.rows - 1;
-        src[i] = reinterpret_cast<const char *>(p.x) + row * p.ldx * (X8 ? 1 : 2) + lk;
+        x[i] = reinterpret_cast<const char *>(p.x) + row * p.ldx * (X8 ? 1 : 2) + lk;
     }
     const uint8_t *xs[NB];
-    if constexpr (X8) {
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const int64_t row = b0 + 16 * b + r < p.rows ? b0 + 16 * b + r : p.rows - 1;
-            xs[b] = p.x_scales + row * 4 * p.C + g;
-        }
+    for (int b = 0; b < NB; ++b) {
+        const int64_t row = b0 + 16 * b + r < p.rows ? b0 + 16 * b + r : p.rows - 1;
+        xs[b] = X8 ? p.x_scales + row * 4 * p.C + g : nullptr;
     }
     const int64_t plane = X8 ? 0 : p.rows * p.ldx * 2;
 
@@ -174,69 +180,73 @@ __global__ void __launch_bounds__(64 * NWV) mx_few_rows_kernel(const MxLinear p)
 #pragma unroll
         for (int b = 0; b < NB; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    // step s: K tile wave + NWV (s / planes), plane s % planes
-    const int mine = wave < p.C ? (p.C - wave + NWV - 1) / NWV : 0;
-    u32x4 wn[MT], xn[NL];
-    int wsn[MT], xsn[NB];
-    auto load = [&](int c, int plane_at) __attribute__((always_inline)) {
-#pragma unroll
-        for (int a = 0; a < MT; ++a) {
-            wn[a] = *reinterpret_cast<const u32x4 *>(w[a] + (int64_t)c * 1024);
-            wsn[a] = ws[a][(c >> 2) * 256 + (c & 3)];
-        }
-#pragma unroll
-        for (int i = 0; i < NL; ++i) xn[i] = *reinterpret_cast<const u32x4 *>(src[i] + plane_at * plane + (int64_t)c * ROW);
-        if constexpr (X8) {
-#pragma unroll
-            for (int b = 0; b < NB; ++b) xsn[b] = xs[b][4 * c];
-        }
+    struct Step {
+        u32x4 w[MT], x[NX];
+        int ws[MT], xs[NB];
     };
-    char *stage = lds + wave * STAGE;
-    const int steps = mine * p.planes;
+    // step s: K tile wave + NWV (s / planes), plane s % planes
+    const int steps = (wave < p.C ? (p.C - wave + NWV - 1) / NWV : 0) * p.planes;
     int c = wave, pl = 0;
-    if (steps) load(c, 0);
-    for (int s = 0; s < steps; ++s) {
-        u32x4 wc[MT];
-        int wsc[MT], xsc[NB];
+    auto load = [&](Step &to) __attribute__((always_inline)) {
 #pragma unroll
         for (int a = 0; a < MT; ++a) {
-            wc[a] = wn[a];
-            wsc[a] = wsn[a];
+            to.w[a] = *reinterpret_cast<const u32x4 *>(w[a] + (int64_t)c * 1024);
+            to.ws[a] = ws[a][(c >> 2) * 256 + (c & 3)];
         }
+#pragma unroll
+        for (int i = 0; i < NX; ++i) to.x[i] = *reinterpret_cast<const u32x4 *>(x[i] + pl * plane + (int64_t)c * ROW);
         if constexpr (X8) {
 #pragma unroll
-            for (int b = 0; b < NB; ++b) xsc[b] = xsn[b];
+            for (int b = 0; b < NB; ++b) to.xs[b] = xs[b][4 * (int64_t)c];
         }
-#pragma unroll
-        for (int i = 0; i < NL; ++i) *reinterpret_cast<u32x4 *>(stage + (LR * i + lr) * PITCH + lk) = xn[i];
-        // the region is this wave's alone: LDS operations of one wave are in order, and only the compiler has to keep it
-        asm volatile("" ::: "memory");
         if (++pl == p.planes) {
             pl = 0;
             c += NWV;
         }
-        if (s + 1 < steps) load(c, pl);
+    };
+    char *stage = lds + wave * STAGE;
+    auto put = [&](const Step &of) __attribute__((always_inline)) {
+        // LDS operations of one wave are in order: only the compiler has to keep it
+        asm volatile("" ::: "memory");
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const char *at = stage + (16 * b + r) * PITCH;
-            if constexpr (X8) {
-                const u32x4 lo = *reinterpret_cast<const u32x4 *>(at + 16 * g);
-                const u32x4 hi = *reinterpret_cast<const u32x4 *>(at + 64 + 16 * g);
+        for (int i = 0; i < NX; ++i) *reinterpret_cast<u32x4 *>(stage + (LR * i + lr) * PITCH + lk) = of.x[i];
+        asm volatile("" ::: "memory");
+    };
+    auto products = [&](const Step &of) __attribute__((always_inline)) {
+        if constexpr (X8) {
 #pragma unroll
-                for (int a = 0; a < MT; ++a) acc[a][b] = mfma_mx(wc[a], wsc[a], lo, hi, xsc[b], acc[a][b]);
-            } else {
-                bf16x8 f[4];
+            for (int b = 0; b < NB; ++b) {
+                const char *at = stage + (16 * b + r) * PITCH + 16 * g;
+                const u32x4 lo = *reinterpret_cast<const u32x4 *>(at), hi = *reinterpret_cast<const u32x4 *>(at + 64);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) f[i] = *reinterpret_cast<const bf16x8 *>(at + 64 * g + 16 * i);
+                for (int a = 0; a < MT; ++a) acc[a][b] = mfma_mx(of.w[a], of.ws[a], lo, hi, of.xs[b], acc[a][b]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                bf16x8 f[NB];
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+                    f[b] = *reinterpret_cast<const bf16x8 *>(stage + (16 * b + r) * PITCH + 64 * g + 16 * i);
 #pragma unroll
                 for (int a = 0; a < MT; ++a) {
-                    const float scale = mx_value(wsc[a]);
+                    const bf16x8 v = to_bf16(of.w[a][i], mx_value(of.ws[a]));
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[a][b] = mfma_pair(to_bf16(wc[a][i], scale), f[i], acc[a][b]);
+                    for (int b = 0; b < NB; ++b) acc[a][b] = mfma_pair(v, f[b], acc[a][b]);
                 }
             }
         }
-        asm volatile("" ::: "memory");
+    };
+    Step even, odd;
+    if (steps > 0) load(even);
+    for (int s = 0; s < steps; s += 2) {
+        put(even);
+        if (s + 1 < steps) load(odd);
+        products(even);
+        if (s + 1 == steps) break;
+        put(odd);
+        if (s + 2 < steps) load(even);
+        products(odd);
     }
     // the waves' sums, halves onto halves
     f32x4 *red = reinterpret_cast<f32x4 *>(lds);
@@ -267,72 +277,86 @@ __global__ void __launch_bounds__(64 * NWV) mx_few_rows_kernel(const MxLinear p)
     }
 }
 
-// Many rows: a workgroup owns BM rows and BN / 16 weight tiles, its WM x WN waves BM / WM x BN / WN each.  The rows'
-// K tiles go to LDS asynchronously, NBUF - 1 steps ahead, in 16-byte units swizzled so that the 16
-// rows of a fragment lie on distinct banks; a wave loads its weights' fragments from global memory, a step
-// ahead: they lie there as it needs them.
-template <bool X8, bool GATED, int BM, int BN, int WM, int WN, int NBUF>
-__global__ void __launch_bounds__(64 * WM * WN) mx_tile_kernel(const MxLinear p, int mb, int nb) {
+// Many rows: a workgroup owns BM rows and BN / 16 weight tiles, its WM x WN waves BM / WM x BN / WN each.  The K tiles of
+// both go to LDS asynchronously, a step ahead.  In LDS a row of x is cut into 16-byte units whose places
+// are swizzled so that the 16 rows of a fragment lie on distinct banks; of the two weight tiles that
+// weight_row mixes the second has its rows' places moved by four for the same reason.
+// Two workgroups share a CU: one's barriers, first copies and stores lie under the other's products.  At K = 2048
+// that is the larger part: 65,536 rows in 8 bits, N 8192: 930 us (2,360 TFLOP/s); one workgroup of 256 x 256 and
+// three stages 1,240, its next tile's copies begun under the stores 1,220; at K = N = 8192, 16,384 rows 790 us
+// (2,780 TFLOP/s) against 880.  The weights' fragments straight from global memory into registers: 1,360
+// (the wait for them is a wait for the copies behind them too).  bf16 rows: 1,760 us (1,250 TFLOP/s); there the LDS
+// for two workgroups allows 64 x 256, and the conversions share the issue slots with twice the products' time.
+template <bool X8, bool GATED, int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(64 * WM * WN, 2 * WM * WN / 4) mx_tile_kernel(const MxLinear p, uint32_t mb, uint32_t nb) {
     constexpr int ROW = X8 ? 128 : 256, UPR = ROW / 16, NWV = WM * WN;
     constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
-    constexpr int DMAS = BM * ROW / 1024 / NWV;                       // a wave's copies of a step
-    static_assert(BM * ROW % (1024 * NWV) == 0 && BM % 64 == 0, "whole copies");
-    static_assert(!X8 || BM / 64 <= NWV, "a wave copies the scales of 64 rows");
-    __shared__ __attribute__((aligned(16))) char xb[NBUF][BM * ROW];
-    __shared__ __attribute__((aligned(16))) uint32_t xsb[X8 ? NBUF : 1][X8 ? BM : 4];
+    constexpr uint32_t BAND = 8;
+    constexpr int DX = BM * ROW / 1024 / NWV, DW = BN / 16 / NWV;                     // a wave's copies of a step
+    static_assert(BM * ROW % (1024 * NWV) == 0 && BN % (16 * NWV) == 0 && BM % 64 == 0 && BN % 64 == 0, "whole copies");
+    static_assert(BM / 64 <= NWV && BN / 64 <= NWV, "a wave copies the scales of 64 rows of each");
+    struct Stage {
+        char x[BM * ROW];
+        char w[BN / 16][1024];
+        char ws[BN / 16][256];                                        // of four K tiles
+        uint32_t xs[X8 ? BM : 4];
+    };
+    __shared__ __attribute__((aligned(16))) Stage stage[2];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, r = lane & 15, wm = wave / WN, wn = wave % WN;
 
-    // an XCD (every eighth workgroup) walks a run of its own of the tiles, eight row blocks under each column block:
-    // its L2 holds those rows and meets every weight once for eight blocks
-    const int64_t total = (int64_t)mb * nb, per = (total + 7) / 8;
-    const int64_t id = (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    // an XCD (every eighth workgroup) walks a run of its own of the tiles, BAND row blocks under each column block: its
+    // L2 holds those rows and meets every weight once for BAND blocks
+    const uint32_t total = mb * nb, per = (total + 7) / 8, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
     if ((blockIdx.x >> 3) >= per || id >= total) return;
-    const int64_t band = id / (8 * (int64_t)nb);
-    const int high = mb - band * 8 < 8 ? (int)(mb - band * 8) : 8;
-    const int64_t in = id - band * 8 * nb;
-    const int64_t m0 = (band * 8 + in % high) * BM;
-    const int t0 = (int)(in / high) * (BN / 16) + wn * FN;
+    const uint32_t band = id / (BAND * nb), high = mb - band * BAND < BAND ? mb - band * BAND : BAND, in = id - band * BAND * nb;
+    const int64_t m0 = (int64_t)(band * BAND + in % high) * BM;
+    const int t0 = (int)(in / high) * (BN / 16);
 
     const int C4 = (p.C + 3) / 4;
-    const uint8_t *w[FN], *ws[FN];
+    // rows and weights past the end are the last ones again: their results are not stored
+    auto swz = [](int R) { return X8 ? (R >> 1) & 7 : R & 15; };      // unit u of row R lies at u ^ swz(R)
+    auto moved = [](int t) { return GATED ? (t >> 1 & 1) * 4 : (t & 1) * 4; };
+    const char *src[DX + DW], *wsrc, *xsrc = nullptr;
 #pragma unroll
-    for (int a = 0; a < FN; ++a) {
-        const int t = t0 + a < p.T ? t0 + a : p.T - 1;
-        w[a] = p.w + (int64_t)t * p.C * 1024 + lane * 16;
-        ws[a] = p.w_scales + (int64_t)t * C4 * 256 + lane * 4;
-    }
-    // copy i of this wave fills units 64 (wave DMAS + i) .. + 63 of the tile; unit u of row R lies at u ^ swz(R)
-    auto swz = [](int R) { return X8 ? (R >> 1) & 7 : R & 15; };
-    const char *src[DMAS];
-#pragma unroll
-    for (int i = 0; i < DMAS; ++i) {
-        const int at = 64 * (wave * DMAS + i) + lane, R = at / UPR, u = at % UPR ^ swz(R);
+    for (int i = 0; i < DX; ++i) {
+        const int at = 64 * (wave * DX + i) + lane, R = at / UPR, u = at % UPR ^ swz(R);
         const int64_t row = m0 + R < p.rows ? m0 + R : p.rows - 1;
         src[i] = reinterpret_cast<const char *>(p.x) + row * p.ldx * (X8 ? 1 : 2) + u * 16;
     }
-    // every wave copies the scales of 64 rows, so that all have as many copies on their way: where there are
-    // more waves than that, some copy the same
-    const int sblock = wave % (BM / 64);
-    const uint8_t *xsrc = nullptr;
-    if constexpr (X8) {
-        const int64_t row = m0 + 64 * sblock + lane < p.rows ? m0 + 64 * sblock + lane : p.rows - 1;
-        xsrc = p.x_scales + row * 4 * p.C;
+#pragma unroll
+    for (int i = 0; i < DW; ++i) {
+        const int a = wave * DW + i;
+        const int64_t t = t0 + a < p.T ? t0 + a : p.T - 1;
+        src[DX + i] = reinterpret_cast<const char *>(p.w) + t * p.C * 1024 + (lane ^ moved(a)) * 16;
+    }
+    // the scales: where there are more waves than blocks of 64 rows, some copy the same
+    const int wblock = wave % (BN / 64), xblock = wave % (BM / 64);
+    {
+        const int64_t t = t0 + 4 * wblock + g < p.T ? t0 + 4 * wblock + g : p.T - 1;
+        wsrc = reinterpret_cast<const char *>(p.w_scales) + t * C4 * 256 + r * 16;
+        if constexpr (X8) {
+            const int64_t row = m0 + 64 * xblock + lane < p.rows ? m0 + 64 * xblock + lane : p.rows - 1;
+            xsrc = reinterpret_cast<const char *>(p.x_scales) + row * 4 * p.C;
+        }
     }
     const int64_t plane = X8 ? 0 : p.rows * p.ldx * 2;
     const int steps = p.C * p.planes;
 
-    int ic = 0, ip = 0, is = 0;                                       // the next copy's K tile, plane and buffer
+    int ic = 0, ip = 0, is = 0;                                       // the next copy's K tile, plane and stage
     auto copy = [&]() __attribute__((always_inline)) {
+        Stage &to = stage[is];
 #pragma unroll
-        for (int i = 0; i < DMAS; ++i)
-            lds_dma16(src[i] + ip * plane + (int64_t)ic * ROW, xb[is] + (wave * DMAS + i) * 1024);
-        if constexpr (X8) lds_dma4(xsrc + 4 * (int64_t)ic, xsb[is] + 64 * sblock);
+        for (int i = 0; i < DX; ++i) lds_dma16(src[i] + ip * plane + (int64_t)ic * ROW, to.x + (wave * DX + i) * 1024);
+#pragma unroll
+        for (int i = 0; i < DW; ++i) lds_dma16(src[DX + i] + (int64_t)ic * 1024, to.w[wave * DW + i]);
+        lds_dma16(wsrc + (int64_t)(ic >> 2) * 256, to.ws[4 * wblock]);
+        if constexpr (X8) lds_dma4(xsrc + 4 * (int64_t)ic, to.xs + 64 * xblock);
         if (++ip == p.planes) {
             ip = 0;
             ++ic;
         }
-        is = is + 1 == NBUF ? 0 : is + 1;
+        is ^= 1;
     };
 
     f32x4 acc[FM][FN];
@@ -340,71 +364,75 @@ __global__ void __launch_bounds__(64 * WM * WN) mx_tile_kernel(const MxLinear p,
     for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int a = 0; a < FN; ++a) acc[i][a] = f32x4{0.f, 0.f, 0.f, 0.f};
-    u32x4 wn_[FN];
-    int wsn[FN];
-    auto load = [&](int c) __attribute__((always_inline)) {
+    // where a lane's weights lie in a stage
+    int wat[FN], wsat[FN];
 #pragma unroll
-        for (int a = 0; a < FN; ++a) {
-            wn_[a] = *reinterpret_cast<const u32x4 *>(w[a] + (int64_t)c * 1024);
-            wsn[a] = ws[a][(c >> 2) * 256 + (c & 3)];
-        }
-    };
-    load(0);
-#pragma unroll
-    for (int s = 0; s < NBUF - 1; ++s)
-        if (s < steps) copy();
-    int c = 0, pl = 0, buf = 0;
+    for (int a = 0; a < FN; ++a) {
+        const WeightRow at = weight_row<GATED, FN>(a, wn * FN, r);
+        wat[a] = at.tile * 1024 + ((16 * g + at.row) ^ moved(at.tile)) * 16;
+        wsat[a] = at.tile * 256 + (16 * g + at.row) * 4;
+    }
+    copy();
+    int c = 0, pl = 0;
     for (int s = 0; s < steps; ++s) {
-        // this step's copies have landed: of this wave's copies only those of the NBUF - 2 steps after it may
-        // still be on their way (loads that the compiler places in between make the wait longer, never shorter)
-        if (NBUF > 2 && s + NBUF - 2 < steps)
-            asm volatile("s_waitcnt vmcnt(%0)" :: "n"((NBUF - 2) * (DMAS + (X8 ? 1 : 0))) : "memory");
-        else
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        lds_barrier();
-        u32x4 wc[FN];
-        int wsc[FN];
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");              // this wave's copies of this step have landed
+        lds_barrier();                                                // all waves' have, and the last step's stage is read
+        if (s + 1 < steps) copy();
+        const Stage &from = stage[s & 1];
+        u32x4 w[FN];
+        int ws[FN];
 #pragma unroll
         for (int a = 0; a < FN; ++a) {
-            wc[a] = wn_[a];
-            wsc[a] = wsn[a];
+            w[a] = *reinterpret_cast<const u32x4 *>(from.w[0] + wat[a]);
+            ws[a] = reinterpret_cast<const uint8_t *>(from.ws[0])[wsat[a] + (c & 3)];
+        }
+        // x's fragments are read one ahead of the products that take them
+        if constexpr (X8) {
+            u32x4 lo[2], hi[2];
+            int xs[2];
+            auto read = [&](int i) __attribute__((always_inline)) {
+                const int R = (wm * FM + i) * 16 + r;
+                lo[i & 1] = *reinterpret_cast<const u32x4 *>(from.x + R * ROW + (g ^ swz(R)) * 16);
+                hi[i & 1] = *reinterpret_cast<const u32x4 *>(from.x + R * ROW + ((4 + g) ^ swz(R)) * 16);
+                xs[i & 1] = reinterpret_cast<const uint8_t *>(from.xs + R)[g];
+            };
+            read(0);
+            unroll<FM>([&](auto ii) __attribute__((always_inline)) {
+                constexpr int i = decltype(ii)::value;
+                if constexpr (i + 1 < FM) read(i + 1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int a = 0; a < FN; ++a) acc[i][a] = mfma_mx(w[a], ws[a], lo[i & 1], hi[i & 1], xs[i & 1], acc[i][a]);
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        } else {
+            bf16x8 x[2];
+            auto read = [&](int i) __attribute__((always_inline)) {                  // product i / FM of row tile i % FM
+                const int R = (wm * FM + i % FM) * 16 + r;
+                x[i & 1] = *reinterpret_cast<const bf16x8 *>(from.x + R * ROW + ((4 * g + i / FM) ^ swz(R)) * 16);
+            };
+            read(0);
+            bf16x8 f[FN];
+            unroll<4 * FM>([&](auto ii) __attribute__((always_inline)) {
+                constexpr int i = decltype(ii)::value;
+                if constexpr (i + 1 < 4 * FM) read(i + 1);
+                if constexpr (i % FM == 0) {
+#pragma unroll
+                    for (int a = 0; a < FN; ++a) f[a] = to_bf16(w[a][i / FM], mx_value(ws[a]));
+                }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int a = 0; a < FN; ++a) acc[i % FM][a] = mfma_pair(f[a], x[i & 1], acc[i % FM][a]);
+                __builtin_amdgcn_sched_barrier(0);
+            });
         }
         if (++pl == p.planes) {
             pl = 0;
             ++c;
         }
-        if (s + 1 < steps) load(c);
-        if (s + NBUF - 1 < steps) copy();
-        const char *tile = xb[buf];
-        if constexpr (X8) {
-#pragma unroll
-            for (int i = 0; i < FM; ++i) {
-                const int R = (wm * FM + i) * 16 + r;
-                const u32x4 lo = *reinterpret_cast<const u32x4 *>(tile + R * ROW + (g ^ swz(R)) * 16);
-                const u32x4 hi = *reinterpret_cast<const u32x4 *>(tile + R * ROW + ((4 + g) ^ swz(R)) * 16);
-                const int xs = reinterpret_cast<const uint8_t *>(xsb[buf] + R)[g];
-#pragma unroll
-                for (int a = 0; a < FN; ++a) acc[i][a] = mfma_mx(wc[a], wsc[a], lo, hi, xs, acc[i][a]);
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                bf16x8 f[FN];
-#pragma unroll
-                for (int a = 0; a < FN; ++a) f[a] = to_bf16(wc[a][k], mx_value(wsc[a]));
-#pragma unroll
-                for (int i = 0; i < FM; ++i) {
-                    const int R = (wm * FM + i) * 16 + r;
-                    const bf16x8 x = *reinterpret_cast<const bf16x8 *>(tile + R * ROW + ((4 * g + k) ^ swz(R)) * 16);
-#pragma unroll
-                    for (int a = 0; a < FN; ++a) acc[i][a] = mfma_pair(f[a], x, acc[i][a]);
-                }
-            }
-        }
-        buf = buf + 1 == NBUF ? 0 : buf + 1;
     }
 #pragma unroll
-    for (int i = 0; i < FM; ++i) epilogue<GATED, FN>(p, m0 + (wm * FM + i) * 16 + r, t0, g, acc[i]);
+    for (int i = 0; i < FM; ++i) epilogue<GATED, FN>(p, m0 + (wm * FM + i) * 16 + r, t0 + wn * FN, g, acc[i]);
 }
 
 namespace {
@@ -416,27 +444,48 @@ hipError_t few_rows_go(const MxLinear &p, int tiles, hipStream_t stream) {
     return hipGetLastError();
 }
 
-template <bool X8, bool GATED, int BM, int BN, int WM, int WN, int NBUF>
+template <bool X8, bool GATED, int BM, int BN, int WM, int WN>
 hipError_t tile_go(const MxLinear &p, int tiles, hipStream_t stream) {
     const int64_t mb = (p.rows + BM - 1) / BM, nb = (tiles + BN / 16 - 1) / (BN / 16);
-    const int64_t blocks = (mb * nb + 7) / 8 * 8;
-    hipLaunchKernelGGL((mx_tile_kernel<X8, GATED, BM, BN, WM, WN, NBUF>), dim3((unsigned)blocks), dim3(64 * WM * WN), 0, stream,
-                       p, (int)mb, (int)nb);
+    hipLaunchKernelGGL((mx_tile_kernel<X8, GATED, BM, BN, WM, WN>), dim3((unsigned)((mb * nb + 7) / 8 * 8)), dim3(64 * WM * WN), 0,
+                       stream, p, (uint32_t)mb, (uint32_t)nb);
     return hipGetLastError();
 }
 
+// The variant: the largest tiles that still give every CU a workgroup (a larger tile reads less, the smaller ones'
+// traffic bounds them), us for bf16 / 8-bit rows:
+//   64 rows, K 5632, N 2048: 2 tiles x 16 rows (256 workgroups) 8.6 / 8.2, 1 x 16 (512) 9.6 / 8.9, 2 x 32 (128) 10.7 / 9.7
+//   32 rows, K 2048, N 8192: 2 x 32 (256) 8.0 / 7.2, 2 x 16 (512) 7.9 / 7.6, 4 x 32 (128) 9.6 / 8.3
+// The kernel for few rows up to where 4 x 32 makes one workgroup a CU: it has the whole sum in flight.  128 rows, K 5632,
+// N 2048: 11.0 / 9.9, 64 x 64 tiles 26.6 / 18.8; 128 rows, K 2048, N 8192 (512 of 4 x 32): 15.4 / 13.6, tiles 13.9 / 11.0.
+// Tiles: largest with 5 workgroups for 4 CUs.  512 rows, K 2048, N 8192: 64 x 128 (512) 24.1 / 15.9, 64 x 64 (1,024) 27.6 /
+// 22.9; 256 rows: 64 x 64 (512) 17.0 / 13.2, 64 x 128 (256) 18.2 / 14.6; 8-bit rows, N 32768, 512 rows: 128 x 256
+// (512) 34.3, 64 x 256 38.2, 256 rows: 64 x 256 (512) 22.2, 128 x 256 (256) 25.3.
 template <bool X8, bool GATED>
 hipError_t mx_linear_t(const MxLinear &p, hipStream_t stream) {
     // the output's padding to whole 128s of columns counts as tiles (8-bit outputs: 8 pairs a 128)
     const int tiles = GATED && p.out == MX8 ? (p.N + 127) / 128 * 16 : p.T;
-    if (p.rows <= 16) return few_rows_go<X8, GATED, GATED ? 4 : 1, 1, 8>(p, tiles, stream);
-    if (p.rows <= 64) return few_rows_go<X8, GATED, GATED ? 4 : 1, 4, 8>(p, tiles, stream);
     const int64_t cus = device_cu_count();
-    if ((p.rows + 255) / 256 * ((tiles + 15) / 16) >= cus) {
-        if constexpr (X8) return tile_go<X8, GATED, 256, 256, 2, 4, 3>(p, tiles, stream);
-        else return tile_go<X8, GATED, 256, 256, 2, 4, 2>(p, tiles, stream);
+    auto few = [&](int mt, int nb) { return (int64_t)((tiles + mt - 1) / mt) * ((p.rows + 16 * nb - 1) / (16 * nb)); };
+    if (p.rows <= 32 || few(4, 2) <= cus) {
+        if (p.rows > 16 && few(4, 2) >= cus) return few_rows_go<X8, GATED, 4, 2, 8>(p, tiles, stream);
+        if constexpr (GATED) {
+            return few_rows_go<X8, GATED, 4, 1, 8>(p, tiles, stream);
+        } else {
+            if (p.rows > 16 && few(2, 2) >= cus) return few_rows_go<X8, GATED, 2, 2, 8>(p, tiles, stream);
+            if (few(4, 1) >= cus) return few_rows_go<X8, GATED, 4, 1, 8>(p, tiles, stream);
+            if (few(2, 1) >= cus) return few_rows_go<X8, GATED, 2, 1, 8>(p, tiles, stream);
+            return few_rows_go<X8, GATED, 1, 1, 8>(p, tiles, stream);
+        }
     }
-    return tile_go<X8, GATED, 64, 128, 2, 2, 3>(p, tiles, stream);
+    auto fills = [&](int bm, int bn) { return 4 * ((p.rows + bm - 1) / bm) * ((tiles + bn / 16 - 1) / (bn / 16)) >= 5 * cus; };
+    if constexpr (X8)
+        if (fills(128, 256)) return tile_go<X8, GATED, 128, 256, 2, 2>(p, tiles, stream);
+    if (fills(64, 256)) return tile_go<X8, GATED, 64, 256, 1, 4>(p, tiles, stream);
+    if (fills(64, 128)) return tile_go<X8, GATED, 64, 128, 2, 2>(p, tiles, stream);
+    // a gated block of 32 columns takes four tiles of a wave
+    if constexpr (GATED) return tile_go<X8, GATED, 64, 64, 4, 1>(p, tiles, stream);
+    else return tile_go<X8, GATED, 64, 64, 2, 2>(p, tiles, stream);
 }
 
 }  // namespace
