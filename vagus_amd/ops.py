@@ -90,7 +90,8 @@ def _aligned(t):
     a view that starts mid-vector is copied."""
     if t is None:
         return None
-    t = t.contiguous()
+    if not t.is_contiguous():
+        t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
@@ -2093,15 +2094,22 @@ def _mx_source(name, t, dims=None):
     K = t.shape[-1]
     if t.dim() != 2:
         t = t.reshape(-1, K)
-    if (t.stride(1) != 1 and K > 1) or (t.stride(0) < K and t.shape[0] > 1):
-        t = t.contiguous()
-    return t, t.stride(0) if t.shape[0] > 1 else K
+    ld, one = t.stride()
+    if t.shape[0] <= 1:
+        ld = K
+    if (one != 1 and K > 1) or ld < K:
+        t, ld = t.contiguous(), K
+    return t, ld
 
 
-def _mx_rows(lead, K: int, device) -> MXRows:
+def _mx_rows(lead, K: int, like) -> MXRows:
+    """Room for rows of K columns beside `like`."""
     C = _blocks_of(K)
-    return MXRows(torch.empty((*lead, 128 * C), dtype=torch.float8_e4m3fn, device=device),
-                  torch.empty((*lead, 4 * C), dtype=torch.uint8, device=device), K)
+    out = MXRows.__new__(MXRows)                          # of the right shapes: nothing to check
+    out.values = like.new_empty((*lead, 128 * C), dtype=torch.float8_e4m3fn)
+    out.scales = like.new_empty((*lead, 4 * C), dtype=torch.uint8)
+    out.size = K
+    return out
 
 
 def mx_quantize(x) -> MXRows:
@@ -2109,7 +2117,7 @@ def mx_quantize(x) -> MXRows:
     power of two with amax <= 464 scale, elements rounded to nearest, ties to even.  A block with a NaN or an infinity is
     NaN.  No autograd."""
     rows, ld = _mx_source('x', x)
-    out = _mx_rows(x.shape[:-1], x.shape[-1], x.device)
+    out = _mx_rows(x.shape[:-1], x.shape[-1], x)
     _launch(x.get_device(), _lib.load().vgdr_mx_quantize, _DTYPES[x.dtype], rows.data_ptr(), ld, out.values.data_ptr(),
             out.scales.data_ptr(), rows.shape[0], x.shape[-1])
     return out
@@ -2152,13 +2160,13 @@ def mx_rms_norm(x, weight, eps: float = 1e-6, residual=None, out_residual=None, 
         assert residual.shape == x.shape and residual.dtype == x.dtype, 'residual must match x'
         r = _aligned(residual)
         if out_residual is None:
-            h = torch.empty_like(xs)
+            h = x.new_empty(x.shape)
         else:
             assert out_residual.shape == x.shape and out_residual.dtype == x.dtype and out_residual.is_contiguous() \
                 and out_residual.data_ptr() % 16 == 0, 'out_residual: contiguous, aligned, shaped and typed as x'
             h = out_residual
-    out = _mx_rows(x.shape[:-1], D, x.device)
-    y = torch.empty_like(xs) if norm_out else None
+    out = _mx_rows(x.shape[:-1], D, x)
+    y = x.new_empty(x.shape) if norm_out else None
     _launch(index, _lib.load().vgdr_mx_rms_norm, _DTYPES[x.dtype], xs.data_ptr(), _ptr(r), _ptr(h), w.data_ptr(), _ptr(y),
             out.values.data_ptr(), out.scales.data_ptr(), xs.numel() // max(D, 1), D, float(eps))
     got = (out,) + ((y,) if norm_out else ()) + ((h,) if residual is not None else ())
@@ -2193,14 +2201,15 @@ def _mx_product(x, w: MXWeight, gated: bool, quantize: bool, out_dtype):
     lead, cols = x.shape[:-1], n // 2 if gated else n
     R = v.numel() // v.shape[-1]
     lib = _lib.load()
-    nbytes = lib.vgdr_mx_linear_workspace_size(code, R, k)
+    # bf16 and 8-bit rows of whole 128s of columns are read where they lie
+    nbytes = 0 if rows8 or (code == _lib.VGDR_BF16 and k % 128 == 0) else lib.vgdr_mx_linear_workspace_size(code, R, k)
     if nbytes:
         ws = torch.empty((nbytes,), dtype=torch.uint8, device=v.device)
     if quantize:
-        y = _mx_rows(lead, cols, v.device)
+        y = _mx_rows(lead, cols, v)
         yp, ys, out = y.values.data_ptr(), y.scales.data_ptr(), _lib.VGDR_MX8
     else:
-        y = torch.empty((*lead, cols), dtype=dt, device=v.device)
+        y = v.new_empty((*lead, cols), dtype=dt)
         yp, ys, out = y.data_ptr(), None, _DTYPES[dt]
     _launch(index, lib.vgdr_mx_linear, code, v.data_ptr(), ld, _ptr(xs), w.values.data_ptr(), w.scales.data_ptr(), int(gated),
             out, yp, ys, _ptr(ws), nbytes, R, n, k)
