@@ -72,6 +72,34 @@ def _plain_module(m, cls) -> bool:
         or nn.modules.module._has_any_global_hook()))
 
 
+class MXLinear(nn.Module):
+    """A bias-free linear map whose weights are 4-bit numbers with a scale for each 32 (ops.MXWeight), as buffers: what
+    serving reads a quarter of.  gated: the FFN's input projection, its two halves' tiles by turns
+    (ops.mx_swiglu).  No autograd.  The reference has no quantised layers."""
+
+    def __init__(self, weight: ops.MXWeight):
+        super().__init__()
+        self.shape, self.gated = tuple(weight.shape), weight.gated
+        self.register_buffer('values', weight.values)
+        self.register_buffer('scales', weight.scales)
+
+    @property
+    def weight(self) -> ops.MXWeight:
+        return ops.MXWeight(self.values, self.scales, self.shape, self.gated)
+
+    def rows(self, first: int, n: int) -> ops.MXWeight:
+        """The n rows from `first` on (multiples of 16) as a weight of their own, in place."""
+        assert not self.gated and first % 16 == 0 and n % 16 == 0 and 0 <= first and first + n <= self.shape[0]
+        t = slice(first // 16, (first + n) // 16)
+        return ops.MXWeight(self.values[t], self.scales[t], (n, self.shape[1]))
+
+    def forward(self, x):
+        return ops.mx_linear(x, self.weight)
+
+    def extra_repr(self) -> str:
+        return f'{self.shape[1]}, {self.shape[0]}' + (', gated' if self.gated else '')
+
+
 def parse_fusions(spec) -> frozenset:
     """`fused=` as the reference accepts it (linear_attention.py:95-112): True
     (all), False / None (none), or a subset ('gate', 'conv,gate', 'scan' =
@@ -288,6 +316,34 @@ class GatedDeltaNet(nn.Module):
             on = on - {'gate'}
         return on
 
+    def quantize_weights_(self) -> None:
+        """W_q, W_k, W_v, W_g (as one map, w_in, whose rows they are) and W_o become 4-bit weights (MXLinear), in place and for
+        good; what decides how the state decays and is written (W_a, W_b, the short conv, A_log, dt_bias) keeps
+        its type.  For serving: forward, decode_step, draft_step and prefill_packed without autograd."""
+        if hasattr(self, 'w_in'):
+            return
+        mods = [self.wq, self.wk, self.wv, self.wg] + ([self.wo] if self.out_proj else [])
+        if not all(_plain_module(m, nn.Linear) and m.bias is None for m in mods):
+            raise NotImplementedError('4-bit weights stand for plain bias-free nn.Linear projections')
+        if any(m.weight.shape[0] % 16 for m in mods[:4]):
+            raise NotImplementedError(f'4-bit projections have multiples of 16 columns; got {[m.weight.shape[0] for m in mods[:4]]}')
+        w_in = MXLinear(ops.mx_weight(torch.cat([m.weight.detach() for m in mods[:4]])))
+        wo = MXLinear(ops.mx_weight(self.wo.weight)) if self.out_proj else None
+        del self.wq, self.wk, self.wv, self.wg
+        self.w_in = w_in
+        if wo is not None:
+            self.wo = wo
+
+    def _project(self, x, x8=None) -> dict:
+        """q, k, v and the output gate of 4-bit projections, each a tensor of its own; x8: x as 8-bit rows, which then
+        meet the weights in its place."""
+        H, dk, dv = self.head_count, self.key_head_dim, self.value_head_dim
+        y, at = {}, 0
+        for n, width in zip(('wq', 'wk', 'wv', 'wg'), (H * dk, H * dk, H * dv, H * dv)):
+            y[n] = ops.mx_linear(x if x8 is None else x8, self.w_in.rows(at, width), out_dtype=x.dtype)
+            at += width
+        return y
+
     def _input_projections(self) -> tuple:
         """The names of the projections that read the layer's input."""
         return ('wq', 'wk', 'wv', 'wg') + {'none': (), 'scalar': ('wa',), 'vector': ('wa1',)}[self.gate] \
@@ -297,6 +353,8 @@ class GatedDeltaNet(nn.Module):
         """Whether the projections are plain bias-free nn.Linear modules (and the
         methods that call them this class's own), so that a grouped product may
         stand for their calls."""
+        if hasattr(self, 'w_in'):
+            return False
         names = self._input_projections() + (('wa2',) if self.gate == 'vector' else ()) \
             + (('wo',) if self.out_proj else ())
         mods = [getattr(self, n) for n in names]
@@ -310,13 +368,13 @@ class GatedDeltaNet(nn.Module):
         projections of x already formed, by name."""
         g = beta = None
         H, dk = self.head_count, self.key_head_dim
-        out = lambda n: proj[n] if proj else getattr(self, n)(x)  # noqa: E731
+        out = lambda n: proj[n] if proj and n in proj else getattr(self, n)(x)  # noqa: E731
         if self.gate == 'scalar':
             assert not raw_gate, 'the fused gate activation is KDA-only (vector gate)'
             g = -self.A_log.float().exp() * F.softplus(out('wa').float() + self.dt_bias.float())
         elif self.gate == 'vector':
             B, L = x.shape[0], x.shape[1]
-            f = ops.projections(proj['wa1'], self.wa2.weight)[0] if proj else self.wa2(self.wa1(x))
+            f = ops.projections(proj['wa1'], self.wa2.weight)[0] if proj and 'wa1' in proj else self.wa2(self.wa1(x))
             if raw_gate:
                 g = f.view(B, L, H, dk)
             elif self.gate_lower_bound is not None:
@@ -375,9 +433,10 @@ class GatedDeltaNet(nn.Module):
                             lower_bound=self.gate_lower_bound, cu_seqlens=cu_seqlens,
                             whole_sequences=self.whole_sequences)
 
-    def _output(self, o, x, *, proj: dict | None = None):
+    def _output(self, o, x, *, proj: dict | None = None, rows8: bool = False):
         """RMSNorm(o) x SiLU(W_g x) per head, then W_o (:814-825): one HIP pass
-        for the epilogue.  proj: the projections of x already formed, by name."""
+        for the epilogue.  proj: the projections of x already formed, by name.
+        rows8: a 4-bit W_o takes the epilogue's rows in 8 bits."""
         B, L = x.shape[0], x.shape[1]
         gate = (proj['wg'] if proj else self.wg(x)).view(B, L, self.head_count, self.value_head_dim)
         if _autograd(o, gate, self.o_norm.gamma):
@@ -391,7 +450,9 @@ class GatedDeltaNet(nn.Module):
             o = ops.rms_norm_gated(o.to(gate.dtype), gate, self.o_norm.gamma, eps=self.o_norm.eps).reshape(B, L, -1)
         if not self.out_proj:
             return o
-        return ops.projections(o, self.wo.weight)[0] if proj else self.wo(o)
+        if rows8:
+            return ops.mx_linear(ops.mx_quantize(o), self.wo.weight, out_dtype=o.dtype)
+        return ops.projections(o, self.wo.weight)[0] if proj and not hasattr(self, 'w_in') else self.wo(o)
 
     # --- training / stateless --------------------------------------------
 
@@ -403,11 +464,11 @@ class GatedDeltaNet(nn.Module):
             names = self._input_projections()
             y = dict(zip(names, ops.projections(x, *(getattr(self, n).weight for n in names))))
         else:
-            y = {}
-        qp, kp, vp = (y[n] if grouped else getattr(self, n)(x) for n in ('wq', 'wk', 'wv'))
+            y = self._project(x) if hasattr(self, 'w_in') else {}
+        qp, kp, vp = (y[n] if y else getattr(self, n)(x) for n in ('wq', 'wk', 'wv'))
         on = self._active_fusions(qp)
         q, k, v = self._heads(qp, kp, vp, l2norm='l2norm' not in on)
-        kw = dict(proj=y) if grouped else {}
+        kw = dict(proj=y) if y else {}
         g, beta = self._gates(x, raw_gate='gate' in on, raw_beta='beta' in on, **kw)
         beta, w = self._write(x, k, g, beta)
         o, _ = self._scan(q, k, v, g, beta, None, fusions=on, w=w)
@@ -486,6 +547,8 @@ class GatedDeltaNet(nn.Module):
         H, dk, dv = self.head_count, self.key_head_dim, self.value_head_dim
         vec, scalar = self.gate == 'vector', self.gate == 'scalar' and not raw_gate
         raw_gate = raw_gate and self.gate == 'scalar'
+        if hasattr(self, 'w_in'):
+            return self._decode_inputs_4bit(x, scalar, raw_gate)
         names = self._input_projections()
         mods = [self._modules.get(n) for n in names]
         x2 = x.reshape(B, -1)
@@ -521,6 +584,31 @@ class GatedDeltaNet(nn.Module):
         g, beta = self._gates(x, raw_gate=vec, raw_beta=self.delta)
         return self.wq(x), self.wk(x), self.wv(x), self.wg(x), g, beta if self.delta else None, None
 
+    def _decode_inputs_4bit(self, x, scalar: bool, raw_gate: bool):
+        """_decode_inputs with 4-bit projections: q, k, v and the output gate are one product's column blocks."""
+        B = x.shape[0]
+        H, dk, dv = self.head_count, self.key_head_dim, self.value_head_dim
+        y = self.w_in(x.reshape(B, -1))
+        ld, out, at = y.shape[1], [], y.storage_offset()
+        for n in (H * dk, H * dk, H * dv, H * dv):
+            out.append(y.as_strided((B, 1, n), (ld, n, 1), at))
+            at += n
+        if type(self)._gates is not GatedDeltaNet._gates:
+            g, beta = self._gates(x, raw_gate=self.gate == 'vector', raw_beta=self.delta)
+            return *out, g, beta, None
+        if scalar:                                              # the decode kernel forms both
+            wb = self.wb.weight if hasattr(self, 'wb') else None
+            if all(_plain_module(m, nn.Linear) and m.bias is None and m.weight.dtype == x.dtype
+                   for m in (self.wa,) + ((self.wb,) if wb is not None else ())):
+                return *out, None, None, (x, self.wa.weight, wb, self.A_log, self.dt_bias)
+            g, beta = self._gates(x, raw_beta=self.delta)
+            return *out, g, beta, None
+        beta = self.wb(x).float().view(B, 1, H) if self.delta and hasattr(self, 'wb') else None
+        if raw_gate:
+            return *out, self.wa(x).view(B, 1, H), beta, (self.A_log, self.dt_bias)
+        g = self.wa2(self.wa1(x)).view(B, 1, H, dk) if self.gate == 'vector' else None
+        return *out, g, beta, None
+
     @torch.no_grad()
     def decode_step(self, x):
         """Consume the next block (B, L, dim), advancing the state (:918-952).
@@ -547,7 +635,8 @@ class GatedDeltaNet(nn.Module):
             self.cache_len += L
             o = o.reshape(B, L, H * dv)
             return self.wo(o) if self.out_proj else o
-        qp, kp, vp = self.wq(x), self.wk(x), self.wv(x)
+        y = self._project(x) if hasattr(self, 'w_in') else {}
+        qp, kp, vp = (y[n] if y else getattr(self, n)(x) for n in ('wq', 'wk', 'wv'))
         if self.short_conv_size is not None:
             qp = self.conv_q(qp, 'silu', conv_cache=self.qp_cache)
             kp = self.conv_k(kp, 'silu', conv_cache=self.kp_cache)
@@ -564,7 +653,7 @@ class GatedDeltaNet(nn.Module):
             o, S = self._scan(q, k, v, g, beta, self.state, w=w)
             self.state.copy_(S)
         self.cache_len += L
-        return self._output(o, x)
+        return self._output(o, x, **(dict(proj=y) if y else {}))
 
     def begin_drafts(self, capacity: int) -> None:
         """Room for blocks of up to `capacity` drafted tokens a stream (draft_step), none pending.
@@ -620,12 +709,14 @@ class GatedDeltaNet(nn.Module):
         ops.commit_drafts(self.state, self._drafted, accepted, **conv)
 
     @torch.no_grad()
-    def prefill_packed(self, x, cu_seqlens, *, rows=None):
+    def prefill_packed(self, x, cu_seqlens, *, rows=None, x8=None):
         """Push ragged blocks, packed as x (1, T, dim) with cu_seqlens (N + 1),
         into cache rows: block n continues the stream of row rows[n] (default:
         row n) from its state and conv tail, which it advances.  Returns the
         layer output (1, T, dim).  The reference's Generator has no such call:
-        its decode_step takes equal-length rows only (generator.py:19-22)."""
+        its decode_step takes equal-length rows only (generator.py:19-22).
+        x8: x as 8-bit rows (ops.MXRows), which 4-bit projections then take in
+        x's place, as W_o the epilogue's; the gates' projections take x."""
         assert x.shape[0] == 1, 'prefill_packed takes a packed batch (1, T, dim)'
         N = cu_seqlens.numel() - 1
         rows = list(range(N)) if rows is None else list(rows)
@@ -633,7 +724,9 @@ class GatedDeltaNet(nn.Module):
         assert self.state.shape[0] > 0, 'No state allocated. Call reset_cache or load_cache first.'
         T = x.shape[1]
         H, dk, dv = self.head_count, self.key_head_dim, self.value_head_dim
-        qp, kp, vp = self.wq(x), self.wk(x), self.wv(x)
+        assert x8 is None or hasattr(self, 'w_in'), '8-bit rows are for 4-bit weights (quantize_weights_)'
+        y = self._project(x, x8) if hasattr(self, 'w_in') else {}
+        qp, kp, vp = (y[n] if y else getattr(self, n)(x) for n in ('wq', 'wk', 'wv'))
         on = self._active_fusions(qp)
         whole = rows == list(range(self.state.shape[0]))
         idx = None if whole else torch.as_tensor(rows, dtype=torch.long, device=x.device)
@@ -658,4 +751,4 @@ class GatedDeltaNet(nn.Module):
             self.state.copy_(S)
         else:
             self.state.index_copy_(0, idx, S)
-        return self._output(o, x)
+        return self._output(o, x, **(dict(proj=y, rows8=x8 is not None) if y else {}))

@@ -33,7 +33,7 @@ import torch
 from torch import nn
 
 from . import ops
-from .layer import GatedDeltaNet, RMSNorm
+from .layer import GatedDeltaNet, MXLinear, RMSNorm, _plain_module
 
 
 def _add_norm(norm: RMSNorm, x, delta=None, *, inplace: bool = False):
@@ -55,9 +55,25 @@ def _add_norm(norm: RMSNorm, x, delta=None, *, inplace: bool = False):
     return x, norm(x)
 
 
-def _ffn(ffn: 'FFN', h):
+def _add_norm8(norm: RMSNorm, x, delta, *, norm_out: bool):
+    """_add_norm for a prompt's packed rows with the norm in 8 bits (ops.mx_rms_norm): (x + delta in x itself, the norm as
+    MXRows, with norm_out in x's type too, else None)."""
+    if delta is None:
+        got = ops.mx_rms_norm(x, norm.gamma, norm.eps, norm_out=norm_out)
+        return (x, *got) if norm_out else (x, got, None)
+    in_place = x.is_contiguous() and x.data_ptr() % 16 == 0
+    got = ops.mx_rms_norm(x, norm.gamma, norm.eps, residual=delta, out_residual=x if in_place else None, norm_out=norm_out)
+    return (got[2], got[0], got[1]) if norm_out else (got[1], got[0], None)
+
+
+def _ffn(ffn: 'FFN', h, dtype=None):
     """The FFN with its SwiGLU as one HIP pass (ops.swiglu) for GPU tensors
-    without autograd; the module's expression otherwise."""
+    without autograd; the module's expression otherwise.  With 4-bit weights h may be 8-bit rows: then so are the
+    activations between the two products, and dtype is the result's."""
+    if isinstance(h, ops.MXRows):
+        return ops.mx_linear(ops.mx_swiglu(h, ffn.l1.weight, quantize=True), ffn.l2.weight, out_dtype=dtype)
+    if isinstance(ffn.l1, MXLinear):
+        return ffn(h)
     if (h.is_cuda and not torch.is_grad_enabled() and h.dtype in (torch.bfloat16, torch.float16, torch.float32)
             and ffn.hidden_dim % (16 // h.element_size()) == 0):
         return ffn.l2(ops.swiglu(ffn.l1(h)))
@@ -78,7 +94,17 @@ class FFN(nn.Module):
         nn.init.normal_(self.l1.weight, std=init_std)
         nn.init.normal_(self.l2.weight, std=init_std / math.sqrt(2 * layer_count) if layer_count else init_std)
 
+    def quantize_weights_(self) -> None:
+        """Both projections become 4-bit weights (MXLinear), in place and for good; no autograd from then on."""
+        if isinstance(self.l1, MXLinear):
+            return
+        if not all(_plain_module(m, nn.Linear) and m.bias is None for m in (self.l1, self.l2)):
+            raise NotImplementedError('4-bit weights stand for plain bias-free nn.Linear projections')
+        self.l1, self.l2 = MXLinear(ops.mx_weight(self.l1.weight, gated=True)), MXLinear(ops.mx_weight(self.l2.weight))
+
     def forward(self, x):
+        if isinstance(self.l1, MXLinear):
+            return self.l2(ops.mx_swiglu(x, self.l1.weight))
         x1, xgate = torch.chunk(self.l1(x), 2, dim=-1)
         return self.l2(self.silu(x1) * xgate)
 
@@ -120,6 +146,13 @@ class Block(nn.Module):
         _, h = _add_norm(self.rmsnorm1, x)
         x, h = _add_norm(self.rmsnorm2, x, self.att.prefill_packed(h, cu_seqlens, rows=rows))
         return x + _ffn(self.ffn, h)
+
+    def _stream8(self, x, delta, cu_seqlens, rows):
+        """_stream over packed prompts with 4-bit weights whose rows are 8-bit: both norms give them, and the mixer's
+        gates take the first norm in x's type."""
+        x, h8, h = _add_norm8(self.rmsnorm1, x, delta, norm_out=True)
+        x, h8, _ = _add_norm8(self.rmsnorm2, x, self.att.prefill_packed(h, cu_seqlens, rows=rows, x8=h8), norm_out=False)
+        return x, _ffn(self.ffn, h8, x.dtype)
 
     def _stream(self, x, delta, step):
         """One block over the residual stream x with the previous block's
@@ -212,6 +245,30 @@ class GDNLM(nn.Module):
     def from_config(cls, config: dict) -> 'GDNLM':
         return cls(**config)
 
+    def quantize_weights_(self, *, prompt_bits: int = 8, head: bool = True) -> 'GDNLM':
+        """The blocks' large projections (q, k, v, output gate, W_o, both of the FFN) and the head become 4-bit weights with
+        a scale for each 32 (layer.MXLinear), in place and for good, on the GPU: a decode step reads a quarter of the bytes.
+        The embedding, the norms, the short convs and the gates' projections keep their type.  Packed prompts
+        (prefill_packed) go through the products as 8-bit rows, at twice the rate of 16-bit ones, or with prompt_bits=16
+        as they are; other calls take 16-bit rows.  No autograd from then on.  A state_dict of the quantised model loads into one
+        that was quantised.  Returns self."""
+        assert prompt_bits in (8, 16), f'prompt_bits must be 8 or 16; got {prompt_bits}'
+        if head and not isinstance(self.head, MXLinear) and not (_plain_module(self.head, nn.Linear) and self.head.bias is None):
+            raise NotImplementedError('4-bit weights stand for a plain bias-free nn.Linear head')
+        for blk in self.blocks:
+            blk.att.quantize_weights_()
+            blk.ffn.quantize_weights_()
+        if head and not isinstance(self.head, MXLinear):
+            self.head = MXLinear(ops.mx_weight(self.head.weight))
+        # mx_rms_norm's rows: multiples of 8
+        self.prompt_bits = prompt_bits if self.config['dim'] % 8 == 0 and self.config['dim'] <= 16384 else 16
+        return self
+
+    def _quantized(self) -> list:
+        """The 4-bit weights' buffers: none before quantize_weights_."""
+        maps = [m for blk in self.blocks for m in (getattr(blk.att, 'w_in', None), getattr(blk.att, 'wo', None), blk.ffn.l1, blk.ffn.l2)]
+        return [t for m in maps + [self.head] if isinstance(m, MXLinear) for t in (m.values, m.scales)]
+
     def forward(self, tokens, is_causal: bool = True, return_hidden: bool = False):
         x = self.embedding(tokens)
         for blk in self.blocks:
@@ -275,7 +332,11 @@ class GDNLM(nn.Module):
         x = self.embedding(tokens.reshape(1, -1))
         delta = None
         for blk in self.blocks:
-            x, delta = blk._stream(x, delta, lambda h, blk=blk: blk.att.prefill_packed(h, cu_seqlens, rows=rows))
+            if (getattr(self, 'prompt_bits', 16) == 8 and x.dtype in (torch.bfloat16, torch.float16)
+                    and blk.rmsnorm1.gamma.dtype == x.dtype == blk.rmsnorm2.gamma.dtype):
+                x, delta = blk._stream8(x, delta, cu_seqlens, rows)
+            else:
+                x, delta = blk._stream(x, delta, lambda h, blk=blk: blk.att.prefill_packed(h, cu_seqlens, rows=rows))
         if not last_logits:
             return None
         last = (cu_seqlens[1:] - 1).long()
@@ -364,7 +425,7 @@ class RaggedGenerator:
         (storage and version: load_state_dict, an optimizer step or .to()
         change one of them) and each layer's state and conv-cache buffers.  A
         replay is valid only while the addresses are unchanged."""
-        key = [(p.data_ptr(), p._version) for p in self.model.parameters()]
+        key = [(p.data_ptr(), p._version) for p in (*self.model.parameters(), *self.model._quantized())]
         for blk in self.model.blocks:
             att = blk.att
             key += [(t.data_ptr(), t.dtype) for t in (att.state,) + (att._caches() if att.short_conv_size else ())]
