@@ -128,7 +128,8 @@ def test_entry_points_check_their_arguments():
         a = dict(dt=1, x=4096, ld=128, v=8192, s=12288, rows=2, cols=128) | o
         return L.vgdr_mx_quantize(a['dt'], a['x'], a['ld'], a['v'], a['s'], a['rows'], a['cols'], None)
     assert q(dt=3) == q(dt=-1) == q(x=None) == q(v=None) == q(s=None) == q(v=8200) == q(rows=-1) == q(cols=0) == q(ld=127) == bad
-    assert q(v=4096) == q(rows=1 << 40) == q(cols=(1 << 24) + 1, ld=1 << 25) == bad
+    assert q(v=4096) == q(cols=(1 << 24) + 1, ld=1 << 25) == bad
+    assert q(rows=1 << 40) == q(rows=1 << 28) == no                    # more threads than a launch has
     assert q(rows=0, x=None) == _lib.VGDR_OK
 
     def w(**o):
@@ -142,6 +143,7 @@ def test_entry_points_check_their_arguments():
     assert n(dim=4) == n(dim=132) == n(dim=16392) == n(dim=0) == no
     assert n(dt=3) == n(x=4100) == n(v=4096) == n(y=4096) == n(y=12288) == n(eps=-1.0) == n(eps=float('nan')) == n(rows=-1) == bad
     assert n(r=12288) == n(xo=12288) == n(g=None) == bad
+    assert n(rows=1 << 24) == no
 
     def p(**o):
         a = dict(xd=1, x=4096, ld=128, xs=None, v=8192, s=12288, gated=0, od=1, y=16384, ys=None, ws=None, nb=0, rows=2, n=32, k=128) | o
@@ -152,6 +154,7 @@ def test_entry_points_check_their_arguments():
     assert p(k=1 << 25) == p(n=1 << 25) == p(ld=120) == p(ld=132) == p(x=4104) == p(v=None) == p(y=None) == p(y=4096) == bad
     assert p(xd=3) == p(gated=1, od=3) == bad                         # scales of 8-bit rows are missing
     assert p(xd=0) == p(xd=2) == p(k=100) == bad                      # the workspace is missing
+    assert p(rows=1 << 30) == no
     assert p(xd=0, ws=20480, nb=3 * 2 * 256 - 1) == bad and b'workspace' in L.vgdr_last_error()
     assert L.vgdr_mx_linear_workspace_size(0, 2, 100) == 3 * 2 * 256 and L.vgdr_mx_linear_workspace_size(2, 2, 128) == 2 * 2 * 256
     assert L.vgdr_mx_linear_workspace_size(1, 2, 128) == L.vgdr_mx_linear_workspace_size(3, 2, 100) == 0

@@ -31,6 +31,9 @@ int hip_status(hipError_t e, const char *what) {
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 constexpr int64_t MX_MOST = 1 << 24;              // rows of weights, columns
+constexpr int64_t MX_THREADS = 0xffffff00;        // of a launch, in workgroups of 256
+// threads for rows of cols columns, eight each, padded to whole 128s
+int64_t mx_threads(int64_t rows, int64_t cols) { return rows > MX_THREADS ? rows : rows * ((cols + 127) / 128 * 16); }
 
 // checks of what is rounded to block-scaled numbers
 int check_mx_source(const char *fn, int dtype, int64_t ld, int64_t rows, int64_t cols) {
@@ -1173,8 +1176,7 @@ int vgdr_mx_quantize(int dtype, const void *x, int64_t ldx, void *values, void *
     const char *fn = "vgdr_mx_quantize";
     if (int rc = check_mx_source(fn, dtype, ldx, rows, cols)) return rc;
     if (rows == 0) return VGDR_OK;
-    if (rows > (int64_t)0x7fffffff * 256 / ((cols + 127) / 128 * 16))
-        return fail(VGDR_ERR_INVALID, "%s: too many rows", fn);
+    if (mx_threads(rows, cols) > MX_THREADS) return fail(VGDR_ERR_UNSUPPORTED, "%s: more than 2^35 elements", fn);
     if (!x || !values || !scales) return fail(VGDR_ERR_INVALID, "%s: x, values and scales are required", fn);
     if (!aligned16(values) || !aligned16(scales)) return fail(VGDR_ERR_INVALID, "%s: values and scales must be 16-byte aligned", fn);
     if (x == values) return fail(VGDR_ERR_INVALID, "%s: values must not alias x", fn);
@@ -1190,7 +1192,7 @@ int vgdr_mx_weight(int dtype, const void *w, int64_t ldw, void *values, void *sc
     if (rows < 1 || rows > MX_MOST) return fail(VGDR_ERR_INVALID, "%s: rows=%lld (1 to 2^24)", fn, (long long)rows);
     if (gated != 0 && gated != 1) return fail(VGDR_ERR_INVALID, "%s: gated=%d", fn, gated);
     if (gated && rows % 2) return fail(VGDR_ERR_INVALID, "%s: a gated pair has an even number of rows, got %lld", fn, (long long)rows);
-    if ((rows + 31) / 16 * ((cols + 511) / 512) > 0x7fffffffLL) return fail(VGDR_ERR_INVALID, "%s: too many tiles", fn);
+    if ((rows + 31) / 16 * ((cols + 511) / 512) > MX_THREADS / 256) return fail(VGDR_ERR_UNSUPPORTED, "%s: too many tiles", fn);
     if (!w || !values || !scales) return fail(VGDR_ERR_INVALID, "%s: w, values and scales are required", fn);
     if (!aligned16(values) || !aligned16(scales)) return fail(VGDR_ERR_INVALID, "%s: values and scales must be 16-byte aligned", fn);
     vgdr::MxQuantize p{vgdr::MX_WEIGHT, w, ldw, rows, cols, (uint8_t *)values, (uint8_t *)scales, gated != 0};
@@ -1208,7 +1210,7 @@ int vgdr_mx_rms_norm(int dtype, const void *x, const void *residual, void *x_out
         return fail(VGDR_ERR_UNSUPPORTED, "%s: dim=%lld (supported: a multiple of 8, at most 16384)", fn, (long long)dim);
     if (!(eps >= 0.f)) return fail(VGDR_ERR_INVALID, "%s: eps must be >= 0", fn);
     if (rows == 0) return VGDR_OK;
-    if (rows > 0x7fffffffLL) return fail(VGDR_ERR_INVALID, "%s: too many rows", fn);
+    if (rows > MX_THREADS / 256) return fail(VGDR_ERR_UNSUPPORTED, "%s: %lld rows (at most 2^24 - 1)", fn, (long long)rows);
     if (!x || !gamma || !values || !scales) return fail(VGDR_ERR_INVALID, "%s: x, gamma, values and scales are required", fn);
     if (!aligned16(x) || !aligned16(gamma) || !aligned16(values) || !aligned16(scales) || !aligned16(residual) ||
         !aligned16(x_out) || !aligned16(y))
@@ -1242,7 +1244,7 @@ int vgdr_mx_linear(int x_dtype, const void *x, int64_t ldx, const void *x_scales
         return fail(VGDR_ERR_INVALID, "%s: n=%lld k=%lld (1 to 2^24)", fn, (long long)n, (long long)k);
     if (gated && n % 2) return fail(VGDR_ERR_INVALID, "%s: a gated pair has an even number of rows, got %lld", fn, (long long)n);
     if (rows == 0) return VGDR_OK;
-    if ((rows + 63) / 64 * ((n + 255) / 128) > 0x7fffffffLL) return fail(VGDR_ERR_INVALID, "%s: too many rows", fn);
+    if (!x8 && mx_threads(rows, k) > MX_THREADS) return fail(VGDR_ERR_UNSUPPORTED, "%s: more than 2^35 elements", fn);
     if (!x || !w_values || !w_scales || !y || (x8 && !x_scales) || (y8 && !y_scales))
         return fail(VGDR_ERR_INVALID, "%s: x, the weights, y and the scales of 8-bit rows are required", fn);
     if (!aligned16(x) || !aligned16(x_scales) || !aligned16(w_values) || !aligned16(w_scales) || !aligned16(y) || !aligned16(y_scales))

@@ -447,6 +447,7 @@ hipError_t few_rows_go(const MxLinear &p, int tiles, hipStream_t stream) {
 template <bool X8, bool GATED, int BM, int BN, int WM, int WN>
 hipError_t tile_go(const MxLinear &p, int tiles, hipStream_t stream) {
     const int64_t mb = (p.rows + BM - 1) / BM, nb = (tiles + BN / 16 - 1) / (BN / 16);
+    if (mb * nb > 0xfffff0) return hipErrorInvalidConfiguration;      // a launch has at most 2^32 - 1 threads
     hipLaunchKernelGGL((mx_tile_kernel<X8, GATED, BM, BN, WM, WN>), dim3((unsigned)((mb * nb + 7) / 8 * 8)), dim3(64 * WM * WN), 0,
                        stream, p, (uint32_t)mb, (uint32_t)nb);
     return hipGetLastError();
@@ -456,8 +457,10 @@ hipError_t tile_go(const MxLinear &p, int tiles, hipStream_t stream) {
 // traffic bounds them), us for bf16 / 8-bit rows:
 //   64 rows, K 5632, N 2048: 2 tiles x 16 rows (256 workgroups) 8.6 / 8.2, 1 x 16 (512) 9.6 / 8.9, 2 x 32 (128) 10.7 / 9.7
 //   32 rows, K 2048, N 8192: 2 x 32 (256) 8.0 / 7.2, 2 x 16 (512) 7.9 / 7.6, 4 x 32 (128) 9.6 / 8.3
-// The kernel for few rows up to where 4 x 32 makes one workgroup a CU: it has the whole sum in flight.  128 rows, K 5632,
-// N 2048: 11.0 / 9.9, 64 x 64 tiles 26.6 / 18.8; 128 rows, K 2048, N 8192 (512 of 4 x 32): 15.4 / 13.6, tiles 13.9 / 11.0.
+// The kernel for few rows up to where 4 x 32 makes one workgroup a CU: it has the whole sum in flight (128 rows, K 5632,
+// N 2048: 11.0 / 9.9, 64 x 64 tiles 26.6 / 18.8), and for bf16 rows, whose tiles convert the weights, up to two, with four
+// waves each so that both are on the CU: 64 rows, K 2048, gated 11264: 12.8 / 12.0 (eight waves 15.9 / 13.0), tiles 14.8 /
+// 10.8; 96 rows: 16.9 / 16.1, tiles 17.8 / 12.6.
 // Tiles: largest with 5 workgroups for 4 CUs.  512 rows, K 2048, N 8192: 64 x 128 (512) 24.1 / 15.9, 64 x 64 (1,024) 27.6 /
 // 22.9; 256 rows: 64 x 64 (512) 17.0 / 13.2, 64 x 128 (256) 18.2 / 14.6; 8-bit rows, N 32768, 512 rows: 128 x 256
 // (512) 34.3, 64 x 256 38.2, 256 rows: 64 x 256 (512) 22.2, 128 x 256 (256) 25.3.
@@ -467,8 +470,9 @@ hipError_t mx_linear_t(const MxLinear &p, hipStream_t stream) {
     const int tiles = GATED && p.out == MX8 ? (p.N + 127) / 128 * 16 : p.T;
     const int64_t cus = device_cu_count();
     auto few = [&](int mt, int nb) { return (int64_t)((tiles + mt - 1) / mt) * ((p.rows + 16 * nb - 1) / (16 * nb)); };
-    if (p.rows <= 32 || few(4, 2) <= cus) {
-        if (p.rows > 16 && few(4, 2) >= cus) return few_rows_go<X8, GATED, 4, 2, 8>(p, tiles, stream);
+    if (p.rows <= 32 || few(4, 2) <= (X8 ? 1 : 2) * cus) {
+        if (p.rows > 16 && few(4, 2) > cus) return few_rows_go<X8, GATED, 4, 2, 4>(p, tiles, stream);
+        if (p.rows > 16 && few(4, 2) == cus) return few_rows_go<X8, GATED, 4, 2, 8>(p, tiles, stream);
         if constexpr (GATED) {
             return few_rows_go<X8, GATED, 4, 1, 8>(p, tiles, stream);
         } else {
