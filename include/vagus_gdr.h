@@ -761,8 +761,8 @@ int vgdr_mx_rms_norm(int dtype, const void *x, const void *residual, void *x_out
  * x_scales) and 4-bit weights of n rows, in out_dtype (an element type).  gated: y [rows, n / 2] =
  * silu(x W1^T) (x W2^T) (the FFN's input half, infra/components/ffn.py:48-50) with sums, activation and product in fp32
  * and one rounding, in an element type or VGDR_MX8 (y_scales).  Products and sums are fp32: bf16, fp16 and fp32 rows
- * meet the weights exactly (as one, two and three bf16 numbers an element).  workspace:
- * vgdr_mx_linear_workspace_size bytes (0: none), calls that overlap have their own.  At most 2^24 rows of weights and columns.
+ * meet the weights exactly (as one, two and three bf16 numbers an element).  ldx does not matter for one row.  workspace:
+ * vgdr_mx_linear_workspace_size bytes (0: none, as for up to 32 rows), calls that overlap have their own.  At most 2^24 rows of weights and columns.
  */
 int64_t vgdr_mx_linear_workspace_size(int x_dtype, int64_t rows, int64_t k);
 int vgdr_mx_linear(int x_dtype, const void *x, int64_t ldx, const void *x_scales, const void *w_values, const void *w_scales,

@@ -153,12 +153,12 @@ def test_entry_points_check_their_arguments():
     assert p(xd=4) == p(xd=-1) == p(od=4) == p(gated=2) == p(gated=1, n=31) == p(rows=-1) == p(n=0) == p(k=0) == bad
     assert p(k=1 << 25) == p(n=1 << 25) == p(ld=120) == p(ld=132) == p(x=4104) == p(v=None) == p(y=None) == p(y=4096) == bad
     assert p(xd=3) == p(gated=1, od=3) == bad                         # scales of 8-bit rows are missing
-    assert p(xd=0) == p(xd=2) == p(k=100) == bad                      # the workspace is missing
+    assert p(xd=0, rows=33) == p(xd=2, rows=33) == p(k=100, rows=33) == bad        # the workspace is missing
     assert p(rows=1 << 30) == no
-    assert p(xd=0, ws=20480, nb=3 * 2 * 256 - 1) == bad and b'workspace' in L.vgdr_last_error()
-    assert L.vgdr_mx_linear_workspace_size(0, 2, 100) == 3 * 2 * 256 and L.vgdr_mx_linear_workspace_size(2, 2, 128) == 2 * 2 * 256
-    assert L.vgdr_mx_linear_workspace_size(1, 2, 128) == L.vgdr_mx_linear_workspace_size(3, 2, 100) == 0
-    assert L.vgdr_mx_linear_workspace_size(1, 2, 130) == 2 * 512
+    assert p(xd=0, rows=40, ws=20480, nb=3 * 40 * 256 - 1) == bad and b'workspace' in L.vgdr_last_error()
+    size = L.vgdr_mx_linear_workspace_size
+    assert size(0, 40, 100) == 3 * 40 * 256 and size(2, 40, 128) == 2 * 40 * 256 and size(1, 33, 130) == 33 * 512
+    assert size(1, 40, 128) == size(3, 40, 100) == size(0, 32, 100) == size(0, 0, 100) == 0
     assert p(rows=0, x=None) == _lib.VGDR_OK
 
 
@@ -311,7 +311,7 @@ def within(got, want, err, dt):
     return float(off.max())
 
 
-SHAPES = [(1, 128, 16), (1, 2048, 512), (2, 1, 1), (3, 40, 17), (5, 1000, 100), (15, 130, 33), (16, 512, 64), (17, 640, 48),
+SHAPES = [(1, 128, 16), (1, 2048, 512), (1, 1001, 40), (2, 1, 1), (1, 3, 4200), (20, 333, 4100), (32, 700, 8200), (3, 40, 17), (5, 1000, 100), (15, 130, 33), (16, 512, 64), (17, 640, 48),
           (33, 1024, 130), (64, 256, 100), (65, 128, 16), (130, 384, 257), (300, 1000, 70)]
 
 

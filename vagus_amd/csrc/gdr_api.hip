@@ -1223,7 +1223,7 @@ int vgdr_mx_rms_norm(int dtype, const void *x, const void *residual, void *x_out
 }
 
 int64_t vgdr_mx_linear_workspace_size(int x_dtype, int64_t rows, int64_t k) {
-    if (rows <= 0 || k <= 0 || k > MX_MOST || rows > 0x7fffffffLL) return 0;
+    if (rows <= vgdr::MX_RAW_ROWS || k <= 0 || k > MX_MOST || rows > 0x7fffffffLL) return 0;
     if (x_dtype == VGDR_F32 || x_dtype == VGDR_F16 || (x_dtype == VGDR_BF16 && k % 128))
         return (x_dtype == VGDR_F32 ? 3 : x_dtype == VGDR_F16 ? 2 : 1) * rows * ((k + 127) / 128 * 256);
     return 0;
@@ -1249,7 +1249,7 @@ int vgdr_mx_linear(int x_dtype, const void *x, int64_t ldx, const void *x_scales
         return fail(VGDR_ERR_INVALID, "%s: x, the weights, y and the scales of 8-bit rows are required", fn);
     if (!aligned16(x) || !aligned16(x_scales) || !aligned16(w_values) || !aligned16(w_scales) || !aligned16(y) || !aligned16(y_scales))
         return fail(VGDR_ERR_INVALID, "%s: every tensor must be 16-byte aligned", fn);
-    if (!x8 && (ldx % 8 || ldx < k)) return fail(VGDR_ERR_INVALID, "%s: ldx=%lld (a multiple of 8, at least k)", fn, (long long)ldx);
+    if (!x8 && rows > 1 && (ldx % 8 || ldx < k)) return fail(VGDR_ERR_INVALID, "%s: ldx=%lld (a multiple of 8, at least k)", fn, (long long)ldx);
     if (y == x || y == w_values) return fail(VGDR_ERR_INVALID, "%s: y must not alias an input", fn);
     const int64_t need = vgdr_mx_linear_workspace_size(x_dtype, rows, k);
     if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
@@ -1260,12 +1260,16 @@ int vgdr_mx_linear(int x_dtype, const void *x, int64_t ldx, const void *x_scales
     p.T = (int)(gated ? 2 * ((n / 2 + 15) / 16) : (n + 15) / 16);
     p.N = (int)(gated ? n / 2 : n);
     p.x = x;
+    p.x_type = x_dtype;
     p.ldx = x8 ? 128 * (int64_t)p.C : ldx;
     p.planes = 1;
+    p.K = (int)k;
     if (need) {
         vgdr::MxQuantize q{vgdr::MX_PLANES, x, ldx, rows, k, (uint8_t *)workspace, nullptr, false};
         if (int rc = hip_status(vgdr::mx_quantize(x_dtype, q, stream), "vgdr_mx_linear launch")) return rc;
         p.x = workspace;
+        p.x_type = VGDR_BF16;
+        p.K = 128 * p.C;
         p.ldx = 128 * (int64_t)p.C;
         p.planes = x_dtype == VGDR_F32 ? 3 : x_dtype == VGDR_F16 ? 2 : 1;
     }
@@ -1276,7 +1280,6 @@ int vgdr_mx_linear(int x_dtype, const void *x, int64_t ldx, const void *x_scales
     p.y_scales = (uint8_t *)y_scales;
     p.rows = rows;
     p.out = out_dtype;
-    p.x8 = x8;
     p.gated = gated != 0;
     return hip_status(vgdr::mx_linear(p, stream), "vgdr_mx_linear launch");
 }

@@ -446,15 +446,16 @@ hipError_t mx_rms_norm(int dtype, const MxNorm &p, hipStream_t stream);
 
 // Products with 4-bit weights (gdr_mx_linear.hip).
 constexpr int MX8 = 3;            // beside the element types: rows in 8 bits with scales
+constexpr int MX_RAW_ROWS = 32;   // up to which rows of any type and width are taken as they are
 struct MxLinear {
-    const void *x;                // bf16 [planes][rows][ldx], or 8-bit [rows][128 C]
+    const void *x;                // [rows][ldx] in x_type, or bf16 [planes][rows][ldx]
     const uint8_t *x_scales;      // [rows][4 C]
     const uint8_t *w, *w_scales;  // T tiles of 16 rows, C tiles of 128 columns
     void *y;                      // [rows, N] in `out`; MX8: [rows, 128 ceil(N / 128)]
     uint8_t *y_scales;
     int64_t rows, ldx;
-    int planes, T, C, N, out;     // N: the output's columns
-    bool x8, gated;
+    int x_type, planes, T, C, K, N, out;              // N: the output's columns; K: x's (planes: 128 C)
+    bool gated;
 };
 hipError_t mx_linear(const MxLinear &p, hipStream_t stream);
 

@@ -156,9 +156,8 @@ __global__ void __launch_bounds__(256) mx_rms_norm_kernel(const E *x, const E *r
     }
 }
 
-// Rows of fp16 or fp32 (or of bf16 of a width that is no multiple of 128) as bf16 planes [P][R][Kp] whose sum they are: bf16 has
-// 8 bits, so fp16's 11 take two planes and fp32's 24 three.  A product of a plane's element with a 4-bit weight
-// is exact in fp32, so the product kernels need one form of 16-bit rows.
+// Many rows of fp16 or fp32 (or of bf16 of a width that is no multiple of 128) as bf16 planes [P][R][Kp] whose sum they are.  A
+// product of a plane's element with a 4-bit weight is exact in fp32, so the tiles need one form of 16-bit rows.
 template <typename E, int P>
 __global__ void __launch_bounds__(256) mx_planes_kernel(const E *__restrict__ x, int64_t ldx, __bf16 *out, int64_t rows,
                                                         int64_t K, int64_t Kp, bool vec) {
@@ -167,19 +166,16 @@ __global__ void __launch_bounds__(256) mx_planes_kernel(const E *__restrict__ x,
     const int64_t c = (i - row * per) * 8;
     float v[8];
     load8(v, x + row * ldx, c, K, vec);
+    bf16x8 o[P];
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-        bf16x8 o;
+    for (int e = 0; e < 8; ++e) {
+        __bf16 part[P];
+        split(part, v[e]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            // cut off, not rounded: the largest fp32 numbers stay finite; an infinity or a NaN is the first plane's
-            const uint32_t u = __builtin_bit_cast(uint32_t, v[e]);
-            const bool finite = (u & 0x7f800000u) != 0x7f800000u;
-            o[e] = finite ? __builtin_bit_cast(__bf16, (uint16_t)(u >> 16)) : (__bf16)v[e];
-            v[e] = finite ? v[e] - (float)o[e] : 0.f;
-        }
-        *reinterpret_cast<bf16x8 *>(out + (p * rows + row) * Kp + c) = o;
+        for (int p = 0; p < P; ++p) o[p][e] = part[p];
     }
+#pragma unroll
+    for (int p = 0; p < P; ++p) *reinterpret_cast<bf16x8 *>(out + (p * rows + row) * Kp + c) = o[p];
 }
 
 namespace {

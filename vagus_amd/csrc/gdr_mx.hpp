@@ -66,4 +66,17 @@ __device__ __forceinline__ float round_to_odd(double x) {
     return __builtin_bit_cast(float, u);
 }
 
+// v as the sum of P bf16 numbers: cut off, not rounded, so that the largest fp32 numbers stay finite; an infinity or a
+// NaN is the first part's.  bf16 has 8 bits: fp16's 11 take two parts, fp32's 24 three.
+template <int P>
+__device__ __forceinline__ void split(__bf16 (&out)[P], float v) {
+#pragma unroll
+    for (int q = 0; q < P; ++q) {
+        const uint32_t u = __builtin_bit_cast(uint32_t, v);
+        const bool finite = (u & 0x7f800000u) != 0x7f800000u;
+        out[q] = finite ? __builtin_bit_cast(__bf16, (uint16_t)(u >> 16)) : (__bf16)v;
+        v = finite ? v - (float)out[q] : 0.f;
+    }
+}
+
 }  // namespace vgdr

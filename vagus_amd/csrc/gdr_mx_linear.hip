@@ -138,10 +138,16 @@ __device__ __forceinline__ void epilogue(const MxLinear &p, int64_t row, int t0,
 // region of its own, which needs no barrier: a load covers whole rows of a tile there, where fragments
 // straight from global memory would have every lane in a line of its own, and the address unit bounds those
 // (64 rows, K 5632, N 2048: 9.6 us; 64 rows, K and N 8192: 25).
-template <bool X8, bool GATED, int MT, int NB, int NWV>
+// X: the rows' type (0 fp32, 1 bf16, 2 fp16, MX8).  fp32 and fp16 rows become three and two bf16 planes on their way
+// into LDS; their K, and bf16's, may end inside a tile.
+template <int X, bool GATED, int MT, int NB, int NWV>
 __global__ void __launch_bounds__(64 * NWV) mx_few_rows_kernel(const MxLinear p) {
-    constexpr int ROW = X8 ? 128 : 256, PITCH = ROW + 16, LR = 1024 / ROW, NX = 16 * NB / LR;
-    constexpr int STAGE = 16 * NB * PITCH, RED = NWV / 2 * MT * NB * 64 * 16;
+    typedef std::conditional_t<X == 0, float, std::conditional_t<X == 1, __bf16, std::conditional_t<X == 2, _Float16, uint8_t>>> E;
+    constexpr bool X8 = X == MX8;
+    constexpr int ES = (int)sizeof(E), VE = 16 / ES, P = X == 0 ? 3 : X == 2 ? 2 : 1;
+    constexpr int ROW = 128 * ES, LR = 1024 / ROW, NX = 16 * NB / LR;
+    constexpr int PITCH = (X8 ? 128 : 256) + 16, PLANE = 16 * NB * PITCH;
+    constexpr int STAGE = P * PLANE, RED = NWV / 2 * MT * NB * 64 * 16;
     constexpr int LDS = STAGE * NWV > RED ? STAGE * NWV : RED;
     __shared__ __attribute__((aligned(16))) char lds[LDS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -159,12 +165,12 @@ __global__ void __launch_bounds__(64 * NWV) mx_few_rows_kernel(const MxLinear p)
         ws[a] = p.w_scales + t * C4 * 256 + (16 * g + at.row) * 4;
     }
     // a lane loads 16 bytes of row lane / (64 / LR) + LR i; rows past the end are the last one again
-    const int lr = lane / (64 / LR), lk = lane % (64 / LR) * 16;
-    const char *x[NX];
+    const int lr = lane / (64 / LR), lk = lane % (64 / LR) * VE;
+    const E *x[NX];
 #pragma unroll
     for (int i = 0; i < NX; ++i) {
         const int64_t row = b0 + LR * i + lr < p.rows ? b0 + LR * i + lr : p.rows - 1;
-        x[i] = reinterpret_cast<const char *>(p.x) + row * p.ldx * (X8 ? 1 : 2) + lk;
+        x[i] = reinterpret_cast<const E *>(p.x) + row * p.ldx + lk;
     }
     const uint8_t *xs[NB];
 #pragma unroll
@@ -172,7 +178,7 @@ __global__ void __launch_bounds__(64 * NWV) mx_few_rows_kernel(const MxLinear p)
         const int64_t row = b0 + 16 * b + r < p.rows ? b0 + 16 * b + r : p.rows - 1;
         xs[b] = X8 ? p.x_scales + row * 4 * p.C + g : nullptr;
     }
-    const int64_t plane = X8 ? 0 : p.rows * p.ldx * 2;
+    const int64_t plane = p.rows * p.ldx;                             // of bf16 rows that are planes already
 
     f32x4 acc[MT][NB];
 #pragma unroll
@@ -193,8 +199,19 @@ __global__ void __launch_bounds__(64 * NWV) mx_few_rows_kernel(const MxLinear p)
             to.w[a] = *reinterpret_cast<const u32x4 *>(w[a] + (int64_t)c * 1024);
             to.ws[a] = ws[a][(c >> 2) * 256 + (c & 3)];
         }
+        if (X8 || 128 * (c + 1) <= p.K) {
 #pragma unroll
-        for (int i = 0; i < NX; ++i) to.x[i] = *reinterpret_cast<const u32x4 *>(x[i] + pl * plane + (int64_t)c * ROW);
+            for (int i = 0; i < NX; ++i) to.x[i] = *reinterpret_cast<const u32x4 *>(x[i] + pl * plane + 128 * (int64_t)c);
+        } else {
+            typedef E V __attribute__((ext_vector_type(VE)));
+#pragma unroll
+            for (int i = 0; i < NX; ++i) {
+                V v;
+#pragma unroll
+                for (int e = 0; e < VE; ++e) v[e] = 128 * c + lk + e < p.K ? x[i][pl * plane + 128 * (int64_t)c + e] : (E)0;
+                to.x[i] = __builtin_bit_cast(u32x4, v);
+            }
+        }
         if constexpr (X8) {
 #pragma unroll
             for (int b = 0; b < NB; ++b) to.xs[b] = xs[b][4 * (int64_t)c];
@@ -209,7 +226,26 @@ __global__ void __launch_bounds__(64 * NWV) mx_few_rows_kernel(const MxLinear p)
         // LDS operations of one wave are in order: only the compiler has to keep it
         asm volatile("" ::: "memory");
 #pragma unroll
-        for (int i = 0; i < NX; ++i) *reinterpret_cast<u32x4 *>(stage + (LR * i + lr) * PITCH + lk) = of.x[i];
+        for (int i = 0; i < NX; ++i) {
+            char *to = stage + (LR * i + lr) * PITCH + lk * (X8 ? 1 : 2);
+            if constexpr (P == 1) {
+                *reinterpret_cast<u32x4 *>(to) = of.x[i];
+            } else {
+                typedef E V __attribute__((ext_vector_type(VE)));
+                typedef __bf16 O __attribute__((ext_vector_type(VE)));
+                const V v = __builtin_bit_cast(V, of.x[i]);
+                O o[P];
+#pragma unroll
+                for (int e = 0; e < VE; ++e) {
+                    __bf16 part[P];
+                    split(part, (float)v[e]);
+#pragma unroll
+                    for (int q = 0; q < P; ++q) o[q][e] = part[q];
+                }
+#pragma unroll
+                for (int q = 0; q < P; ++q) *reinterpret_cast<O *>(to + q * PLANE) = o[q];
+            }
+        }
         asm volatile("" ::: "memory");
     };
     auto products = [&](const Step &of) __attribute__((always_inline)) {
@@ -224,15 +260,19 @@ __global__ void __launch_bounds__(64 * NWV) mx_few_rows_kernel(const MxLinear p)
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                bf16x8 f[NB];
+                bf16x8 f[P][NB];
 #pragma unroll
-                for (int b = 0; b < NB; ++b)
-                    f[b] = *reinterpret_cast<const bf16x8 *>(stage + (16 * b + r) * PITCH + 64 * g + 16 * i);
+                for (int q = 0; q < P; ++q)
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+                        f[q][b] = *reinterpret_cast<const bf16x8 *>(stage + q * PLANE + (16 * b + r) * PITCH + 64 * g + 16 * i);
 #pragma unroll
                 for (int a = 0; a < MT; ++a) {
                     const bf16x8 v = to_bf16(of.w[a][i], mx_value(of.ws[a]));
 #pragma unroll
-                    for (int b = 0; b < NB; ++b) acc[a][b] = mfma_pair(v, f[b], acc[a][b]);
+                    for (int q = 0; q < P; ++q)
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) acc[a][b] = mfma_pair(v, f[q][b], acc[a][b]);
                 }
             }
         }
@@ -437,10 +477,10 @@ __global__ void __launch_bounds__(64 * WM * WN, 2 * WM * WN / 4) mx_tile_kernel(
 
 namespace {
 
-template <bool X8, bool GATED, int MT, int NB, int NWV>
+template <int X, bool GATED, int MT, int NB, int NWV>
 hipError_t few_rows_go(const MxLinear &p, int tiles, hipStream_t stream) {
     const dim3 grid((unsigned)((tiles + MT - 1) / MT), (unsigned)((p.rows + 16 * NB - 1) / (16 * NB)));
-    hipLaunchKernelGGL((mx_few_rows_kernel<X8, GATED, MT, NB, NWV>), grid, dim3(64 * NWV), 0, stream, p);
+    hipLaunchKernelGGL((mx_few_rows_kernel<X, GATED, MT, NB, NWV>), grid, dim3(64 * NWV), 0, stream, p);
     return hipGetLastError();
 }
 
@@ -464,39 +504,52 @@ hipError_t tile_go(const MxLinear &p, int tiles, hipStream_t stream) {
 // Tiles: largest with 5 workgroups for 4 CUs.  512 rows, K 2048, N 8192: 64 x 128 (512) 24.1 / 15.9, 64 x 64 (1,024) 27.6 /
 // 22.9; 256 rows: 64 x 64 (512) 17.0 / 13.2, 64 x 128 (256) 18.2 / 14.6; 8-bit rows, N 32768, 512 rows: 128 x 256
 // (512) 34.3, 64 x 256 38.2, 256 rows: 64 x 256 (512) 22.2, 128 x 256 (256) 25.3.
-template <bool X8, bool GATED>
+// Rows that the kernel for few rows converts itself (MX_RAW_ROWS at most) stay as they are: fp32 or fp16, or of a width that
+// ends inside a tile.  7 rows of fp32, K 1000, N 1337: one launch instead of two.
+template <int X, bool GATED>
 hipError_t mx_linear_t(const MxLinear &p, hipStream_t stream) {
+    constexpr bool X8 = X == MX8;
     // the output's padding to whole 128s of columns counts as tiles (8-bit outputs: 8 pairs a 128)
     const int tiles = GATED && p.out == MX8 ? (p.N + 127) / 128 * 16 : p.T;
     const int64_t cus = device_cu_count();
     auto few = [&](int mt, int nb) { return (int64_t)((tiles + mt - 1) / mt) * ((p.rows + 16 * nb - 1) / (16 * nb)); };
-    if (p.rows <= 32 || few(4, 2) <= (X8 ? 1 : 2) * cus) {
-        if (p.rows > 16 && few(4, 2) > cus) return few_rows_go<X8, GATED, 4, 2, 4>(p, tiles, stream);
-        if (p.rows > 16 && few(4, 2) == cus) return few_rows_go<X8, GATED, 4, 2, 8>(p, tiles, stream);
-        if constexpr (GATED) {
-            return few_rows_go<X8, GATED, 4, 1, 8>(p, tiles, stream);
-        } else {
-            if (p.rows > 16 && few(2, 2) >= cus) return few_rows_go<X8, GATED, 2, 2, 8>(p, tiles, stream);
-            if (few(4, 1) >= cus) return few_rows_go<X8, GATED, 4, 1, 8>(p, tiles, stream);
-            if (few(2, 1) >= cus) return few_rows_go<X8, GATED, 2, 1, 8>(p, tiles, stream);
-            return few_rows_go<X8, GATED, 1, 1, 8>(p, tiles, stream);
+    if constexpr (X == 0 || X == 2) {
+        if (GATED || few(4, 1) >= cus) return few_rows_go<X, GATED, 4, 1, 8>(p, tiles, stream);
+        if constexpr (!GATED) {
+            if (few(2, 1) >= cus) return few_rows_go<X, GATED, 2, 1, 8>(p, tiles, stream);
+            return few_rows_go<X, GATED, 1, 1, 8>(p, tiles, stream);
         }
+    } else {
+        if (p.rows <= MX_RAW_ROWS || few(4, 2) <= (X8 ? 1 : 2) * cus) {
+            if (p.rows > 16 && few(4, 2) > cus) return few_rows_go<X, GATED, 4, 2, 4>(p, tiles, stream);
+            if (p.rows > 16 && few(4, 2) == cus) return few_rows_go<X, GATED, 4, 2, 8>(p, tiles, stream);
+            if constexpr (GATED) {
+                return few_rows_go<X, GATED, 4, 1, 8>(p, tiles, stream);
+            } else {
+                if (p.rows > 16 && few(2, 2) >= cus) return few_rows_go<X, GATED, 2, 2, 8>(p, tiles, stream);
+                if (few(4, 1) >= cus) return few_rows_go<X, GATED, 4, 1, 8>(p, tiles, stream);
+                if (few(2, 1) >= cus) return few_rows_go<X, GATED, 2, 1, 8>(p, tiles, stream);
+                return few_rows_go<X, GATED, 1, 1, 8>(p, tiles, stream);
+            }
+        }
+        auto fills = [&](int bm, int bn) { return 4 * ((p.rows + bm - 1) / bm) * ((tiles + bn / 16 - 1) / (bn / 16)) >= 5 * cus; };
+        if constexpr (X8)
+            if (fills(128, 256)) return tile_go<X8, GATED, 128, 256, 2, 2>(p, tiles, stream);
+        if (fills(64, 256)) return tile_go<X8, GATED, 64, 256, 1, 4>(p, tiles, stream);
+        if (fills(64, 128)) return tile_go<X8, GATED, 64, 128, 2, 2>(p, tiles, stream);
+        // a gated block of 32 columns takes four tiles of a wave
+        if constexpr (GATED) return tile_go<X8, GATED, 64, 64, 4, 1>(p, tiles, stream);
+        else return tile_go<X8, GATED, 64, 64, 2, 2>(p, tiles, stream);
     }
-    auto fills = [&](int bm, int bn) { return 4 * ((p.rows + bm - 1) / bm) * ((tiles + bn / 16 - 1) / (bn / 16)) >= 5 * cus; };
-    if constexpr (X8)
-        if (fills(128, 256)) return tile_go<X8, GATED, 128, 256, 2, 2>(p, tiles, stream);
-    if (fills(64, 256)) return tile_go<X8, GATED, 64, 256, 1, 4>(p, tiles, stream);
-    if (fills(64, 128)) return tile_go<X8, GATED, 64, 128, 2, 2>(p, tiles, stream);
-    // a gated block of 32 columns takes four tiles of a wave
-    if constexpr (GATED) return tile_go<X8, GATED, 64, 64, 4, 1>(p, tiles, stream);
-    else return tile_go<X8, GATED, 64, 64, 2, 2>(p, tiles, stream);
 }
 
 }  // namespace
 
 hipError_t mx_linear(const MxLinear &p, hipStream_t stream) {
-    if (p.x8) return p.gated ? mx_linear_t<true, true>(p, stream) : mx_linear_t<true, false>(p, stream);
-    return p.gated ? mx_linear_t<false, true>(p, stream) : mx_linear_t<false, false>(p, stream);
+    if (p.x_type == MX8) return p.gated ? mx_linear_t<MX8, true>(p, stream) : mx_linear_t<MX8, false>(p, stream);
+    if (p.x_type == 0) return p.gated ? mx_linear_t<0, true>(p, stream) : mx_linear_t<0, false>(p, stream);
+    if (p.x_type == 2) return p.gated ? mx_linear_t<2, true>(p, stream) : mx_linear_t<2, false>(p, stream);
+    return p.gated ? mx_linear_t<1, true>(p, stream) : mx_linear_t<1, false>(p, stream);
 }
 
 }  // namespace vgdr

@@ -1732,7 +1732,7 @@ def _stream_counts(name, t, N, index):
 
 def _launch(index, fn, *args):
     """fn(*args, stream) on GPU `index`'s current stream, with that GPU current."""
-    if index == torch.cuda.current_device():
+    if index == torch._C._cuda_getDevice():               # a tensor is on it: the GPU is initialised
         _lib.check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
     else:
         with torch.cuda.device(index):
@@ -2191,7 +2191,7 @@ def _mx_product(x, w: MXWeight, gated: bool, quantize: bool, out_dtype):
     else:
         dt = x.dtype if out_dtype is None else out_dtype
         v, ld = _mx_source('x', x)
-        if v.data_ptr() % 16 or ld % 8:
+        if v.data_ptr() % 16 or (ld % 8 and v.shape[0] > 1):
             pad = -k % 8                                              # rows of whole 16-byte units
             v = F.pad(v, (0, pad)) if pad else v.clone(memory_format=torch.contiguous_format)
             ld = k + pad
@@ -2201,8 +2201,8 @@ def _mx_product(x, w: MXWeight, gated: bool, quantize: bool, out_dtype):
     lead, cols = x.shape[:-1], n // 2 if gated else n
     R = v.numel() // v.shape[-1]
     lib = _lib.load()
-    # bf16 and 8-bit rows of whole 128s of columns are read where they lie
-    nbytes = 0 if rows8 or (code == _lib.VGDR_BF16 and k % 128 == 0) else lib.vgdr_mx_linear_workspace_size(code, R, k)
+    # few rows, and bf16 and 8-bit ones of whole 128s of columns, are read where they lie
+    nbytes = 0 if rows8 or R <= 32 or (code == _lib.VGDR_BF16 and k % 128 == 0) else lib.vgdr_mx_linear_workspace_size(code, R, k)
     if nbytes:
         ws = torch.empty((nbytes,), dtype=torch.uint8, device=v.device)
     if quantize:
