@@ -70,12 +70,15 @@ __device__ __forceinline__ float round_to_odd(double x) {
 // NaN is the first part's.  bf16 has 8 bits: fp16's 11 take two parts, fp32's 24 three.
 template <int P>
 __device__ __forceinline__ void split(__bf16 (&out)[P], float v) {
+    uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const bool finite = (u & 0x7f800000u) != 0x7f800000u;
+    out[0] = finite ? __builtin_bit_cast(__bf16, (uint16_t)(u >> 16)) : (__bf16)v;
+    float left = finite ? v - __builtin_bit_cast(float, u & 0xffff0000u) : 0.f;
 #pragma unroll
-    for (int q = 0; q < P; ++q) {
-        const uint32_t u = __builtin_bit_cast(uint32_t, v);
-        const bool finite = (u & 0x7f800000u) != 0x7f800000u;
-        out[q] = finite ? __builtin_bit_cast(__bf16, (uint16_t)(u >> 16)) : (__bf16)v;
-        v = finite ? v - (float)out[q] : 0.f;
+    for (int q = 1; q < P; ++q) {
+        u = __builtin_bit_cast(uint32_t, left);
+        out[q] = __builtin_bit_cast(__bf16, (uint16_t)(u >> 16));
+        left -= __builtin_bit_cast(float, u & 0xffff0000u);
     }
 }
 

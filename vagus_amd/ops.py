@@ -2087,7 +2087,8 @@ def _mx_source(name, t, dims=None):
     """(t as rows (R, K), their distance in elements) for a kernel that rounds them."""
     if t.get_device() < 0:
         _check_device(t)
-    _check_grad(t)
+    if t.requires_grad:
+        _check_grad(t)
     if t.dtype not in _DTYPES:
         raise NotImplementedError(f'{name} must be one of {list(_DTYPES)}; got {t.dtype}')
     assert t.dim() >= 1 and t.shape[-1] >= 1 and (dims is None or t.dim() == dims), f'{name}: shape {tuple(t.shape)}'
@@ -2174,45 +2175,53 @@ def mx_rms_norm(x, weight, eps: float = 1e-6, residual=None, out_residual=None, 
 
 
 def _mx_product(x, w: MXWeight, gated: bool, quantize: bool, out_dtype):
-    assert isinstance(w, MXWeight) and w.gated == gated, \
-        f'{"mx_swiglu takes a gated" if gated else "mx_linear takes an ungated"} MXWeight (mx_weight); got {type(w).__name__}'
+    # a decode step calls this four times a layer: few Python calls on the usual way through
+    if type(w) is not MXWeight or w.gated != gated:
+        raise AssertionError(f'{"mx_swiglu takes a gated" if gated else "mx_linear takes an ungated"} MXWeight (mx_weight); '
+                             f'got {type(w).__name__}')
     n, k = w.shape
-    rows8 = isinstance(x, MXRows)
-    assert (x.size if rows8 else x.shape[-1] if x.dim() else 0) == k, f'x must be (..., {k}); got {tuple(x.shape)}'
-    index = x.values.get_device() if rows8 else x.get_device()
-    if index < 0:
-        _check_device(x.values if rows8 else x)
-    _all_on(index, w.values, w.scales, x.scales if rows8 else None)
-    xs = ws = None
+    wv, ws = w.values, w.scales
+    index = wv.get_device()
+    rows8 = type(x) is MXRows
+    work = scales = None
+    nbytes = 0
     if rows8:
+        v, scales, code, ld = x.values, x.scales, _lib.VGDR_MX8, 0
+        if x.size != k:
+            raise AssertionError(f'x must be (..., {k}); got {tuple(x.shape)}')
+        if v.get_device() != index or scales.get_device() != index or ws.get_device() != index:
+            _all_on(index, v, scales, ws)
+        v, scales = _aligned(v), _aligned(scales)
+        lead, R = v.shape[:-1], v.numel() // v.shape[-1]
         dt = torch.bfloat16 if out_dtype is None else out_dtype
-        v, xs = _aligned(x.values), _aligned(x.scales)
-        code, ld = _lib.VGDR_MX8, 0
     else:
-        dt = x.dtype if out_dtype is None else out_dtype
+        if x.get_device() != index or ws.get_device() != index:
+            _all_on(index, x, ws)
+        assert x.dim() and x.shape[-1] == k, f'x must be (..., {k}); got {tuple(x.shape)}'
         v, ld = _mx_source('x', x)
-        if v.data_ptr() % 16 or (ld % 8 and v.shape[0] > 1):
+        R, lead = v.shape[0], x.shape[:-1]
+        if v.data_ptr() % 16 or (ld % 8 and R > 1):
             pad = -k % 8                                              # rows of whole 16-byte units
             v = F.pad(v, (0, pad)) if pad else v.clone(memory_format=torch.contiguous_format)
             ld = k + pad
         code = _DTYPES[x.dtype]
-    if dt not in _DTYPES:
+        dt = x.dtype if out_dtype is None else out_dtype
+        # few rows, and bf16 ones of whole 128s of columns, are read where they lie
+        if R > 32 and (code != _lib.VGDR_BF16 or k % 128):
+            nbytes = _lib.load().vgdr_mx_linear_workspace_size(code, R, k)
+            work = torch.empty((nbytes,), dtype=torch.uint8, device=v.device)
+    out = _DTYPES.get(dt)
+    if out is None:
         raise NotImplementedError(f'out_dtype must be one of {list(_DTYPES)}; got {dt}')
-    lead, cols = x.shape[:-1], n // 2 if gated else n
-    R = v.numel() // v.shape[-1]
-    lib = _lib.load()
-    # few rows, and bf16 and 8-bit ones of whole 128s of columns, are read where they lie
-    nbytes = 0 if rows8 or R <= 32 or (code == _lib.VGDR_BF16 and k % 128 == 0) else lib.vgdr_mx_linear_workspace_size(code, R, k)
-    if nbytes:
-        ws = torch.empty((nbytes,), dtype=torch.uint8, device=v.device)
+    cols = n // 2 if gated else n
     if quantize:
         y = _mx_rows(lead, cols, v)
         yp, ys, out = y.values.data_ptr(), y.scales.data_ptr(), _lib.VGDR_MX8
     else:
-        y = v.new_empty((*lead, cols), dtype=dt)
-        yp, ys, out = y.data_ptr(), None, _DTYPES[dt]
-    _launch(index, lib.vgdr_mx_linear, code, v.data_ptr(), ld, _ptr(xs), w.values.data_ptr(), w.scales.data_ptr(), int(gated),
-            out, yp, ys, _ptr(ws), nbytes, R, n, k)
+        y = v.new_empty((*lead, cols)) if dt is v.dtype else v.new_empty((*lead, cols), dtype=dt)
+        yp, ys = y.data_ptr(), None
+    _launch(index, _lib.load().vgdr_mx_linear, code, v.data_ptr(), ld, _ptr(scales), wv.data_ptr(), ws.data_ptr(), gated,
+            out, yp, ys, _ptr(work), nbytes, R, n, k)
     return y
 
 
