@@ -35,6 +35,13 @@ __device__ __forceinline__ f32x4 mfma_mx(u32x4 w, int ws, u32x4 lo, u32x4 hi, in
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 0, 0, ws, 0, xs);
 }
 
+// Behind the loop of matrix instructions: whichever way the loop was left, their results pass their wait states here
+// before anything reads them.  Tied to the accumulators instead, it cost the largest products 4 %.
+__device__ __forceinline__ void settle() {
+    asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 // silu(a) b.  Where the result is rounded to 16 or 8 bits, by the hardware's exponential and
 // reciprocal (a few 2^-23); fp32 results take the accurate ones, which cost an epilogue three times as much.
 __device__ __forceinline__ float gated_product(float a, float b, bool accurate) {
@@ -127,16 +134,18 @@ __device__ __forceinline__ void epilogue(const MxLinear &p, int64_t row, int t0,
 
 }  // namespace
 
+constexpr int BF16_TAIL = 4;
+
 // Few rows: a workgroup owns MT weight tiles and 16 NB rows; its NWV waves take every NWV-th K tile, the next one's loads
 // ahead of this one's products, and meet in LDS, in a fixed order.  A wave passes its rows' tiles through an LDS
 // region of its own, which needs no barrier: a load covers whole rows of a tile there, where fragments
 // straight from global memory would have every lane in a line of its own, and the address unit bounds those
 // (64 rows, K 5632, N 2048: 9.6 us; 64 rows, K and N 8192: 25).
-// X: the rows' type (0 fp32, 1 bf16, 2 fp16, MX8).  fp32 and fp16 rows become three and two bf16 planes on their way
-// into LDS; their K, and bf16's, may end inside a tile.
+// X: the rows' type (0 fp32, 1 bf16, 2 fp16, MX8, BF16_TAIL).  fp32 and fp16 rows become three and two bf16 planes on their way
+// into LDS; their K, and BF16_TAIL's, may end inside a tile (a check that costs the others half a microsecond).
 template <int X, bool GATED, int MT, int NB, int NWV>
-__global__ void __launch_bounds__(64 * NWV) mx_few_rows_kernel(const MxLinear p) {
-    typedef std::conditional_t<X == 0, float, std::conditional_t<X == 1, __bf16, std::conditional_t<X == 2, _Float16, uint8_t>>> E;
+__global__ void __launch_bounds__(64 * NWV, 2) mx_few_rows_kernel(const MxLinear p) {
+    typedef std::conditional_t<X == 0, float, std::conditional_t<X == 1 || X == BF16_TAIL, __bf16, std::conditional_t<X == 2, _Float16, uint8_t>>> E;
     constexpr bool X8 = X == MX8;
     constexpr int ES = (int)sizeof(E), VE = 16 / ES, P = X == 0 ? 3 : X == 2 ? 2 : 1;
     constexpr int ROW = 128 * ES, LR = 1024 / ROW, NX = 16 * NB / LR;
@@ -197,7 +206,7 @@ __global__ void __launch_bounds__(64 * NWV) mx_few_rows_kernel(const MxLinear p)
             to.w[a] = *reinterpret_cast<const u32x4 *>(w[a] + (int64_t)c * 1024);
             to.ws[a] = ws[a][(c >> 2) * 256 + (c & 3)];
         }
-        if (X8 || 128 * (c + 1) <= p.K) {
+        if (X8 || X == 1 || 128 * (c + 1) <= p.K) {
 #pragma unroll
             for (int i = 0; i < NX; ++i)
                 if (P == 1 || LR * i < live) to.x[i] = *reinterpret_cast<const u32x4 *>(x[i] + pl * plane + 128 * (int64_t)c);
@@ -289,6 +298,7 @@ __global__ void __launch_bounds__(64 * NWV) mx_few_rows_kernel(const MxLinear p)
         if (s + 2 < steps) load(even);
         products(odd);
     }
+    settle();
     // the waves' sums, halves onto halves
     f32x4 *red = reinterpret_cast<f32x4 *>(lds);
 #pragma unroll
@@ -471,6 +481,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2 * WM * WN / 4) mx_tile_kernel(
             ++c;
         }
     }
+    settle();
 #pragma unroll
     for (int i = 0; i < FM; ++i) epilogue<GATED, FN>(p, m0 + (wm * FM + i) * 16 + r, t0 + wn * FN, g, acc[i]);
 }
@@ -499,8 +510,8 @@ hipError_t tile_go(const MxLinear &p, int tiles, hipStream_t stream) {
 //   32 rows, K 2048, N 8192: 2 x 32 (256) 8.0 / 7.2, 2 x 16 (512) 7.9 / 7.6, 4 x 32 (128) 9.6 / 8.3
 // The kernel for few rows up to where 4 x 32 makes one workgroup a CU: it has the whole sum in flight (128 rows, K 5632,
 // N 2048: 11.0 / 9.9, 64 x 64 tiles 26.6 / 18.8), and for bf16 rows, whose tiles convert the weights, up to two, with four
-// waves each so that both are on the CU: 64 rows, K 2048, gated 11264: 12.8 / 12.0 (eight waves 15.9 / 13.0), tiles 14.8 /
-// 10.8; 96 rows: 16.9 / 16.1, tiles 17.8 / 12.6.
+// waves each so that both are on the CU: 64 rows, K 2048, gated 11264: 13.2 / 11.1 (eight waves 16.2 / 14.3), tiles 14.8 /
+// 10.8; 96 rows: 16.8 / 15.0, tiles 17.8 / 12.6.
 // Tiles: largest with 5 workgroups for 4 CUs.  512 rows, K 2048, N 8192: 64 x 128 (512) 24.1 / 15.9, 64 x 64 (1,024) 27.6 /
 // 22.9; 256 rows: 64 x 64 (512) 17.0 / 13.2, 64 x 128 (256) 18.2 / 14.6; 8-bit rows, N 32768, 512 rows: 128 x 256
 // (512) 34.3, 64 x 256 38.2, 256 rows: 64 x 256 (512) 22.2, 128 x 256 (256) 25.3.
@@ -513,7 +524,7 @@ hipError_t mx_linear_t(const MxLinear &p, hipStream_t stream) {
     const int tiles = GATED && p.out == MX8 ? (p.N + 127) / 128 * 16 : p.T;
     const int64_t cus = device_cu_count();
     auto few = [&](int mt, int nb) { return (int64_t)((tiles + mt - 1) / mt) * ((p.rows + 16 * nb - 1) / (16 * nb)); };
-    if constexpr (X == 0 || X == 2) {
+    if constexpr (X == 0 || X == 2 || X == BF16_TAIL) {
         if (GATED || few(4, 1) >= cus) return few_rows_go<X, GATED, 4, 1, 8>(p, tiles, stream);
         if constexpr (!GATED) {
             if (few(2, 1) >= cus) return few_rows_go<X, GATED, 2, 1, 8>(p, tiles, stream);
@@ -549,6 +560,7 @@ hipError_t mx_linear(const MxLinear &p, hipStream_t stream) {
     if (p.x_type == MX8) return p.gated ? mx_linear_t<MX8, true>(p, stream) : mx_linear_t<MX8, false>(p, stream);
     if (p.x_type == 0) return p.gated ? mx_linear_t<0, true>(p, stream) : mx_linear_t<0, false>(p, stream);
     if (p.x_type == 2) return p.gated ? mx_linear_t<2, true>(p, stream) : mx_linear_t<2, false>(p, stream);
+    if (p.K % 128) return p.gated ? mx_linear_t<BF16_TAIL, true>(p, stream) : mx_linear_t<BF16_TAIL, false>(p, stream);
     return p.gated ? mx_linear_t<1, true>(p, stream) : mx_linear_t<1, false>(p, stream);
 }
 
