@@ -115,7 +115,9 @@ def test_containers_refuse_what_they_cannot_be():
 def test_cpu_tensors_are_refused():
     x = torch.zeros(2, 128)
     w = ops.MXWeight(torch.zeros(2, 1, 4, 16, 16, dtype=torch.uint8), torch.ones(2, 1, 4, 16, 4, dtype=torch.uint8), (32, 128))
-    for f in (lambda: ops.mx_quantize(x), lambda: ops.mx_weight(x), lambda: ops.mx_rms_norm(x, x[0]), lambda: ops.mx_linear(x, w)):
+    rows = ops.MXRows(torch.zeros(2, 128, dtype=torch.float8_e4m3fn), torch.ones(2, 4, dtype=torch.uint8), 128)
+    for f in (lambda: ops.mx_quantize(x), lambda: ops.mx_weight(x), lambda: ops.mx_rms_norm(x, x[0]), lambda: ops.mx_linear(x, w),
+              lambda: ops.mx_linear(rows, w)):
         with pytest.raises(RuntimeError, match='ROCm GPU'):
             f()
 
@@ -438,6 +440,23 @@ def test_products_of_infinities_stay_in_their_rows(R):
     x[1, 5] = float('inf')
     y = ops.mx_linear(ops.mx_quantize(x), w)
     assert bool(torch.isnan(y[1]).all()) and torch.equal(y[0], clean[0])
+
+
+@gpu
+@pytest.mark.parametrize('R', [2, 100])
+def test_a_gated_block_that_is_not_finite(R):
+    case('mx_swiglu: an infinity in one row', R)
+    w = ops.mx_weight(randn(2 * 96, 256, seed=15), gated=True)
+    for rows in (randn(R, 256, seed=16).bfloat16(), randn(R, 256, seed=16)):
+        clean = ops.mx_swiglu(rows, w, quantize=True)
+        rows[1, 7] = float('inf')
+        got = ops.mx_swiglu(rows, w, quantize=True)
+        y = ops.mx_swiglu(rows, w)
+        assert not bool(torch.isfinite(y[1]).all()) and bool(torch.isfinite(y[0]).all())
+        bad = ~torch.isfinite(y.float()).view(R, 3, 32).all(-1)
+        assert torch.equal(got.scales[:, :3] == 255, bad) and torch.equal(got.scales[0], clean.scales[0])
+        assert torch.equal(torch.isnan(got.dequantize()).view(R, 3, 32).all(-1), bad)
+        assert torch.equal(got.values.view(torch.uint8)[0], clean.values.view(torch.uint8)[0])
 
 
 @gpu

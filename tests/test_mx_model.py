@@ -103,6 +103,10 @@ def test_what_4_bit_projections_do_not_stand_for():
     with pytest.raises(NotImplementedError, match='head'):
         m.quantize_weights_()
     assert isinstance(m.blocks[0].ffn.l1, nn.Linear)
+    m.blocks[0].ffn.l1.register_forward_pre_hook(lambda *a: None)         # nothing of the model, not a part of it
+    with pytest.raises(NotImplementedError, match='plain'):
+        m.quantize_weights_(head=False)
+    assert hasattr(m.blocks[0].att, 'wq')
 
 
 # --- the layer ------------------------------------------------------------------------

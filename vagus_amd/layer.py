@@ -322,17 +322,23 @@ class GatedDeltaNet(nn.Module):
         its type.  For serving: forward, decode_step, draft_step and prefill_packed without autograd."""
         if hasattr(self, 'w_in'):
             return
-        mods = [self.wq, self.wk, self.wv, self.wg] + ([self.wo] if self.out_proj else [])
-        if not all(_plain_module(m, nn.Linear) and m.bias is None for m in mods):
-            raise NotImplementedError('4-bit weights stand for plain bias-free nn.Linear projections')
-        if any(m.weight.shape[0] % 16 for m in mods[:4]):
-            raise NotImplementedError(f'4-bit projections have multiples of 16 columns; got {[m.weight.shape[0] for m in mods[:4]]}')
-        w_in = MXLinear(ops.mx_weight(torch.cat([m.weight.detach() for m in mods[:4]])))
+        self._check_4bit()
+        w_in = MXLinear(ops.mx_weight(torch.cat([m.weight.detach() for m in (self.wq, self.wk, self.wv, self.wg)])))
         wo = MXLinear(ops.mx_weight(self.wo.weight)) if self.out_proj else None
         del self.wq, self.wk, self.wv, self.wg
         self.w_in = w_in
         if wo is not None:
             self.wo = wo
+
+    def _check_4bit(self) -> None:
+        """Refuses what quantize_weights_ does not stand for."""
+        if hasattr(self, 'w_in'):
+            return
+        mods = [self.wq, self.wk, self.wv, self.wg] + ([self.wo] if self.out_proj else [])
+        if not all(_plain_module(m, nn.Linear) and m.bias is None for m in mods):
+            raise NotImplementedError('4-bit weights stand for plain bias-free nn.Linear projections')
+        if any(m.weight.shape[0] % 16 for m in mods[:4]):
+            raise NotImplementedError(f'4-bit projections have multiples of 16 columns; got {[m.weight.shape[0] for m in mods[:4]]}')
 
     def _project(self, x, x8=None) -> dict:
         """q, k, v and the output gate of 4-bit projections, each a tensor of its own; x8: x as 8-bit rows, which then

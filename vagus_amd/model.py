@@ -98,9 +98,13 @@ class FFN(nn.Module):
         """Both projections become 4-bit weights (MXLinear), in place and for good; no autograd from then on."""
         if isinstance(self.l1, MXLinear):
             return
-        if not all(_plain_module(m, nn.Linear) and m.bias is None for m in (self.l1, self.l2)):
-            raise NotImplementedError('4-bit weights stand for plain bias-free nn.Linear projections')
+        self._check_4bit()
         self.l1, self.l2 = MXLinear(ops.mx_weight(self.l1.weight, gated=True)), MXLinear(ops.mx_weight(self.l2.weight))
+
+    def _check_4bit(self) -> None:
+        """Refuses what quantize_weights_ does not stand for."""
+        if not isinstance(self.l1, MXLinear) and not all(_plain_module(m, nn.Linear) and m.bias is None for m in (self.l1, self.l2)):
+            raise NotImplementedError('4-bit weights stand for plain bias-free nn.Linear projections')
 
     def forward(self, x):
         if isinstance(self.l1, MXLinear):
@@ -255,6 +259,9 @@ class GDNLM(nn.Module):
         assert prompt_bits in (8, 16), f'prompt_bits must be 8 or 16; got {prompt_bits}'
         if head and not isinstance(self.head, MXLinear) and not (_plain_module(self.head, nn.Linear) and self.head.bias is None):
             raise NotImplementedError('4-bit weights stand for a plain bias-free nn.Linear head')
+        for blk in self.blocks:                       # all of it or nothing
+            blk.att._check_4bit()
+            blk.ffn._check_4bit()
         for blk in self.blocks:
             blk.att.quantize_weights_()
             blk.ffn.quantize_weights_()

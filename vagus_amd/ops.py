@@ -2176,13 +2176,15 @@ def mx_rms_norm(x, weight, eps: float = 1e-6, residual=None, out_residual=None, 
 
 def _mx_product(x, w: MXWeight, gated: bool, quantize: bool, out_dtype):
     # a decode step calls this four times a layer: few Python calls on the usual way through
-    if type(w) is not MXWeight or w.gated != gated:
+    if not isinstance(w, MXWeight) or w.gated != gated:
         raise AssertionError(f'{"mx_swiglu takes a gated" if gated else "mx_linear takes an ungated"} MXWeight (mx_weight); '
                              f'got {type(w).__name__}')
     n, k = w.shape
     wv, ws = w.values, w.scales
     index = wv.get_device()
-    rows8 = type(x) is MXRows
+    if index < 0:
+        _check_device(wv)
+    rows8 = isinstance(x, MXRows)
     work = scales = None
     nbytes = 0
     if rows8:
