@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(256) mx_rows_kernel(const E *__restrict__ x, i
 template <typename E>
 __global__ void __launch_bounds__(256) mx_weight_kernel(const E *__restrict__ w, int64_t ldw, uint8_t *values,
                                                         uint8_t *scales, int64_t n, int64_t K, int64_t C, int64_t tiles,
-                                                        bool gated) {
+                                                        bool gated, bool vec) {
     const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int64_t C4 = (C + 3) / 4, t = unit / (4 * C4), c = unit - t * 4 * C4;   // c past C: a scale alone
     if (t >= tiles) return;
@@ -70,11 +70,9 @@ __global__ void __launch_bounds__(256) mx_weight_kernel(const E *__restrict__ w,
     float v[32];
     uint32_t amax = 0;
 #pragma unroll
-    for (int e = 0; e < 32; ++e) {
-        const int64_t k = 128 * c + 32 * g + e;
-        v[e] = live && k < K ? (float)row[k] : 0.f;
-        amax = max(amax, abs_bits(v[e]));
-    }
+    for (int e = 0; e < 32; e += 8) load8(*reinterpret_cast<float(*)[8]>(v + e), row, 128 * c + 32 * g + e, live ? K : 0, vec);
+#pragma unroll
+    for (int e = 0; e < 32; ++e) amax = max(amax, abs_bits(v[e]));
     const int b = mx_scale<4>(amax);
     if (c < C) {
         const float inv = b == 255 ? 0.f : mx_inverse(b);
@@ -196,7 +194,7 @@ hipError_t quantize_t(const MxQuantize &p, hipStream_t stream) {
     }
     const int64_t C = Kp / 128, tiles = p.gated ? 2 * ((p.rows / 2 + 15) / 16) : (p.rows + 15) / 16;
     hipLaunchKernelGGL((mx_weight_kernel<E>), dim3((unsigned)(tiles * ((C + 3) / 4))), dim3(256), 0, stream, x, p.ldx, p.values,
-                       p.scales, p.rows, p.K, C, tiles, p.gated);
+                       p.scales, p.rows, p.K, C, tiles, p.gated, vec);
     return hipGetLastError();
 }
 
