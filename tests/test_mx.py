@@ -508,7 +508,7 @@ def test_calls_that_are_refused():
     for f in (lambda: ops.mx_linear(x, wg), lambda: ops.mx_swiglu(x, w), lambda: ops.mx_linear(x[:, :100], w), lambda: ops.mx_linear(x, x),
               lambda: ops.mx_weight(x[0]), lambda: ops.mx_weight(x[:3], gated=True), lambda: ops.mx_weight(x[:0]),
               lambda: ops.mx_rms_norm(x, x[0].half()), lambda: ops.mx_rms_norm(x, x[0], residual=x[:2]),
-              lambda: ops.mx_rms_norm(x, x[0], residual=x, out_residual=x.half())):
+              lambda: ops.mx_rms_norm(x, x[0], residual=x, out_residual=x.half()), lambda: ops.mx_rms_norm(x, x[0], out_residual=x.clone())):
         with pytest.raises(AssertionError):
             f()
     for f in (lambda: ops.mx_quantize(x.double()), lambda: ops.mx_linear(x.double(), w), lambda: ops.mx_linear(x, w, out_dtype=torch.float64),

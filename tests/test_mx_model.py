@@ -23,7 +23,7 @@ from torch import nn
 from oracle import mx
 from vagus_amd import ops
 from vagus_amd.layer import GatedDeltaNet, MXLinear
-from vagus_amd.model import FFN, GDNLM, RaggedGenerator
+from vagus_amd.model import FFN, GDNLM, RaggedGenerator, _ffn
 
 DEV = 'cuda'
 gpu = pytest.mark.gpu
@@ -107,6 +107,15 @@ def test_what_4_bit_projections_do_not_stand_for():
     with pytest.raises(NotImplementedError, match='plain'):
         m.quantize_weights_(head=False)
     assert hasattr(m.blocks[0].att, 'wq')
+
+
+def test_another_module_in_the_place_of_an_ffn_runs():
+    h = torch.randn(2, 3, 64)
+    with torch.no_grad():
+        assert torch.equal(_ffn(nn.Identity(), h), h)
+    m = GDNLM(vocab_size=50, dim=64, layer_count=1, head_count=1, key_head_dim=64, value_head_dim=64, gate='scalar')
+    m.blocks[0].ffn = nn.Identity()
+    assert m._quantized() == []
 
 
 # --- the layer ------------------------------------------------------------------------
@@ -319,6 +328,24 @@ def test_generator():
         blk.ffn.l1 = MXLinear(ops.mx_weight(src.ffn.l1.weight, gated=True))     # moved
     gen.prefill(texts)
     assert torch.equal(gen.generate(12), run(m, graph=False))
+
+
+@gpu
+def test_weights_quantised_in_inference_mode():
+    case('quantize_weights_ within inference_mode, generation outside of it, a state_dict')
+    m, want = pair(torch.float32)
+    with torch.inference_mode():
+        m.quantize_weights_()
+    text = [torch.arange(7) % 300]
+
+    def run(mm):
+        gen = RaggedGenerator(mm)
+        gen.prefill(text)
+        return gen.generate(6)
+    tokens = run(m)
+    assert not any(t.is_inference() for t in m._quantized()) and torch.equal(tokens, run(want))
+    m.load_state_dict({n: t.clone() for n, t in m.state_dict().items()})
+    assert torch.equal(run(m), tokens)
 
 
 @gpu

@@ -316,6 +316,7 @@ class GatedDeltaNet(nn.Module):
             on = on - {'gate'}
         return on
 
+    @torch.inference_mode(False)                       # buffers for calls from outside of it too
     def quantize_weights_(self) -> None:
         """W_q, W_k, W_v, W_g (as one map, w_in, whose rows they are) and W_o become 4-bit weights (MXLinear), in place and for
         good; what decides how the state decays and is written (W_a, W_b, the short conv, A_log, dt_bias) keeps

@@ -72,7 +72,7 @@ def _ffn(ffn: 'FFN', h, dtype=None):
     activations between the two products, and dtype is the result's."""
     if isinstance(h, ops.MXRows):
         return ops.mx_linear(ops.mx_swiglu(h, ffn.l1.weight, quantize=True), ffn.l2.weight, out_dtype=dtype)
-    if isinstance(ffn.l1, MXLinear):
+    if isinstance(getattr(ffn, 'l1', None), MXLinear):
         return ffn(h)
     if (h.is_cuda and not torch.is_grad_enabled() and h.dtype in (torch.bfloat16, torch.float16, torch.float32)
             and ffn.hidden_dim % (16 // h.element_size()) == 0):
@@ -94,6 +94,7 @@ class FFN(nn.Module):
         nn.init.normal_(self.l1.weight, std=init_std)
         nn.init.normal_(self.l2.weight, std=init_std / math.sqrt(2 * layer_count) if layer_count else init_std)
 
+    @torch.inference_mode(False)                       # buffers for calls from outside of it too
     def quantize_weights_(self) -> None:
         """Both projections become 4-bit weights (MXLinear), in place and for good; no autograd from then on."""
         if isinstance(self.l1, MXLinear):
@@ -249,6 +250,7 @@ class GDNLM(nn.Module):
     def from_config(cls, config: dict) -> 'GDNLM':
         return cls(**config)
 
+    @torch.inference_mode(False)                       # buffers for calls from outside of it too
     def quantize_weights_(self, *, prompt_bits: int = 8, head: bool = True) -> 'GDNLM':
         """The blocks' large projections (q, k, v, output gate, W_o, both of the FFN) and the head become 4-bit weights with
         a scale for each 32 (layer.MXLinear), in place and for good, on the GPU: a decode step reads a quarter of the bytes.
@@ -273,7 +275,7 @@ class GDNLM(nn.Module):
 
     def _quantized(self) -> list:
         """The 4-bit weights' buffers: none before quantize_weights_."""
-        maps = [m for blk in self.blocks for m in (getattr(blk.att, 'w_in', None), getattr(blk.att, 'wo', None), blk.ffn.l1, blk.ffn.l2)]
+        maps = [getattr(m, n, None) for blk in self.blocks for m, n in ((blk.att, 'w_in'), (blk.att, 'wo'), (blk.ffn, 'l1'), (blk.ffn, 'l2'))]
         return [t for m in maps + [self.head] if isinstance(m, MXLinear) for t in (m.values, m.scales)]
 
     def forward(self, tokens, is_causal: bool = True, return_hidden: bool = False):
@@ -432,7 +434,7 @@ class RaggedGenerator:
         (storage and version: load_state_dict, an optimizer step or .to()
         change one of them) and each layer's state and conv-cache buffers.  A
         replay is valid only while the addresses are unchanged."""
-        key = [(p.data_ptr(), p._version) for p in (*self.model.parameters(), *self.model._quantized())]
+        key = [(p.data_ptr(), 0 if p.is_inference() else p._version) for p in (*self.model.parameters(), *self.model._quantized())]
         for blk in self.model.blocks:
             att = blk.att
             key += [(t.data_ptr(), t.dtype) for t in (att.state,) + (att._caches() if att.short_conv_size else ())]

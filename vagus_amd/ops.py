@@ -2155,6 +2155,7 @@ def mx_rms_norm(x, weight, eps: float = 1e-6, residual=None, out_residual=None, 
     D = x.shape[-1]
     assert weight.shape == (D,) and weight.dtype == x.dtype, \
         f'weight must be ({D},) in {x.dtype}; got {tuple(weight.shape)} {weight.dtype}'
+    assert out_residual is None or residual is not None, 'out_residual takes x + residual: there is no residual'
     xs, w = _aligned(x), _aligned(weight)
     r = h = None
     if residual is not None:
