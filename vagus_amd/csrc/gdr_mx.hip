@@ -42,7 +42,10 @@ __device__ __forceinline__ void store8(uint8_t *values, uint8_t *scales, int64_t
 
 }  // namespace
 
-// Rows x [R, K] (ldx apart) to 8 bits: a thread eight elements, four threads a block.
+// Rows x [R, K] (ldx apart) to 8 bits: b = 2^s the smallest with amax <= 464 b, v = rne(x / b), exact but for that one
+// rounding.  A thread eight elements, four threads a block: 16-byte loads, 8-byte stores, whole
+// lines of both per wave, and the block's largest in two exchanges between neighbours.  Bound by
+// memory: 65,536 rows of 2048 in bf16 71.9 us, 407 MB at 5.7 TB/s.
 template <typename E>
 __global__ void __launch_bounds__(256) mx_rows_kernel(const E *__restrict__ x, int64_t ldx, uint8_t *values,
                                                       uint8_t *scales, int64_t rows, int64_t K, int64_t Kp, bool vec) {
@@ -54,7 +57,9 @@ __global__ void __launch_bounds__(256) mx_rows_kernel(const E *__restrict__ x, i
     store8(values, scales, row * Kp + c, v);
 }
 
-// Weights w [n, K] (ldw apart) to 4 bits in the tiles' order: a wave a tile, lane 16 g + r one block.
+// Weights w [n, K] (ldw apart) to 4 bits in the tiles' order: a wave a tile, lane 16 g + r one block, whose 16 bytes it
+// stores at its own place (a wave's stores are one run of 1024 bytes).  Four waves take the four tiles whose
+// scales share words.  Bound by memory: 8192 x 8192 in bf16 34 us, 170 MB at 5.0 TB/s (element by element 148).
 template <typename E>
 __global__ void __launch_bounds__(256) mx_weight_kernel(const E *__restrict__ w, int64_t ldw, uint8_t *values,
                                                         uint8_t *scales, int64_t n, int64_t K, int64_t C, int64_t tiles,
@@ -91,8 +96,10 @@ __global__ void __launch_bounds__(256) mx_weight_kernel(const E *__restrict__ w,
 }
 
 // h = x + residual, y = h rsqrt(mean h^2 + eps) gamma, y to 8 bits; a workgroup a row, a thread U units of eight
-// elements.  y is formed in 64 bits and rounded once (round_to_odd), so that the bytes are those of the
-// formula itself, whatever the order of the sum.
+// elements, in registers from the read to the rounding: every byte moves once.  y is formed in 64 bits and rounded once
+// (round_to_odd), so that the bytes are those of the formula itself, whatever the order of the sum; a multiply and an
+// add in 64 bits an element, and three multiplies, lie under the loads.  Bound by memory: 65,536 rows of
+// 2048 in bf16 with the residual 182 us, 945 MB at 5.2 TB/s; one row 2.5 us, a launch and two dependent round trips.
 template <typename E, int U>
 __global__ void __launch_bounds__(256) mx_rms_norm_kernel(const E *x, const E *res, E *x_out, const E *__restrict__ gamma,
                                                           float eps, E *y, uint8_t *values, uint8_t *scales, int dim,
@@ -155,7 +162,9 @@ __global__ void __launch_bounds__(256) mx_rms_norm_kernel(const E *x, const E *r
 }
 
 // Many rows of fp16 or fp32 (or of bf16 of a width that is no multiple of 128) as bf16 planes [P][R][Kp] whose sum they are.  A
-// product of a plane's element with a 4-bit weight is exact in fp32, so the tiles need one form of 16-bit rows.
+// product of a plane's element with a 4-bit weight is exact in fp32, so the tiles need one form of 16-bit rows, whose K
+// steps are two or three times as many.  65,536 rows of 2048 against 8192 columns, planes and product: bf16 1,730 us (no
+// planes), fp16 3,390, fp32 5,320 (the library's fp32 product alone: 14,400 at its rate of 153 TFLOP/s).
 template <typename E, int P>
 __global__ void __launch_bounds__(256) mx_planes_kernel(const E *__restrict__ x, int64_t ldx, __bf16 *out, int64_t rows,
                                                         int64_t K, int64_t Kp, bool vec) {

@@ -141,6 +141,9 @@ constexpr int BF16_TAIL = 4;
 // region of its own, which needs no barrier: a load covers whole rows of a tile there, where fragments
 // straight from global memory would have every lane in a line of its own, and the address unit bounds those
 // (64 rows, K 5632, N 2048: 9.6 us; 64 rows, K and N 8192: 25).
+// Bound by latency, a chain of launch, first loads, K / 128 / NWV steps and the meeting in LDS: one row, K 2048, N 8192
+// 4.5 us (8.9 MB of weights, 1.8 us at a copy's rate), 64 rows 7.1 us; one row, gated 11264, 5.8 us, 64 rows 10.6.  A longer
+// way ahead in the loads, sixteen waves, or eight weight tiles a workgroup took as long or longer.
 // X: the rows' type (0 fp32, 1 bf16, 2 fp16, MX8, BF16_TAIL).  fp32 and fp16 rows become three and two bf16 planes on their way
 // into LDS; their K, and BF16_TAIL's, may end inside a tile (a check that costs the others half a microsecond).
 template <int X, bool GATED, int MT, int NB, int NWV>
@@ -333,10 +336,10 @@ __global__ void __launch_bounds__(64 * NWV, 2) mx_few_rows_kernel(const MxLinear
 // are swizzled so that the 16 rows of a fragment lie on distinct banks; of the two weight tiles that
 // weight_row mixes the second has its rows' places moved by four for the same reason.
 // Two workgroups share a CU: one's barriers, first copies and stores lie under the other's products.  At K = 2048
-// that is the larger part: 65,536 rows in 8 bits, N 8192: 930 us (2,360 TFLOP/s); one workgroup of 256 x 256 and
+// that is the larger part: 65,536 rows in 8 bits, N 8192: 925 us (2,380 TFLOP/s); one workgroup of 256 x 256 and
 // three stages 1,240, its next tile's copies begun under the stores 1,220; at K = N = 8192, 16,384 rows 790 us
 // (2,780 TFLOP/s) against 880.  The weights' fragments straight from global memory into registers: 1,360
-// (the wait for them is a wait for the copies behind them too).  bf16 rows: 1,760 us (1,250 TFLOP/s); there the LDS
+// (the wait for them is a wait for the copies behind them too).  bf16 rows: 1,730 us (1,270 TFLOP/s); there the LDS
 // for two workgroups allows 64 x 256, and the conversions share the issue slots with twice the products' time.
 template <bool X8, bool GATED, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN, 2 * WM * WN / 4) mx_tile_kernel(const MxLinear p, uint32_t mb, uint32_t nb) {

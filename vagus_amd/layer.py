@@ -41,6 +41,8 @@ in the reference.  Training: the scans, the short conv and the output epilogue
 differentiate through their HIP backward kernels; where those do not stand for
 the module's expression (autocast, tracing, functorch transforms, hooks on the
 submodule) the conv and the epilogue run as the reference's torch expressions.
+Serving: ``quantize_weights_`` makes W_q, W_k, W_v, W_g and W_o 4-bit weights (``MXLinear``), whose products are HIP kernels
+without a backward.
 """
 from __future__ import annotations
 

@@ -24,6 +24,9 @@ pending.  ``RaggedGenerator.generate_drafted`` feeds a block a step, the pending
 token and tokens drafted from the stream's own text, keeps those that the
 model's probabilities let stand, and samples the token behind them: as many tokens for
 one read of the weights and the states, greedy or at a temperature.
+
+``GDNLM.quantize_weights_`` makes the large projections 4-bit weights for serving: a step then reads a quarter of
+their bytes, and packed prompts go through the products as 8-bit rows.
 """
 from __future__ import annotations
 

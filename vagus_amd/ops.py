@@ -36,6 +36,9 @@ explicit write vector w) through vgdr_scan_bwd, and so are the token-by-token
 calls (fused_recurrent_*, hip_recurrent) without the short conv or the output
 epilogue.  The decode step, the fused epilogue and in-place state updates
 raise NotImplementedError for inputs that require grad.
+
+Serving in fewer bits (mx_weight, mx_quantize, mx_rms_norm, mx_linear, mx_swiglu): 4-bit weights and 8-bit rows with a scale for
+each 32 elements (MXWeight, MXRows), and the norm and the products that take and give them.  No autograd.
 """
 from __future__ import annotations
 
