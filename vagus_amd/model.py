@@ -437,7 +437,8 @@ class RaggedGenerator:
         (storage and version: load_state_dict, an optimizer step or .to()
         change one of them) and each layer's state and conv-cache buffers.  A
         replay is valid only while the addresses are unchanged."""
-        key = [(p.data_ptr(), 0 if p.is_inference() else p._version) for p in (*self.model.parameters(), *self.model._quantized())]
+        quantized = getattr(self.model, '_quantized', list)()       # a model of the caller's own has none
+        key = [(p.data_ptr(), 0 if p.is_inference() else p._version) for p in (*self.model.parameters(), *quantized)]
         for blk in self.model.blocks:
             att = blk.att
             key += [(t.data_ptr(), t.dtype) for t in (att.state,) + (att._caches() if att.short_conv_size else ())]
