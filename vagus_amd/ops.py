@@ -2152,30 +2152,33 @@ def mx_rms_norm(x, weight, eps: float = 1e-6, residual=None, out_residual=None, 
     if index < 0:
         _check_device(x)
     _all_on(index, weight, residual, out_residual)
-    _check_grad(x, weight, residual)
-    if x.dtype not in _DTYPES:
-        raise NotImplementedError(f'x must be one of {list(_DTYPES)}; got {x.dtype}')
-    D = x.shape[-1]
-    assert weight.shape == (D,) and weight.dtype == x.dtype, \
-        f'weight must be ({D},) in {x.dtype}; got {tuple(weight.shape)} {weight.dtype}'
+    if x.requires_grad or weight.requires_grad or residual is not None:
+        _check_grad(x, weight, residual)
+    shape, dt = x.shape, x.dtype
+    code = _DTYPES.get(dt)
+    if code is None:
+        raise NotImplementedError(f'x must be one of {list(_DTYPES)}; got {dt}')
+    D = shape[-1]
+    assert weight.shape == (D,) and weight.dtype is dt, f'weight must be ({D},) in {dt}; got {tuple(weight.shape)} {weight.dtype}'
     assert out_residual is None or residual is not None, 'out_residual takes x + residual: there is no residual'
     xs, w = _aligned(x), _aligned(weight)
     r = h = None
     if residual is not None:
-        assert residual.shape == x.shape and residual.dtype == x.dtype, 'residual must match x'
+        assert residual.shape == shape and residual.dtype is dt, 'residual must match x'
         r = _aligned(residual)
         if out_residual is None:
-            h = x.new_empty(x.shape)
+            h = x.new_empty(shape)
         else:
-            assert out_residual.shape == x.shape and out_residual.dtype == x.dtype and out_residual.is_contiguous() \
+            assert out_residual.shape == shape and out_residual.dtype is dt and out_residual.is_contiguous() \
                 and out_residual.data_ptr() % 16 == 0, 'out_residual: contiguous, aligned, shaped and typed as x'
             h = out_residual
-    out = _mx_rows(x.shape[:-1], D, x)
-    y = x.new_empty(x.shape) if norm_out else None
-    _launch(index, _lib.load().vgdr_mx_rms_norm, _DTYPES[x.dtype], xs.data_ptr(), _ptr(r), _ptr(h), w.data_ptr(), _ptr(y),
+    out = _mx_rows(shape[:-1], D, x)
+    y = x.new_empty(shape) if norm_out else None
+    _launch(index, _lib.load().vgdr_mx_rms_norm, code, xs.data_ptr(), _ptr(r), _ptr(h), w.data_ptr(), _ptr(y),
             out.values.data_ptr(), out.scales.data_ptr(), xs.numel() // max(D, 1), D, float(eps))
-    got = (out,) + ((y,) if norm_out else ()) + ((h,) if residual is not None else ())
-    return got if len(got) > 1 else out
+    if residual is None:
+        return (out, y) if norm_out else out
+    return (out, y, h) if norm_out else (out, h)
 
 
 def _mx_product(x, w: MXWeight, gated: bool, quantize: bool, out_dtype):
