@@ -512,14 +512,19 @@ hipError_t tile_go(const MxLinear &p, int tiles, hipStream_t stream) {
 //   64 rows, K 5632, N 2048: 2 tiles x 16 rows (256 workgroups) 8.6 / 8.2, 1 x 16 (512) 9.6 / 8.9, 2 x 32 (128) 10.7 / 9.7
 //   32 rows, K 2048, N 8192: 2 x 32 (256) 8.0 / 7.2, 2 x 16 (512) 7.9 / 7.6, 4 x 32 (128) 9.6 / 8.3
 // The kernel for few rows up to where 4 x 32 makes one workgroup a CU: it has the whole sum in flight (128 rows, K 5632,
-// N 2048: 11.0 / 9.9, 64 x 64 tiles 26.6 / 18.8), and for bf16 rows, whose tiles convert the weights, up to two, with four
-// waves each so that both are on the CU: 64 rows, K 2048, gated 11264: 13.2 / 11.1 (eight waves 16.2 / 14.3), tiles 14.8 /
-// 10.8; 96 rows: 16.8 / 15.0, tiles 17.8 / 12.6.
+// N 2048: 11.0 / 9.9, 64 x 64 tiles 26.6 / 18.8).  Past that it has four waves, so that two are on a CU (64 rows, K 2048, gated
+// 11264: 13.2 / 11.1, eight waves 16.2 / 14.3), and bf16 rows, whose tiles convert the weights in each of many steps one
+// behind the other, keep it the longer the sum is.  Kernels alone, few / tiles, at N 8192 and gated 8192:
+//   two a CU (128 rows): K 512 5.1 / 4.6 and 5.2 / 5.1, K 1024 6.9 / 6.7 and 7.1 / 7.2, K 2048 9.9 / 10.7 and 9.9 / 11.5
+//   three (192 rows): K 1536 12.0 / 10.7 and 12.2 / 12.4, K 2048 14.1 / 13.2 and 14.2 / 15.6, K 5632 27.9 / 31.5 and 28.5 / 37.0
+//   four (256 rows): K 2048 16.8 / 13.7 and 17.4 / 15.9, K 5632 35.9 / 33.4 and 36.1 / 37.7
+// 8-bit rows: two a CU, K 2048 8.8 / 8.0 and 8.9 / 8.3, K 5632 16.3 / 17.6 and 16.8 / 16.9.
 // Tiles: largest with 5 workgroups for 4 CUs.  512 rows, K 2048, N 8192: 64 x 128 (512) 24.1 / 15.9, 64 x 64 (1,024) 27.6 /
 // 22.9; 256 rows: 64 x 64 (512) 17.0 / 13.2, 64 x 128 (256) 18.2 / 14.6; 8-bit rows, N 32768, 512 rows: 128 x 256
 // (512) 34.3, 64 x 256 38.2, 256 rows: 64 x 256 (512) 22.2, 128 x 256 (256) 25.3.
 // Rows that the kernel for few rows converts itself (MX_RAW_ROWS at most) stay as they are: fp32 or fp16, or of a width that
-// ends inside a tile.  7 rows of fp32, K 1000, N 1337: one launch instead of two.
+// ends inside a tile: one launch instead of two.  Past it, planes first / as they are, fp16 rows, kernels alone: 64 rows, K 2048,
+// N 8192 12.6 / 13.4, N 2048 7.6 / 6.3, N 32000 26.1 / 51.7, gated 11264 16.6 / 19.0; 48 rows, K 5632, N 2048 14.5 / 18.9.
 template <int X, bool GATED>
 hipError_t mx_linear_t(const MxLinear &p, hipStream_t stream) {
     constexpr bool X8 = X == MX8;
@@ -534,7 +539,8 @@ hipError_t mx_linear_t(const MxLinear &p, hipStream_t stream) {
             return few_rows_go<X, GATED, 1, 1, 8>(p, tiles, stream);
         }
     } else {
-        if (p.rows <= MX_RAW_ROWS || few(4, 2) <= (X8 ? 1 : 2) * cus) {
+        const int sum = p.C * p.planes, most = X8 || sum <= 6 ? 1 : sum <= (GATED ? 12 : 16) ? 2 : 3;
+        if (p.rows <= MX_RAW_ROWS || few(4, 2) <= most * cus) {
             if (p.rows > 16 && few(4, 2) > cus) return few_rows_go<X, GATED, 4, 2, 4>(p, tiles, stream);
             if (p.rows > 16 && few(4, 2) == cus) return few_rows_go<X, GATED, 4, 2, 8>(p, tiles, stream);
             if constexpr (GATED) {
