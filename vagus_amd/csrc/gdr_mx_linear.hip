@@ -507,10 +507,14 @@ hipError_t tile_go(const MxLinear &p, int tiles, hipStream_t stream) {
     return hipGetLastError();
 }
 
-// The variant: the largest tiles that still give every CU a workgroup (a larger tile reads less, the smaller ones'
-// traffic bounds them), us for bf16 / 8-bit rows:
-//   64 rows, K 5632, N 2048: 2 tiles x 16 rows (256 workgroups) 8.6 / 8.2, 1 x 16 (512) 9.6 / 8.9, 2 x 32 (128) 10.7 / 9.7
-//   32 rows, K 2048, N 8192: 2 x 32 (256) 8.0 / 7.2, 2 x 16 (512) 7.9 / 7.6, 4 x 32 (128) 9.6 / 8.3
+// The variant of the few-row kernel: the smallest tiles that make at most one workgroup a CU.  Smaller ones leave a part of the
+// CUs a second workgroup to wait for, and read the rows or the weights more often.  Kernels alone, us for bf16 / 8-bit rows:
+//   192 rows, K 5632, N 2048: 4 tiles x 32 rows (192 workgroups) 11.3 / 9.7, 2 x 32 (384) 13.9 / 11.3
+//   16 rows, K 5632, N 6144: 2 x 16 (192) 5.6 / 5.4, 1 x 16 (384) 6.5 / 5.9; as fp32 15.3, 26.6
+//   48 rows, K 5632, N 2048: 2 x 16 (192) 5.7 / 5.4, 1 x 16 (384) 6.6 / 5.9
+// and with the call's host time, one a CU against half of them: 64 rows, K 5632, N 2048: 2 x 16 (256) 8.6 / 8.2, 2 x 32
+// (128) 10.7 / 9.7; 32 rows, K 2048, N 8192: 2 x 32 (256) 8.0 / 7.2, 4 x 32 (128) 9.6 / 8.3.  It costs short sums a
+// little: 192 rows, K 1024, N 2048: 5.2 / 5.1 against 6.1 / 4.9; one row, K 2048, N 12288: 5.0 / 4.4 against 4.7 / 4.1.
 // The kernel for few rows up to where 4 x 32 makes one workgroup a CU: it has the whole sum in flight (128 rows, K 5632,
 // N 2048: 11.0 / 9.9, 64 x 64 tiles 26.6 / 18.8).  Past that it has four waves, so that two are on a CU (64 rows, K 2048, gated
 // 11264: 13.2 / 11.1, eight waves 16.2 / 14.3), and bf16 rows, whose tiles convert the weights in each of many steps one
@@ -533,24 +537,22 @@ hipError_t mx_linear_t(const MxLinear &p, hipStream_t stream) {
     const int64_t cus = device_cu_count();
     auto few = [&](int mt, int nb) { return (int64_t)((tiles + mt - 1) / mt) * ((p.rows + 16 * nb - 1) / (16 * nb)); };
     if constexpr (X == 0 || X == 2 || X == BF16_TAIL) {
-        if (GATED || few(4, 1) >= cus) return few_rows_go<X, GATED, 4, 1, 8>(p, tiles, stream);
         if constexpr (!GATED) {
-            if (few(2, 1) >= cus) return few_rows_go<X, GATED, 2, 1, 8>(p, tiles, stream);
-            return few_rows_go<X, GATED, 1, 1, 8>(p, tiles, stream);
+            if (few(1, 1) <= cus) return few_rows_go<X, GATED, 1, 1, 8>(p, tiles, stream);
+            if (few(2, 1) <= cus) return few_rows_go<X, GATED, 2, 1, 8>(p, tiles, stream);
         }
+        return few_rows_go<X, GATED, 4, 1, 8>(p, tiles, stream);
     } else {
         const int sum = p.C * p.planes, most = X8 || sum <= 6 ? 1 : sum <= (GATED ? 12 : 16) ? 2 : 3;
         if (p.rows <= MX_RAW_ROWS || few(4, 2) <= most * cus) {
-            if (p.rows > 16 && few(4, 2) > cus) return few_rows_go<X, GATED, 4, 2, 4>(p, tiles, stream);
-            if (p.rows > 16 && few(4, 2) == cus) return few_rows_go<X, GATED, 4, 2, 8>(p, tiles, stream);
-            if constexpr (GATED) {
-                return few_rows_go<X, GATED, 4, 1, 8>(p, tiles, stream);
-            } else {
-                if (p.rows > 16 && few(2, 2) >= cus) return few_rows_go<X, GATED, 2, 2, 8>(p, tiles, stream);
-                if (few(4, 1) >= cus) return few_rows_go<X, GATED, 4, 1, 8>(p, tiles, stream);
-                if (few(2, 1) >= cus) return few_rows_go<X, GATED, 2, 1, 8>(p, tiles, stream);
-                return few_rows_go<X, GATED, 1, 1, 8>(p, tiles, stream);
+            if constexpr (!GATED) {
+                if (few(1, 1) <= cus) return few_rows_go<X, GATED, 1, 1, 8>(p, tiles, stream);
+                if (few(2, 1) <= cus) return few_rows_go<X, GATED, 2, 1, 8>(p, tiles, stream);
+                if (p.rows > 16 && few(2, 2) <= cus) return few_rows_go<X, GATED, 2, 2, 8>(p, tiles, stream);
             }
+            if (p.rows <= 16 || few(4, 1) <= cus) return few_rows_go<X, GATED, 4, 1, 8>(p, tiles, stream);
+            if (few(4, 2) <= cus) return few_rows_go<X, GATED, 4, 2, 8>(p, tiles, stream);
+            return few_rows_go<X, GATED, 4, 2, 4>(p, tiles, stream);
         }
         auto fills = [&](int bm, int bn) { return 4 * ((p.rows + bm - 1) / bm) * ((tiles + bn / 16 - 1) / (bn / 16)) >= 5 * cus; };
         if constexpr (X8)
