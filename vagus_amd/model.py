@@ -278,8 +278,7 @@ class GDNLM(nn.Module):
 
     def _quantized(self) -> list:
         """The 4-bit weights' buffers: none before quantize_weights_."""
-        maps = [getattr(m, n, None) for blk in self.blocks for m, n in ((blk.att, 'w_in'), (blk.att, 'wo'), (blk.ffn, 'l1'), (blk.ffn, 'l2'))]
-        return [t for m in maps + [self.head] if isinstance(m, MXLinear) for t in (m.values, m.scales)]
+        return [t for m in self.modules() if isinstance(m, MXLinear) for t in (m.values, m.scales)]
 
     def forward(self, tokens, is_causal: bool = True, return_hidden: bool = False):
         x = self.embedding(tokens)
@@ -433,12 +432,16 @@ class RaggedGenerator:
         return nxt
 
     def _fingerprint(self) -> tuple:
-        """What a recorded decode step holds by address: every parameter
-        (storage and version: load_state_dict, an optimizer step or .to()
-        change one of them) and each layer's state and conv-cache buffers.  A
+        """What a recorded decode step holds by address: every parameter and every 4-bit
+        weight, of whatever module (storage and version: load_state_dict, an optimizer step or .to()
+        change one of them), and each layer's state and conv-cache buffers.  A
         replay is valid only while the addresses are unchanged."""
-        quantized = getattr(self.model, '_quantized', list)()       # a model of the caller's own has none
-        key = [(p.data_ptr(), 0 if p.is_inference() else p._version) for p in (*self.model.parameters(), *quantized)]
+        key, todo = [], [self.model]
+        while todo:                                   # the modules' own tables: twice as fast as parameters(), at every step
+            m = todo.pop()
+            todo += [c for c in m._modules.values() if c is not None]
+            held = (*m._parameters.values(), *m._buffers.values()) if isinstance(m, MXLinear) else m._parameters.values()
+            key += [(t.data_ptr(), 0 if t.is_inference() else t._version) for t in held if t is not None]
         for blk in self.model.blocks:
             att = blk.att
             key += [(t.data_ptr(), t.dtype) for t in (att.state,) + (att._caches() if att.short_conv_size else ())]
