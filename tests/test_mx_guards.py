@@ -7,8 +7,9 @@ import pytest
 import torch
 from torch import nn
 
+from oracle import mx
 from vagus_amd import ops
-from vagus_amd.layer import MXLinear
+from vagus_amd.layer import GatedDeltaNet, MXLinear
 from vagus_amd.model import GDNLM, RaggedGenerator
 
 DEV = 'cuda'
@@ -17,6 +18,16 @@ gpu = pytest.mark.gpu
 
 def case(*what):
     print('\n[case]', *what, flush=True)
+
+
+def rel(a, b):
+    return float((a.double() - b.double()).norm() / b.double().norm())
+
+
+def round_(linear):
+    """The weights that 4 bits leave of linear, in place."""
+    with torch.no_grad():
+        linear.weight.copy_(mx.rounded(linear.weight.double(), 4))
 
 
 def blank(n, k, gated=False, device='cpu'):
@@ -108,3 +119,57 @@ def test_a_model_class_of_the_callers_own_is_recorded_again_when_its_4_bit_weigh
     torch.cuda.synchronize()
     want = run(RaggedGenerator(other), graph=False)
     assert torch.equal(run(gen), want)
+
+
+# --- layers of other classes -------------------------------------------------------------
+
+
+class OwnGates(GatedDeltaNet):
+    """_gates as the class documents it to its callers, without the projections that a grouped product hands on."""
+
+    def _gates(self, x, *, raw_gate=False, raw_beta=False):
+        g, beta = super()._gates(x, raw_gate=raw_gate, raw_beta=raw_beta)
+        return (g if raw_gate else 0.5 * g), beta
+
+
+class OwnOutput(GatedDeltaNet):
+    def _output(self, o, x):
+        return self.wo(o.reshape(*x.shape[:2], -1) * torch.sigmoid(self.wg(x)))
+
+
+def test_a_layer_with_an_output_of_its_own_keeps_its_weights():
+    layer = OwnOutput(dim=64, head_count=1, key_head_dim=64, value_head_dim=64, gate='scalar')
+    with pytest.raises(NotImplementedError, match='_output'):
+        layer.quantize_weights_()
+    m = small()
+    m.blocks[1].att = layer
+    with pytest.raises(NotImplementedError, match='_output'):
+        m.quantize_weights_()
+    assert isinstance(layer.wq, nn.Linear) and isinstance(m.blocks[0].att.wq, nn.Linear)
+
+
+@gpu
+@pytest.mark.parametrize('gate', ['scalar', 'vector'])
+def test_gates_of_a_subclass_take_the_input_alone(gate):
+    case('a subclass whose _gates has no proj: every call of a 4-bit layer', gate)
+    torch.manual_seed(3)
+    with torch.device(DEV):
+        layer = OwnGates(dim=128, head_count=2, key_head_dim=64, value_head_dim=64, gate=gate)
+    want = copy.deepcopy(layer)
+    for n in ('wq', 'wk', 'wv', 'wg', 'wo'):
+        round_(getattr(want, n))
+    layer.quantize_weights_()
+    x = torch.randn(2, 40, 128, device=DEV)
+    cu = torch.tensor([0, 9, 40], dtype=torch.int32, device=DEV)
+    with torch.no_grad():                                     # fp32 sums in other orders: as tests/test_mx_model.py
+        assert rel(layer(x), want(x)) < 1e-4
+    for m in (layer, want):
+        m.reset_cache(2)
+    assert rel(layer.prefill_packed(x[:1], cu), want.prefill_packed(x[:1], cu)) < 1e-4
+    for a, b in ((0, 1), (1, 9), (9, 10)):
+        assert rel(layer.decode_step(x[:, a:b]), want.decode_step(x[:, a:b])) < 1e-4
+    for m in (layer, want):
+        m.begin_drafts(4)
+    none = torch.zeros(2, dtype=torch.int32, device=DEV)
+    assert rel(layer.draft_step(x[:, 10:14], none), want.draft_step(x[:, 10:14], none)) < 1e-4
+    assert rel(layer.state, want.state) < 1e-4

@@ -337,6 +337,8 @@ class GatedDeltaNet(nn.Module):
         """Refuses what quantize_weights_ does not stand for."""
         if hasattr(self, 'w_in'):
             return
+        if type(self)._output is not GatedDeltaNet._output:
+            raise NotImplementedError('4-bit projections feed this class\'s _output: a layer with one of its own may call W_g and W_o itself')
         mods = [self.wq, self.wk, self.wv, self.wg] + ([self.wo] if self.out_proj else [])
         if not all(_plain_module(m, nn.Linear) and m.bias is None for m in mods):
             raise NotImplementedError('4-bit weights stand for plain bias-free nn.Linear projections')
@@ -377,13 +379,13 @@ class GatedDeltaNet(nn.Module):
         projections of x already formed, by name."""
         g = beta = None
         H, dk = self.head_count, self.key_head_dim
-        out = lambda n: proj[n] if proj and n in proj else getattr(self, n)(x)  # noqa: E731
+        out = lambda n: proj[n] if proj else getattr(self, n)(x)  # noqa: E731
         if self.gate == 'scalar':
             assert not raw_gate, 'the fused gate activation is KDA-only (vector gate)'
             g = -self.A_log.float().exp() * F.softplus(out('wa').float() + self.dt_bias.float())
         elif self.gate == 'vector':
             B, L = x.shape[0], x.shape[1]
-            f = ops.projections(proj['wa1'], self.wa2.weight)[0] if proj and 'wa1' in proj else self.wa2(self.wa1(x))
+            f = ops.projections(proj['wa1'], self.wa2.weight)[0] if proj else self.wa2(self.wa1(x))
             if raw_gate:
                 g = f.view(B, L, H, dk)
             elif self.gate_lower_bound is not None:
@@ -477,11 +479,11 @@ class GatedDeltaNet(nn.Module):
         qp, kp, vp = (y[n] if y else getattr(self, n)(x) for n in ('wq', 'wk', 'wv'))
         on = self._active_fusions(qp)
         q, k, v = self._heads(qp, kp, vp, l2norm='l2norm' not in on)
-        kw = dict(proj=y) if y else {}
-        g, beta = self._gates(x, raw_gate='gate' in on, raw_beta='beta' in on, **kw)
+        # the gates' projections are never 4-bit: a _gates of a subclass takes x alone
+        g, beta = self._gates(x, raw_gate='gate' in on, raw_beta='beta' in on, **(dict(proj=y) if grouped else {}))
         beta, w = self._write(x, k, g, beta)
         o, _ = self._scan(q, k, v, g, beta, None, fusions=on, w=w)
-        return self._output(o, x, **kw)
+        return self._output(o, x, **(dict(proj=y) if y else {}))
 
     # --- streaming ---------------------------------------------------------
 
@@ -604,7 +606,7 @@ class GatedDeltaNet(nn.Module):
             at += n
         if type(self)._gates is not GatedDeltaNet._gates:
             g, beta = self._gates(x, raw_gate=self.gate == 'vector', raw_beta=self.delta)
-            return *out, g, beta, None
+            return *out, g, beta if self.delta else None, None
         if scalar:                                              # the decode kernel forms both
             wb = self.wb.weight if hasattr(self, 'wb') else None
             if all(_plain_module(m, nn.Linear) and m.bias is None and m.weight.dtype == x.dtype
