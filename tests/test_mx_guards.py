@@ -10,7 +10,7 @@ from torch import nn
 from oracle import mx
 from vagus_amd import ops
 from vagus_amd.layer import GatedDeltaNet, MXLinear
-from vagus_amd.model import GDNLM, RaggedGenerator
+from vagus_amd.model import FFN, GDNLM, RaggedGenerator
 
 DEV = 'cuda'
 gpu = pytest.mark.gpu
@@ -173,3 +173,26 @@ def test_gates_of_a_subclass_take_the_input_alone(gate):
     none = torch.zeros(2, dtype=torch.int32, device=DEV)
     assert rel(layer.draft_step(x[:, 10:14], none), want.draft_step(x[:, 10:14], none)) < 1e-4
     assert rel(layer.state, want.state) < 1e-4
+
+
+# --- FFNs of other classes ------------------------------------------------------------------
+
+
+class OwnFFN(FFN):
+    def forward(self, x):
+        return 0.5 * super().forward(x)
+
+
+def test_an_ffn_with_a_forward_or_an_activation_of_its_own_keeps_its_weights():
+    one, gelu, patched, hooked = OwnFFN(64, 128), FFN(64, 128), FFN(64, 128), FFN(64, 128)
+    gelu.silu = nn.GELU()
+    patched.forward = lambda x: x
+    hooked.silu.register_forward_hook(lambda *a: None)
+    for ffn in (one, gelu, patched, hooked):
+        with pytest.raises(NotImplementedError, match='of its own'):
+            ffn.quantize_weights_()
+        m = small()
+        m.blocks[1].ffn = ffn
+        with pytest.raises(NotImplementedError, match='of its own'):
+            m.quantize_weights_()
+        assert isinstance(ffn.l1, nn.Linear) and isinstance(m.blocks[0].ffn.l1, nn.Linear)

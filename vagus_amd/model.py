@@ -107,7 +107,11 @@ class FFN(nn.Module):
 
     def _check_4bit(self) -> None:
         """Refuses what quantize_weights_ does not stand for."""
-        if not isinstance(self.l1, MXLinear) and not all(_plain_module(m, nn.Linear) and m.bias is None for m in (self.l1, self.l2)):
+        if isinstance(self.l1, MXLinear):
+            return
+        if type(self).forward is not FFN.forward or 'forward' in self.__dict__ or not _plain_module(self.silu, nn.SiLU):
+            raise NotImplementedError('the 4-bit products form SwiGLU: an FFN with a forward or an activation of its own keeps its weights')
+        if not all(_plain_module(m, nn.Linear) and m.bias is None for m in (self.l1, self.l2)):
             raise NotImplementedError('4-bit weights stand for plain bias-free nn.Linear projections')
 
     def forward(self, x):
