@@ -196,3 +196,82 @@ def test_an_ffn_with_a_forward_or_an_activation_of_its_own_keeps_its_weights():
         with pytest.raises(NotImplementedError, match='of its own'):
             m.quantize_weights_()
         assert isinstance(ffn.l1, nn.Linear) and isinstance(m.blocks[0].ffn.l1, nn.Linear)
+
+
+# --- hooks on 4-bit maps ----------------------------------------------------------------------
+
+
+def quantised_on_the_cpu(m):
+    """m with maps of zeros in the places of its projections, as quantize_weights_ leaves it."""
+    for blk in m.blocks:
+        a, f = blk.att, blk.ffn
+        wide = sum(w.weight.shape[0] for w in (a.wq, a.wk, a.wv, a.wg))
+        del a.wq, a.wk, a.wv, a.wg
+        a.w_in, a.wo = blank(wide, a.dim), blank(a.dim, a.out_width)
+        f.l1, f.l2 = blank(2 * f.hidden_dim, f.dim, True), blank(f.dim, f.hidden_dim)
+    return m
+
+
+@pytest.mark.parametrize('which', ['att.w_in', 'att.wo', 'ffn.l1', 'ffn.l2', 'ffn'])
+def test_a_hooked_map_takes_no_8_bit_rows(which):
+    m = quantised_on_the_cpu(small())
+    assert all(blk._takes8() for blk in m.blocks)
+    for register in ('register_forward_hook', 'register_forward_pre_hook'):
+        handle = getattr(m.blocks[1].get_submodule(which), register)(lambda *a: None)
+        assert m.blocks[0]._takes8() and not m.blocks[1]._takes8()
+        handle.remove()
+        assert m.blocks[1]._takes8()
+    handle = nn.modules.module.register_module_forward_hook(lambda *a: None)
+    assert not m.blocks[0]._takes8()
+    handle.remove()
+
+
+@gpu
+@pytest.mark.parametrize('dtype, bar', [(torch.float32, 1e-4), (torch.bfloat16, 2e-2)])       # as tests/test_mx_model.py
+def test_hooks_on_4_bit_maps_run_on_every_call(dtype, bar):
+    case('hooks that scale what each map gives: forward, prompts, steps, drafts', dtype)
+    m = small(DEV, dim=256, head_count=2, value_head_dim=128).to(dtype).eval()
+    m.head.weight = nn.Parameter(m.head.weight.detach().clone())
+    want = copy.deepcopy(m)
+    for blk in want.blocks:
+        for lin in (blk.att.wq, blk.att.wk, blk.att.wv, blk.att.wg, blk.att.wo, blk.ffn.l1, blk.ffn.l2):
+            round_(lin)
+        for n in ('wq', 'wk', 'wv', 'wg'):
+            getattr(blk.att, n).register_forward_hook(lambda m_, a, o: 2 * o)
+        blk.att.wo.register_forward_hook(lambda m_, a, o: -o)
+        blk.ffn.l2.register_forward_pre_hook(lambda m_, a: (4 * a[0],))
+        blk.ffn.l2.register_forward_hook(lambda m_, a, o: 0.5 * o)
+    round_(want.head)
+    m.quantize_weights_()
+    seen = []
+
+    def hook(name, scale):
+        def f(mod, args, out):
+            assert torch.is_tensor(args[0]) and args[0].dtype is dtype
+            seen.append(name)
+            out = scale * out
+            return out.transpose(-1, -2).contiguous().transpose(-1, -2) if name == 'w_in' else out      # any view of it
+        return f
+    for blk in m.blocks:
+        for mod, name, scale in ((blk.att.w_in, 'w_in', 2), (blk.att.wo, 'wo', -1), (blk.ffn.l1, 'l1', 4), (blk.ffn.l2, 'l2', 0.5)):
+            mod.register_forward_hook(hook(name, scale))
+
+    def both(f):
+        seen.clear()
+        got = f(m)
+        torch.cuda.synchronize()
+        assert seen == 2 * ['w_in', 'wo', 'l1', 'l2'], seen
+        assert rel(got, f(want)) < bar
+    ids = torch.arange(40, device=DEV) % 50
+    cu = torch.tensor([0, 30, 40], dtype=torch.int32, device=DEV)
+    with torch.no_grad():
+        both(lambda k: k(ids.view(2, 20)))
+    for k in (m, want):
+        k.reset_cache(2)
+    both(lambda k: k.prefill_packed(ids, cu))
+    both(lambda k: k.decode_step(ids.view(2, 20)[:, :1]))
+    both(lambda k: k.decode_step(ids.view(2, 20)[:, :7]))
+    for k in (m, want):
+        k.begin_drafts(4)
+    none = torch.zeros(2, dtype=torch.int32, device=DEV)
+    both(lambda k: k.draft_step(ids.view(2, 20)[:, :4], none))

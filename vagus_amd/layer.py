@@ -65,19 +65,24 @@ def _autograd(*ts) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
+def _hooked(m) -> bool:
+    """Whether m's call is more than its class's forward."""
+    return bool('forward' in m.__dict__ or m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks
+                or nn.modules.module._has_any_global_hook())
+
+
 def _plain_module(m, cls) -> bool:
     """Whether m is a cls whose call is its forward alone: no subclass
     (parametrisations make one) and no hooks that a kernel in its place would
     pass by."""
-    return (type(m) is cls and 'forward' not in m.__dict__ and not (
-        m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks
-        or nn.modules.module._has_any_global_hook()))
+    return type(m) is cls and not _hooked(m)
 
 
 class MXLinear(nn.Module):
     """A bias-free linear map whose weights are 4-bit numbers with a scale for each 32 (ops.MXWeight), as buffers: what
-    serving reads a quarter of.  gated: the FFN's input projection, its two halves' tiles by turns
-    (ops.mx_swiglu).  No autograd.  The reference has no quantised layers."""
+    serving reads a quarter of.  gated: the FFN's input projection, its two halves' tiles by turns, whose call gives the
+    activations (ops.mx_swiglu).  No autograd.  Maps with hooks are called as modules, with 16- or 32-bit rows; of plain ones the layers
+    may take parts or feed 8-bit rows instead (_plain_module).  The reference has no quantised layers."""
 
     def __init__(self, weight: ops.MXWeight):
         super().__init__()
@@ -96,7 +101,7 @@ class MXLinear(nn.Module):
         return ops.MXWeight(self.values[t], self.scales[t], (n, self.shape[1]))
 
     def forward(self, x):
-        return ops.mx_linear(x, self.weight)
+        return ops.mx_swiglu(x, self.weight) if self.gated else ops.mx_linear(x, self.weight)
 
     def extra_repr(self) -> str:
         return f'{self.shape[1]}, {self.shape[0]}' + (', gated' if self.gated else '')
@@ -349,8 +354,11 @@ class GatedDeltaNet(nn.Module):
         """q, k, v and the output gate of 4-bit projections, each a tensor of its own; x8: x as 8-bit rows, which then
         meet the weights in its place."""
         H, dk, dv = self.head_count, self.key_head_dim, self.value_head_dim
+        names, widths = ('wq', 'wk', 'wv', 'wg'), (H * dk, H * dk, H * dv, H * dv)
+        if not _plain_module(self.w_in, MXLinear):              # its own call
+            return {n: t.contiguous() for n, t in zip(names, self.w_in(x).split(widths, dim=-1))}
         y, at = {}, 0
-        for n, width in zip(('wq', 'wk', 'wv', 'wg'), (H * dk, H * dk, H * dv, H * dv)):
+        for n, width in zip(names, widths):
             y[n] = ops.mx_linear(x if x8 is None else x8, self.w_in.rows(at, width), out_dtype=x.dtype)
             at += width
         return y
@@ -461,7 +469,7 @@ class GatedDeltaNet(nn.Module):
             o = ops.rms_norm_gated(o.to(gate.dtype), gate, self.o_norm.gamma, eps=self.o_norm.eps).reshape(B, L, -1)
         if not self.out_proj:
             return o
-        if rows8:
+        if rows8 and _plain_module(self.wo, MXLinear):
             return ops.mx_linear(ops.mx_quantize(o), self.wo.weight, out_dtype=o.dtype)
         return ops.projections(o, self.wo.weight)[0] if proj and not hasattr(self, 'w_in') else self.wo(o)
 
@@ -599,7 +607,7 @@ class GatedDeltaNet(nn.Module):
         """_decode_inputs with 4-bit projections: q, k, v and the output gate are one product's column blocks."""
         B = x.shape[0]
         H, dk, dv = self.head_count, self.key_head_dim, self.value_head_dim
-        y = self.w_in(x.reshape(B, -1))
+        y = self.w_in(x.reshape(B, -1)).contiguous()           # a hook may have returned any view
         ld, out, at = y.shape[1], [], y.storage_offset()
         for n in (H * dk, H * dk, H * dv, H * dv):
             out.append(y.as_strided((B, 1, n), (ld, n, 1), at))

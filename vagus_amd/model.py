@@ -36,7 +36,7 @@ import torch
 from torch import nn
 
 from . import ops
-from .layer import GatedDeltaNet, MXLinear, RMSNorm, _plain_module
+from .layer import GatedDeltaNet, MXLinear, RMSNorm, _hooked, _plain_module
 
 
 def _add_norm(norm: RMSNorm, x, delta=None, *, inplace: bool = False):
@@ -116,7 +116,7 @@ class FFN(nn.Module):
 
     def forward(self, x):
         if isinstance(self.l1, MXLinear):
-            return self.l2(ops.mx_swiglu(x, self.l1.weight))
+            return self.l2(self.l1(x))
         x1, xgate = torch.chunk(self.l1(x), 2, dim=-1)
         return self.l2(self.silu(x1) * xgate)
 
@@ -158,6 +158,14 @@ class Block(nn.Module):
         _, h = _add_norm(self.rmsnorm1, x)
         x, h = _add_norm(self.rmsnorm2, x, self.att.prefill_packed(h, cu_seqlens, rows=rows))
         return x + _ffn(self.ffn, h)
+
+    def _takes8(self) -> bool:
+        """Whether the block's products may take 8-bit rows: its 4-bit maps are plain modules, as quantize_weights_ made them.  With
+        hooks or other modules in their places a prompt's rows stay as they are, and the modules are called."""
+        a, f = self.att, self.ffn
+        return (type(f).forward is FFN.forward and not _hooked(f) and _plain_module(getattr(a, 'w_in', None), MXLinear)
+                and (not a.out_proj or _plain_module(a.wo, MXLinear))
+                and _plain_module(f.l1, MXLinear) and f.l1.gated and _plain_module(f.l2, MXLinear))
 
     def _stream8(self, x, delta, cu_seqlens, rows):
         """_stream over packed prompts with 4-bit weights whose rows are 8-bit: both norms give them, and the mixer's
@@ -348,7 +356,7 @@ class GDNLM(nn.Module):
         delta = None
         for blk in self.blocks:
             if (getattr(self, 'prompt_bits', 16) == 8 and x.dtype in (torch.bfloat16, torch.float16)
-                    and blk.rmsnorm1.gamma.dtype == x.dtype == blk.rmsnorm2.gamma.dtype):
+                    and blk.rmsnorm1.gamma.dtype == x.dtype == blk.rmsnorm2.gamma.dtype and blk._takes8()):
                 x, delta = blk._stream8(x, delta, cu_seqlens, rows)
             else:
                 x, delta = blk._stream(x, delta, lambda h, blk=blk: blk.att.prefill_packed(h, cu_seqlens, rows=rows))
