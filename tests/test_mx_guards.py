@@ -10,7 +10,7 @@ from torch import nn
 from oracle import mx
 from vagus_amd import ops
 from vagus_amd.layer import GatedDeltaNet, MXLinear
-from vagus_amd.model import FFN, GDNLM, RaggedGenerator
+from vagus_amd.model import FFN, GDNLM, RaggedGenerator, _ffn
 
 DEV = 'cuda'
 gpu = pytest.mark.gpu
@@ -196,6 +196,29 @@ def test_an_ffn_with_a_forward_or_an_activation_of_its_own_keeps_its_weights():
         with pytest.raises(NotImplementedError, match='of its own'):
             m.quantize_weights_()
         assert isinstance(ffn.l1, nn.Linear) and isinstance(m.blocks[0].ffn.l1, nn.Linear)
+
+
+@gpu
+@pytest.mark.parametrize('four_bits', [False, True])
+@pytest.mark.parametrize('what', ['identity', 'own forward', 'activation', 'hook'])
+def test_other_modules_in_the_place_of_an_ffn_run_on_the_gpu(what, four_bits):
+    case('another module than the FFN that the fused pass stands for', what, four_bits)
+    m = small(DEV, value_head_dim=128, dim=128).to(torch.bfloat16)
+    if four_bits:
+        m.quantize_weights_()
+    with torch.device(DEV):
+        ffn = nn.Identity() if what == 'identity' else (OwnFFN if what == 'own forward' else FFN)(128, 256).to(torch.bfloat16)
+    if what == 'activation':
+        ffn.silu = nn.GELU()
+    if what == 'hook':
+        ffn.register_forward_hook(lambda mod, args, out: out + 1)
+    m.blocks[0].ffn = ffn
+    ids, cu = torch.arange(12, device=DEV), torch.tensor([0, 7, 12], dtype=torch.int32, device=DEV)
+    m.reset_cache(2)
+    assert bool(torch.isfinite(m.prefill_packed(ids, cu)).all()) and bool(torch.isfinite(m.decode_step(ids[:2, None])).all())
+    h = torch.randn(1, 5, 128, device=DEV).bfloat16()
+    with torch.no_grad():
+        assert torch.equal(_ffn(ffn, h), ffn(h))
 
 
 # --- hooks on 4-bit maps ----------------------------------------------------------------------

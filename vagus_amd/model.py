@@ -75,10 +75,9 @@ def _ffn(ffn: 'FFN', h, dtype=None):
     activations between the two products, and dtype is the result's."""
     if isinstance(h, ops.MXRows):
         return ops.mx_linear(ops.mx_swiglu(h, ffn.l1.weight, quantize=True), ffn.l2.weight, out_dtype=dtype)
-    if isinstance(getattr(ffn, 'l1', None), MXLinear):
-        return ffn(h)
     if (h.is_cuda and not torch.is_grad_enabled() and h.dtype in (torch.bfloat16, torch.float16, torch.float32)
-            and ffn.hidden_dim % (16 // h.element_size()) == 0):
+            and type(ffn).forward is FFN.forward and not _hooked(ffn) and _plain_module(ffn._modules.get('silu'), nn.SiLU)
+            and not isinstance(ffn._modules.get('l1'), MXLinear) and ffn.hidden_dim % (16 // h.element_size()) == 0):
         return ffn.l2(ops.swiglu(ffn.l1(h)))
     return ffn(h)
 
