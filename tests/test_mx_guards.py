@@ -298,3 +298,50 @@ def test_hooks_on_4_bit_maps_run_on_every_call(dtype, bar):
         k.begin_drafts(4)
     none = torch.zeros(2, dtype=torch.int32, device=DEV)
     both(lambda k: k.draft_step(ids.view(2, 20)[:, :4], none))
+
+
+# --- all of a model or nothing ------------------------------------------------------------------
+
+
+def held(m):
+    return {n: t.data_ptr() for n, t in m.state_dict(keep_vars=True).items()}, [type(c) for c in m.modules()]
+
+
+@pytest.mark.parametrize('good', [0, 1, 2, 3, 5, 7, 8])
+def test_a_model_that_cannot_be_quantised_stays_as_it_was(monkeypatch, good):
+    m = small()
+    before = held(m)
+    calls = []
+
+    def mx_weight(w, gated=False):
+        calls.append(w.shape)
+        if len(calls) > good:
+            raise RuntimeError('no room')
+        return blank(*w.shape, gated).weight
+    monkeypatch.setattr(ops, 'mx_weight', mx_weight)
+    with pytest.raises(RuntimeError, match='no room'):
+        m.quantize_weights_()
+    assert held(m) == before
+    good = 100
+    calls.clear()
+    m.quantize_weights_()                                     # two blocks of four maps, the head
+    assert len(calls) == 9 and len(m._quantized()) == 18 and all(blk._takes8() for blk in m.blocks)
+
+
+@gpu
+@pytest.mark.parametrize('what', ['cpu', 'fp64', 'head'])
+def test_a_model_with_a_later_part_elsewhere_stays_as_it_was(what):
+    case('quantize_weights_ of a model with a part on the CPU or in fp64', what)
+    m = small(DEV, value_head_dim=128, dim=128)
+    part = m.blocks[1].ffn.l2 if what != 'head' else m.head
+    if what == 'head':
+        part.weight = nn.Parameter(part.weight.detach().clone())
+    part.to('cpu' if what != 'fp64' else torch.float64)
+    before = held(m)
+    with pytest.raises(NotImplementedError if what == 'fp64' else RuntimeError):
+        m.quantize_weights_()
+    assert held(m) == before
+    part.to(DEV, torch.float32)
+    m.quantize_weights_()
+    m.reset_cache(2)
+    assert bool(torch.isfinite(m.decode_step(torch.ones(2, 1, dtype=torch.int64, device=DEV))).all())

@@ -331,12 +331,20 @@ class GatedDeltaNet(nn.Module):
         if hasattr(self, 'w_in'):
             return
         self._check_4bit()
-        w_in = MXLinear(ops.mx_weight(torch.cat([m.weight.detach() for m in (self.wq, self.wk, self.wv, self.wg)])))
-        wo = MXLinear(ops.mx_weight(self.wo.weight)) if self.out_proj else None
-        del self.wq, self.wk, self.wv, self.wg
-        self.w_in = w_in
-        if wo is not None:
-            self.wo = wo
+        self._take_4bit(self._made_4bit())
+
+    def _made_4bit(self) -> dict:
+        """The 4-bit maps of this layer, by name; the layer as it was.  Empty if it has them."""
+        if hasattr(self, 'w_in'):
+            return {}
+        w_in = torch.cat([m.weight.detach() for m in (self.wq, self.wk, self.wv, self.wg)])
+        return dict(w_in=MXLinear(ops.mx_weight(w_in)), **(dict(wo=MXLinear(ops.mx_weight(self.wo.weight))) if self.out_proj else {}))
+
+    def _take_4bit(self, made: dict) -> None:
+        if made:
+            del self.wq, self.wk, self.wv, self.wg
+        for name, m in made.items():
+            setattr(self, name, m)
 
     def _check_4bit(self) -> None:
         """Refuses what quantize_weights_ does not stand for."""

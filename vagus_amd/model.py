@@ -102,7 +102,17 @@ class FFN(nn.Module):
         if isinstance(self.l1, MXLinear):
             return
         self._check_4bit()
-        self.l1, self.l2 = MXLinear(ops.mx_weight(self.l1.weight, gated=True)), MXLinear(ops.mx_weight(self.l2.weight))
+        self._take_4bit(self._made_4bit())
+
+    def _made_4bit(self) -> dict:
+        """The 4-bit maps of this FFN, by name; the FFN as it was.  Empty if it has them."""
+        if isinstance(self.l1, MXLinear):
+            return {}
+        return dict(l1=MXLinear(ops.mx_weight(self.l1.weight, gated=True)), l2=MXLinear(ops.mx_weight(self.l2.weight)))
+
+    def _take_4bit(self, made: dict) -> None:
+        for name, m in made.items():
+            setattr(self, name, m)
 
     def _check_4bit(self) -> None:
         """Refuses what quantize_weights_ does not stand for."""
@@ -275,14 +285,16 @@ class GDNLM(nn.Module):
         assert prompt_bits in (8, 16), f'prompt_bits must be 8 or 16; got {prompt_bits}'
         if head and not isinstance(self.head, MXLinear) and not (_plain_module(self.head, nn.Linear) and self.head.bias is None):
             raise NotImplementedError('4-bit weights stand for a plain bias-free nn.Linear head')
-        for blk in self.blocks:                       # all of it or nothing
-            blk.att._check_4bit()
-            blk.ffn._check_4bit()
-        for blk in self.blocks:
-            blk.att.quantize_weights_()
-            blk.ffn.quantize_weights_()
+        # all of it or nothing: what cannot be quantised (of another device or type, or for want of memory) raises before
+        # anything changes, for which the model holds its weights beside the 4-bit ones until all of these are there
+        parts = [part for blk in self.blocks for part in (blk.att, blk.ffn)]
+        for part in parts:
+            part._check_4bit()
+        made = [part._made_4bit() for part in parts]
         if head and not isinstance(self.head, MXLinear):
             self.head = MXLinear(ops.mx_weight(self.head.weight))
+        for part, maps in zip(parts, made):
+            part._take_4bit(maps)
         # mx_rms_norm's rows: multiples of 8
         self.prompt_bits = prompt_bits if self.config['dim'] % 8 == 0 and self.config['dim'] <= 16384 else 16
         return self
