@@ -221,6 +221,15 @@ def test_other_modules_in_the_place_of_an_ffn_run_on_the_gpu(what, four_bits):
         assert torch.equal(_ffn(ffn, h), ffn(h))
 
 
+@pytest.mark.parametrize('where', ['ffn', 'att'])
+def test_blocks_of_other_modules_are_refused_as_such(where):
+    m = small()
+    setattr(m.blocks[1], where, nn.Identity())
+    with pytest.raises(NotImplementedError, match='Identity'):
+        m.quantize_weights_()
+    assert isinstance(m.blocks[0].ffn.l1, nn.Linear)
+
+
 # --- hooks on 4-bit maps ----------------------------------------------------------------------
 
 

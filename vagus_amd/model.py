@@ -289,6 +289,8 @@ class GDNLM(nn.Module):
         # anything changes, for which the model holds its weights beside the 4-bit ones until all of these are there
         parts = [part for blk in self.blocks for part in (blk.att, blk.ffn)]
         for part in parts:
+            if not isinstance(part, (GatedDeltaNet, FFN)):
+                raise NotImplementedError(f'4-bit weights are for blocks of a GatedDeltaNet and an FFN; got a {type(part).__name__}')
             part._check_4bit()
         made = [part._made_4bit() for part in parts]
         if head and not isinstance(self.head, MXLinear):
