@@ -102,3 +102,17 @@ def test_a_kernel(kind, gated, R, K, n):
         rows_within(rows, want, err)
         again = f(x, w, quantize=True)
         assert torch.equal(again.values.view(torch.uint8), rows.values.view(torch.uint8)) and torch.equal(again.scales, rows.scales)
+
+
+@gpu
+@pytest.mark.parametrize('kind', ['bf16', 'fp16', 'fp32'])
+@pytest.mark.parametrize('R, K, h', [(3, 256, 384), (70, 640, 1024), (300, 256, 4096), (600, 200, 8192)])
+def test_8_bit_results_of_exact_rows_are_the_fp32_result_rounded(R, K, h, kind):
+    case('mx_swiglu to 8 bits against mx_quantize of its fp32 result', kind, R, K, h)
+    # whole 128s of columns: one kernel for both, one order of the sums
+    assert kernel_of(kind, True, True, R, K, 2 * h) == kernel_of(kind, True, False, R, K, 2 * h)
+    x, _ = rows_of(kind, R, K, R + K)
+    w = ops.mx_weight(randn(2 * h, K, seed=h) * 0.2, gated=True)
+    got, want = ops.mx_swiglu(x, w, quantize=True), ops.mx_quantize(ops.mx_swiglu(x, w, out_dtype=FS))
+    assert torch.equal(got.scales, want.scales)
+    assert torch.equal(got.values.view(torch.uint8), want.values.view(torch.uint8))

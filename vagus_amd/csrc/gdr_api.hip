@@ -1281,6 +1281,7 @@ int vgdr_mx_linear(int x_dtype, const void *x, int64_t ldx, const void *x_scales
     p.rows = rows;
     p.out = out_dtype;
     p.gated = gated != 0;
+    p.accurate = out_dtype == VGDR_F32 || (y8 && !x8);
     return hip_status(vgdr::mx_linear(p, stream), "vgdr_mx_linear launch");
 }
 

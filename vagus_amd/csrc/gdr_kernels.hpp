@@ -455,7 +455,7 @@ struct MxLinear {
     uint8_t *y_scales;
     int64_t rows, ldx;
     int x_type, planes, T, C, K, N, out;              // N: the output's columns; K: x's (planes: 128 C)
-    bool gated;
+    bool gated, accurate;         // accurate: the activation by expf and a division
 };
 hipError_t mx_linear(const MxLinear &p, hipStream_t stream);
 
