@@ -354,3 +354,33 @@ def test_a_model_with_a_later_part_elsewhere_stays_as_it_was(what):
     m.quantize_weights_()
     m.reset_cache(2)
     assert bool(torch.isfinite(m.decode_step(torch.ones(2, 1, dtype=torch.int64, device=DEV))).all())
+
+
+# --- layers that are not 4-bit ---------------------------------------------------------------------
+
+
+@gpu
+def test_a_layer_that_is_not_4_bit_searches_for_no_4_bit_map():
+    case('attributes that the calls of an ordinary layer look for in vain')
+    missed = []
+
+    class Watched(GatedDeltaNet):
+        def __getattr__(self, name):
+            try:
+                return super().__getattr__(name)
+            except AttributeError:
+                missed.append(name)
+                raise
+    with torch.device(DEV):
+        layer = Watched(dim=128, head_count=1, key_head_dim=64, value_head_dim=64, gate='scalar')
+    x = torch.randn(2, 8, 128, device=DEV)
+    layer(x).sum().backward()
+    layer.reset_cache(2)
+    with torch.no_grad():
+        layer(x)
+    layer.prefill_packed(x[:1], torch.tensor([0, 3, 8], dtype=torch.int32, device=DEV))
+    layer.decode_step(x[:, :1])
+    layer.decode_step(x)
+    layer.begin_drafts(4)
+    layer.draft_step(x[:, :4], torch.zeros(2, dtype=torch.int32, device=DEV))
+    assert 'w_in' not in missed, missed

@@ -328,14 +328,18 @@ class GatedDeltaNet(nn.Module):
         """W_q, W_k, W_v, W_g (as one map, w_in, whose rows they are) and W_o become 4-bit weights (MXLinear), in place and for
         good; what decides how the state decays and is written (W_a, W_b, the short conv, A_log, dt_bias) keeps
         its type.  For serving: forward, decode_step, draft_step and prefill_packed without autograd."""
-        if hasattr(self, 'w_in'):
+        if self._is_4bit:
             return
         self._check_4bit()
         self._take_4bit(self._made_4bit())
 
+    @property
+    def _is_4bit(self) -> bool:
+        return 'w_in' in self._modules                # its own table: a search for an attribute that is not there raises inside
+
     def _made_4bit(self) -> dict:
         """The 4-bit maps of this layer, by name; the layer as it was.  Empty if it has them."""
-        if hasattr(self, 'w_in'):
+        if self._is_4bit:
             return {}
         w_in = torch.cat([m.weight.detach() for m in (self.wq, self.wk, self.wv, self.wg)])
         return dict(w_in=MXLinear(ops.mx_weight(w_in)), **(dict(wo=MXLinear(ops.mx_weight(self.wo.weight))) if self.out_proj else {}))
@@ -348,7 +352,7 @@ class GatedDeltaNet(nn.Module):
 
     def _check_4bit(self) -> None:
         """Refuses what quantize_weights_ does not stand for."""
-        if hasattr(self, 'w_in'):
+        if self._is_4bit:
             return
         if type(self)._output is not GatedDeltaNet._output:
             raise NotImplementedError('4-bit projections feed this class\'s _output: a layer with one of its own may call W_g and W_o itself')
@@ -380,7 +384,7 @@ class GatedDeltaNet(nn.Module):
         """Whether the projections are plain bias-free nn.Linear modules (and the
         methods that call them this class's own), so that a grouped product may
         stand for their calls."""
-        if hasattr(self, 'w_in'):
+        if self._is_4bit:
             return False
         names = self._input_projections() + (('wa2',) if self.gate == 'vector' else ()) \
             + (('wo',) if self.out_proj else ())
@@ -479,7 +483,7 @@ class GatedDeltaNet(nn.Module):
             return o
         if rows8 and _plain_module(self.wo, MXLinear):
             return ops.mx_linear(ops.mx_quantize(o), self.wo.weight, out_dtype=o.dtype)
-        return ops.projections(o, self.wo.weight)[0] if proj and not hasattr(self, 'w_in') else self.wo(o)
+        return ops.projections(o, self.wo.weight)[0] if proj and not self._is_4bit else self.wo(o)
 
     # --- training / stateless --------------------------------------------
 
@@ -491,7 +495,7 @@ class GatedDeltaNet(nn.Module):
             names = self._input_projections()
             y = dict(zip(names, ops.projections(x, *(getattr(self, n).weight for n in names))))
         else:
-            y = self._project(x) if hasattr(self, 'w_in') else {}
+            y = self._project(x) if self._is_4bit else {}
         qp, kp, vp = (y[n] if y else getattr(self, n)(x) for n in ('wq', 'wk', 'wv'))
         on = self._active_fusions(qp)
         q, k, v = self._heads(qp, kp, vp, l2norm='l2norm' not in on)
@@ -574,7 +578,7 @@ class GatedDeltaNet(nn.Module):
         H, dk, dv = self.head_count, self.key_head_dim, self.value_head_dim
         vec, scalar = self.gate == 'vector', self.gate == 'scalar' and not raw_gate
         raw_gate = raw_gate and self.gate == 'scalar'
-        if hasattr(self, 'w_in'):
+        if self._is_4bit:
             return self._decode_inputs_4bit(x, scalar, raw_gate)
         names = self._input_projections()
         mods = [self._modules.get(n) for n in names]
@@ -662,7 +666,7 @@ class GatedDeltaNet(nn.Module):
             self.cache_len += L
             o = o.reshape(B, L, H * dv)
             return self.wo(o) if self.out_proj else o
-        y = self._project(x) if hasattr(self, 'w_in') else {}
+        y = self._project(x) if self._is_4bit else {}
         qp, kp, vp = (y[n] if y else getattr(self, n)(x) for n in ('wq', 'wk', 'wv'))
         if self.short_conv_size is not None:
             qp = self.conv_q(qp, 'silu', conv_cache=self.qp_cache)
@@ -751,8 +755,8 @@ class GatedDeltaNet(nn.Module):
         assert self.state.shape[0] > 0, 'No state allocated. Call reset_cache or load_cache first.'
         T = x.shape[1]
         H, dk, dv = self.head_count, self.key_head_dim, self.value_head_dim
-        assert x8 is None or hasattr(self, 'w_in'), '8-bit rows are for 4-bit weights (quantize_weights_)'
-        y = self._project(x, x8) if hasattr(self, 'w_in') else {}
+        assert x8 is None or self._is_4bit, '8-bit rows are for 4-bit weights (quantize_weights_)'
+        y = self._project(x, x8) if self._is_4bit else {}
         qp, kp, vp = (y[n] if y else getattr(self, n)(x) for n in ('wq', 'wk', 'wv'))
         on = self._active_fusions(qp)
         whole = rows == list(range(self.state.shape[0]))
