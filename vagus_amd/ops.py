@@ -2016,10 +2016,10 @@ def _blocks_of(n: int) -> int:
     return -(-n // 128)
 
 
-def _powers(scales):
-    """The scale bytes' numbers, fp32: 2^(b - 127), NaN for 255."""
+def _powers(scales, dtype=torch.float32):
+    """The scale bytes' numbers in dtype: 2^(b - 127), NaN for 255."""
     b = scales.to(torch.int32)
-    return torch.where(b == 255, float('nan'), (b << 23).view(torch.float32))
+    return torch.where(b == 255, float('nan'), (b << 23).view(torch.float32)).to(dtype)
 
 
 class MXRows:
@@ -2046,7 +2046,9 @@ class MXRows:
         return self.values.device
 
     def dequantize(self, dtype=torch.float32):
-        v = self.values.float().unflatten(-1, (-1, 32)) * _powers(self.scales)[..., None]
+        """The numbers that the bytes stand for, (..., size); in torch.float64 those above fp32's range too."""
+        wide = torch.promote_types(dtype, torch.float32)
+        v = self.values.to(wide).unflatten(-1, (-1, 32)) * _powers(self.scales, wide)[..., None]
         return v.flatten(-2)[..., :self.size].to(dtype)
 
 
@@ -2073,13 +2075,14 @@ class MXWeight:
         return self.values.device
 
     def dequantize(self, dtype=torch.float32):
-        """The numbers that the bytes stand for, (n, k)."""
+        """The numbers that the bytes stand for, (n, k); in torch.float64 those above fp32's range too."""
         n, k = self.shape
         T, C = self.values.shape[:2]
-        number = torch.tensor([0, .5, 1, 1.5, 2, 3, 4, 6], device=self.device)
+        wide = torch.promote_types(dtype, torch.float32)
+        number = torch.tensor([0, .5, 1, 1.5, 2, 3, 4, 6], dtype=wide, device=self.device)
         number = torch.cat([number, -number])
         code = torch.stack([self.values & 15, self.values >> 4], -1).flatten(-2)          # (T, C, 4, 16, 32)
-        s = _powers(self.scales).permute(0, 1, 4, 2, 3).flatten(1, 2)[:, :C]               # (T, C, 4, 16)
+        s = _powers(self.scales, wide).permute(0, 1, 4, 2, 3).flatten(1, 2)[:, :C]               # (T, C, 4, 16)
         w = (number[code.long()] * s[..., None]).permute(0, 3, 1, 2, 4).reshape(T, 16, 128 * C)[..., :k]
         if self.gated:
             w = w.unflatten(0, (-1, 2)).transpose(0, 1).reshape(2, -1, k)[:, :n // 2]
