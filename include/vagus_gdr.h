@@ -728,8 +728,8 @@ int vgdr_lookup_drafts(const void *history, int token_bytes, int64_t ld, int64_t
 /*
  * Block-scaled numbers: 32 consecutive elements of a row share a scale 2^(b - 127), held as the byte b in 1..254; b = 255:
  * the block had a NaN or an infinity, its values are NaN.  8-bit values are e4m3, 4-bit ones e2m1; the scale
- * is the smallest power of two (at least 2^-126) with amax <= 464 scale (8 bits) or 7 scale (4 bits), elements
- * are rounded to nearest, ties to even, and saturate at 448 and 6.
+ * is the smallest power of two (at least 2^-126; 4 bits: at most 2^125, so that every weight is finite) with amax <= 464 scale
+ * (8 bits) or 7 scale (4 bits), elements are rounded to nearest, ties to even, and saturate at 448 and 6.
  *
  * VGDR_MX8, beside the element types: rows in 8 bits, values [rows, 128 ceil(K / 128)] with bytes
  * [rows, 4 ceil(K / 128)]; padded columns are zeros with b = 1.

@@ -40,6 +40,8 @@ def quantize(x, bits):
     amax = v.abs().amax(-1)
     k = (exponent(amax) - exponent(torch.tensor(TOP[bits], dtype=torch.float64)).item()).clamp(min=-126)
     k = torch.where(amax > TOP[bits] * power(k), k + 1, k)
+    if bits == 4:
+        k = k.clamp(max=125)                                      # every number is finite in bf16
     q = nearest(v / power(k)[..., None], bits)
     q = torch.where(bad[..., None], float('nan'), q)
     return q.flatten(1), torch.where(bad, 255, k + 127).to(torch.uint8)

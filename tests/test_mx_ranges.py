@@ -27,3 +27,29 @@ def test_dequantize_in_64_bits_passes_the_range_of_fp32():
     values[0, 0, 0, 5, 1], scales[0, 0, 0, 5, 0] = 0xf6, 254                                # 4 and -6 times 2^127
     got = ops.MXWeight(values, scales, (16, 128)).dequantize(torch.float64)
     assert got[5, 2] == 2.0 ** 129 and got[5, 3] == -6 * 2.0 ** 127 and int((got != 0).sum()) == 2
+
+
+def test_the_oracles_largest_weights_are_finite_in_bf16():
+    w = torch.full((1, 32), torch.finfo(torch.float32).max)
+    assert torch.equal(mx.rounded(w, 4), torch.full((1, 32), 1.5 * 2.0 ** 127, dtype=torch.float64))
+    for v in (1.75 * 2.0 ** 127, 1.5 * 2.0 ** 127, 2.0 ** 126):           # the first is half a step above the largest
+        w[0, 0] = v
+        assert float(mx.rounded(w[:, :1], 4)) == min(v, 1.5 * 2.0 ** 127)
+
+
+@gpu
+@pytest.mark.parametrize('dt', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('R', [1, 40])
+def test_the_largest_weights(R, dt):
+    case('mx_weight of the largest numbers, products with rows of zeros and of small numbers', R, dt)
+    top = torch.finfo(dt).max
+    w = torch.zeros(32, 256, device=DEV)
+    w[0, 0], w[1, 40], w[2, 200], w[3, 5], w[3, 6] = top, -top, 1.75 * 2.0 ** 127, 1.5 * 2.0 ** 127, -2.0 ** 124
+    w = w.to(dt)
+    got = ops.mx_weight(w)
+    assert torch.equal(got.dequantize(torch.float64), mx.rounded(w, 4)) and bool(torch.isfinite(got.dequantize()).all())
+    x = torch.zeros(R, 256, device=DEV)
+    x[-1, [0, 40, 200, 5]] = 2.0 ** -100
+    want = x.double() @ mx.rounded(w, 4).t()                       # powers of two: nothing is rounded
+    for rows in (x, x.bfloat16(), ops.mx_quantize(x)):
+        assert torch.equal(ops.mx_linear(rows, got, out_dtype=torch.float32).double(), want)

@@ -6,7 +6,9 @@
 // s >= -126, with amax <= 464 2^s (8 bits) or 7 2^s (4 bits): half a step above the format's
 // largest value, so that the block's largest element is off by half a step at most, as every other; a scale
 // twice as large would cost all others a bit.  Elements are rounded to nearest, ties to even, the ends saturate.
-// s >= -126 keeps every scale and its inverse a normal fp32 number; a block of zeros has b = 1.
+// s >= -126 keeps every scale and its inverse a normal fp32 number; a block of zeros has b = 1.  4 bits: s <= 125, so that
+// every weight is a finite bf16 number (6 2^125 = 1.5 2^127, where what is larger ends): as 4 2^126 the largest
+// fp32 numbers would be infinities, and NaN to a row of zeros.
 //
 // Rows in 8 bits: values [rows, 128 ceil(K / 128)] and bytes [rows, 4 ceil(K / 128)]; the padding is zeros with b = 1.
 //
@@ -32,7 +34,7 @@ __device__ __forceinline__ int mx_scale(uint32_t amax) {
     constexpr int TOP = BITS == 8 ? 8 : 2;
     if (amax >= 0x7f800000u) return 255;
     const int b = (int)(amax >> 23) - TOP + ((amax & 0x7fffffu) > HALF ? 1 : 0);
-    return b < 1 ? 1 : b;
+    return b < 1 ? 1 : BITS == 4 && b > 252 ? 252 : b;
 }
 // 2^-(b - 127), for b in 1 .. 253
 __device__ __forceinline__ float mx_inverse(int b) { return __builtin_bit_cast(float, (uint32_t)(254 - b) << 23); }

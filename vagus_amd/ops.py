@@ -2132,7 +2132,7 @@ def mx_quantize(x) -> MXRows:
 
 def mx_weight(w, gated: bool = False) -> MXWeight:
     """w (n, k), fp32, bf16 or fp16, as 4-bit weights (vgdr_mx_weight): a scale for each 32 elements of a row, the smallest
-    power of two with amax <= 7 scale, elements rounded to nearest, ties to even.  gated: w is the FFN's input
+    power of two with amax <= 7 scale (and at most 2^125: larger numbers end at 1.5 2^127), elements rounded to nearest, ties to even.  gated: w is the FFN's input
     projection, its two halves' rows for mx_swiglu.  Done once, where the model is made ready to serve."""
     rows, ld = _mx_source('w', w.detach(), dims=2)
     n, k = w.shape
