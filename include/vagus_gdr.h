@@ -750,7 +750,7 @@ int vgdr_mx_quantize(int dtype, const void *x, int64_t ldx, void *values, void *
 /* Weights w [rows, cols] in dtype to 4 bits in the tiles' order; gated: rows is even. */
 int vgdr_mx_weight(int dtype, const void *w, int64_t ldw, void *values, void *scales, int64_t rows, int64_t cols, int gated,
                    hipStream_t stream);
-/* h = x + residual (rounded to dtype; residual NULL: h = x), written to x_out (may be NULL or x), and the norm
+/* h = x + residual (rounded to dtype; residual NULL: h = x), written to x_out (may be NULL, x or residual; else apart from both), and the norm
  * h rsqrt(mean h^2 + eps) gamma (infra/components/norm_layer.py:15-23) formed in 64 bits and rounded once, to
  * 8-bit rows; y (may be NULL): the norm in dtype with vgdr_rms_norm's roundings.  x, residual [rows, dim] dense; dim a
  * multiple of 8, at most 16384. */

@@ -8,7 +8,7 @@ import torch
 from torch import nn
 
 from oracle import mx
-from vagus_amd import ops
+from vagus_amd import _lib, ops
 from vagus_amd.layer import GatedDeltaNet, MXLinear
 from vagus_amd.model import FFN, GDNLM, RaggedGenerator, _ffn
 
@@ -384,3 +384,47 @@ def test_a_layer_that_is_not_4_bit_searches_for_no_4_bit_map():
     layer.begin_drafts(4)
     layer.draft_step(x[:, :4], torch.zeros(2, dtype=torch.int32, device=DEV))
     assert 'w_in' not in missed, missed
+
+
+# --- results that lie in what is read ----------------------------------------------------------------
+
+
+def test_a_norm_refuses_results_that_overlap():
+    """Every call here is refused before a launch: the addresses are none."""
+    L = _lib.load()
+
+    def n(**o):
+        a = dict(dt=1, x=1 << 20, r=2 << 20, xo=None, g=3 << 20, y=4 << 20, v=5 << 20, s=6 << 20, rows=4, dim=128) | o
+        return L.vgdr_mx_rms_norm(a['dt'], a['x'], a['r'], a['xo'], a['g'], a['y'], a['v'], a['s'], a['rows'], a['dim'], 1e-6, None)
+    row, total = 256, 1024                                    # bf16: bytes of a row, of x
+    for base in (1 << 20, 2 << 20):                           # x, the residual: shifted by rows either way
+        for at in (base - total + 16, base - row, base + 16, base + row, base + total - 16):
+            assert n(xo=at) == n(y=at) == _lib.VGDR_ERR_INVALID, at
+            assert b'alias' in L.vgdr_last_error()
+        for at in (base, base + 16, base + total - 16):                   # the bytes are fewer: 512 and 16
+            assert n(v=at) == n(s=at) == n(v=at - 496) == _lib.VGDR_ERR_INVALID, at
+    for at in (3 << 20, (3 << 20) + 16, (3 << 20) + row - 16):            # gamma
+        assert n(xo=at) == n(y=at) == n(v=at) == n(s=at) == _lib.VGDR_ERR_INVALID, at
+    assert n(y=1 << 20) == n(v=2 << 20) == n(xo=4 << 20) == n(s=(5 << 20) + 16) == n(xo=(5 << 20) + 496) == _lib.VGDR_ERR_INVALID
+    assert n(dt=0, xo=(1 << 20) + 2 * total - 16) == n(xo=1 << 20, y=1 << 20) == _lib.VGDR_ERR_INVALID
+
+
+@gpu
+def test_a_norm_in_place_and_beside_what_it_reads():
+    case('mx_rms_norm into x, into the residual, beside x in one buffer, shifted by a row')
+    D = 256
+    buf = torch.randn(12, D, device=DEV).bfloat16()
+    gamma, res = torch.randn(D, device=DEV).bfloat16(), torch.randn(5, D, device=DEV).bfloat16()
+    x = buf[:5]
+    want, h = ops.mx_rms_norm(x, gamma, residual=res)
+    for out in (buf[5:10], buf[7:12]):
+        rows, got = ops.mx_rms_norm(x, gamma, residual=res, out_residual=out)
+        assert got is out and torch.equal(got, h) and torch.equal(rows.values.view(torch.uint8), want.values.view(torch.uint8))
+    for out in (buf[1:6], buf[4:9]):
+        with pytest.raises(AssertionError, match='alias'):
+            ops.mx_rms_norm(x, gamma, residual=res, out_residual=out)
+    r = res.clone()
+    rows, got = ops.mx_rms_norm(x, gamma, residual=r, out_residual=r)
+    assert got is r and torch.equal(r, h) and torch.equal(rows.scales, want.scales)
+    rows, got = ops.mx_rms_norm(x, gamma, residual=res, out_residual=x)
+    assert got is x and torch.equal(x, h) and torch.equal(rows.scales, want.scales)

@@ -35,6 +35,12 @@ constexpr int64_t MX_THREADS = 0xffffff00;        // of a launch, in workgroups 
 // threads for rows of cols columns, eight each, padded to whole 128s
 int64_t mx_threads(int64_t rows, int64_t cols) { return rows > MX_THREADS ? rows : rows * ((cols + 127) / 128 * 16); }
 
+// whether two dense ranges share bytes, NULL none
+bool overlap(const void *a, int64_t na, const void *b, int64_t nb) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a && b && x < y + (uintptr_t)nb && y < x + (uintptr_t)na;
+}
+
 // checks of what is rounded to block-scaled numbers
 int check_mx_source(const char *fn, int dtype, int64_t ld, int64_t rows, int64_t cols) {
     if (dtype != VGDR_F32 && dtype != VGDR_BF16 && dtype != VGDR_F16)
@@ -1215,9 +1221,17 @@ int vgdr_mx_rms_norm(int dtype, const void *x, const void *residual, void *x_out
     if (!aligned16(x) || !aligned16(gamma) || !aligned16(values) || !aligned16(scales) || !aligned16(residual) ||
         !aligned16(x_out) || !aligned16(y))
         return fail(VGDR_ERR_INVALID, "%s: every tensor must be 16-byte aligned", fn);
-    if (values == x || (residual && values == residual) || (x_out && values == x_out) ||
-        (y && (y == x || y == residual || y == x_out || y == values)))
-        return fail(VGDR_ERR_INVALID, "%s: values and y must not alias x, residual or x_out", fn);
+    // a workgroup writes its row while others still read theirs: x_out is x or the residual itself, or apart from all that is read
+    const int64_t es = dtype == VGDR_F32 ? 4 : 2, n = rows * dim * es, nv = rows * ((dim + 127) / 128 * 128), ns = nv / 32;
+    const void *out[] = {values, scales, y, x_out}, *in[] = {x, residual, gamma};
+    const int64_t out_n[] = {nv, ns, n, n}, in_n[] = {n, n, dim * es};
+    for (int i = 0; i < 4; ++i) {
+        for (int j = 0; j < 3; ++j)
+            if (overlap(out[i], out_n[i], in[j], in_n[j]) && !(i == 3 && j < 2 && out[i] == in[j]))
+                return fail(VGDR_ERR_INVALID, "%s: values, scales, y and x_out must not alias an input (x_out may be x or residual)", fn);
+        for (int j = 0; j < i; ++j)
+            if (overlap(out[i], out_n[i], out[j], out_n[j])) return fail(VGDR_ERR_INVALID, "%s: the results must not alias each other", fn);
+    }
     vgdr::MxNorm p{x, residual, x_out, y, gamma, (uint8_t *)values, (uint8_t *)scales, rows, (int)dim, eps};
     return hip_status(vgdr::mx_rms_norm(dtype, p, stream), "vgdr_mx_rms_norm launch");
 }

@@ -2147,7 +2147,7 @@ def mx_weight(w, gated: bool = False) -> MXWeight:
 
 def mx_rms_norm(x, weight, eps: float = 1e-6, residual=None, out_residual=None, norm_out: bool = False):
     """rms_norm with its result as rows in 8 bits (vgdr_mx_rms_norm): h = x + residual, rounded to x's dtype (into
-    out_residual, a new tensor by default), and h rsqrt(mean h^2 + eps) weight, formed in 64 bits and rounded once, to
+    out_residual: x or residual themselves or a tensor apart from both, a new one by default), and h rsqrt(mean h^2 + eps) weight, formed in 64 bits and rounded once, to
     the bytes that mx_quantize would give of it.  Returns the MXRows; with norm_out also the norm
     in x's dtype, rounded as rms_norm's; with residual also h: rows, (rows, h), (rows, y) or (rows, y, h).
     x, residual, weight in one dtype, the last dim a multiple of 8; no autograd."""
