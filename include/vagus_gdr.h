@@ -759,9 +759,12 @@ int vgdr_mx_rms_norm(int dtype, const void *x, const void *residual, void *x_out
 /*
  * y [rows, n] = x W^T for x [rows, k] (x_dtype: an element type with ldx a multiple of 8, or VGDR_MX8 with
  * x_scales) and 4-bit weights of n rows, in out_dtype (an element type).  gated: y [rows, n / 2] =
- * silu(x W1^T) (x W2^T) (the FFN's input half, infra/components/ffn.py:48-50) with sums, activation and product in fp32
- * and one rounding, in an element type or VGDR_MX8 (y_scales).  Products and sums are fp32: bf16, fp16 and fp32 rows
- * meet the weights exactly (as one, two and three bf16 numbers an element).  ldx does not matter for one row.  workspace:
+ * silu(x W1^T) (x W2^T) (the FFN's input half, infra/components/ffn.py:48-50) with activation and product in fp32
+ * and one rounding, in an element type or VGDR_MX8 (y_scales).  Products and sums of 16- and 32-bit rows are fp32: bf16, fp16 and
+ * fp32 rows meet the weights as one, two and three bf16 numbers an element, which is exact (fp32 rows: down to 2^-133, the least of
+ * bf16).  8-bit rows are summed 128 products at a time by the scaled matrix instruction, in fewer bits than fp32, and in fp32 from one
+ * 128 to the next: the results are off by some 1.2e-5 of their size (rms; 5e-8 with bf16 rows), by less than 2^-13 of the sum of |x w| where measured; an
+ * 8-bit result whose largest element lies that near the border of a scale has the next scale.  ldx does not matter for one row.  workspace:
  * vgdr_mx_linear_workspace_size bytes (0: none, as for up to 32 rows), calls that overlap have their own.  At most 2^24 rows of weights and columns.
  */
 int64_t vgdr_mx_linear_workspace_size(int x_dtype, int64_t rows, int64_t k);

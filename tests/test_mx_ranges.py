@@ -53,3 +53,20 @@ def test_the_largest_weights(R, dt):
     want = x.double() @ mx.rounded(w, 4).t()                       # powers of two: nothing is rounded
     for rows in (x, x.bfloat16(), ops.mx_quantize(x)):
         assert torch.equal(ops.mx_linear(rows, got, out_dtype=torch.float32).double(), want)
+
+
+@gpu
+@pytest.mark.parametrize('R', [2, 40])
+@pytest.mark.parametrize('e', [-100, -115, -122, -126])
+def test_small_fp32_rows_are_held_down_to_the_least_of_bf16(R, e):
+    """Parts are cut at 2^-133, so an element is off by less than that; 2 (3 K + 64) 2^-24 of sum |x w| for the sums,
+    2^-24 of the result for its rounding (as tests/test_mx.py)."""
+    case('mx_linear: fp32 rows about 2 to the', e, R)
+    K = 200
+    g = torch.Generator(DEV).manual_seed(R)
+    x = (torch.rand(R, K, generator=g, device=DEV) - 0.5) * 2.0 ** e
+    w = ops.mx_weight(torch.randn(40, K, generator=g, device=DEV) * 2.0 ** 110)
+    wd = w.dequantize(torch.float64)
+    want, A = x.double() @ wd.t(), x.double().abs() @ wd.abs().t()
+    tol = 2.0 ** -133 * wd.abs().sum(1) + A * 2 * (3 * K + 64) * 2 ** -24 + want.abs() * 2 ** -24
+    assert bool(((ops.mx_linear(x, w).double() - want).abs() <= tol).all())

@@ -69,7 +69,7 @@ __device__ __forceinline__ float round_to_odd(double x) {
 }
 
 // v as the sum of P bf16 numbers: cut off, not rounded, so that the largest fp32 numbers stay finite; an infinity or a
-// NaN is the first part's.  bf16 has 8 bits: fp16's 11 take two parts, fp32's 24 three.
+// NaN is the first part's.  bf16 has 8 bits: fp16's 11 take two parts, fp32's 24 three.  What lies below bf16's least, 2^-133, is cut.
 template <int P>
 __device__ __forceinline__ void split(__bf16 (&out)[P], float v) {
     uint32_t u = __builtin_bit_cast(uint32_t, v);

@@ -28,7 +28,9 @@ __device__ __forceinline__ bf16x8 to_bf16(uint32_t q, float scale) {
     return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// 4-bit rows of A, 8-bit rows of B, their blocks' scale bytes
+// 4-bit rows of A, 8-bit rows of B, their blocks' scale bytes.  The instruction sums its 128 products in fewer bits than fp32
+// (results off by 1.2e-5 rms at K 128 to 8192; bf16 rows 1e-8 to 1.3e-7) and adds to fp32.  Taken for its rate, twice bf16's: the
+// rows' rounding to 8 bits is off by 2.6e-2 of a result, 2,000 times that.
 __device__ __forceinline__ f32x4 mfma_mx(u32x4 w, int ws, u32x4 lo, u32x4 hi, int xs, f32x4 c) {
     const i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
     const i32x8 b = {(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};

@@ -2147,9 +2147,10 @@ def mx_weight(w, gated: bool = False) -> MXWeight:
 
 def mx_rms_norm(x, weight, eps: float = 1e-6, residual=None, out_residual=None, norm_out: bool = False):
     """rms_norm with its result as rows in 8 bits (vgdr_mx_rms_norm): h = x + residual, rounded to x's dtype (into
-    out_residual: x or residual themselves or a tensor apart from both, a new one by default), and h rsqrt(mean h^2 + eps) weight, formed in 64 bits and rounded once, to
-    the bytes that mx_quantize would give of it.  Returns the MXRows; with norm_out also the norm
-    in x's dtype, rounded as rms_norm's; with residual also h: rows, (rows, h), (rows, y) or (rows, y, h).
+    out_residual: x or residual themselves or a tensor apart from both, a new one by default), and
+    h rsqrt(mean h^2 + eps) weight, formed in 64 bits and rounded once, to the bytes that mx_quantize would give of it.
+    Returns the MXRows; with norm_out also the norm in x's dtype, rounded as rms_norm's; with residual also h: rows, (rows, h),
+    (rows, y) or (rows, y, h).
     x, residual, weight in one dtype, the last dim a multiple of 8; no autograd."""
     index = x.get_device()
     if index < 0:
@@ -2239,13 +2240,14 @@ def _mx_product(x, w: MXWeight, gated: bool, quantize: bool, out_dtype):
 
 def mx_linear(x, w: MXWeight, out_dtype=None):
     """F.linear(x, w) with 4-bit weights (vgdr_mx_linear), for one row as for a batch of prompts: x (..., k) in fp32, bf16 or
-    fp16, which meets the weights exactly, or MXRows; fp32 sums, rounded once to out_dtype (x's; bf16
+    fp16, which meets the weights exactly (fp32 down to 2^-133) in fp32 sums, or MXRows, whose sums the scaled matrix instruction forms in
+    fewer bits (off by some 1.2e-5 of a result, rms; the rows' own rounding is 2.6e-2); rounded once to out_dtype (x's; bf16
     for MXRows).  A block of weights or of an MXRows that is NaN makes NaN what it takes part in.  No autograd."""
     return _mx_product(x, w, False, False, out_dtype)
 
 
 def mx_swiglu(x, w: MXWeight, quantize: bool = False, out_dtype=None):
-    """swiglu(F.linear(x, w)) with gated 4-bit weights (mx_weight(w, gated=True)) in one kernel: both products, the
+    """swiglu(F.linear(x, w)) with gated 4-bit weights (mx_weight(w, gated=True)) in one kernel: both products with sums as mx_linear's, the
     activation and their product in fp32, rounded once (the module rounds four times, infra/components/ffn.py:48-50),
     to out_dtype as mx_linear, or with `quantize` to MXRows, which the FFN's second product reads.  No autograd."""
     return _mx_product(x, w, True, quantize, out_dtype)
