@@ -258,6 +258,16 @@ def test_a_hooked_map_takes_no_8_bit_rows(which):
     handle.remove()
 
 
+def test_a_layer_with_prompts_of_its_own_takes_no_8_bit_rows():
+    class Own(GatedDeltaNet):
+        def prefill_packed(self, x, cu_seqlens, *, rows=None):
+            return 2 * super().prefill_packed(x, cu_seqlens, rows=rows)
+    m = small()
+    m.blocks[1].att = Own(dim=64, head_count=1, key_head_dim=64, value_head_dim=64, gate='scalar')
+    quantised_on_the_cpu(m)
+    assert m.blocks[0]._takes8() and not m.blocks[1]._takes8()
+
+
 @gpu
 @pytest.mark.parametrize('dtype, bar', [(torch.float32, 1e-4), (torch.bfloat16, 2e-2)])       # as tests/test_mx_model.py
 def test_hooks_on_4_bit_maps_run_on_every_call(dtype, bar):
