@@ -369,6 +369,11 @@ def test_a_model_with_a_later_part_elsewhere_stays_as_it_was(what):
 # --- layers that are not 4-bit ---------------------------------------------------------------------
 
 
+def test_an_ordinary_model_says_how_it_takes_prompts():
+    m = small()
+    assert m.prompt_bits == 16 and 'prompt_bits' not in m.__dict__
+
+
 @gpu
 def test_a_layer_that_is_not_4_bit_searches_for_no_4_bit_map():
     case('attributes that the calls of an ordinary layer look for in vain')

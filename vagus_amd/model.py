@@ -196,6 +196,8 @@ class Block(nn.Module):
 class GDNLM(nn.Module):
     """The reference's GDNLM (gdn_lm.py:20-195) for the all-GDN layout."""
 
+    prompt_bits = 16                                  # of packed prompts' rows in the products; quantize_weights_ sets it
+
     def __init__(self,
                  vocab_size: int,
                  dim: int,
@@ -279,10 +281,10 @@ class GDNLM(nn.Module):
     def quantize_weights_(self, *, prompt_bits: int = 8, head: bool = True) -> 'GDNLM':
         """The blocks' large projections (q, k, v, output gate, W_o, both of the FFN) and the head become 4-bit weights with
         a scale for each 32 (layer.MXLinear), in place and for good, on the GPU: a decode step reads a quarter of the bytes.
-        The embedding, the norms, the short convs and the gates' projections keep their type.  Packed prompts
-        (prefill_packed) go through the products as 8-bit rows, at twice the rate of 16-bit ones, or with prompt_bits=16
-        as they are; other calls take 16-bit rows.  No autograd from then on.  A state_dict of the quantised model loads into one
-        that was quantised.  Returns self."""
+        The embedding, the norms, the short convs and the gates' projections keep their type.  Unless prompt_bits is 16 the
+        activations of packed prompts (prefill_packed) are rounded too: a 16-bit model's go through the products as 8-bit rows, at
+        twice the rate of 16-bit ones.  Other calls take the rows as they are.  No autograd from then on.  A state_dict of the
+        quantised model loads into one that was quantised.  Returns self."""
         assert prompt_bits in (8, 16), f'prompt_bits must be 8 or 16; got {prompt_bits}'
         if head and not isinstance(self.head, MXLinear) and not (_plain_module(self.head, nn.Linear) and self.head.bias is None):
             raise NotImplementedError('4-bit weights stand for a plain bias-free nn.Linear head')
@@ -369,7 +371,7 @@ class GDNLM(nn.Module):
         x = self.embedding(tokens.reshape(1, -1))
         delta = None
         for blk in self.blocks:
-            if (getattr(self, 'prompt_bits', 16) == 8 and x.dtype in (torch.bfloat16, torch.float16)
+            if (self.prompt_bits == 8 and x.dtype in (torch.bfloat16, torch.float16)
                     and blk.rmsnorm1.gamma.dtype == x.dtype == blk.rmsnorm2.gamma.dtype and blk._takes8()):
                 x, delta = blk._stream8(x, delta, cu_seqlens, rows)
             else:
