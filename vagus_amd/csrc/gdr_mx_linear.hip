@@ -144,10 +144,11 @@ constexpr int BF16_TAIL = 4;
 // ahead of this one's products, and meet in LDS, in a fixed order.  A wave passes its rows' tiles through an LDS
 // region of its own, which needs no barrier: a load covers whole rows of a tile there, where fragments
 // straight from global memory would have every lane in a line of its own, and the address unit bounds those
-// (64 rows, K 5632, N 2048: 9.6 us; 64 rows, K and N 8192: 25).
-// Bound by latency, a chain of launch, first loads, K / 128 / NWV steps and the meeting in LDS: one row, K 2048, N 8192
-// 4.5 us (8.9 MB of weights, 1.8 us at a copy's rate), 64 rows 7.1 us; one row, gated 11264, 5.8 us, 64 rows 10.6.  A longer
-// way ahead in the loads, sixteen waves, or eight weight tiles a workgroup took as long or longer.
+// (64 rows, K 5632, N 2048: 9.6 us, 5.9 through LDS; 64 rows, K and N 8192: 25, 17.7).
+// Bound by latency, a chain of launch, first loads, K / 128 / NWV steps and the meeting in LDS.  Recorded, with the weights in the
+// caches / from memory, as a model's step finds them: one row, K 2048, N 8192 3.7 / 5.0 us (8.9 MB of weights, 1.8 us at a copy's
+// rate), 64 rows 7.4 / 8.5; one row, gated 11264, 5.1 / 6.4, 64 rows 9.7 / 11.5.  A longer way ahead in the loads, sixteen
+// waves, or eight weight tiles a workgroup took as long or longer.
 // X: the rows' type (0 fp32, 1 bf16, 2 fp16, MX8, BF16_TAIL).  fp32 and fp16 rows become three and two bf16 planes on their way
 // into LDS; their K, and BF16_TAIL's, may end inside a tile (a check that costs the others half a microsecond).
 template <int X, bool GATED, int MT, int NB, int NWV>
@@ -512,24 +513,26 @@ hipError_t tile_go(const MxLinear &p, int tiles, hipStream_t stream) {
 }
 
 // The variant of the few-row kernel: the smallest tiles that make at most one workgroup a CU.  Smaller ones leave a part of the
-// CUs a second workgroup to wait for, and read the rows or the weights more often.  Kernels alone, us for bf16 / 8-bit rows:
-//   192 rows, K 5632, N 2048: 4 tiles x 32 rows (192 workgroups) 11.3 / 9.7, 2 x 32 (384) 13.9 / 11.3
-//   16 rows, K 5632, N 6144: 2 x 16 (192) 5.6 / 5.4, 1 x 16 (384) 6.5 / 5.9; as fp32 15.3, 26.6
-//   48 rows, K 5632, N 2048: 2 x 16 (192) 5.7 / 5.4, 1 x 16 (384) 6.6 / 5.9
-// and with the call's host time, one a CU against half of them: 64 rows, K 5632, N 2048: 2 x 16 (256) 8.6 / 8.2, 2 x 32
-// (128) 10.7 / 9.7; 32 rows, K 2048, N 8192: 2 x 32 (256) 8.0 / 7.2, 4 x 32 (128) 9.6 / 8.3.  It costs short sums a
-// little: 192 rows, K 1024, N 2048: 5.2 / 5.1 against 6.1 / 4.9; one row, K 2048, N 12288: 5.0 / 4.4 against 4.7 / 4.1.
+// CUs a second workgroup to wait for, and read the rows or the weights more often.  Kernels alone, recorded, the weights in the
+// caches, us for bf16 / 8-bit rows:
+//   192 rows, K 5632, N 2048: 4 tiles x 32 rows (192 workgroups) 11.7 / 9.7, 2 x 32 (384) 13.9 / 11.5
+//   16 rows, K 5632, N 6144: 2 x 16 (192) 5.7 / 5.5, 1 x 16 (384) 6.7 / 6.2; as fp32 15.7, 26.6
+//   48 rows, K 5632, N 2048: 2 x 16 (192) 5.5 / 5.3, 1 x 16 (384) 6.4 / 6.0
+// and one a CU against half of them: 64 rows, K 5632, N 2048: 2 x 16 (256) 5.9 / 5.5, 2 x 32 (128) 8.0 / 7.0; 32 rows, K 2048,
+// N 8192: 2 x 32 (256) 5.3 / 4.8, 4 x 32 (128) 6.8 / 6.2.  It costs short sums a
+// little: 192 rows, K 1024, N 2048: 5.3 / 5.0 against 6.1 / 4.9; one row, K 2048, N 12288: 5.1 / 4.4 against 4.8 / 4.2.
 // The kernel for few rows up to where 4 x 32 makes one workgroup a CU: it has the whole sum in flight (128 rows, K 5632,
-// N 2048: 11.0 / 9.9, 64 x 64 tiles 26.6 / 18.8).  Past that it has four waves, so that two are on a CU (64 rows, K 2048, gated
-// 11264: 13.2 / 11.1, eight waves 16.2 / 14.3), and bf16 rows, whose tiles convert the weights in each of many steps one
-// behind the other, keep it the longer the sum is.  Kernels alone, few / tiles, at N 8192 and gated 8192:
-//   two a CU (128 rows): K 512 5.1 / 4.6 and 5.2 / 5.1, K 1024 6.9 / 6.7 and 7.1 / 7.2, K 2048 9.9 / 10.7 and 9.9 / 11.5
-//   three (192 rows): K 1536 12.0 / 10.7 and 12.2 / 12.4, K 2048 14.1 / 13.2 and 14.2 / 15.6, K 5632 27.9 / 31.5 and 28.5 / 37.0
-//   four (256 rows): K 2048 16.8 / 13.7 and 17.4 / 15.9, K 5632 35.9 / 33.4 and 36.1 / 37.7
-// 8-bit rows: two a CU, K 2048 8.8 / 8.0 and 8.9 / 8.3, K 5632 16.3 / 17.6 and 16.8 / 16.9.
-// Tiles: largest with 5 workgroups for 4 CUs.  512 rows, K 2048, N 8192: 64 x 128 (512) 24.1 / 15.9, 64 x 64 (1,024) 27.6 /
-// 22.9; 256 rows: 64 x 64 (512) 17.0 / 13.2, 64 x 128 (256) 18.2 / 14.6; 8-bit rows, N 32768, 512 rows: 128 x 256
-// (512) 34.3, 64 x 256 38.2, 256 rows: 64 x 256 (512) 22.2, 128 x 256 (256) 25.3.
+// N 2048: 8.7 / 7.4, 64 x 64 tiles 24.4 / 15.5).  Past that it has four waves, so that two are on a CU (64 rows, K 2048, gated
+// 11264: 9.7 / 8.8, eight waves 12.8 / 10.5), and bf16 rows, whose tiles convert the weights in each of many steps one
+// behind the other, keep it the longer the sum is.  Few / tiles, at N 8192 and gated 8192:
+//   two a CU (128 rows): K 512 5.1 / 4.8 and 5.3 / 5.0, K 1024 7.0 / 6.9 and 7.2 / 7.1, K 2048 10.1 / 10.9 and 10.1 / 11.2
+//   three (192 rows): K 1536 12.3 / 10.7 and 12.2 / 12.1, K 2048 14.1 / 13.0 and 14.2 / 15.2, K 5632 28.4 / 30.5 and 26.9 / 35.9
+//   four (256 rows): K 2048 17.1 / 13.3 and 16.8 / 15.4, K 5632 34.1 / 31.3 and 33.9 / 36.4
+// 8-bit rows: two a CU, K 2048 8.6 / 8.3 and 9.2 / 8.3, K 5632 17.2 / 19.0 and 17.1 / 23.4; with the weights from memory the few-row
+// kernel is ahead throughout (9.9 / 14.4 and 10.3 / 14.5, 20.3 / 32.8 and 20.8 / 33.1).
+// Tiles: largest with 5 workgroups for 4 CUs.  512 rows, K 2048, N 8192: 64 x 128 (512) 21.9 / 12.0, 64 x 64 (1,024) 23.7 /
+// 18.5; 256 rows: 64 x 64 (512) 13.4 / 10.2, 64 x 128 (256) 14.5 / 9.8, from memory 15.1 / 14.8 and 15.7 / 15.6; 8-bit rows,
+// N 32768, 512 rows: 128 x 256 (512) 33.5, 64 x 256 34.7, 256 rows: 64 x 256 (512) 19.2, 128 x 256 (256) 22.5.
 // Rows that the kernel for few rows converts itself (MX_RAW_ROWS at most) stay as they are: fp32 or fp16, or of a width that
 // ends inside a tile: one launch instead of two.  Past it, planes first / as they are, fp16 rows, kernels alone: 64 rows, K 2048,
 // N 8192 12.6 / 13.4, N 2048 7.6 / 6.3, N 32000 26.1 / 51.7, gated 11264 16.6 / 19.0; 48 rows, K 5632, N 2048 14.5 / 18.9.
