@@ -94,6 +94,22 @@ def test_a_recorded_step_knows_every_4_bit_weight():
         kept.append(changes(lambda: m.embedding.weight.mul_(2)))
 
 
+def test_a_recorded_step_of_an_object_that_is_no_module():
+    m = small()
+    m.blocks[1].ffn.l2 = blank(64, m.blocks[1].ffn.hidden_dim)
+
+    class Plain:
+        blocks, parameters = m.blocks, m.parameters
+    m.reset_cache(1)
+    gen = RaggedGenerator(Plain())
+    keys = [gen._fingerprint()]
+    for change in (lambda: m.head.weight.mul_(2), lambda: m.blocks[1].ffn.l2.values.fill_(1), lambda: m.blocks[0].ffn.l1.weight.mul_(2)):
+        with torch.no_grad():
+            change()
+        keys.append(gen._fingerprint())
+    assert len(set(keys)) == 4 and keys[-1] == gen._fingerprint()
+
+
 @gpu
 def test_a_model_class_of_the_callers_own_is_recorded_again_when_its_4_bit_weights_move():
     case('4-bit layers in another model class: replaced, then loaded into')

@@ -465,6 +465,8 @@ class RaggedGenerator:
         change one of them), and each layer's state and conv-cache buffers.  A
         replay is valid only while the addresses are unchanged."""
         key, todo = [], [self.model]
+        if not isinstance(self.model, nn.Module):     # a caller's own object around blocks and parameters
+            key, todo = [(p.data_ptr(), 0 if p.is_inference() else p._version) for p in self.model.parameters()], list(self.model.blocks)
         while todo:                                   # the modules' own tables: twice as fast as parameters(), at every step
             m = todo.pop()
             todo += [c for c in m._modules.values() if c is not None]
