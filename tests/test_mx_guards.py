@@ -283,6 +283,18 @@ def test_a_layer_with_prompts_of_its_own_takes_no_8_bit_rows():
     quantised_on_the_cpu(m)
     assert m.blocks[0]._takes8() and not m.blocks[1]._takes8()
 
+    class Around(nn.Module):
+        """A layer's calls handed on by name."""
+
+        def __init__(self, layer):
+            super().__init__()
+            self.layer = layer
+
+        def __getattr__(self, name):
+            return super().__getattr__(name) if name == 'layer' else getattr(self._modules['layer'], name)
+    m.blocks[0].att = Around(m.blocks[0].att)
+    assert not m.blocks[0]._takes8()
+
 
 @gpu
 @pytest.mark.parametrize('dtype, bar', [(torch.float32, 1e-4), (torch.bfloat16, 2e-2)])       # as tests/test_mx_model.py

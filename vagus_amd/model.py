@@ -173,7 +173,7 @@ class Block(nn.Module):
         hooks or other modules in their places a prompt's rows stay as they are, and the modules are called."""
         a, f = self.att, self.ffn
         return (type(f).forward is FFN.forward and not _hooked(f)
-                and type(a).prefill_packed is GatedDeltaNet.prefill_packed and _plain_module(getattr(a, 'w_in', None), MXLinear)
+                and getattr(type(a), 'prefill_packed', None) is GatedDeltaNet.prefill_packed and _plain_module(getattr(a, 'w_in', None), MXLinear)
                 and (not a.out_proj or _plain_module(a.wo, MXLinear))
                 and _plain_module(f.l1, MXLinear) and f.l1.gated and _plain_module(f.l2, MXLinear))
 
